@@ -410,6 +410,153 @@ int velox_hip_attention_decode(const float* d_qkv, uint16_t* d_kv_layer, uint32_
                                uint32_t d, uint32_t s_max, uint32_t pos, float theta, uint32_t splits,
                                float* d_out, hipStream_t stream);
 
+/* ---- paged KV cache: rotary positions, append, attention, pages (no counterpart in the reference, whose
+ *      caches are one contiguous block per sequence) ----
+ * A cache is described by a plain struct over device memory that the caller owns (velox_hip_paged_bytes gives
+ * the sizes). Every entry point checks the description (EINVAL), launches on `stream` with the stream's device
+ * current, allocates nothing, does not synchronize and can be captured into a hipGraph. The library keeps
+ * nothing between calls; a call's workspace or scratch is the call's own until the stream has passed it.
+ *
+ * A page holds page_size positions (a multiple of 32) of one layer in the layout of an arena's layer cache of
+ * page_size positions: K [num_kv_heads][page_size][head_dim], then V [num_kv_heads][page_size / 32][head_dim][32]
+ * (velox_hip_attention_decode). So an arena's kv_cache_pool is such a pool too: its sequences' caches are pages of
+ * s_cap positions.
+ * Position p of sequence s lies in page table[s * table_stride + p / page_size]. An entry that is no page number
+ * (VELOX_HIP_NO_PAGE, or >= n_pages) and positions past max_pages entries have no memory: attention leaves such
+ * positions out as a mask does, the append drops their k and v. */
+#define VELOX_HIP_NO_PAGE 0xFFFFFFFFu
+#define VELOX_HIP_NO_SEQ 0xFFFFFFFFu
+typedef struct VeloxHipPagedCache {
+    void* pool;             /* page p of layer l at pool + l * layer_stride + p * page bytes; 16-byte aligned */
+    uint64_t layer_stride;  /* bytes, a multiple of 16, at least n_pages * page bytes (any value with one layer) */
+    uint32_t dtype;         /* VELOX_DT_F16 or VELOX_DT_BF16 */
+    uint32_t num_layers, num_kv_heads, head_dim;  /* head_dim 64 or 128 */
+    uint32_t n_pages, page_size;
+    uint32_t n_seqs, max_pages, table_stride;     /* n_seqs <= 4096; table rows of max_pages entries */
+    uint32_t reserved;      /* 0 */
+    uint32_t* table;        /* [n_seqs][table_stride] page numbers */
+    uint32_t* lens;         /* [n_seqs] positions of each sequence, new rows included; below 2^31 */
+    uint32_t* refs;         /* [n_pages] how many table entries (and other holders) name a page; 0: free.
+                               NULL where the caller keeps the pages: velox_hip_pages_* then refuse */
+    uint32_t* scratch;      /* velox_hip_pages_* only, velox_hip_paged_bytes' scratch_bytes */
+} VeloxHipPagedCache;
+/* Sizes of a description's memory (its pointers are not looked at): page_bytes one page of one layer. Any
+ * output may be NULL. */
+int velox_hip_paged_bytes(const VeloxHipPagedCache* c, uint64_t* page_bytes, uint64_t* pool_bytes,
+                          uint64_t* table_bytes, uint64_t* refs_bytes, uint64_t* scratch_bytes);
+
+/* Activation rows: element e of head h of row r at data[r * row_stride + h * head_stride + e] (strides in
+ * elements; slices of fused q/k/v rows are such rows). Any alignment of the element type. */
+typedef struct VeloxHipRows {
+    void* data;
+    uint32_t dtype;         /* VELOX_DT_F32, _F16 or _BF16 */
+    uint32_t heads;
+    uint64_t row_stride, head_stride;
+} VeloxHipRows;
+
+/* ---- rotary positions ----
+ * Pair j of a head's first rot_dim values turns by position * f_j: (a, b) -> amplitude (a cos - b sin,
+ * b cos + a sin); the values behind rot_dim pass. HALF pairs (j, j + rot_dim / 2), INTERLEAVED (2j, 2j + 1).
+ * f_j = theta^(-2j / rot_dim), scaled for long contexts:
+ *   LINEAR  f / factor;
+ *   BANDS   pairs with at least high_turns turns within original_len positions keep f, those with at most
+ *           low_turns get f / factor, between them the share (turns - low_turns) / (high_turns - low_turns) of f
+ *           and the rest of f / factor (Llama-3.1's rule);
+ *   YARN    f for pairs below floor(pair(high_turns)), f / factor from ceil(pair(low_turns)), a linear ramp
+ *           between, pair(n) = rot_dim ln(original_len / (2 pi n)) / (2 ln theta) (the YaRN paper's rule).
+ * Angles are formed in 64 bits, so that far positions keep their phase. */
+#define VELOX_ROPE_HALF 0u
+#define VELOX_ROPE_INTERLEAVED 1u
+#define VELOX_ROPE_PLAIN 0u
+#define VELOX_ROPE_LINEAR 1u
+#define VELOX_ROPE_BANDS 2u
+#define VELOX_ROPE_YARN 3u
+typedef struct VeloxHipRopeConfig {
+    uint32_t rot_dim;       /* even, 2..256 */
+    uint32_t layout, scaling;
+    uint32_t original_len;  /* BANDS, YARN */
+    double theta, factor;   /* factor: >= 1 (PLAIN ignores it) */
+    double low_turns, high_turns; /* 0, 0: BANDS 1 and 4, YARN 1 and 32 */
+    double amplitude;       /* 0: YARN 0.1 ln(factor) + 1, else 1 */
+} VeloxHipRopeConfig;
+typedef struct VeloxHipRope VeloxHipRope; /* opaque; host memory only, usable on every device */
+int velox_hip_rope_create(const VeloxHipRopeConfig* cfg, VeloxHipRope** out);
+void velox_hip_rope_destroy(VeloxHipRope* r);
+/* f_j (rot_dim / 2 values, radians per position) and the amplitude; either may be NULL. */
+int velox_hip_rope_frequencies(const VeloxHipRope* r, double* freq, double* amplitude);
+/* out[r] = x[r] turned by d_positions[r] for r < n_rows (out may be x itself: the same data and strides; other
+ * overlaps are not allowed). The two have the same dtype and heads. */
+int velox_hip_rope_rows(const VeloxHipRope* r, const VeloxHipRows* x, const VeloxHipRows* out, uint32_t n_rows,
+                        uint32_t head_dim, const uint32_t* d_positions, hipStream_t stream);
+/* The new rows of a layer: q turned into q_out, k turned and v into the pages (rounded to the cache's type).
+ * Rows d_q_start[s] .. d_q_start[s + 1] are sequence s's, its last one at position lens[s] - 1 (d_q_start NULL:
+ * row s is sequence s's, n_rows <= n_seqs). Rows behind the last sequence, and rows in front of position 0, are
+ * left as they were. rope NULL: no rotation. q and q_out may both be NULL, or the same rows. No two sequences
+ * may write the same page (velox_hip_pages_extend sees to it). */
+int velox_hip_rope_append(const VeloxHipPagedCache* c, uint32_t layer, const VeloxHipRope* rope, const VeloxHipRows* q,
+                          const VeloxHipRows* k, const VeloxHipRows* v, const VeloxHipRows* q_out,
+                          const uint32_t* d_q_start, uint32_t n_rows, hipStream_t stream);
+
+/* ---- attention over the pages ----
+ * o = sum_j softmax_j(scale q . k_j) v_j over the positions j that the row at position t sees: j <= t and
+ * (window == 0, or j > t - window, or j < sinks). Head h reads KV head h / (heads / num_kv_heads). A row that
+ * sees nothing gives 0. scale 0: 1 / sqrt(head_dim). q and out: any element types (q of another type than the
+ * cache's is not rounded to it). What masked or unwritten places of the pages hold does not matter.
+ *
+ * paged_attention: row s is the newest position of sequence s (t = lens[s] - 1), s < n_seqs. Long caches are
+ * split over workgroups and joined. max_len: an upper bound of lens that the split is planned by (0: max_pages *
+ * page_size); longer sequences are still right. workspace: velox_hip_paged_attention_bytes of the same cache, heads and
+ * bounds, enough for every mask (may be 0 bytes: NULL), 16-byte aligned.
+ *
+ * paged_prompt_attention: the rows of a ragged batch as in velox_hip_rope_append; every row sees what its own
+ * position allows. max_rows: an upper bound of a sequence's rows that the split is planned by (0: n_rows). Rows
+ * behind the last sequence, and in front of position 0, are left as they were. */
+typedef struct VeloxHipAttnMask {
+    uint32_t window, sinks;
+} VeloxHipAttnMask;
+int velox_hip_paged_attention_bytes(const VeloxHipPagedCache* c, uint32_t heads, uint32_t max_len,
+                                    uint64_t* bytes);
+int velox_hip_paged_attention(const VeloxHipPagedCache* c, uint32_t layer, const VeloxHipRows* q, const VeloxHipRows* out,
+                              VeloxHipAttnMask mask, float scale, uint32_t max_len, void* workspace,
+                              uint64_t workspace_bytes, hipStream_t stream);
+int velox_hip_paged_prompt_attention_bytes(const VeloxHipPagedCache* c, uint32_t heads, uint32_t n_rows,
+                                           uint32_t max_rows, uint32_t max_len, uint64_t* bytes);
+int velox_hip_paged_prompt_attention(const VeloxHipPagedCache* c, uint32_t layer, const VeloxHipRows* q,
+                                     const VeloxHipRows* out, const uint32_t* d_q_start, uint32_t n_rows,
+                                     VeloxHipAttnMask mask, float scale, uint32_t max_rows, uint32_t max_len,
+                                     void* workspace, uint64_t workspace_bytes, hipStream_t stream);
+
+/* ---- pages ----
+ * The bookkeeping lives on the device (table, lens, refs), so that captured steps can cross page borders. Every
+ * rule goes by index: the same state and arguments give the same pages. Table entries past a sequence's pages are
+ * VELOX_HIP_NO_PAGE (reset writes them), and refs is at least the number of entries that name a page: a holder
+ * outside the table (a kept prefix) adds its own count. Entries that are no page number are passed over.
+ * Calls on one cache are ordered by the caller (one stream).
+ *
+ * reset: no sequence has a page, every page is free.
+ * extend: lens[s] += d_add[s] for every sequence, with the pages that takes: first, where the sequence's last page
+ *   is partly filled and others hold it too, a page of its own to which every layer's data is copied (of several
+ *   sequences that extend such a page, with nobody else holding it, the last one keeps the original), then new
+ *   pages behind. Pages are the lowest free ones, given out in the order of the sequences. A sequence whose
+ *   positions would pass max_pages is refused: it stays as it was. So is the first that the free pages do not
+ *   suffice for, and all behind it that extend.
+ * fork: every sequence s becomes what sequence d_src[s] was (its pages shared), all at once: d_src[s] == s stays, a
+ *   number >= n_seqs (VELOX_HIP_NO_SEQ) leaves it empty. Pages that nobody holds any more are free.
+ * free: the sequences d_seqs[0 .. n) are empty (numbers >= n_seqs are passed over; one may appear twice).
+ * trim: frees the pages that no later row of a window sees: whole pages inside [sinks, lens[s] + 1 - window)
+ *   become VELOX_HIP_NO_PAGE, the length stays. window >= 1.
+ * compact: the live pages fill the front of the pool: the k-th free place among the first L (L live pages) takes
+ *   the k-th live page behind them, data of every layer, refs and table entries included (holders outside the table
+ *   are not told: not while there are any).
+ * status: {sequences that the last extend refused, free pages now}; synchronizes the stream. */
+int velox_hip_pages_reset(const VeloxHipPagedCache* c, hipStream_t stream);
+int velox_hip_pages_extend(const VeloxHipPagedCache* c, const uint32_t* d_add, hipStream_t stream);
+int velox_hip_pages_fork(const VeloxHipPagedCache* c, const uint32_t* d_src, hipStream_t stream);
+int velox_hip_pages_free(const VeloxHipPagedCache* c, const uint32_t* d_seqs, uint32_t n, hipStream_t stream);
+int velox_hip_pages_trim(const VeloxHipPagedCache* c, uint32_t window, uint32_t sinks, hipStream_t stream);
+int velox_hip_pages_compact(const VeloxHipPagedCache* c, hipStream_t stream);
+int velox_hip_pages_status(const VeloxHipPagedCache* c, uint32_t* refused, uint32_t* free_pages, hipStream_t stream);
+
 /* ---- runner (velox_cuda_runner.cu:327-726 flow: plan, alloc, load, capture, prefill, decode) ---- */
 typedef struct VeloxHipRunOptions {
     const char* model;       /* builtin config name (unless model_file or weights_path is given) */

@@ -109,6 +109,37 @@ class MlaRunReport(C.Structure):
                                           "wall_ms")] + [("status", C.c_int)]
 
 
+NO_PAGE = NO_SEQ = 0xFFFFFFFF
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS, ROPE_YARN = 0, 1, 2, 3
+
+
+class PagedCacheDesc(C.Structure):
+    """VeloxHipPagedCache: a paged KV cache over memory the caller owns."""
+    _fields_ = [
+        ("pool", C.c_void_p), ("layer_stride", C.c_uint64), ("dtype", C.c_uint32), ("num_layers", C.c_uint32),
+        ("num_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32),
+        ("n_seqs", C.c_uint32), ("max_pages", C.c_uint32), ("table_stride", C.c_uint32), ("reserved", C.c_uint32),
+        ("table", C.c_void_p), ("lens", C.c_void_p), ("refs", C.c_void_p), ("scratch", C.c_void_p),
+    ]
+
+
+class Rows(C.Structure):
+    """VeloxHipRows: activation rows [row][head][element] by strides in elements."""
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_uint32), ("heads", C.c_uint32), ("row_stride", C.c_uint64),
+                ("head_stride", C.c_uint64)]
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [("rot_dim", C.c_uint32), ("layout", C.c_uint32), ("scaling", C.c_uint32), ("original_len", C.c_uint32),
+                ("theta", C.c_double), ("factor", C.c_double), ("low_turns", C.c_double), ("high_turns", C.c_double),
+                ("amplitude", C.c_double)]
+
+
+class AttnMask(C.Structure):
+    _fields_ = [("window", C.c_uint32), ("sinks", C.c_uint32)]
+
+
 MLA_Q_A, MLA_Q_B, MLA_KV_A, MLA_KV_B, MLA_O, MLA_NORM, MLA_Q_A_NORM, MLA_KV_A_NORM = range(1, 9)
 
 
@@ -223,6 +254,25 @@ _SIGS = {
     "velox_hip_mla_arena_check": (_I, [C.POINTER(Arena), C.POINTER(MlaConfig)]),
     "velox_hip_mla_graph_step": (None, [C.POINTER(Arena), _U64, _P]),
     "velox_hip_mla_decode": (None, [C.POINTER(Arena), _U32, C.c_size_t, _U64, _P]),
+    "velox_hip_paged_bytes": (_I, [C.POINTER(PagedCacheDesc)] + [C.POINTER(_U64)] * 5),
+    "velox_hip_rope_create": (_I, [C.POINTER(RopeConfig), C.POINTER(_P)]),
+    "velox_hip_rope_destroy": (None, [_P]),
+    "velox_hip_rope_frequencies": (_I, [_P, C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+    "velox_hip_rope_rows": (_I, [_P, C.POINTER(Rows), C.POINTER(Rows), _U32, _U32, _P, _P]),
+    "velox_hip_rope_append": (_I, [C.POINTER(PagedCacheDesc), _U32, _P] + [C.POINTER(Rows)] * 4 + [_P, _U32, _P]),
+    "velox_hip_paged_attention_bytes": (_I, [C.POINTER(PagedCacheDesc), _U32, _U32, C.POINTER(_U64)]),
+    "velox_hip_paged_attention": (_I, [C.POINTER(PagedCacheDesc), _U32, C.POINTER(Rows), C.POINTER(Rows), AttnMask, _F,
+                                       _U32, _P, _U64, _P]),
+    "velox_hip_paged_prompt_attention_bytes": (_I, [C.POINTER(PagedCacheDesc), _U32, _U32, _U32, _U32, C.POINTER(_U64)]),
+    "velox_hip_paged_prompt_attention": (_I, [C.POINTER(PagedCacheDesc), _U32, C.POINTER(Rows), C.POINTER(Rows), _P, _U32,
+                                              AttnMask, _F, _U32, _U32, _P, _U64, _P]),
+    "velox_hip_pages_reset": (_I, [C.POINTER(PagedCacheDesc), _P]),
+    "velox_hip_pages_extend": (_I, [C.POINTER(PagedCacheDesc), _P, _P]),
+    "velox_hip_pages_fork": (_I, [C.POINTER(PagedCacheDesc), _P, _P]),
+    "velox_hip_pages_free": (_I, [C.POINTER(PagedCacheDesc), _P, _U32, _P]),
+    "velox_hip_pages_trim": (_I, [C.POINTER(PagedCacheDesc), _U32, _U32, _P]),
+    "velox_hip_pages_compact": (_I, [C.POINTER(PagedCacheDesc), _P]),
+    "velox_hip_pages_status": (_I, [C.POINTER(PagedCacheDesc), C.POINTER(_U32), C.POINTER(_U32), _P]),
     "velox_hip_arena_check": (_I, [C.POINTER(Arena), C.POINTER(ModelConfig)]),
     "velox_hip_record_error": (None, [_I]),
     "velox_hip_decode": (None, [C.POINTER(Arena), _U32, C.c_size_t, _U64, _P]),

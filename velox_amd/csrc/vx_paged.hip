@@ -1,0 +1,495 @@
+// vx_paged.hip -- the paged KV cache: rotary positions, the append to the pages, the pages' bookkeeping.
+#include "vx_paged.h"
+
+namespace {
+
+// ---- elements ----
+__device__ __forceinline__ float vx_load(const void* p, size_t i, uint32_t dtype) {
+    if (dtype == VELOX_DT_F32) return ((const float*)p)[i];
+    if (dtype == VELOX_DT_F16) return (float)((const _Float16*)p)[i];
+    return (float)((const __bf16*)p)[i];
+}
+// The fp32 value rounded once (to nearest even) to the element type.
+__device__ __forceinline__ void vx_store(void* p, size_t i, uint32_t dtype, float v) {
+    if (dtype == VELOX_DT_F32) ((float*)p)[i] = v;
+    else if (dtype == VELOX_DT_F16) ((_Float16*)p)[i] = (_Float16)v;
+    else ((__bf16*)p)[i] = (__bf16)v;
+}
+
+// cos and sin of position * f_j, times the amplitude. The angle is position * f_j / 2 pi turns in 64 bits (a
+// product in 32 would be off by 2^-24 of a position's whole angle: 0.06 rad at position 10^6); its fraction of
+// a turn, at most one half, is exact to 2^-25 in fp32.
+__device__ __forceinline__ float2 vx_turn(const VxRopeTable& t, uint32_t j, uint32_t pos) {
+    const double turns = (double)pos * t.turns[j];
+    const float f = (float)(turns - rint(turns));
+    float s, c;
+    sincospif(2.0f * f, &s, &c);
+    return make_float2(c * t.amp, s * t.amp);
+}
+
+// ---- rotation of rows: one workgroup per kRows rows, the rows' cos/sin shared by all heads through LDS ----
+constexpr int kRopeThreads = 256;
+
+__global__ __launch_bounds__(kRopeThreads) void vx_rope_rows_kernel(VxRopeTable t, VxRowsView x, VxRowsView o, uint32_t n_rows,
+                                                                    uint32_t d, const uint32_t* __restrict__ positions) {
+    __shared__ float2 cs[kVxMaxRopePairs];
+    const uint32_t half = t.rot / 2, row = blockIdx.x;
+    const uint32_t pos = positions[row];
+    for (uint32_t j = threadIdx.x; j < half; j += kRopeThreads) cs[j] = vx_turn(t, j, pos);
+    __syncthreads();
+    const uint32_t units = half + (d - t.rot);  // a pair, or one value behind them
+    for (uint32_t i = threadIdx.x; i < units * x.heads; i += kRopeThreads) {
+        const uint32_t h = i / units, u = i % units;
+        const size_t xb = (size_t)row * x.rs + (size_t)h * x.hs, ob = (size_t)row * o.rs + (size_t)h * o.hs;
+        if (u < half) {
+            const uint32_t e0 = t.interleaved ? 2 * u : u, e1 = t.interleaved ? 2 * u + 1 : u + half;
+            const float a = vx_load(x.data, xb + e0, x.dtype), b = vx_load(x.data, xb + e1, x.dtype);
+            vx_store(o.data, ob + e0, o.dtype, a * cs[u].x - b * cs[u].y);
+            vx_store(o.data, ob + e1, o.dtype, b * cs[u].x + a * cs[u].y);
+        } else {
+            const uint32_t e = t.rot + u - half;
+            vx_store(o.data, ob + e, o.dtype, vx_load(x.data, xb + e, x.dtype));
+        }
+    }
+}
+
+// ---- ragged batches ----
+// Rows [lo, hi) of sequence s and the position of row lo; positions may be negative.
+struct VxSpan {
+    uint32_t lo, hi;
+    int64_t pos0;
+};
+__device__ __forceinline__ VxSpan vx_span(const uint32_t* q_start, const uint32_t* lens, uint32_t n_rows, uint32_t s) {
+    VxSpan r;
+    r.lo = q_start ? min(q_start[s], n_rows) : s;
+    r.hi = q_start ? min(q_start[s + 1], n_rows) : min(s + 1u, n_rows);
+    r.hi = max(r.hi, r.lo);
+    r.pos0 = (int64_t)lens[s] - (int64_t)(r.hi - r.lo);
+    return r;
+}
+
+// The sequence and index within it of 32-position block `item` of the batch, blocks counted over the sequences
+// in order; false behind the last. Every wave walks the sequences 64 at a time.
+__device__ __forceinline__ bool vx_find_block(const VxAppendArgs& a, uint32_t item, uint32_t& seq, uint32_t& blk) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t base = 0;
+    for (uint32_t s0 = 0; s0 < a.c.n_seqs; s0 += 64) {
+        const uint32_t s = s0 + lane;
+        uint32_t n = 0;
+        if (s < a.c.n_seqs) {
+            const VxSpan r = vx_span(a.q_start, a.c.lens, a.n_rows, s);
+            const int64_t end = r.pos0 + (r.hi - r.lo), from = r.pos0 > 0 ? r.pos0 : 0;
+            if (end > from) n = (uint32_t)(((end + 31) >> 5) - (from >> 5));
+        }
+        uint32_t upto = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(upto, o);
+            if (lane >= (uint32_t)o) upto += v;
+        }
+        const uint64_t hit = __ballot(item < base + upto);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            seq = s0 + (uint32_t)l;
+            blk = item - base - (uint32_t)(__shfl(upto, l) - __shfl(n, l));
+            return true;
+        }
+        base += __shfl(upto, 63);
+    }
+    return false;
+}
+
+// ---- append: a workgroup takes one 32-position block (a V block of the pages, up to 32 rows) of a sequence ----
+__global__ __launch_bounds__(256) void vx_rope_append_kernel(VxRopeTable t, VxAppendArgs a) {
+    __shared__ float2 cs[32][kVxMaxRopePairs / 2];
+    uint32_t seq, blk;
+    if (!vx_find_block(a, blockIdx.x, seq, blk)) return;
+    const VxSpan r = vx_span(a.q_start, a.c.lens, a.n_rows, seq);
+    const int64_t from = r.pos0 > 0 ? r.pos0 : 0, end = r.pos0 + (r.hi - r.lo);
+    const int64_t p0 = ((from >> 5) + blk) << 5;  // the block's first position
+    const uint32_t i0 = (uint32_t)((from > p0 ? from : p0) - p0), i1 = (uint32_t)((end < p0 + 32 ? end : p0 + 32) - p0);
+    const uint32_t row0 = r.lo + (uint32_t)(p0 + i0 - r.pos0), n = i1 - i0;  // rows row0 .. row0 + n at positions p0 + i0 ..
+    const uint32_t half = t.rot / 2, d = a.c.d, hkv = a.c.hkv;
+    for (uint32_t i = threadIdx.x; i < n * half; i += 256) cs[i / half][i % half] = vx_turn(t, i % half, (uint32_t)(p0 + i0 + i / half));
+    const uint64_t pi = (uint64_t)p0 / a.c.page_size;
+    uint32_t page = kVxNoPage;
+    if (pi < a.c.max_pages) page = a.c.table[(size_t)seq * a.c.table_stride + pi];
+    const bool have = page < a.c.n_pages;
+    uint16_t* kp = (uint16_t*)(a.c.pool + (size_t)(have ? page : 0u) * a.c.page_bytes);
+    uint16_t* vp = kp + (size_t)hkv * a.c.page_size * d;
+    const uint32_t in_page = (uint32_t)((uint64_t)p0 % a.c.page_size);
+    __syncthreads();
+    const uint32_t hq = a.q.data ? a.q.heads : 0, heads = hq + 2 * hkv;
+    const uint32_t units = half + (d - t.rot);
+    for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < n * heads * units; i += gridDim.y * 256) {
+        const uint32_t u = i % units, h = i / units % heads, w = i / units / heads;
+        const uint32_t row = row0 + w;
+        const bool pair = u < half;
+        const uint32_t e0 = pair ? (t.interleaved ? 2 * u : u) : t.rot + u - half;
+        const uint32_t e1 = pair ? (t.interleaved ? 2 * u + 1 : u + half) : e0;
+        const VxRowsView& x = h < hq ? a.q : h < hq + hkv ? a.k : a.v;
+        const uint32_t hh = h < hq ? h : h < hq + hkv ? h - hq : h - hq - hkv;
+        const size_t xb = (size_t)row * x.rs + (size_t)hh * x.hs;
+        float y0 = vx_load(x.data, xb + e0, x.dtype), y1 = pair ? vx_load(x.data, xb + e1, x.dtype) : 0.0f;
+        if (pair && h < hq + hkv) {
+            const float2 c = cs[w][u];
+            const float a0 = y0, b0 = y1;
+            y0 = a0 * c.x - b0 * c.y;
+            y1 = b0 * c.x + a0 * c.y;
+        }
+        if (h < hq) {
+            const size_t ob = (size_t)row * a.qo.rs + (size_t)hh * a.qo.hs;
+            vx_store(a.qo.data, ob + e0, a.qo.dtype, y0);
+            if (pair) vx_store(a.qo.data, ob + e1, a.qo.dtype, y1);
+        } else if (have && h < hq + hkv) {
+            uint16_t* to = kp + ((size_t)hh * a.c.page_size + in_page + i0 + w) * d;
+            vx_store(to, e0, a.c.dtype, y0);
+            if (pair) vx_store(to, e1, a.c.dtype, y1);
+        } else if (have) {
+            uint16_t* to = vp + ((size_t)hh * (a.c.page_size / 32) + in_page / 32) * d * 32;
+            const uint32_t slot = vx_vslot(i0 + w);
+            vx_store(to, (size_t)e0 * 32 + slot, a.c.dtype, y0);
+            if (pair) vx_store(to, (size_t)e1 * 32 + slot, a.c.dtype, y1);
+        }
+    }
+}
+
+// ---- pages ----
+constexpr int kPageThreads = 1024;
+
+// Sum over the threads before this one; total: the workgroup's sum. Two barriers.
+__device__ __forceinline__ uint32_t vx_scan(uint32_t v, uint32_t& total) {
+    __shared__ uint32_t part[kPageThreads / 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t upto = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t w = __shfl_up(upto, o);
+        if (lane >= (uint32_t)o) upto += w;
+    }
+    __syncthreads();  // part of an earlier call is read
+    if (lane == 63) part[wave] = upto;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPageThreads / 64; ++w) {
+        if ((uint32_t)w < wave) before += part[w];
+        all += part[w];
+    }
+    total = all;
+    return before + upto - v;
+}
+
+__global__ void vx_pages_reset_kernel(VxPages p) {
+    const size_t n = (size_t)p.n_seqs * p.max_pages, step = (size_t)gridDim.x * blockDim.x;
+    const size_t i0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    for (size_t i = i0; i < n; i += step) p.table[i / p.max_pages * p.table_stride + i % p.max_pages] = kVxNoPage;
+    for (size_t i = i0; i < p.n_pages; i += step) p.refs[i] = 0;
+    for (size_t i = i0; i < p.n_seqs; i += step) p.lens[i] = 0;
+    for (size_t i = i0; i < kVxPagesHead; i += step) p.scratch[i] = 0;
+}
+
+// One workgroup: who needs what (a thread per sequence), the lowest free pages (a scan of refs that ends when
+// it has enough), then a thread per page given out.
+__global__ __launch_bounds__(kPageThreads) void vx_pages_extend_kernel(VxPages p, const uint32_t* __restrict__ add) {
+    __shared__ uint32_t s_upto[kVxMaxPagedSeqs];  // pages given to sequences up to this one, itself included
+    __shared__ uint32_t s_old[kVxMaxPagedSeqs];   // pages it had; bit 31: its last one is copied
+    __shared__ uint32_t s_spot[kVxMaxPagedSeqs];  // the shared last page it would write
+    __shared__ uint32_t s_moves, s_granted, s_refused;
+    const uint32_t tid = threadIdx.x, n = p.n_seqs, per = (n + kPageThreads - 1) / kPageThreads;
+    const uint32_t a0 = min(tid * per, n), a1 = min(a0 + per, n);
+    uint32_t* src = p.scratch + kVxPagesHead;
+    uint32_t* dst = src + vx_pages_moves(p.n_seqs, p.n_pages);
+    uint32_t* list = dst + vx_pages_moves(p.n_seqs, p.n_pages);
+    if (tid == 0) s_moves = s_granted = s_refused = 0;
+    const auto pages_of = [&](uint64_t len) { return (len + p.page_size - 1) / p.page_size; };
+    const auto fits_in = [&](uint64_t len, uint64_t grow) {
+        return grow && pages_of(len + grow) <= p.max_pages && len + grow < 0x80000000ull;
+    };
+    int any = 0;
+    for (uint32_t s = a0; s < a1; ++s) {
+        const uint64_t len = p.lens[s], grow = add[s], old = pages_of(len);
+        const bool fits = fits_in(len, grow);
+        uint32_t spot = kVxNoPage;
+        if (fits && len % p.page_size) {
+            const uint32_t last = p.table[(size_t)s * p.table_stride + old - 1];
+            if (last < p.n_pages && p.refs[last] > 1) spot = last;
+        }
+        s_spot[s] = spot;
+        s_old[s] = (uint32_t)(fits ? old : 0);
+        any |= spot != kVxNoPage;
+    }
+    any = __syncthreads_or(any);
+    uint32_t mine = 0;
+    for (uint32_t s = a0; s < a1; ++s) {
+        const uint64_t len = p.lens[s], grow = add[s];
+        const bool fits = fits_in(len, grow);
+        uint32_t need = fits ? (uint32_t)(pages_of(len + grow) - pages_of(len)) : 0;
+        const uint32_t spot = any ? s_spot[s] : kVxNoPage;
+        if (spot != kVxNoPage) {
+            uint32_t same = 0;
+            bool later = false;
+            for (uint32_t j = 0; j < n; ++j) {
+                const bool eq = s_spot[j] == spot;
+                same += eq;
+                later |= eq && j > s;
+            }
+            if (later || same != p.refs[spot]) {  // else it is the last of all its holders and keeps the page
+                s_old[s] |= 0x80000000u;
+                ++need;
+            }
+        }
+        mine += need;
+        s_upto[s] = mine;  // within this thread's sequences, for now
+    }
+    uint32_t total;
+    const uint32_t before = vx_scan(mine, total);
+    for (uint32_t s = a0; s < a1; ++s) s_upto[s] += before;
+    // the lowest free pages
+    uint32_t found = 0;
+    for (uint32_t base = 0; base < p.n_pages && found < total; base += kPageThreads * 8) {
+        uint32_t free = 0;
+        const uint32_t first = base + tid * 8;
+        for (uint32_t k = 0; k < 8 && first + k < p.n_pages; ++k) free |= (p.refs[first + k] == 0) << k;
+        uint32_t got;
+        uint32_t rank = found + vx_scan(__popc(free), got);
+        for (; free; free &= free - 1, ++rank)
+            if (rank < total) list[rank] = first + __builtin_ctz(free);
+        found += got;
+    }
+    __syncthreads();
+    // sequences in order until the pages run out; the refused are then the last that extend
+    for (uint32_t s = a0; s < a1; ++s) {
+        const uint64_t len = p.lens[s], grow = add[s];
+        if (!grow) continue;
+        const bool fits = pages_of(len + grow) <= p.max_pages;
+        if (!fits || s_upto[s] > found) {
+            atomicAdd(&s_refused, 1u);
+            continue;
+        }
+        atomicMax(&s_granted, s_upto[s]);
+        p.lens[s] = (uint32_t)(len + grow);
+        if (s_old[s] >> 31) {
+            const uint32_t old = s_old[s] & 0x7FFFFFFFu, from = s_spot[s];
+            const uint32_t to = list[s ? s_upto[s - 1] : 0u];
+            const uint32_t m = atomicAdd(&s_moves, 1u);
+            src[m] = from;
+            dst[m] = to;
+            p.table[(size_t)s * p.table_stride + old - 1] = to;
+            p.refs[to] = 1;
+            atomicSub(&p.refs[from], 1u);
+        }
+    }
+    __syncthreads();
+    for (uint32_t r = tid; r < s_granted; r += kPageThreads) {
+        uint32_t lo = 0, hi = n - 1;  // the first sequence with s_upto > r
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (s_upto[mid] > r) hi = mid;
+            else lo = mid + 1;
+        }
+        const uint32_t copied = s_old[lo] >> 31, k = r - (lo ? s_upto[lo - 1] : 0u);
+        if (k < copied) continue;  // written above
+        p.table[(size_t)lo * p.table_stride + (s_old[lo] & 0x7FFFFFFFu) + k - copied] = list[r];
+        p.refs[list[r]] = 1;
+    }
+    if (tid == 0) {
+        p.scratch[0] = s_refused;
+        p.scratch[2] = s_moves;
+    }
+}
+
+// Copies the moves' pages of every layer. Work items of 16 KiB, dealt over the grid.
+constexpr uint32_t kMoveItem = 16384;
+__device__ __forceinline__ void vx_copy_moves(const VxPages& p, uint32_t wg, uint32_t n_wgs) {
+    const uint32_t moves = p.scratch[2];
+    const uint32_t* src = p.scratch + kVxPagesHead;
+    const uint32_t* dst = src + vx_pages_moves(p.n_seqs, p.n_pages);
+    const uint32_t parts = (uint32_t)((p.page_bytes + kMoveItem - 1) / kMoveItem);
+    const uint64_t items = (uint64_t)moves * p.n_layers * parts;
+    for (uint64_t i = wg; i < items; i += n_wgs) {
+        const uint32_t part = (uint32_t)(i % parts), layer = (uint32_t)(i / parts % p.n_layers), m = (uint32_t)(i / parts / p.n_layers);
+        uint8_t* base = p.pool + (size_t)layer * p.layer_stride + (size_t)part * kMoveItem;
+        const uint32_t bytes = (uint32_t)min((uint64_t)kMoveItem, p.page_bytes - (uint64_t)part * kMoveItem);
+        const uint4* f = (const uint4*)(base + (size_t)src[m] * p.page_bytes);
+        uint4* t = (uint4*)(base + (size_t)dst[m] * p.page_bytes);
+        for (uint32_t k = threadIdx.x; k < bytes / 16; k += blockDim.x) t[k] = f[k];
+    }
+}
+__global__ __launch_bounds__(256) void vx_pages_copy_kernel(VxPages p) { vx_copy_moves(p, blockIdx.x, gridDim.x); }
+
+// A workgroup takes a few columns of the table: all its entries are read into LDS before one is written, so
+// that every sequence takes its parent's old pages whatever the order. References change by the difference;
+// the sums do not depend on the order of the atomics. Workgroup 0 does the lengths.
+constexpr uint32_t kForkWords = 16384;
+__global__ __launch_bounds__(256) void vx_pages_fork_kernel(VxPages p, const uint32_t* __restrict__ from, uint32_t cols) {
+    __shared__ uint32_t old[kForkWords];
+    const uint32_t n = p.n_seqs, c0 = blockIdx.x * cols, nc = min(cols, p.max_pages - c0);
+    for (uint32_t i = threadIdx.x; i < n * nc; i += 256) old[i] = p.table[(size_t)(i / nc) * p.table_stride + c0 + i % nc];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n * nc; i += 256) {
+        const uint32_t s = i / nc, c = i % nc, f = from[s];
+        const uint32_t was = old[i], now = f < n ? old[f * nc + c] : kVxNoPage;
+        if (was == now) continue;
+        p.table[(size_t)s * p.table_stride + c0 + c] = now;
+        if (now < p.n_pages) atomicAdd(&p.refs[now], 1u);
+        if (was < p.n_pages) atomicSub(&p.refs[was], 1u);
+    }
+    if (blockIdx.x == 0) {
+        __syncthreads();
+        for (uint32_t s = threadIdx.x; s < n; s += 256) old[s] = p.lens[s];
+        __syncthreads();
+        for (uint32_t s = threadIdx.x; s < n; s += 256) {
+            const uint32_t f = from[s], len = f < n ? old[f] : 0u;
+            if (len != old[s]) p.lens[s] = len;
+        }
+    }
+}
+
+// An entry leaves the table by an exchange, so that a sequence listed twice gives its pages back once.
+__device__ __forceinline__ void vx_drop(const VxPages& p, uint32_t s, uint32_t j) {
+    const uint32_t was = atomicExch(&p.table[(size_t)s * p.table_stride + j], kVxNoPage);
+    if (was < p.n_pages) atomicSub(&p.refs[was], 1u);
+}
+__global__ void vx_pages_free_kernel(VxPages p, const uint32_t* __restrict__ seqs, uint32_t n) {
+    for (uint32_t i = blockIdx.y; i < n; i += gridDim.y) {
+        const uint32_t s = seqs[i];
+        if (s >= p.n_seqs) continue;
+        for (uint32_t j = blockIdx.x * blockDim.x + threadIdx.x; j < p.max_pages; j += gridDim.x * blockDim.x) vx_drop(p, s, j);
+        if (blockIdx.x == 0 && threadIdx.x == 0) p.lens[s] = 0;
+    }
+}
+__global__ void vx_pages_trim_kernel(VxPages p, uint32_t window, uint32_t sinks) {
+    for (uint32_t s = blockIdx.y; s < p.n_seqs; s += gridDim.y) {
+        const uint64_t len = p.lens[s];
+        if (len + 1 <= window) continue;
+        const uint64_t j0 = ((uint64_t)sinks + p.page_size - 1) / p.page_size;
+        const uint64_t j1 = min((len + 1 - window) / p.page_size, (uint64_t)p.max_pages);
+        for (uint64_t j = j0 + blockIdx.x * blockDim.x + threadIdx.x; j < j1; j += gridDim.x * blockDim.x) vx_drop(p, s, (uint32_t)j);
+    }
+}
+
+__global__ __launch_bounds__(kPageThreads) void vx_pages_count_kernel(VxPages p) {
+    uint32_t free = 0, total;
+    for (uint32_t i = threadIdx.x; i < p.n_pages; i += kPageThreads) free += p.refs[i] == 0;
+    vx_scan(free, total);
+    if (threadIdx.x == 0) p.scratch[1] = total;
+}
+
+// One workgroup plans the moves: with L live pages, the k-th free place below L takes the k-th live page from
+// L on (there are as many of the one as of the other), and the map of pages from L on says where each went.
+__global__ __launch_bounds__(kPageThreads) void vx_pages_plan_kernel(VxPages p) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t* src = p.scratch + kVxPagesHead;
+    uint32_t* dst = src + vx_pages_moves(p.n_seqs, p.n_pages);
+    uint32_t* map = dst + vx_pages_moves(p.n_seqs, p.n_pages);
+    uint32_t live = 0, total;
+    for (uint32_t i = tid; i < p.n_pages; i += kPageThreads) live += p.refs[i] != 0;
+    vx_scan(live, total);
+    uint32_t holes = 0, moved = 0;
+    for (uint32_t base = 0; base < p.n_pages; base += kPageThreads * 8) {
+        uint32_t hole = 0, move = 0;
+        const uint32_t first = base + tid * 8;
+        for (uint32_t k = 0; k < 8 && first + k < p.n_pages; ++k) {
+            const bool is = p.refs[first + k] != 0;
+            if (first + k < total) hole |= (uint32_t)!is << k;
+            else if (is) move |= 1u << k;
+            else map[first + k] = kVxNoPage;
+        }
+        // at most 8192 of either in a tile: both counts in one scan
+        uint32_t got;
+        const uint32_t at = vx_scan(__popc(hole) | __popc(move) << 16, got);
+        uint32_t h = holes + (at & 0xFFFFu), m = moved + (at >> 16);
+        for (; hole; hole &= hole - 1) dst[h++] = first + __builtin_ctz(hole);
+        for (; move; move &= move - 1) src[m++] = first + __builtin_ctz(move);
+        holes += got & 0xFFFFu;
+        moved += got >> 16;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < moved; i += kPageThreads) {
+        const uint32_t a = src[i], b = dst[i];
+        map[a] = b;
+        p.refs[b] = p.refs[a];
+        p.refs[a] = 0;
+    }
+    if (tid == 0) {
+        p.scratch[2] = moved;
+        p.scratch[3] = total;
+    }
+}
+// The table follows the map, beside the copies of the data.
+__global__ __launch_bounds__(256) void vx_pages_move_kernel(VxPages p, uint32_t table_wgs) {
+    if (blockIdx.x >= table_wgs) {
+        vx_copy_moves(p, blockIdx.x - table_wgs, gridDim.x - table_wgs);
+        return;
+    }
+    const uint32_t live = p.scratch[3];
+    const uint32_t* map = p.scratch + kVxPagesHead + 2 * (size_t)vx_pages_moves(p.n_seqs, p.n_pages);
+    const size_t n = (size_t)p.n_seqs * p.max_pages;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)table_wgs * 256) {
+        uint32_t* e = &p.table[i / p.max_pages * p.table_stride + i % p.max_pages];
+        const uint32_t was = *e;
+        if (was >= live && was < p.n_pages) *e = map[was];
+    }
+}
+
+uint32_t grid_of(uint64_t items, uint32_t most) { return (uint32_t)(items < 1 ? 1 : items > most ? most : items); }
+uint32_t copy_grid(const VxPages& p, uint64_t moves) {
+    return grid_of(moves * p.n_layers * ((p.page_bytes + kMoveItem - 1) / kMoveItem), 2048);
+}
+
+}  // namespace
+
+hipError_t vx_launch_rope_rows(const VxRopeTable& t, const VxRowsView& x, const VxRowsView& out, uint32_t n_rows,
+                               uint32_t d, const uint32_t* positions, hipStream_t st) {
+    vx_rope_rows_kernel<<<n_rows, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions);
+    return hipGetLastError();
+}
+
+hipError_t vx_launch_rope_append(const VxRopeTable& t, const VxAppendArgs& a, hipStream_t st) {
+    // a sequence's rows touch at most rows / 32 + 2 blocks
+    const uint64_t blocks = (uint64_t)a.n_rows / 32 + 2ull * a.c.n_seqs;
+    const uint32_t grid = (uint32_t)(blocks < a.n_rows ? blocks : a.n_rows);
+    vx_rope_append_kernel<<<dim3(grid, 8), 256, 0, st>>>(t, a);
+    return hipGetLastError();
+}
+
+hipError_t vx_launch_pages_reset(const VxPages& p, hipStream_t st) {
+    const uint64_t n = (uint64_t)p.n_seqs * p.max_pages;
+    vx_pages_reset_kernel<<<grid_of(((n > p.n_pages ? n : p.n_pages) + 255) / 256, 1024), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+hipError_t vx_launch_pages_extend(const VxPages& p, const uint32_t* add, hipStream_t st) {
+    vx_pages_extend_kernel<<<1, kPageThreads, 0, st>>>(p, add);
+    vx_pages_copy_kernel<<<copy_grid(p, p.n_seqs), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+hipError_t vx_launch_pages_fork(const VxPages& p, const uint32_t* src, hipStream_t st) {
+    const uint32_t most = kForkWords / p.n_seqs, cols = most < p.max_pages ? most : p.max_pages;
+    vx_pages_fork_kernel<<<(p.max_pages + cols - 1) / cols, 256, 0, st>>>(p, src, cols);
+    return hipGetLastError();
+}
+
+hipError_t vx_launch_pages_free(const VxPages& p, const uint32_t* seqs, uint32_t n, hipStream_t st) {
+    vx_pages_free_kernel<<<dim3(grid_of((p.max_pages + 255) / 256, 64), grid_of(n, 4096)), 256, 0, st>>>(p, seqs, n);
+    return hipGetLastError();
+}
+
+hipError_t vx_launch_pages_trim(const VxPages& p, uint32_t window, uint32_t sinks, hipStream_t st) {
+    vx_pages_trim_kernel<<<dim3(grid_of((p.max_pages + 255) / 256, 64), grid_of(p.n_seqs, 4096)), 256, 0, st>>>(p, window, sinks);
+    return hipGetLastError();
+}
+
+hipError_t vx_launch_pages_compact(const VxPages& p, hipStream_t st) {
+    vx_pages_plan_kernel<<<1, kPageThreads, 0, st>>>(p);
+    const uint32_t table_wgs = grid_of(((uint64_t)p.n_seqs * p.max_pages + 1023) / 1024, 256);
+    vx_pages_move_kernel<<<table_wgs + copy_grid(p, p.n_pages / 2), 256, 0, st>>>(p, table_wgs);
+    return hipGetLastError();
+}
+
+hipError_t vx_launch_pages_count(const VxPages& p, hipStream_t st) {
+    vx_pages_count_kernel<<<1, kPageThreads, 0, st>>>(p);
+    return hipGetLastError();
+}
