@@ -46,6 +46,7 @@ struct VxPagedAttnArgs {
     uint32_t window, sinks;
     float scale;
     uint32_t splits;
+    uint64_t span;   // token form: positions of a row at most, as planned
     float* part_o;   // [row][head][split][d]
     float* part_ml;  // [row][head][split][2]: maximum (log2 domain), sum
 };
