@@ -461,10 +461,10 @@ __device__ __forceinline__ uint32_t vx_v_swizzle(uint32_t e) { return (e >> 1 & 
 template <class E, int D, int QT, int PT>
 __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPagedAttnArgs a, uint32_t tiles) {
     constexpr int NK = D / 16, NM = D / 32, RB = D / 8;
-    constexpr uint32_t kChunk = 32u * D * 2u, kBuf = 4u * kChunk;  // K or V of a chunk; K, K, V, V of a step
+    constexpr uint32_t kChunk = 32u * D * 2u, kBuf = 4u * kChunk;  // K or V of a chunk; of a step
     constexpr uint32_t kUnits = kChunk / 1024u;                    // 1 KiB units of a chunk's K or V
     typedef typename E::v8 v8;
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kBuf];
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kBuf];  // K of two steps, V of two steps
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t col = lane & 31u, grp = lane >> 5;
     const uint32_t G = a.q.heads / a.c.hkv, kvh = blockIdx.x % a.c.hkv;
@@ -477,15 +477,15 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     const uint32_t c0 = min(blockIdx.y * per, ch.n), c1 = min(c0 + per, ch.n);
     const uint32_t* table = a.c.table + (size_t)rt.seq * a.c.table_stride;
 
-    // this lane's pair
+    // this lane's pair; -1: a position of a pair that is not there
     const uint32_t pr = r0 + 32 * wave + col, row = rt.lo + pr / G, head = kvh * G + pr % G;
     const bool mine = pr < r1;
-    const int64_t t = mine ? rt.pos0 + pr / G : -1, low = vx_low(t, a.window);
-    // the wave's positions: all of its pairs see [all_low, all_t], none sees past any_t or, but for sinks, before any_low
-    const uint32_t w0 = min(r0 + 32 * wave, r1 - 1), w1 = min(r0 + 32 * wave + 31, r1 - 1);
-    const bool some = r0 + 32 * wave < r1;
-    const int64_t any_t = some ? rt.pos0 + w1 / G : -1, all_t = rt.pos0 + w0 / G, all_low = vx_low(any_t, a.window);
-    const int64_t any_low = vx_low(all_t, a.window);
+    const auto position = [&](uint32_t pair) { return (int)max((int64_t)-1, rt.pos0 + pair / G); };
+    const int t = mine ? position(pr) : -1, low = (int)vx_low(t, a.window);
+    const int sinks = (int)min(a.sinks, 0x7FFFFFFFu);
+    // all pairs of the wave see [all_low, all_t]; none of the workgroup sees past last_t or, but for sinks, before ch.low
+    const int all_t = position(min(r0 + 32 * wave, r1 - 1)), all_low = (int)vx_low(position(min(r0 + 32 * wave + 31, r1 - 1)), a.window);
+    const int last_t = position(r1 - 1);
 
     v8 qf[QT][NK];
     float to_log2 = fabsf(a.scale) * kLog2e;
@@ -542,25 +542,23 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     const auto page_of = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(i & 63u)); };
     const auto place_of = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)places, (int)(i & 63u)); };
 
-    // staging: unit u of a step is a KiB of K (u < 2 kUnits) or V of its first or second chunk
+    // staging: the waves share the KiBs of a step's K (or V), two chunks' worth
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
-    const auto stage = [&](uint32_t i, uint32_t buf) {  // i: the step's first chunk, counted from the last look_up
+    const uint32_t my_chunk = wave >> 1, my_unit = (wave & 1u) * (kUnits / 2);
+    uint32_t k_off[kUnits / 2], v_off[kUnits / 2];
 #pragma unroll
-        for (uint32_t k = 0; k < kUnits; ++k) {  // 4 kUnits over 4 waves
-            const uint32_t u = wave * kUnits + k;  // wave w: 0, 1 the chunks' K, 2, 3 their V
-            const uint32_t c = wave & 1u, page = page_of(i + c), place = place_of(i + c);
-            const uint8_t* base = a.c.pool + (size_t)(page < a.c.n_pages ? page : 0u) * a.c.page_bytes +
-                                  (size_t)((wave < 2 ? 0u : a.c.hkv) + kvh) * a.c.page_size * D * 2 + (size_t)place * D * 2;
-            uint32_t off;
-            if (wave < 2) {
-                const uint32_t s = 64u * k + lane, p = s / RB;
-                off = p * D * 2 + 16u * (s % RB ^ vx_k_swizzle<D>(p));
-            } else {
-                const uint32_t s = 64u * k + lane, e = s / 4;
-                off = e * 64 + 16u * (s % 4 ^ vx_v_swizzle(e));
-            }
-            vx_load_lds(base, off, lds0 + buf * kBuf + u * 1024u);
-        }
+    for (uint32_t j = 0; j < kUnits / 2; ++j) {
+        const uint32_t i = 64u * (my_unit + j) + lane, p = i / RB, e = i / 4;
+        k_off[j] = p * D * 2 + 16u * (i % RB ^ vx_k_swizzle<D>(p));
+        v_off[j] = e * 64 + 16u * (i % 4 ^ vx_v_swizzle(e));
+    }
+    // K of the step whose chunks are in lanes i and i + 1
+    const auto stage = [&](uint32_t i, const uint32_t (&off)[kUnits / 2], uint32_t head0, uint32_t to) {
+        const uint32_t page = page_of(i + my_chunk), place = place_of(i + my_chunk);
+        const uint8_t* base = a.c.pool + (size_t)(page < a.c.n_pages ? page : 0u) * a.c.page_bytes +
+                              ((size_t)(head0 + kvh) * a.c.page_size + place) * (D * 2);
+#pragma unroll
+        for (uint32_t j = 0; j < kUnits / 2; ++j) vx_load_lds(base, off[j], lds0 + to + my_chunk * kChunk + (my_unit + j) * 1024u);
     };
 
     vx_f16 o[NM];
@@ -569,65 +567,66 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;  // the pair's maximum (as far as the weights are taken against it), this lane's sum
-    const uint32_t kp = (col & 7u) | (col >> 3 & 1u) << 4 | (col >> 4) << 3;  // position of this lane's K row
+    // where this lane reads its K row (position kp of a chunk; the block of step c of the products at ^ 32 c) and V rows
+    const uint32_t kp = (col & 7u) | (col >> 3 & 1u) << 4 | (col >> 4) << 3;
+    const uint32_t k_at = kp * D * 2 + 16u * (grp ^ vx_k_swizzle<D>(kp));
+    const uint32_t v_at = col * 64 + 16u * (grp ^ vx_v_swizzle(col));
 
-    if (c0 < c1) {
-        look_up(c0);
-        stage(0, 0);
-    }
-    uint32_t seen_from = c0;  // the chunk that lane 0 looked up
-    for (uint32_t i = c0, buf = 0; i < c1; i += 2, buf ^= 1) {
-        const uint32_t at = i - seen_from;
-        const uint32_t page0 = page_of(at), page1 = page_of(at + 1);
-        vx_wait_loads<0>();
-        vx_barrier();  // step i is in LDS, and step i - 2 is read by everyone
-        if (i + 2 < c1) {
-            if (at + 2 == 64) {
-                look_up(i + 2);
-                seen_from = i + 2;
-            }
-            stage(i + 2 - seen_from, buf ^ 1);
+    typedef vx_f16 Scores[2];
+    const auto scores = [&](vx_f16& s, int b, uint32_t buf) {  // chunk b of a step
+        const unsigned char* kb = lds + buf * (2 * kChunk) + b * kChunk;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+            const v8 k = *(const v8*)(kb + (k_at ^ 32u * c));
+#pragma unroll
+            for (int u = QT - 1; u >= 0; --u) s = E::mfma(k, qf[u][c], s);
         }
-        const uint32_t base0 = vx_chunk_base(ch, i), base1 = vx_chunk_base(ch, i + 1);
-        const bool have0 = page0 < a.c.n_pages && (int64_t)base0 <= any_t;
-        const bool have1 = i + 1 < c1 && page1 < a.c.n_pages && (int64_t)base1 <= any_t;
-        if (!have0 && !have1) continue;
-        const unsigned char* kb = lds + buf * kBuf;
-        const unsigned char* vb = kb + 2 * kChunk;
-        vx_f16 s[2];
+    };
+    // place of position p in the chunk at base: -1 in front of it, 32 or more behind it
+    const auto place_in = [](int p, uint32_t base) { return max(-1, min(64, p - (int)base)); };
+    struct Step {  // two chunks of the walk; uniform
+        uint32_t base[2];
+        bool have[2], masked, hidden;  // some pair of the wave does not see all; some place is seen by no pair
+    };
+    const auto step_of = [&](uint32_t i, uint32_t at) {
+        Step x;
+        x.masked = x.hidden = false;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NK; ++c) {
-                const v8 k = *(const v8*)(kb + b * kChunk + kp * D * 2 + 16u * ((2 * c + grp) ^ vx_k_swizzle<D>(kp)));
-#pragma unroll
-                for (int u = QT - 1; u >= 0; --u) s[b] = E::mfma(k, qf[u][c], s[b]);
-            }
+            const uint32_t base = vx_chunk_base(ch, i + b);
+            x.base[b] = base;
+            x.have[b] = i + b < c1 && page_of(at + b) < a.c.n_pages;
+            x.masked |= !x.have[b] || (int)base + 31 > all_t || (int)base < all_low;
+            x.hidden |= !x.have[b] || (int)base + 31 > last_t || (int64_t)base < ch.low;
         }
-        // hidden positions
-        bool masked[2];
+        x.masked = __builtin_amdgcn_readfirstlane(x.masked);
+        x.hidden = __builtin_amdgcn_readfirstlane(x.hidden);
+        return x;
+    };
+    // Hides what the mask hides, and moves the maximum where a score passes it by more than 8 (the weights may pass 1
+    // by 2^8 until then: a bf16 or fp16 weight keeps its relative precision, and the rescaling is rare).
+    const auto bound = [&](Scores& s, const Step& x) {
+        if (x.masked) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const uint32_t base = b ? base1 : base0;
-            const bool have = b ? have1 : have0;
-            masked[b] = !have || (int64_t)base + 31 > all_t || (int64_t)base < all_low;
-            if (masked[b]) {
+            for (int b = 0; b < 2; ++b) {
+                const int pt = (x.have[b] ? place_in(t, x.base[b]) : -1) - 4 * (int)grp, pl = place_in(low, x.base[b]) - 4 * (int)grp,
+                          ps = place_in(sinks, x.base[b]) - 4 * (int)grp;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int64_t p = (int64_t)base + 16 * (r >> 2 & 1) + 8 * (r >> 3) + 4 * grp + (r & 3);
-                    if (!have || p > t || (p < low && p >= (int64_t)a.sinks)) s[b][r] = -INFINITY;
+                    const int p = 16 * (r >> 2 & 1) + 8 * (r >> 3) + (r & 3);
+                    const bool hidden = (p > pt) | ((p < pl) & (p >= ps));
+                    s[b][r] = hidden ? -INFINITY : s[b][r];
                 }
             }
         }
-        float top = -INFINITY;
+        float top = s[0][0];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
         top = vx_max_pair(top) * to_log2;
-        // the weights may pass 1 by 2^8 before the maximum they are taken against moves
         if (__ballot(top > m + 8.0f || (m == -INFINITY && top != -INFINITY))) {
             const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
@@ -635,49 +634,122 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
 #pragma unroll
             for (int n = 0; n < NM; ++n) o[n] *= f;
         }
+    };
+    // Places of V that no pair sees may hold anything (0 times NaN is NaN): the workgroup zeroes them in LDS.
+    const auto clear = [&](const Step& x, uint32_t buf) {
+        for (uint32_t i = threadIdx.x; i < 2 * D * 4; i += kPromptThreads) {
+            const uint32_t b = i / (D * 4), e = i / 4 % D, j = i % 4 ^ vx_v_swizzle(e);  // j: slots 8 j .. 8 j + 7 of row e
+            const uint32_t base = b ? x.base[1] : x.base[0];
+            const int pt = (b ? x.have[1] : x.have[0]) ? place_in(last_t, base) : -1, pl = place_in((int)ch.low, base), ps = place_in(sinks, base);
+            vx_u4* at = (vx_u4*)(lds + 4 * kChunk + buf * (2 * kChunk) + 16 * i);
+            vx_u4 v = *at;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int p = 16 * (k >> 2) + 4 * (int)j + (k & 3);
+                if ((p > pt) | ((p < pl) & (p >= ps))) v[k / 2] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
+            }
+            *at = v;
+        }
+        vx_barrier();
+    };
+    // o += V^T P^T of a chunk
+    const auto add = [&](const vx_f16& s, int b, uint32_t buf) {
+        const unsigned char* vb = lds + 4 * kChunk + buf * (2 * kChunk) + b * kChunk;
         const float ref = m == -INFINITY ? 0.0f : m;
+        v8 pf[PT][2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            v8 pf[PT][2];
+        for (int r = 0; r < 16; ++r) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], to_log2, -ref));
+            l += p;
+            float rest = p;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], to_log2, -ref));
-                l += p;
-                float rest = p;
-#pragma unroll
-                for (int u = 0; u < PT; ++u) {
-                    const typename E::elt v = (typename E::elt)rest;
-                    pf[u][r >> 3][r & 7] = v;
-                    rest -= (float)v;
-                }
+            for (int u = 0; u < PT; ++u) {
+                const typename E::elt v = (typename E::elt)rest;
+                pf[u][r >> 3][r & 7] = v;
+                rest -= (float)v;
             }
-            // places of hidden positions may hold anything: those that no pair of the wave sees are zeroed
-            vx_u4 keep[2];
-            if (masked[b]) {
+        }
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t k = 0;
+            for (int n = 0; n < NM; ++n) {
+                const v8 v = *(const v8*)(vb + 2048 * n + (v_at ^ 32u * h));
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int64_t p = (int64_t)(b ? base1 : base0) + 16 * (w >> 1) + 8 * h + 4 * grp + 2 * (w & 1) + e;
-                            if ((b ? have1 : have0) && p <= any_t && (p >= any_low || p < (int64_t)a.sinks)) k |= 0xFFFFu << 16 * e;
-                        }
-                        keep[h][w] = k;
+                for (int u = PT - 1; u >= 0; --u) o[n] = E::mfma(v, pf[u][h], o[n]);
+            }
+    };
+
+    // The walk, a step of two chunks at a time: while step i's weights are formed and added, the scores of step
+    // i + 1 are multiplied (PIPE). LDS: K of steps i + 1 and i + 2, V of steps i and i + 1, each in two buffers.
+    // With q in several terms the registers hold one step's scores only.
+    constexpr bool PIPE = QT == 1;
+    const uint32_t n_steps = (c1 - c0 + 1) / 2;
+    uint32_t first = 0;  // the step whose chunks are in lanes 0 and 1
+    const auto at = [&](uint32_t i) {  // the lane of step i's first chunk; i never falls behind the last look_up
+        if (i - first >= 32) {
+            look_up(c0 + 2 * i);
+            first = i;
+        }
+        return 2 * (i - first);
+    };
+    if (n_steps) {
+        look_up(c0);
+        stage(0, k_off, 0, 0);
+        Step now = step_of(c0, 0), next = now;
+        Scores s;
+        if constexpr (PIPE) {
+            vx_wait_loads<0>();
+            vx_barrier();
+            stage(0, v_off, a.c.hkv, 4 * kChunk);
+            if (n_steps > 1) {
+                next = step_of(c0 + 2, 2);
+                stage(2, k_off, 0, 2 * kChunk);
+            }
+            scores(s[0], 0, 0);
+            scores(s[1], 1, 0);
+            bound(s, now);
+        } else {
+            stage(0, v_off, a.c.hkv, 4 * kChunk);
+        }
+        for (uint32_t i = 0; i < n_steps; ++i) {
+            const uint32_t buf = i & 1u;
+            const bool more = i + 1 < n_steps;
+            vx_wait_loads<0>();
+            vx_barrier();  // step i is in LDS, and the buffers of what follows are read by everyone
+            Step after = next;
+            if (more) {
+                uint32_t j = at(i + 1);
+                stage(j, v_off, a.c.hkv, 4 * kChunk + (buf ^ 1) * (2 * kChunk));
+                if constexpr (PIPE) {
+                    if (i + 2 < n_steps) {
+                        j = at(i + 2);
+                        after = step_of(c0 + 2 * (i + 2), j);
+                        stage(j, k_off, 0, buf * (2 * kChunk));
                     }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int n = 0; n < NM; ++n) {
-                    const uint32_t e = 32 * n + col;
-                    vx_u4 w = *(const vx_u4*)(vb + b * kChunk + e * 64 + 16u * ((2 * h + grp) ^ vx_v_swizzle(e)));
-                    if (masked[b]) w &= keep[h];
-                    const v8 v = __builtin_bit_cast(v8, w);
-#pragma unroll
-                    for (int u = PT - 1; u >= 0; --u) o[n] = E::mfma(v, pf[u][h], o[n]);
+                } else {
+                    next = step_of(c0 + 2 * (i + 1), j);
+                    stage(j, k_off, 0, (buf ^ 1) * (2 * kChunk));
                 }
+            }
+            if (now.hidden) clear(now, buf);
+            if constexpr (PIPE) {
+                Scores u;  // behind the last step this multiplies what an earlier one left in LDS, to no use
+                scores(u[0], 0, buf ^ 1);
+                add(s[0], 0, buf);
+                scores(u[1], 1, buf ^ 1);
+                add(s[1], 1, buf);
+                if (more) bound(u, next);
+                s[0] = u[0];
+                s[1] = u[1];
+            } else {
+                scores(s[0], 0, buf);
+                scores(s[1], 1, buf);
+                bound(s, now);
+                add(s[0], 0, buf);
+                add(s[1], 1, buf);
+            }
+            now = next;
+            next = after;
         }
     }
 
