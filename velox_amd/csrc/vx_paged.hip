@@ -27,9 +27,104 @@ __device__ __forceinline__ float2 vx_turn(const VxRopeTable& t, uint32_t j, uint
     return make_float2(c * t.amp, s * t.amp);
 }
 
-// ---- rotation of rows: one workgroup per kRows rows, the rows' cos/sin shared by all heads through LDS ----
+// A pair turned by cs = (cos, sin); the same roundings wherever it is done (the empty statement keeps the values in
+// fp32: a product, a sum and the conversion to fp16 would become one instruction in some places and not in others).
+__device__ __forceinline__ float2 vx_rotate(float a, float b, float2 cs) {
+    float x = __builtin_fmaf(a, cs.x, -(b * cs.y)), y = __builtin_fmaf(b, cs.x, a * cs.y);
+    asm("" : "+v"(x), "+v"(y));
+    return make_float2(x, y);
+}
+
+// A unit of a head's values with 16-byte loads and stores: V pairs (half layout: V values of each half), or V values
+// (interleaved pairs, or values behind rot_dim, which pass).
+template <class T>
+struct alignas(16) VxVec {
+    static constexpr int V = 16 / sizeof(T);
+    T v[V];
+};
+template <class T>
+__device__ __forceinline__ uint32_t vx_units(const VxRopeTable& t, uint32_t d) {
+    constexpr uint32_t V = VxVec<T>::V;
+    return (t.interleaved ? t.rot : t.rot / 2) / V + (d - t.rot) / V;
+}
+// Unit u of the head at x turned by the row's cos / sin table cs, V values at a time given to put(first element,
+// values).
+template <class T, class Put>
+__device__ __forceinline__ void vx_turn_unit(const VxRopeTable& t, const T* x, uint32_t u, const float2* cs, Put put) {
+    constexpr uint32_t V = VxVec<T>::V;
+    const uint32_t half = t.rot / 2, pair_units = (t.interleaved ? t.rot : half) / V;
+    float y[V];
+    if (u >= pair_units) {
+        const uint32_t e = t.rot + (u - pair_units) * V;
+        const VxVec<T> a = *(const VxVec<T>*)(x + e);
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) y[i] = (float)a.v[i];
+        put(e, y);
+    } else if (t.interleaved) {
+        const VxVec<T> a = *(const VxVec<T>*)(x + u * V);
+#pragma unroll
+        for (uint32_t i = 0; i < V; i += 2) {
+            const float2 r = vx_rotate((float)a.v[i], (float)a.v[i + 1], cs[u * (V / 2) + i / 2]);
+            y[i] = r.x;
+            y[i + 1] = r.y;
+        }
+        put(u * V, y);
+    } else {
+        const VxVec<T> a = *(const VxVec<T>*)(x + u * V), b = *(const VxVec<T>*)(x + half + u * V);
+        float z[V];
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) {
+            const float2 r = vx_rotate((float)a.v[i], (float)b.v[i], cs[u * V + i]);
+            y[i] = r.x;
+            z[i] = r.y;
+        }
+        put(u * V, y);
+        put(half + u * V, z);
+    }
+}
+template <class O, int V>
+__device__ __forceinline__ void vx_put(O* to, const float* y) {
+    struct alignas(V * sizeof(O)) Out {
+        O v[V];
+    } o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.v[i] = (O)y[i];
+    *(Out*)to = o;
+}
+
+// ---- rotation of rows: a workgroup takes kRows rows, whose cos / sin all heads share through LDS ----
+// Bound by its bytes: 4001 rows of 64 heads of 128 (fp16, 131 MB moved) take @@ us (@@ TB/s).
 constexpr int kRopeThreads = 256;
 
+template <class T>
+__global__ __launch_bounds__(kRopeThreads) void vx_rope_vec_kernel(VxRopeTable t, VxRowsView x, VxRowsView o, uint32_t n_rows,
+                                                                   uint32_t d, const uint32_t* __restrict__ positions, uint32_t per) {
+    constexpr int V = VxVec<T>::V;
+    __shared__ float2 cs[kRopeThreads > 2 * kVxMaxRopePairs ? kRopeThreads : 2 * kVxMaxRopePairs];
+    const uint32_t half = t.rot / 2, row0 = blockIdx.x * per, n = min(per, n_rows - row0);  // n * half <= 256
+    for (uint32_t i = threadIdx.x; i < n * half; i += kRopeThreads) cs[i] = vx_turn(t, i % half, positions[row0 + i / half]);
+    __syncthreads();
+    const uint32_t units = vx_units<T>(t, d), step = kRopeThreads / units;  // a thread keeps its unit
+    if (step) {
+        const uint32_t u = threadIdx.x % units;
+        if (threadIdx.x / units >= step) return;
+        for (uint32_t i = threadIdx.x / units; i < n * x.heads; i += step) {
+            const uint32_t w = i / x.heads, h = i % x.heads;
+            T* to = (T*)o.data + (size_t)(row0 + w) * o.rs + (size_t)h * o.hs;
+            vx_turn_unit<T>(t, (const T*)x.data + (size_t)(row0 + w) * x.rs + (size_t)h * x.hs, u, cs + w * half,
+                            [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
+        }
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < n * x.heads * units; i += kRopeThreads) {
+        const uint32_t w = i / units / x.heads, h = i / units % x.heads;
+        T* to = (T*)o.data + (size_t)(row0 + w) * o.rs + (size_t)h * o.hs;
+        vx_turn_unit<T>(t, (const T*)x.data + (size_t)(row0 + w) * x.rs + (size_t)h * x.hs, i % units, cs + w * half,
+                        [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
+    }
+}
+
+// The same value by value, for rows without 16-byte alignment and pairs that do not fill vectors.
 __global__ __launch_bounds__(kRopeThreads) void vx_rope_rows_kernel(VxRopeTable t, VxRowsView x, VxRowsView o, uint32_t n_rows,
                                                                     uint32_t d, const uint32_t* __restrict__ positions) {
     __shared__ float2 cs[kVxMaxRopePairs];
@@ -44,8 +139,9 @@ __global__ __launch_bounds__(kRopeThreads) void vx_rope_rows_kernel(VxRopeTable 
         if (u < half) {
             const uint32_t e0 = t.interleaved ? 2 * u : u, e1 = t.interleaved ? 2 * u + 1 : u + half;
             const float a = vx_load(x.data, xb + e0, x.dtype), b = vx_load(x.data, xb + e1, x.dtype);
-            vx_store(o.data, ob + e0, o.dtype, a * cs[u].x - b * cs[u].y);
-            vx_store(o.data, ob + e1, o.dtype, b * cs[u].x + a * cs[u].y);
+            const float2 r = vx_rotate(a, b, cs[u]);
+            vx_store(o.data, ob + e0, o.dtype, r.x);
+            vx_store(o.data, ob + e1, o.dtype, r.y);
         } else {
             const uint32_t e = t.rot + u - half;
             vx_store(o.data, ob + e, o.dtype, vx_load(x.data, xb + e, x.dtype));
@@ -72,6 +168,11 @@ __device__ __forceinline__ VxSpan vx_span(const uint32_t* q_start, const uint32_
 // in order; false behind the last. Every wave walks the sequences 64 at a time.
 __device__ __forceinline__ bool vx_find_block(const VxAppendArgs& a, uint32_t item, uint32_t& seq, uint32_t& blk) {
     const uint32_t lane = threadIdx.x & 63u;
+    if (!a.q_start) {
+        seq = item;
+        blk = 0;
+        return a.c.lens[item] > 0;
+    }
     uint32_t base = 0;
     for (uint32_t s0 = 0; s0 < a.c.n_seqs; s0 += 64) {
         const uint32_t s = s0 + lane;
@@ -99,55 +200,133 @@ __device__ __forceinline__ bool vx_find_block(const VxAppendArgs& a, uint32_t it
     return false;
 }
 
-// ---- append: a workgroup takes one 32-position block (a V block of the pages, up to 32 rows) of a sequence ----
-__global__ __launch_bounds__(256) void vx_rope_append_kernel(VxRopeTable t, VxAppendArgs a) {
-    __shared__ float2 cs[32][kVxMaxRopePairs / 2];
+// ---- append: workgroups (x) take a 32-position block (a V block of the pages, up to 32 rows) of a sequence each;
+// y deals its heads ----
+struct VxBlock {
+    uint32_t row0, n, i0;  // rows row0 .. row0 + n at places i0 .. of the block
+    uint32_t in_page;      // the block's place in its page
+    uint16_t *k, *v;       // the page's K and V; NULL: no page
+};
+__device__ __forceinline__ bool vx_block(const VxRopeTable& t, const VxAppendArgs& a, VxBlock& b, float2 (*cs)[kVxMaxRopePairs / 2]) {
     uint32_t seq, blk;
-    if (!vx_find_block(a, blockIdx.x, seq, blk)) return;
+    if (!vx_find_block(a, blockIdx.x, seq, blk)) return false;
     const VxSpan r = vx_span(a.q_start, a.c.lens, a.n_rows, seq);
     const int64_t from = r.pos0 > 0 ? r.pos0 : 0, end = r.pos0 + (r.hi - r.lo);
     const int64_t p0 = ((from >> 5) + blk) << 5;  // the block's first position
-    const uint32_t i0 = (uint32_t)((from > p0 ? from : p0) - p0), i1 = (uint32_t)((end < p0 + 32 ? end : p0 + 32) - p0);
-    const uint32_t row0 = r.lo + (uint32_t)(p0 + i0 - r.pos0), n = i1 - i0;  // rows row0 .. row0 + n at positions p0 + i0 ..
-    const uint32_t half = t.rot / 2, d = a.c.d, hkv = a.c.hkv;
-    for (uint32_t i = threadIdx.x; i < n * half; i += 256) cs[i / half][i % half] = vx_turn(t, i % half, (uint32_t)(p0 + i0 + i / half));
+    b.i0 = (uint32_t)((from > p0 ? from : p0) - p0);
+    b.n = (uint32_t)((end < p0 + 32 ? end : p0 + 32) - p0) - b.i0;
+    b.row0 = r.lo + (uint32_t)(p0 + b.i0 - r.pos0);
+    const uint32_t half = t.rot / 2;
     const uint64_t pi = (uint64_t)p0 / a.c.page_size;
     uint32_t page = kVxNoPage;
     if (pi < a.c.max_pages) page = a.c.table[(size_t)seq * a.c.table_stride + pi];
+    for (uint32_t i = threadIdx.x; i < b.n * half; i += 256) cs[i / half][i % half] = vx_turn(t, i % half, (uint32_t)(p0 + b.i0 + i / half));
     const bool have = page < a.c.n_pages;
-    uint16_t* kp = (uint16_t*)(a.c.pool + (size_t)(have ? page : 0u) * a.c.page_bytes);
-    uint16_t* vp = kp + (size_t)hkv * a.c.page_size * d;
-    const uint32_t in_page = (uint32_t)((uint64_t)p0 % a.c.page_size);
+    b.k = have ? (uint16_t*)(a.c.pool + (size_t)page * a.c.page_bytes) : nullptr;
+    b.v = have ? b.k + (size_t)a.c.hkv * a.c.page_size * a.c.d : nullptr;
+    b.in_page = (uint32_t)((uint64_t)p0 % a.c.page_size);
     __syncthreads();
-    const uint32_t hq = a.q.data ? a.q.heads : 0, heads = hq + 2 * hkv;
+    return true;
+}
+
+// T: the rows' type, C: the cache's. K and q by units of 16 bytes; V by 8 dimensions of the 8 positions that share
+// 16 bytes of a V block, transposed in registers, so that whole blocks leave as whole lines.
+template <class T, class C>
+__global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxAppendArgs a) {
+    constexpr int V = VxVec<T>::V;
+    __shared__ float2 cs[32][kVxMaxRopePairs / 2];
+    VxBlock b;
+    if (!vx_block(t, a, b, cs)) return;
+    const uint32_t d = a.c.d, hkv = a.c.hkv, hq = a.q.data ? a.q.heads : 0, heads = hq + hkv;
+    const uint32_t units = vx_units<T>(t, d), step = 256 / units;  // d <= 128: at most 32 units
+    const uint32_t u = threadIdx.x % units, mine = threadIdx.x / units;
+    if (mine < step)
+        for (uint32_t i = blockIdx.y * step + mine; i < b.n * heads; i += gridDim.y * step) {
+            const uint32_t w = i / heads, h = i % heads;
+            if (h < hq) {
+                T* to = (T*)a.qo.data + (size_t)(b.row0 + w) * a.qo.rs + (size_t)h * a.qo.hs;
+                vx_turn_unit<T>(t, (const T*)a.q.data + (size_t)(b.row0 + w) * a.q.rs + (size_t)h * a.q.hs, u, cs[w],
+                                [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
+            } else if (b.k) {
+                C* to = (C*)b.k + ((size_t)(h - hq) * a.c.page_size + b.in_page + b.i0 + w) * d;
+                vx_turn_unit<T>(t, (const T*)a.k.data + (size_t)(b.row0 + w) * a.k.rs + (size_t)(h - hq) * a.k.hs, u, cs[w],
+                                [&](uint32_t e, const float* y) { vx_put<C, V>(to + e, y); });
+            }
+        }
+    if (!b.v) return;
+    const uint32_t groups = d / 8;
+    // from the last workgroup of the block on: the first ones have rows left over
+    for (uint32_t i = (gridDim.y - 1 - blockIdx.y) * 256 + threadIdx.x; i < hkv * groups * 4; i += gridDim.y * 256) {
+        const uint32_t e0 = i % groups * 8, j = i / groups % 4, h = i / groups / 4;  // slots 8 j .. 8 j + 7 of 8 dimensions
+        C x[8][8];
+        uint32_t there = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t p = 16 * (k >> 2) + 4 * j + (k & 3);  // the position of slot 8 j + k
+            if (p - b.i0 < b.n) {
+                there |= 1u << k;
+                const T* from = (const T*)a.v.data + (size_t)(b.row0 + p - b.i0) * a.v.rs + (size_t)h * a.v.hs + e0;
+#pragma unroll
+                for (int q = 0; q < 8 / V; ++q) {
+                    const VxVec<T> y = ((const VxVec<T>*)from)[q];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[k][q * V + e] = (C)(float)y.v[e];
+                }
+            }
+        }
+        C* to = (C*)b.v + ((size_t)h * a.c.page_size + b.in_page) * d + e0 * 32 + 8 * j;
+        if (there == 255u) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                struct alignas(16) Out {
+                    C v[8];
+                } o;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) o.v[k] = x[k][e];
+                *(Out*)(to + e * 32) = o;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (there >> k & 1)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) to[e * 32 + k] = x[k][e];
+        }
+    }
+}
+
+// The same value by value, for rows of several types or without 16-byte alignment, and pairs that do not fill vectors.
+__global__ __launch_bounds__(256) void vx_append_rows_kernel(VxRopeTable t, VxAppendArgs a) {
+    __shared__ float2 cs[32][kVxMaxRopePairs / 2];
+    VxBlock b;
+    if (!vx_block(t, a, b, cs)) return;
+    const uint32_t half = t.rot / 2, d = a.c.d, hkv = a.c.hkv, hq = a.q.data ? a.q.heads : 0, heads = hq + 2 * hkv;
     const uint32_t units = half + (d - t.rot);
-    for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < n * heads * units; i += gridDim.y * 256) {
+    for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < b.n * heads * units; i += gridDim.y * 256) {
         const uint32_t u = i % units, h = i / units % heads, w = i / units / heads;
-        const uint32_t row = row0 + w;
         const bool pair = u < half;
         const uint32_t e0 = pair ? (t.interleaved ? 2 * u : u) : t.rot + u - half;
         const uint32_t e1 = pair ? (t.interleaved ? 2 * u + 1 : u + half) : e0;
         const VxRowsView& x = h < hq ? a.q : h < hq + hkv ? a.k : a.v;
         const uint32_t hh = h < hq ? h : h < hq + hkv ? h - hq : h - hq - hkv;
-        const size_t xb = (size_t)row * x.rs + (size_t)hh * x.hs;
+        const size_t xb = (size_t)(b.row0 + w) * x.rs + (size_t)hh * x.hs;
         float y0 = vx_load(x.data, xb + e0, x.dtype), y1 = pair ? vx_load(x.data, xb + e1, x.dtype) : 0.0f;
         if (pair && h < hq + hkv) {
-            const float2 c = cs[w][u];
-            const float a0 = y0, b0 = y1;
-            y0 = a0 * c.x - b0 * c.y;
-            y1 = b0 * c.x + a0 * c.y;
+            const float2 r = vx_rotate(y0, y1, cs[w][u]);
+            y0 = r.x;
+            y1 = r.y;
         }
         if (h < hq) {
-            const size_t ob = (size_t)row * a.qo.rs + (size_t)hh * a.qo.hs;
+            const size_t ob = (size_t)(b.row0 + w) * a.qo.rs + (size_t)hh * a.qo.hs;
             vx_store(a.qo.data, ob + e0, a.qo.dtype, y0);
             if (pair) vx_store(a.qo.data, ob + e1, a.qo.dtype, y1);
-        } else if (have && h < hq + hkv) {
-            uint16_t* to = kp + ((size_t)hh * a.c.page_size + in_page + i0 + w) * d;
+        } else if (b.k && h < hq + hkv) {
+            uint16_t* to = b.k + ((size_t)hh * a.c.page_size + b.in_page + b.i0 + w) * d;
             vx_store(to, e0, a.c.dtype, y0);
             if (pair) vx_store(to, e1, a.c.dtype, y1);
-        } else if (have) {
-            uint16_t* to = vp + ((size_t)hh * (a.c.page_size / 32) + in_page / 32) * d * 32;
-            const uint32_t slot = vx_vslot(i0 + w);
+        } else if (b.k) {
+            uint16_t* to = b.v + ((size_t)hh * (a.c.page_size / 32) + b.in_page / 32) * d * 32;
+            const uint32_t slot = vx_vslot(b.i0 + w);
             vx_store(to, (size_t)e0 * 32 + slot, a.c.dtype, y0);
             if (pair) vx_store(to, (size_t)e1 * 32 + slot, a.c.dtype, y1);
         }
@@ -440,17 +619,50 @@ uint32_t copy_grid(const VxPages& p, uint64_t moves) {
 
 }  // namespace
 
+// Whether 16-byte loads and stores fit rows of type elements.
+static bool vx_vec_rows(const VxRowsView& r) {
+    const uint32_t v = r.dtype == VELOX_DT_F32 ? 4 : 8;
+    return (uintptr_t)r.data % 16 == 0 && r.rs % v == 0 && (r.heads == 1 || r.hs % v == 0);
+}
+static bool vx_vec_pairs(const VxRopeTable& t, uint32_t dtype, uint32_t d) {
+    const uint32_t v = dtype == VELOX_DT_F32 ? 4 : 8;
+    return d % v == 0 && (t.interleaved ? t.rot % v == 0 : t.rot % (2 * v) == 0);
+}
+
 hipError_t vx_launch_rope_rows(const VxRopeTable& t, const VxRowsView& x, const VxRowsView& out, uint32_t n_rows,
                                uint32_t d, const uint32_t* positions, hipStream_t st) {
-    vx_rope_rows_kernel<<<n_rows, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions);
+    if (vx_vec_rows(x) && vx_vec_rows(out) && vx_vec_pairs(t, x.dtype, d)) {
+        // a thread for every angle where the rows fill the GPU several times over, one row a workgroup below
+        const uint32_t most = 2 * kRopeThreads / t.rot, share = n_rows / 1024, per = share < 1 ? 1 : share < most ? share : most;
+        const uint32_t grid = (n_rows + per - 1) / per;
+        if (x.dtype == VELOX_DT_F32) vx_rope_vec_kernel<float><<<grid, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions, per);
+        else if (x.dtype == VELOX_DT_F16) vx_rope_vec_kernel<_Float16><<<grid, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions, per);
+        else vx_rope_vec_kernel<__bf16><<<grid, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions, per);
+    } else {
+        vx_rope_rows_kernel<<<n_rows, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions);
+    }
     return hipGetLastError();
+}
+
+template <class T>
+static void vx_append_vec(const VxRopeTable& t, const VxAppendArgs& a, dim3 grid, hipStream_t st) {
+    if (a.c.dtype == VELOX_DT_F16) vx_append_vec_kernel<T, _Float16><<<grid, 256, 0, st>>>(t, a);
+    else vx_append_vec_kernel<T, __bf16><<<grid, 256, 0, st>>>(t, a);
 }
 
 hipError_t vx_launch_rope_append(const VxRopeTable& t, const VxAppendArgs& a, hipStream_t st) {
     // a sequence's rows touch at most rows / 32 + 2 blocks
-    const uint64_t blocks = (uint64_t)a.n_rows / 32 + 2ull * a.c.n_seqs;
-    const uint32_t grid = (uint32_t)(blocks < a.n_rows ? blocks : a.n_rows);
-    vx_rope_append_kernel<<<dim3(grid, 8), 256, 0, st>>>(t, a);
+    const uint64_t bound = (uint64_t)a.n_rows / 32 + 2ull * a.c.n_seqs;
+    const uint32_t blocks = (uint32_t)(bound < a.n_rows ? bound : a.n_rows);
+    // every workgroup of a block computes its angles again: no more of them than fill the GPU
+    const uint32_t y = blocks >= 512 ? 1 : blocks >= 256 ? 2 : blocks >= 128 ? 4 : 8;
+    const dim3 grid(blocks, y);
+    const bool vec = (!a.q.data || (vx_vec_rows(a.q) && vx_vec_rows(a.qo) && a.q.dtype == a.k.dtype)) && vx_vec_rows(a.k) &&
+                     vx_vec_rows(a.v) && a.k.dtype == a.v.dtype && vx_vec_pairs(t, a.k.dtype, a.c.d);
+    if (!vec) vx_append_rows_kernel<<<grid, 256, 0, st>>>(t, a);
+    else if (a.k.dtype == VELOX_DT_F32) vx_append_vec<float>(t, a, grid, st);
+    else if (a.k.dtype == VELOX_DT_F16) vx_append_vec<_Float16>(t, a, grid, st);
+    else vx_append_vec<__bf16>(t, a, grid, st);
     return hipGetLastError();
 }
 
