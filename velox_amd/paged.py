@@ -8,7 +8,6 @@ values: -1 is VELOX_HIP_NO_PAGE / VELOX_HIP_NO_SEQ. Calls can be captured into a
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import torch
@@ -20,20 +19,15 @@ _LAYOUTS = {"half": L.ROPE_HALF, "interleaved": L.ROPE_INTERLEAVED}
 _SCALINGS = {"none": L.ROPE_PLAIN, "linear": L.ROPE_LINEAR, "bands": L.ROPE_BANDS, "yarn": L.ROPE_YARN}
 
 
+# the current device and a device's current stream as plain numbers: torch.cuda.current_stream builds an object for
+# every call, a good part of a small operator's host time
+_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
-
-
-def _on(device: torch.device):
-    """The device's guard, if it is not the current one."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _gpu(t: torch.Tensor, what: str) -> torch.device:
@@ -41,23 +35,38 @@ def _gpu(t: torch.Tensor, what: str) -> torch.device:
     return t.device
 
 
+def _call(fn, index: int, *args) -> None:
+    """fn(*args, stream) on device `index`, its current stream."""
+    if _device() == index:
+        rc = fn(*args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
+    if rc:
+        L.check(rc, fn.__name__)
+
+
 def _words(t: torch.Tensor, n: int, device: torch.device, what: str) -> int:
     """The address of an int32 vector of n elements (n < 0: any length)."""
-    _need(_gpu(t, what) == device and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(),
-          f"{what}: a contiguous int32 vector on {device} is wanted")
-    _need(n < 0 or t.numel() == n, f"{what}: {n} elements are wanted, got {t.numel()}")
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 vector on {device} is wanted")
+    if n >= 0 and t.numel() != n:
+        raise ValueError(f"{what}: {n} elements are wanted, got {t.numel()}")
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, device: torch.device, what: str, heads: int = 0, dim: int = 0) -> L.Rows:
-    """[row][head][element] as VeloxHipRows; the elements of a head are next to each other."""
-    _need(_gpu(t, what) == device and t.dim() == 3 and t.dtype in _DTYPES,
-          f"{what}: a float32, float16 or bfloat16 tensor [row][head][element] on {device} is wanted")
-    _need((not heads or t.shape[1] == heads) and (not dim or t.shape[2] == dim),
-          f"{what}: heads and head size {heads, dim} are wanted, got {tuple(t.shape[1:])}")
+def _rows(t: torch.Tensor, device: torch.device, what: str, heads: int = 0, dim: int = 0) -> tuple[L.Rows, int]:
+    """[row][head][element] as VeloxHipRows, and its rows; the elements of a head are next to each other."""
+    code = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
+    if code is None or t.device != device or t.dim() != 3:
+        raise ValueError(f"{what}: a float32, float16 or bfloat16 tensor [row][head][element] on {device} is wanted")
+    n, h, d = t.shape
+    if (heads and h != heads) or (dim and d != dim):
+        raise ValueError(f"{what}: heads and head size {heads, dim} are wanted, got {h, d}")
     rs, hs, es = t.stride()
-    _need(es == 1 or t.shape[2] == 1, f"{what}: a head's elements have to be next to each other")
-    return L.Rows(t.data_ptr(), _DTYPES[t.dtype], t.shape[1], rs, hs)
+    if es != 1 and d != 1:
+        raise ValueError(f"{what}: a head's elements have to be next to each other")
+    return L.Rows(t.data_ptr(), code, h, rs, hs), n
 
 
 class PagedCache:
@@ -108,12 +117,11 @@ class PagedCache:
             self._scratch = torch.zeros(scratch.value // 4, dtype=torch.int32, device=device)
             d.scratch = self._scratch.data_ptr()
         self.desc = d
-        self._ref = C.byref(d)
+        self._ref, self._index = C.byref(d), device.index
 
     # -- pages ----------------------------------------------------------------------------------
     def _pages(self, name: str, *args) -> None:
-        with _on(self.device):
-            L.check(getattr(self.lib, "velox_hip_pages_" + name)(self._ref, *args, _stream(self.device)), "pages_" + name)
+        _call(getattr(self.lib, "velox_hip_pages_" + name), self._index, self._ref, *args)
 
     def reset(self) -> None:
         """No sequence has a page, every page is free."""
@@ -198,13 +206,12 @@ def rope(turn: Rope, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor
     _need(bool(turn.handle), "rope: the handle is closed")
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=device)
-    xr, o = _rows(x, device, "x"), _rows(out, device, "out")
+    xr, n = _rows(x, device, "x")
+    o, _ = _rows(out, device, "out")
     _need(out.shape == x.shape and out.dtype == x.dtype, "out: the shape and type of x are wanted")
-    at = _words(positions, x.shape[0], device, "positions")
+    at = _words(positions, n, device, "positions")
     if x.numel():
-        with _on(device):
-            L.check(turn.lib.velox_hip_rope_rows(turn.handle, C.byref(xr), C.byref(o), x.shape[0], x.shape[2], at, _stream(device)),
-                    "rope_rows")
+        _call(turn.lib.velox_hip_rope_rows, device.index, turn.handle, xr, o, n, x.shape[2], at)
     return out
 
 
@@ -215,22 +222,22 @@ def rope_append(cache: PagedCache, layer: int, turn: Rope | None, q: torch.Tenso
     device, d = cache.device, cache.head_dim
     _need(turn is None or bool(turn.handle), "rope_append: the handle is closed")
     _need(layer >= 0, "layer has to be at least 0")
-    kr, vr = _rows(k, device, "k", cache.num_kv_heads, d), _rows(v, device, "v", cache.num_kv_heads, d)
-    n = k.shape[0]
-    _need(v.shape[0] == n, "k and v: as many rows of each are wanted")
+    kr, n = _rows(k, device, "k", cache.num_kv_heads, d)
+    vr, vn = _rows(v, device, "v", cache.num_kv_heads, d)
+    _need(vn == n, "k and v: as many rows of each are wanted")
     qr = qo = None
     if q is not None:
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        qr, qo = C.byref(_rows(q, device, "q", 0, d)), C.byref(_rows(q_out, device, "q_out", q.shape[1], d))
-        _need(q.shape[0] == n and q_out.shape[0] == n, "q and q_out: as many rows as k are wanted")
+        qr, qn = _rows(q, device, "q", 0, d)
+        qo, on = _rows(q_out, device, "q_out", qr.heads, d)
+        _need(qn == n and on == n, "q and q_out: as many rows as k are wanted")
     else:
         _need(q_out is None, "q_out without q")
     start = _words(q_start, cache.n_seqs + 1, device, "q_start") if q_start is not None else None
     if n:
-        with _on(device):
-            L.check(cache.lib.velox_hip_rope_append(cache._ref, layer, turn.handle if turn is not None else None, qr, C.byref(kr),
-                                                    C.byref(vr), qo, start, n, _stream(device)), "rope_append")
+        _call(cache.lib.velox_hip_rope_append, cache._index, cache._ref, layer, turn.handle if turn is not None else None, qr, kr, vr,
+              qo, start, n)
     return q_out
 
 
@@ -242,7 +249,8 @@ def _mask(window: int, sinks: int) -> L.AttnMask:
 def _space(workspace: torch.Tensor | None, device: torch.device) -> tuple[int | None, int]:
     if workspace is None:
         return None, 0
-    _need(_gpu(workspace, "workspace") == device and workspace.is_contiguous(), f"workspace: contiguous memory on {device} is wanted")
+    if not isinstance(workspace, torch.Tensor) or workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace: contiguous memory on {device} is wanted")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
@@ -252,18 +260,16 @@ def attention(cache: PagedCache, layer: int, q: torch.Tensor, *, window: int = 0
     max_len bounds lens for planning; workspace: cache.attention_workspace of the same bounds (None: made here)."""
     device = cache.device
     _need(layer >= 0 and max_len >= 0, "layer and max_len have to be at least 0")
-    qr = _rows(q, device, "q", 0, cache.head_dim)
-    _need(q.shape[0] == cache.n_seqs, f"q: {cache.n_seqs} rows are wanted")
+    qr, n = _rows(q, device, "q", 0, cache.head_dim)
+    _need(n == cache.n_seqs, f"q: {cache.n_seqs} rows are wanted")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    o = _rows(out, device, "out", q.shape[1], cache.head_dim)
-    _need(out.shape[0] == q.shape[0], "out: as many rows as q are wanted")
+    o, on = _rows(out, device, "out", qr.heads, cache.head_dim)
+    _need(on == n, "out: as many rows as q are wanted")
     if workspace is None:
-        workspace = cache.attention_workspace(q.shape[1], max_len=max_len)
+        workspace = cache.attention_workspace(qr.heads, max_len=max_len)
     space, size = _space(workspace, device)
-    with _on(device):
-        L.check(cache.lib.velox_hip_paged_attention(cache._ref, layer, C.byref(qr), C.byref(o), _mask(window, sinks), scale, max_len,
-                                                    space, size, _stream(device)), "paged_attention")
+    _call(cache.lib.velox_hip_paged_attention, cache._index, cache._ref, layer, qr, o, _mask(window, sinks), scale, max_len, space, size)
     return out
 
 
@@ -274,20 +280,17 @@ def prompt_attention(cache: PagedCache, layer: int, q: torch.Tensor, q_start: to
     the last of them its newest position. Rows behind the last sequence are not written."""
     device = cache.device
     _need(layer >= 0 and max_len >= 0 and max_rows >= 0, "layer, max_rows and max_len have to be at least 0")
-    qr = _rows(q, device, "q", 0, cache.head_dim)
+    qr, n = _rows(q, device, "q", 0, cache.head_dim)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    o = _rows(out, device, "out", q.shape[1], cache.head_dim)
-    n = q.shape[0]
-    _need(out.shape[0] == n, "out: as many rows as q are wanted")
+    o, on = _rows(out, device, "out", qr.heads, cache.head_dim)
+    _need(on == n, "out: as many rows as q are wanted")
     start = _words(q_start, cache.n_seqs + 1, device, "q_start")
     if n == 0:
         return out
     if workspace is None:
-        workspace = cache.prompt_workspace(q.shape[1], total_rows=n, max_rows=max_rows, max_len=max_len)
+        workspace = cache.prompt_workspace(qr.heads, total_rows=n, max_rows=max_rows, max_len=max_len)
     space, size = _space(workspace, device)
-    with _on(device):
-        L.check(cache.lib.velox_hip_paged_prompt_attention(cache._ref, layer, C.byref(qr), C.byref(o), start, n, _mask(window, sinks),
-                                                           scale, max_rows, max_len, space, size, _stream(device)),
-                "paged_prompt_attention")
+    _call(cache.lib.velox_hip_paged_prompt_attention, cache._index, cache._ref, layer, qr, o, start, n, _mask(window, sinks), scale,
+          max_rows, max_len, space, size)
     return out
