@@ -45,12 +45,16 @@ struct VxEight {
 struct VxBf16 {
     typedef __bf16 elt;
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ float sum2(v2 a, float c) { return __builtin_amdgcn_fdot2_f32_bf16(a, v2{(__bf16)1.0f, (__bf16)1.0f}, c, false); }
     static __device__ __forceinline__ vx_f4 mfma(v8 a, v8 b, vx_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ vx_f16 mfma(v8 a, v8 b, vx_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 struct VxF16 {
     typedef _Float16 elt;
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ float sum2(v2 a, float c) { return __builtin_amdgcn_fdot2(a, v2{(_Float16)1.0f, (_Float16)1.0f}, c, false); }
     static __device__ __forceinline__ vx_f4 mfma(v8 a, v8 b, vx_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ vx_f16 mfma(v8 a, v8 b, vx_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
@@ -394,9 +398,11 @@ __device__ __forceinline__ void vx_wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void vx_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-// 16 bytes per lane from base + off (off per lane) to the 1 KiB of LDS at byte offset lds (base and lds uniform).
+// 16 bytes per lane from base + off (off per lane) to the 1 KiB of LDS at byte offset lds (base and lds uniform). It
+// stays between the barrier before it and the wait behind it (volatile statements keep their order); LDS reads may
+// pass it, so it must not write what is read before that wait.
 __device__ __forceinline__ void vx_load_lds(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0");
 }
 // The other lane of a pair (lane ^ 32) and this one: larger value, sum.
 __device__ __forceinline__ float vx_max_pair(float v) {
@@ -495,71 +501,89 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
 #pragma unroll
             for (int c = 0; c < NK; ++c) raw[c].read(a.q.data, (size_t)row * a.q.rs + (size_t)head * a.q.hs + 16 * c + 8 * grp, a.q.dtype);
         }
-        float x[NK][8], big = 0.0f;
+        if constexpr (QT == 1) {  // the cache's type: as it lies
+            const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
-        for (int c = 0; c < NK; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = mine ? raw[c].at(i, a.q.dtype) : 0.0f;
-                x[c][i] = a.scale < 0.0f ? -v : v;
-                big = fmaxf(big, fabsf(v));
-            }
-        if constexpr (QT == 2) {
-            big = vx_max_pair(big);
-            const int e = big > 0.0f && big < INFINITY ? 14 - ilogbf(big) : 0;
+            for (int c = 0; c < NK; ++c) qf[0][c] = mine ? __builtin_bit_cast(v8, raw[c].w[0] ^ sign) : v8{};
+        } else {
+            float x[NK][8], big = 0.0f;
 #pragma unroll
             for (int c = 0; c < NK; ++c)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[c][i] = ldexpf(x[c][i], e);
-            to_log2 = ldexpf(to_log2, -e);
-        }
-#pragma unroll
-        for (int c = 0; c < NK; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float rest = x[c][i];
-#pragma unroll
-                for (int u = 0; u < QT; ++u) {
-                    const typename E::elt v = (typename E::elt)rest;
-                    qf[u][c][i] = v;
-                    rest -= (float)v;
+                for (int i = 0; i < 8; ++i) {
+                    const float v = mine ? raw[c].at(i, a.q.dtype) : 0.0f;
+                    x[c][i] = a.scale < 0.0f ? -v : v;
+                    big = fmaxf(big, fabsf(v));
                 }
+            if constexpr (QT == 2) {
+                big = vx_max_pair(big);
+                const int e = big > 0.0f && big < INFINITY ? 14 - ilogbf(big) : 0;
+#pragma unroll
+                for (int c = 0; c < NK; ++c)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[c][i] = ldexpf(x[c][i], e);
+                to_log2 = ldexpf(to_log2, -e);
             }
+#pragma unroll
+            for (int c = 0; c < NK; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float rest = x[c][i];
+#pragma unroll
+                    for (int u = 0; u < QT; ++u) {
+                        const typename E::elt v = (typename E::elt)rest;
+                        qf[u][c][i] = v;
+                        rest -= (float)v;
+                    }
+                }
+        }
     }
 
-    // page and place of the next 64 chunks, one a lane
-    uint32_t pages, places;
-    const auto look_up = [&](uint32_t first) {
-        const uint32_t i = first + lane;
-        pages = kVxNoPage;
-        places = 0;
+    // where the K of the next 64 chunks lies in the pool, one a lane, and which of them have a page (page 0 stands in
+    // for the others, and for chunks past the last)
+    uint32_t place_lo, place_hi;
+    uint64_t paged, partial, hidden;  // chunks with a page; that not all pairs of the wave see whole; with places no pair sees
+    uint32_t first = 0;               // the step whose chunks are in lanes 0 and 1
+    const auto look_up = [&](uint32_t step) {
+        const uint32_t i = c0 + 2 * step + lane, base = vx_chunk_base(ch, i);
+        uint32_t page = kVxNoPage, place = 0;
         if (i < c1) {
-            const uint32_t base = vx_chunk_base(ch, i), j = base / a.c.page_size;
-            places = base - j * a.c.page_size;
-            if (j < a.c.max_pages) pages = table[j];
+            const uint32_t j = base / a.c.page_size;
+            place = base - j * a.c.page_size;
+            if (j < a.c.max_pages) page = table[j];
         }
+        const bool have = page < a.c.n_pages;
+        partial = __ballot(!have || (int)base + 31 > all_t || (int)base < all_low);
+        hidden = __ballot(!have || (int)base + 31 > last_t || (int)base < (int)ch.low);
+        const uint64_t at = (have ? (uint64_t)page * a.c.page_bytes : 0) + ((uint64_t)kvh * a.c.page_size + place) * (D * 2);
+        place_lo = (uint32_t)at;
+        place_hi = (uint32_t)(at >> 32);
+        paged = __ballot(have);
+        first = step;
     };
-    const auto page_of = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(i & 63u)); };
-    const auto place_of = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)places, (int)(i & 63u)); };
 
-    // staging: the waves share the KiBs of a step's K (or V), two chunks' worth
+    // staging: each wave brings a quarter of a step's K and V, KiB by KiB
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
     const uint32_t my_chunk = wave >> 1, my_unit = (wave & 1u) * (kUnits / 2);
-    uint32_t k_off[kUnits / 2], v_off[kUnits / 2];
+    const uint32_t my_lds = lds0 + my_chunk * kChunk + my_unit * 1024u;
+    const uint64_t v_from_k = (uint64_t)a.c.hkv * a.c.page_size * (D * 2);
+    uint32_t k_off[kUnits / 2];
+    const uint32_t v_off = (16u * my_unit + lane / 4) * 64 + 16u * (lane % 4 ^ vx_v_swizzle(lane / 4));  // 16 rows a unit
 #pragma unroll
     for (uint32_t j = 0; j < kUnits / 2; ++j) {
-        const uint32_t i = 64u * (my_unit + j) + lane, p = i / RB, e = i / 4;
+        const uint32_t i = 64u * (my_unit + j) + lane, p = i / RB;
         k_off[j] = p * D * 2 + 16u * (i % RB ^ vx_k_swizzle<D>(p));
-        v_off[j] = e * 64 + 16u * (i % 4 ^ vx_v_swizzle(e));
     }
-    // K of the step whose chunks are in lanes i and i + 1
-    const auto stage = [&](uint32_t i, const uint32_t (&off)[kUnits / 2], uint32_t head0, uint32_t to) {
-        const uint32_t page = page_of(i + my_chunk), place = place_of(i + my_chunk);
-        const uint8_t* base = a.c.pool + (size_t)(page < a.c.n_pages ? page : 0u) * a.c.page_bytes +
-                              ((size_t)(head0 + kvh) * a.c.page_size + place) * (D * 2);
-#pragma unroll
-        for (uint32_t j = 0; j < kUnits / 2; ++j) vx_load_lds(base, off[j], lds0 + to + my_chunk * kChunk + (my_unit + j) * 1024u);
+    const auto source = [&](uint32_t step) {  // this wave's chunk of a step that the lanes hold
+        const int l = (int)(2 * (step - first) + my_chunk);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)place_lo, l), hi = (uint32_t)__builtin_amdgcn_readlane((int)place_hi, l);
+        return (const uint8_t*)a.c.pool + ((uint64_t)hi << 32 | lo);
     };
+    const auto load_k = [&](const uint8_t* from, uint32_t buf, uint32_t j) { vx_load_lds(from, k_off[j], my_lds + buf * (2 * kChunk) + j * 1024u); };
+    const auto load_v = [&](const uint8_t* from, uint32_t buf, uint32_t j) {
+        vx_load_lds(from + v_from_k + j * 1024u, v_off, my_lds + (4 + 2 * buf) * kChunk + j * 1024u);
+    };
+    constexpr uint32_t NU = kUnits / 2;
 
     vx_f16 o[NM];
 #pragma unroll
@@ -586,33 +610,23 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     };
     // place of position p in the chunk at base: -1 in front of it, 32 or more behind it
     const auto place_in = [](int p, uint32_t base) { return max(-1, min(64, p - (int)base)); };
-    struct Step {  // two chunks of the walk; uniform
-        uint32_t base[2];
-        bool have[2], masked, hidden;  // some pair of the wave does not see all; some place is seen by no pair
+    struct Step {  // two chunks of the walk, a bit for each
+        uint32_t chunk, have, partial, hidden;
     };
-    const auto step_of = [&](uint32_t i, uint32_t at) {
-        Step x;
-        x.masked = x.hidden = false;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const uint32_t base = vx_chunk_base(ch, i + b);
-            x.base[b] = base;
-            x.have[b] = i + b < c1 && page_of(at + b) < a.c.n_pages;
-            x.masked |= !x.have[b] || (int)base + 31 > all_t || (int)base < all_low;
-            x.hidden |= !x.have[b] || (int)base + 31 > last_t || (int64_t)base < ch.low;
-        }
-        x.masked = __builtin_amdgcn_readfirstlane(x.masked);
-        x.hidden = __builtin_amdgcn_readfirstlane(x.hidden);
-        return x;
+    const auto step_of = [&](uint32_t step) {
+        const uint32_t at = 2 * (step - first);
+        return Step{c0 + 2 * step, (uint32_t)(paged >> at) & 3u, (uint32_t)(partial >> at) & 3u, (uint32_t)(hidden >> at) & 3u};
     };
     // Hides what the mask hides, and moves the maximum where a score passes it by more than 8 (the weights may pass 1
     // by 2^8 until then: a bf16 or fp16 weight keeps its relative precision, and the rescaling is rare).
     const auto bound = [&](Scores& s, const Step& x) {
-        if (x.masked) {
+        if (x.partial) {
+            asm volatile("");  // a branch, not 64 selects in every step
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const int pt = (x.have[b] ? place_in(t, x.base[b]) : -1) - 4 * (int)grp, pl = place_in(low, x.base[b]) - 4 * (int)grp,
-                          ps = place_in(sinks, x.base[b]) - 4 * (int)grp;
+                const uint32_t base = vx_chunk_base(ch, x.chunk + b);
+                const int pt = (x.have >> b & 1u ? place_in(t, base) : -1) - 4 * (int)grp, pl = place_in(low, base) - 4 * (int)grp,
+                          ps = place_in(sinks, base) - 4 * (int)grp;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int p = 16 * (r >> 2 & 1) + 8 * (r >> 3) + (r & 3);
@@ -639,8 +653,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     const auto clear = [&](const Step& x, uint32_t buf) {
         for (uint32_t i = threadIdx.x; i < 2 * D * 4; i += kPromptThreads) {
             const uint32_t b = i / (D * 4), e = i / 4 % D, j = i % 4 ^ vx_v_swizzle(e);  // j: slots 8 j .. 8 j + 7 of row e
-            const uint32_t base = b ? x.base[1] : x.base[0];
-            const int pt = (b ? x.have[1] : x.have[0]) ? place_in(last_t, base) : -1, pl = place_in((int)ch.low, base), ps = place_in(sinks, base);
+            const uint32_t base = vx_chunk_base(ch, x.chunk + b);
+            const int pt = x.have >> b & 1u ? place_in(last_t, base) : -1, pl = place_in((int)ch.low, base), ps = place_in(sinks, base);
             vx_u4* at = (vx_u4*)(lds + 4 * kChunk + buf * (2 * kChunk) + 16 * i);
             vx_u4 v = *at;
 #pragma unroll
@@ -652,7 +666,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
         }
         vx_barrier();
     };
-    // o += V^T P^T of a chunk
+    // o += V^T P^T of a chunk. Weights of one term are summed as they are rounded, two by two: what the row is divided
+    // by is the sum of what it was made of.
     const auto add = [&](const vx_f16& s, int b, uint32_t buf) {
         const unsigned char* vb = lds + 4 * kChunk + buf * (2 * kChunk) + b * kChunk;
         const float ref = m == -INFINITY ? 0.0f : m;
@@ -660,7 +675,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], to_log2, -ref));
-            l += p;
+            if constexpr (PT > 1) l += p;
             float rest = p;
 #pragma unroll
             for (int u = 0; u < PT; ++u) {
@@ -668,6 +683,10 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
                 pf[u][r >> 3][r & 7] = v;
                 rest -= (float)v;
             }
+        }
+        if constexpr (PT == 1) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) l = E::sum2(typename E::v2{pf[0][r >> 3][r & 7], pf[0][r >> 3][(r & 7) + 1]}, l);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -680,77 +699,90 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     };
 
     // The walk, a step of two chunks at a time: while step i's weights are formed and added, the scores of step
-    // i + 1 are multiplied (PIPE). LDS: K of steps i + 1 and i + 2, V of steps i and i + 1, each in two buffers.
-    // With q in several terms the registers hold one step's scores only.
+    // i + 1 are multiplied and the loads of what follows go out between the products (issued in one go they held a
+    // wave up for 1800 of a step's 4500 clocks). LDS: K of steps i + 1 and i + 2, V of steps i and i + 1, each in two
+    // buffers. With q in several terms the registers hold one step's scores only (PIPE false).
     constexpr bool PIPE = QT == 1;
     const uint32_t n_steps = (c1 - c0 + 1) / 2;
-    uint32_t first = 0;  // the step whose chunks are in lanes 0 and 1
-    const auto at = [&](uint32_t i) {  // the lane of step i's first chunk; i never falls behind the last look_up
-        if (i - first >= 32) {
-            look_up(c0 + 2 * i);
-            first = i;
-        }
-        return 2 * (i - first);
-    };
     if (n_steps) {
-        look_up(c0);
-        stage(0, k_off, 0, 0);
-        Step now = step_of(c0, 0), next = now;
+        look_up(0);
+        const uint8_t* from = source(0);
+#pragma unroll
+        for (uint32_t j = 0; j < NU; ++j) load_k(from, 0, j);
+        Step now = step_of(0), next = now;
         Scores s;
         if constexpr (PIPE) {
             vx_wait_loads<0>();
             vx_barrier();
-            stage(0, v_off, a.c.hkv, 4 * kChunk);
-            if (n_steps > 1) {
-                next = step_of(c0 + 2, 2);
-                stage(2, k_off, 0, 2 * kChunk);
+            const uint8_t* from1 = source(1);
+            next = step_of(1);
+#pragma unroll
+            for (uint32_t j = 0; j < NU; ++j) {
+                load_v(from, 0, j);
+                load_k(from1, 1, j);
             }
             scores(s[0], 0, 0);
             scores(s[1], 1, 0);
             bound(s, now);
         } else {
-            stage(0, v_off, a.c.hkv, 4 * kChunk);
+#pragma unroll
+            for (uint32_t j = 0; j < NU; ++j) load_v(from, 0, j);
         }
-        for (uint32_t i = 0; i < n_steps; ++i) {
-            const uint32_t buf = i & 1u;
-            const bool more = i + 1 < n_steps;
+        const auto begin = [&](uint32_t i) {
             vx_wait_loads<0>();
             vx_barrier();  // step i is in LDS, and the buffers of what follows are read by everyone
-            Step after = next;
-            if (more) {
-                uint32_t j = at(i + 1);
-                stage(j, v_off, a.c.hkv, 4 * kChunk + (buf ^ 1) * (2 * kChunk));
-                if constexpr (PIPE) {
-                    if (i + 2 < n_steps) {
-                        j = at(i + 2);
-                        after = step_of(c0 + 2 * (i + 2), j);
-                        stage(j, k_off, 0, buf * (2 * kChunk));
-                    }
-                } else {
-                    next = step_of(c0 + 2 * (i + 1), j);
-                    stage(j, k_off, 0, (buf ^ 1) * (2 * kChunk));
+            if (i + 2 - first >= 32) look_up(i + 1);
+        };
+        if constexpr (PIPE) {
+            // behind the last step the loads and the scores go on with what is there, to no use
+            const auto go = [&](uint32_t i, uint32_t buf, Scores& s, Scores& u) {
+                begin(i);
+                const uint8_t *from1 = source(i + 1), *from2 = source(i + 2);
+                const Step after = step_of(i + 2);
+                if (now.hidden) clear(now, buf);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const auto load = [&](uint32_t j) {
+                        if (b == 0) load_v(from1, buf ^ 1, j);
+                        else load_k(from2, buf, j);
+                    };
+#pragma unroll
+                    for (uint32_t j = 0; j < NU / 2; ++j) load(j);
+                    scores(u[b], b, buf ^ 1);
+#pragma unroll
+                    for (uint32_t j = NU / 2; j < NU; ++j) load(j);
+                    add(s[b], b, buf);
                 }
+                if (i + 1 < n_steps) bound(u, next);
+                now = next;
+                next = after;
+            };
+            Scores u;
+            for (uint32_t i = 0; i < n_steps; i += 2) {
+                go(i, 0, s, u);
+                if (i + 1 < n_steps) go(i + 1, 1, u, s);
             }
-            if (now.hidden) clear(now, buf);
-            if constexpr (PIPE) {
-                Scores u;  // behind the last step this multiplies what an earlier one left in LDS, to no use
-                scores(u[0], 0, buf ^ 1);
-                add(s[0], 0, buf);
-                scores(u[1], 1, buf ^ 1);
-                add(s[1], 1, buf);
-                if (more) bound(u, next);
-                s[0] = u[0];
-                s[1] = u[1];
-            } else {
+        } else {
+            for (uint32_t i = 0; i < n_steps; ++i) {
+                const uint32_t buf = i & 1u;
+                begin(i);
+                const uint8_t* from1 = source(i + 1);
+                next = step_of(i + 1);
+#pragma unroll
+                for (uint32_t j = 0; j < NU; ++j) {
+                    load_k(from1, buf ^ 1, j);
+                    load_v(from1, buf ^ 1, j);
+                }
+                if (now.hidden) clear(now, buf);
                 scores(s[0], 0, buf);
                 scores(s[1], 1, buf);
                 bound(s, now);
                 add(s[0], 0, buf);
                 add(s[1], 1, buf);
+                now = next;
             }
-            now = next;
-            next = after;
         }
+        vx_wait_loads<0>();  // nothing may land in LDS that is another workgroup's by then
     }
 
     l = vx_sum_pair(l);
