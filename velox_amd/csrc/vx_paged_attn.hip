@@ -428,8 +428,9 @@ __device__ __forceinline__ bool vx_find_tile(const VxPagedAttnArgs& a, uint32_t 
     uint32_t base = 0;
     for (uint32_t s0 = 0; s0 < a.c.n_seqs; s0 += 64) {
         const uint32_t s = s0 + lane;
-        uint32_t n = 0, lo = 0, rows = 0;
+        uint32_t n = 0, lo = 0, rows = 0, len = 0;
         if (s < a.c.n_seqs) {
+            len = a.c.lens[s];
             lo = min(a.q_start[s], a.n_rows);
             rows = max(min(a.q_start[s + 1], a.n_rows), lo) - lo;
             n = (uint32_t)(((uint64_t)rows * G + kPromptRows - 1) / kPromptRows);
@@ -447,7 +448,7 @@ __device__ __forceinline__ bool vx_find_tile(const VxPagedAttnArgs& a, uint32_t 
             r.tile = item - base - (uint32_t)(__builtin_amdgcn_readlane((int)upto, l) - __builtin_amdgcn_readlane((int)n, l));
             r.lo = (uint32_t)__builtin_amdgcn_readlane((int)lo, l);
             r.rows = (uint32_t)__builtin_amdgcn_readlane((int)rows, l);
-            r.pos0 = (int64_t)a.c.lens[r.seq] - (int64_t)r.rows;
+            r.pos0 = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)len, l) - (int64_t)r.rows;
             return true;
         }
         base += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
@@ -493,50 +494,11 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     const int all_t = position(min(r0 + 32 * wave, r1 - 1)), all_low = (int)vx_low(position(min(r0 + 32 * wave + 31, r1 - 1)), a.window);
     const int last_t = position(r1 - 1);
 
-    v8 qf[QT][NK];
-    float to_log2 = fabsf(a.scale) * kLog2e;
-    {
-        VxEight raw[NK];
-        if (mine) {
+    // q is requested before the table and the first K, and brought into its operands behind them
+    VxEight raw[NK];
+    if (mine) {
 #pragma unroll
-            for (int c = 0; c < NK; ++c) raw[c].read(a.q.data, (size_t)row * a.q.rs + (size_t)head * a.q.hs + 16 * c + 8 * grp, a.q.dtype);
-        }
-        if constexpr (QT == 1) {  // the cache's type: as it lies
-            const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-            for (int c = 0; c < NK; ++c) qf[0][c] = mine ? __builtin_bit_cast(v8, raw[c].w[0] ^ sign) : v8{};
-        } else {
-            float x[NK][8], big = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NK; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = mine ? raw[c].at(i, a.q.dtype) : 0.0f;
-                    x[c][i] = a.scale < 0.0f ? -v : v;
-                    big = fmaxf(big, fabsf(v));
-                }
-            if constexpr (QT == 2) {
-                big = vx_max_pair(big);
-                const int e = big > 0.0f && big < INFINITY ? 14 - ilogbf(big) : 0;
-#pragma unroll
-                for (int c = 0; c < NK; ++c)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[c][i] = ldexpf(x[c][i], e);
-                to_log2 = ldexpf(to_log2, -e);
-            }
-#pragma unroll
-            for (int c = 0; c < NK; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float rest = x[c][i];
-#pragma unroll
-                    for (int u = 0; u < QT; ++u) {
-                        const typename E::elt v = (typename E::elt)rest;
-                        qf[u][c][i] = v;
-                        rest -= (float)v;
-                    }
-                }
-        }
+        for (int c = 0; c < NK; ++c) raw[c].read(a.q.data, (size_t)row * a.q.rs + (size_t)head * a.q.hs + 16 * c + 8 * grp, a.q.dtype);
     }
 
     // where the K of the next 64 chunks lies in the pool, one a lane, and which of them have a page (page 0 stands in
@@ -584,6 +546,61 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
         vx_load_lds(from + v_from_k + j * 1024u, v_off, my_lds + (4 + 2 * buf) * kChunk + j * 1024u);
     };
     constexpr uint32_t NU = kUnits / 2;
+
+    const uint32_t n_steps = (c1 - c0 + 1) / 2;
+    constexpr bool PIPE = QT == 1;
+    look_up(0);
+    if (n_steps) {  // K and V of the first step, with PIPE K of the second
+        const uint8_t *from = source(0), *from1 = source(1);
+#pragma unroll
+        for (uint32_t j = 0; j < NU; ++j) load_k(from, 0, j);
+#pragma unroll
+        for (uint32_t j = 0; j < NU; ++j) load_v(from, 0, j);
+        if constexpr (PIPE) {
+#pragma unroll
+            for (uint32_t j = 0; j < NU; ++j) load_k(from1, 1, j);
+        }
+    }
+    v8 qf[QT][NK];
+    float to_log2 = fabsf(a.scale) * kLog2e;
+    {
+        if constexpr (QT == 1) {  // the cache's type: as it lies
+            const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+            for (int c = 0; c < NK; ++c) qf[0][c] = mine ? __builtin_bit_cast(v8, raw[c].w[0] ^ sign) : v8{};
+        } else {
+            float x[NK][8], big = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NK; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = mine ? raw[c].at(i, a.q.dtype) : 0.0f;
+                    x[c][i] = a.scale < 0.0f ? -v : v;
+                    big = fmaxf(big, fabsf(v));
+                }
+            if constexpr (QT == 2) {
+                big = vx_max_pair(big);
+                const int e = big > 0.0f && big < INFINITY ? 14 - ilogbf(big) : 0;
+#pragma unroll
+                for (int c = 0; c < NK; ++c)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[c][i] = ldexpf(x[c][i], e);
+                to_log2 = ldexpf(to_log2, -e);
+            }
+#pragma unroll
+            for (int c = 0; c < NK; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float rest = x[c][i];
+#pragma unroll
+                    for (int u = 0; u < QT; ++u) {
+                        const typename E::elt v = (typename E::elt)rest;
+                        qf[u][c][i] = v;
+                        rest -= (float)v;
+                    }
+                }
+        }
+    }
 
     vx_f16 o[NM];
 #pragma unroll
@@ -702,31 +719,16 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     // i + 1 are multiplied and the loads of what follows go out between the products (issued in one go they held a
     // wave up for 1800 of a step's 4500 clocks). LDS: K of steps i + 1 and i + 2, V of steps i and i + 1, each in two
     // buffers. With q in several terms the registers hold one step's scores only (PIPE false).
-    constexpr bool PIPE = QT == 1;
-    const uint32_t n_steps = (c1 - c0 + 1) / 2;
     if (n_steps) {
-        look_up(0);
-        const uint8_t* from = source(0);
-#pragma unroll
-        for (uint32_t j = 0; j < NU; ++j) load_k(from, 0, j);
         Step now = step_of(0), next = now;
         Scores s;
         if constexpr (PIPE) {
-            vx_wait_loads<0>();
+            vx_wait_loads<2 * NU>();  // the first K; the V and the next K may be on their way
             vx_barrier();
-            const uint8_t* from1 = source(1);
             next = step_of(1);
-#pragma unroll
-            for (uint32_t j = 0; j < NU; ++j) {
-                load_v(from, 0, j);
-                load_k(from1, 1, j);
-            }
             scores(s[0], 0, 0);
             scores(s[1], 1, 0);
             bound(s, now);
-        } else {
-#pragma unroll
-            for (uint32_t j = 0; j < NU; ++j) load_v(from, 0, j);
         }
         const auto begin = [&](uint32_t i) {
             vx_wait_loads<0>();
@@ -740,6 +742,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
                 const uint8_t *from1 = source(i + 1), *from2 = source(i + 2);
                 const Step after = step_of(i + 2);
                 if (now.hidden) clear(now, buf);
+                __builtin_amdgcn_s_setprio(1);  // before the other workgroup's waves that stage or take maxima: 479 -> 470 us
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const auto load = [&](uint32_t j) {
@@ -753,6 +756,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
                     for (uint32_t j = NU / 2; j < NU; ++j) load(j);
                     add(s[b], b, buf);
                 }
+                __builtin_amdgcn_s_setprio(0);
                 if (i + 1 < n_steps) bound(u, next);
                 now = next;
                 next = after;
