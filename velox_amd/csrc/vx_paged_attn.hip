@@ -33,13 +33,55 @@ struct VxEight {
         if (dtype == VELOX_DT_F32) __builtin_memcpy(w, (const float*)p + i, 32);
         else __builtin_memcpy(w, (const uint16_t*)p + i, 16);
     }
-    __device__ __forceinline__ float at(int i, uint32_t dtype) const {
-        const uint32_t f = w[i / 4][i & 3], h = w[0][i / 2] >> 16 * (i & 1) & 0xFFFFu;
-        return dtype == VELOX_DT_F32   ? __builtin_bit_cast(float, f)
-               : dtype == VELOX_DT_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h)
-                                       : __builtin_bit_cast(float, h << 16);
-    }
 };
+template <int N>
+__device__ __forceinline__ void vx_widen(const VxEight (&raw)[N], uint32_t dtype, float (&x)[N][8]) {
+    if (dtype == VELOX_DT_F32) {
+        asm volatile("");  // three branches, not selects of three values each
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t f = raw[c].w[i / 4][i & 3];
+                x[c][i] = __builtin_bit_cast(float, f);
+            }
+    } else if (dtype == VELOX_DT_F16) {
+        asm volatile("");
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint16_t h = (uint16_t)(raw[c].w[0][i / 2] >> 16 * (i & 1));
+                x[c][i] = (float)__builtin_bit_cast(_Float16, h);
+            }
+    } else {
+        asm volatile("");
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t f = i & 1 ? raw[c].w[0][i / 2] & 0xFFFF0000u : raw[c].w[0][i / 2] << 16;
+                x[c][i] = __builtin_bit_cast(float, f);
+            }
+    }
+}
+// The power of two that brings a head's largest value to [2^13, 2^14) (none for 0, infinities and NaN; of values below
+// 2^-87 no more than 2^100, so that it stays a number).
+__device__ __forceinline__ int vx_to_2_14(float big) {
+    return big > 0.0f && big < INFINITY ? min(14 - __builtin_amdgcn_frexp_expf(big), 100) : 0;
+}
+// Four values side by side, each rounded once, at any alignment.
+__device__ __forceinline__ void vx_store4(void* p, size_t i, uint32_t dtype, vx_f4 v) {
+    if (dtype == VELOX_DT_F32) {
+        __builtin_memcpy((float*)p + i, &v, 16);
+    } else if (dtype == VELOX_DT_F16) {
+        const _Float16 h[4] = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+        __builtin_memcpy((uint16_t*)p + i, h, 8);
+    } else {
+        const __bf16 h[4] = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        __builtin_memcpy((uint16_t*)p + i, h, 8);
+    }
+}
 
 // The cache's element type: eight of them are an MFMA operand.
 struct VxBf16 {
@@ -88,7 +130,7 @@ __device__ __forceinline__ uint32_t vx_chunk_base(const VxChunks& c, uint32_t i)
 // tiles); its waves take the split's chunks in turn and meet in LDS. A wave holds one chunk's K and V (16 KB at
 // head size 128) in registers while the next one's are on their way. q of another type than the cache's enters as
 // QT terms of the cache's type whose sum keeps fp32's precision (three of bf16; two of fp16, of which each
-// head's largest value is brought to 2^14 first, so that the second term stays in range), the weights as PT.
+// head's largest value is brought to 2^13 first, so that the second term stays in range), the weights as PT.
 // Non-temporal loads (NT) where the caches cannot hold the K and V anyway: Llama-3-8B's heads, 4 sequences of 91000 to
 // 131000 positions 330 -> 292 us (5.9 -> 6.7 TB/s); 32 sequences of Qwen2.5-7B (90 MB, in the memory-side cache from
 // one call to the next) 21.8 us without, 23.6 with.
@@ -112,7 +154,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
     const uint32_t kvh = blockIdx.y / ng, g0 = blockIdx.y % ng * 16, gn = min(16u, G - g0);
     const uint32_t seq = blockIdx.z, split = blockIdx.x, h0 = kvh * G + g0;
     // q: column col is head h0 + col. The requests go out first; the first chunk's follow before q is widened.
-    VxEight raw[NC];
+    VxEight raw[NC] = {};
     if (col < gn) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) raw[c].read(a.q.data, (size_t)seq * a.q.rs + (size_t)(h0 + col) * a.q.hs + 32 * c + 8 * grp, a.q.dtype);
@@ -165,18 +207,16 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
     float to_log2 = a.scale * kLog2e;
     {
         float x[NC][8];
-        float big = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[c][i] = col < gn ? raw[c].at(i, a.q.dtype) : 0.0f;
-                big = fmaxf(big, fabsf(x[c][i]));
-            }
+        vx_widen(raw, a.q.dtype, x);
         if constexpr (QT == 2) {
+            float big = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[c][i]));
             big = fmaxf(big, __shfl_xor(big, 16));
             big = fmaxf(big, __shfl_xor(big, 32));
-            const int e = big > 0.0f && big < INFINITY ? 14 - ilogbf(big) : 0;
+            const int e = vx_to_2_14(big);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -495,7 +535,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     const int last_t = position(r1 - 1);
 
     // q is requested before the table and the first K, and brought into its operands behind them
-    VxEight raw[NK];
+    VxEight raw[NK] = {};
     if (mine) {
 #pragma unroll
         for (int c = 0; c < NK; ++c) raw[c].read(a.q.data, (size_t)row * a.q.rs + (size_t)head * a.q.hs + 16 * c + 8 * grp, a.q.dtype);
@@ -567,31 +607,27 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
         if constexpr (QT == 1) {  // the cache's type: as it lies
             const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
-            for (int c = 0; c < NK; ++c) qf[0][c] = mine ? __builtin_bit_cast(v8, raw[c].w[0] ^ sign) : v8{};
+            for (int c = 0; c < NK; ++c) qf[0][c] = __builtin_bit_cast(v8, raw[c].w[0] ^ sign);
         } else {
-            float x[NK][8], big = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NK; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = mine ? raw[c].at(i, a.q.dtype) : 0.0f;
-                    x[c][i] = a.scale < 0.0f ? -v : v;
-                    big = fmaxf(big, fabsf(v));
-                }
+            float x[NK][8];
+            vx_widen(raw, a.q.dtype, x);
+            float by = a.scale < 0.0f ? -1.0f : 1.0f;
             if constexpr (QT == 2) {
-                big = vx_max_pair(big);
-                const int e = big > 0.0f && big < INFINITY ? 14 - ilogbf(big) : 0;
+                float big = 0.0f;
 #pragma unroll
                 for (int c = 0; c < NK; ++c)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[c][i] = ldexpf(x[c][i], e);
+                    for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[c][i]));
+                big = vx_max_pair(big);
+                const int e = vx_to_2_14(big);
+                by = ldexpf(by, e);
                 to_log2 = ldexpf(to_log2, -e);
             }
 #pragma unroll
             for (int c = 0; c < NK; ++c)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float rest = x[c][i];
+                    float rest = x[c][i] * by;
 #pragma unroll
                     for (int u = 0; u < QT; ++u) {
                         const typename E::elt v = (typename E::elt)rest;
@@ -800,8 +836,9 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
 #pragma unroll
         for (int n = 0; n < NM; ++n)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                vx_store(a.out.data, to + 32 * n + 8 * (r >> 2) + 4 * grp + (r & 3), a.out.dtype, l != 0.0f ? o[n][r] * inv : 0.0f);
+            for (int q = 0; q < 4; ++q)
+                vx_store4(a.out.data, to + 32 * n + 8 * q + 4 * grp, a.out.dtype,
+                          vx_f4{o[n][4 * q], o[n][4 * q + 1], o[n][4 * q + 2], o[n][4 * q + 3]} * inv);
     } else {
         const size_t part = ((size_t)row * a.q.heads + head) * a.splits + blockIdx.y;
 #pragma unroll
