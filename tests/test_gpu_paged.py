@@ -227,6 +227,42 @@ def test_prompt_rows_in_front_of_position_0_stay():
     f.check(x[6:], out[6:], 0, 6, 0, 0, True)
 
 
+@pytest.mark.parametrize("q,kv", [("bf16", "bf16"), ("f32", "bf16"), ("f16", "f16"), ("f32", "f16")])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_rows_do_not_see_what_later_or_left_positions_hold(q, kv, value):
+    """A K or V value that is no number reaches the rows that see its position and no others."""
+    d, window, sinks, n, rows = 64, 50, 2, 400, 300
+    for where in (1, 130, 199, 300, 399):
+        f = Filled([n], 1, d, 64, kv)
+        cell = f.pool[0, int(f.table[0, where // 64])]
+        v = cell[64 * d:].view(2, d, 32)
+        v[where % 64 // 32, 5, int(SLOT[where % 32])] = value
+        x = queries(rows, 3, 1, d, q)
+        t = torch.arange(n - rows, n, device="cuda")
+        sees = (t >= where) & ((t < where + window) | (where < sinks))
+        out = paged.prompt_attention(f.cache, 0, x, ints([0, rows]), window=window, sinks=sinks)
+        # the seeing rows get no number: infinity, or NaN where a weight is held in terms of both signs (p0 inf + p1 inf)
+        assert torch.equal(torch.isfinite(out[:, :, 5]), ~sees.view(-1, 1).expand(rows, 3))
+        keep = [e for e in range(d) if e != 5]
+        other = out.clone()
+        other[:, :, 5] = 0
+        f.v[0][:, 0, 5] = 0  # that dimension is looked at above
+        f.check(x, other, 0, 0, window, sinks, q == kv)
+        assert torch.isfinite(out[:, :, keep]).all()
+        one = paged.attention(f.cache, 0, x[-1:], window=window, sinks=sinks)
+        assert torch.isfinite(one[0, :, 5]).all() == (not bool(sees[-1])) and torch.isfinite(one[:, :, keep]).all()
+        f = Filled([n], 1, d, 64, kv)
+        cell = f.pool[0, int(f.table[0, where // 64])]
+        cell[:64 * d].view(64, d)[where % 64, 9] = value
+        out = paged.prompt_attention(f.cache, 0, x, ints([0, rows]), window=window, sinks=sinks)
+        assert torch.isfinite(out[~sees]).all()
+        for i in (~sees).nonzero().flatten()[::37].tolist():  # a few rows by themselves
+            g = Filled([n], 1, d, 64, kv)
+            g.lens[0] = n - rows + i + 1
+            g.k[0], g.v[0] = g.k[0][:g.lens[0]], g.v[0][:g.lens[0]]
+            g.check(x[i:i + 1], out[i:i + 1], 0, i, window, sinks, q == kv)
+
+
 def test_prompt_attention_many_sequences():
     """More sequences than a wave counts at once, most of them without rows."""
     lens = [(i * 13) % 70 for i in range(150)]

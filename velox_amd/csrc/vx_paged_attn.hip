@@ -86,6 +86,7 @@ __device__ __forceinline__ void vx_store4(void* p, size_t i, uint32_t dtype, vx_
 // The cache's element type: eight of them are an MFMA operand.
 struct VxBf16 {
     typedef __bf16 elt;
+    static constexpr uint32_t kExp = 0x7F80u, kOne = 0x0080u;  // the exponent's bits, and the lowest of them
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ float sum2(v2 a, float c) { return __builtin_amdgcn_fdot2_f32_bf16(a, v2{(__bf16)1.0f, (__bf16)1.0f}, c, false); }
@@ -94,6 +95,7 @@ struct VxBf16 {
 };
 struct VxF16 {
     typedef _Float16 elt;
+    static constexpr uint32_t kExp = 0x7C00u, kOne = 0x0400u;
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ float sum2(v2 a, float c) { return __builtin_amdgcn_fdot2(a, v2{(_Float16)1.0f, (_Float16)1.0f}, c, false); }
@@ -512,6 +514,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     constexpr uint32_t kUnits = kChunk / 1024u;                    // 1 KiB units of a chunk's K or V
     typedef typename E::v8 v8;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kBuf];  // K of two steps, V of two steps
+    __shared__ uint32_t s_found;  // settle: 1 + the first chunk of the last step with infinities or NaN, else 0
+    if (threadIdx.x == 0) s_found = 0;
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t col = lane & 31u, grp = lane >> 5;
     const uint32_t G = a.q.heads / a.c.hkv, kvh = blockIdx.x % a.c.hkv;
@@ -532,7 +536,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     const int sinks = (int)min(a.sinks, 0x7FFFFFFFu);
     // all pairs of the wave see [all_low, all_t]; none of the workgroup sees past last_t or, but for sinks, before ch.low
     const int all_t = position(min(r0 + 32 * wave, r1 - 1)), all_low = (int)vx_low(position(min(r0 + 32 * wave + 31, r1 - 1)), a.window);
-    const int last_t = position(r1 - 1);
+    const int first_t = position(r0), last_t = position(r1 - 1), last_low = (int)vx_low(last_t, a.window);
 
     // q is requested before the table and the first K, and brought into its operands behind them
     VxEight raw[NK] = {};
@@ -544,7 +548,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     // where the K of the next 64 chunks lies in the pool, one a lane, and which of them have a page (page 0 stands in
     // for the others, and for chunks past the last)
     uint32_t place_lo, place_hi;
-    uint64_t paged, partial, hidden;  // chunks with a page; that not all pairs of the wave see whole; with places no pair sees
+    // chunks with a page; that not all pairs of the wave, of the workgroup see whole; with places that no pair sees
+    uint64_t paged, partial, mixed, hidden;
     uint32_t first = 0;               // the step whose chunks are in lanes 0 and 1
     const auto look_up = [&](uint32_t step) {
         const uint32_t i = c0 + 2 * step + lane, base = vx_chunk_base(ch, i);
@@ -556,6 +561,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
         }
         const bool have = page < a.c.n_pages;
         partial = __ballot(!have || (int)base + 31 > all_t || (int)base < all_low);
+        mixed = __ballot(!have || (int)base + 31 > first_t || (int)base < last_low);
         hidden = __ballot(!have || (int)base + 31 > last_t || (int)base < (int)ch.low);
         const uint64_t at = (have ? (uint64_t)page * a.c.page_bytes : 0) + ((uint64_t)kvh * a.c.page_size + place) * (D * 2);
         place_lo = (uint32_t)at;
@@ -664,11 +670,12 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     // place of position p in the chunk at base: -1 in front of it, 32 or more behind it
     const auto place_in = [](int p, uint32_t base) { return max(-1, min(64, p - (int)base)); };
     struct Step {  // two chunks of the walk, a bit for each
-        uint32_t chunk, have, partial, hidden;
+        uint32_t chunk, have, partial, mixed, hidden;
     };
     const auto step_of = [&](uint32_t step) {
         const uint32_t at = 2 * (step - first);
-        return Step{c0 + 2 * step, (uint32_t)(paged >> at) & 3u, (uint32_t)(partial >> at) & 3u, (uint32_t)(hidden >> at) & 3u};
+        return Step{c0 + 2 * step, (uint32_t)(paged >> at) & 3u, (uint32_t)(partial >> at) & 3u, (uint32_t)(mixed >> at) & 3u,
+                    (uint32_t)(hidden >> at) & 3u};
     };
     // Hides what the mask hides, and moves the maximum where a score passes it by more than 8 (the weights may pass 1
     // by 2^8 until then: a bf16 or fp16 weight keeps its relative precision, and the rescaling is rare).
@@ -702,20 +709,35 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
             for (int n = 0; n < NM; ++n) o[n] *= f;
         }
     };
-    // Places of V that no pair sees may hold anything (0 times NaN is NaN): the workgroup zeroes them in LDS.
-    const auto clear = [&](const Step& x, uint32_t buf) {
+    // V of a step that not every pair of the workgroup sees whole. A weight of 0 does not keep a place out of the sums
+    // (0 times NaN is NaN), so places that no pair sees are zeroed in LDS, and infinities and NaN of the others too:
+    // the pairs that see those get them behind the walk.
+    const auto settle = [&](const Step& x, uint32_t buf) {
+        unsigned char* vb = lds + 4 * kChunk + buf * (2 * kChunk);
+        uint32_t found = 0;
         for (uint32_t i = threadIdx.x; i < 2 * D * 4; i += kPromptThreads) {
-            const uint32_t b = i / (D * 4), e = i / 4 % D, j = i % 4 ^ vx_v_swizzle(e);  // j: slots 8 j .. 8 j + 7 of row e
-            const uint32_t base = vx_chunk_base(ch, x.chunk + b);
-            const int pt = x.have >> b & 1u ? place_in(last_t, base) : -1, pl = place_in((int)ch.low, base), ps = place_in(sinks, base);
-            vx_u4* at = (vx_u4*)(lds + 4 * kChunk + buf * (2 * kChunk) + 16 * i);
+            vx_u4* at = (vx_u4*)(vb + 16 * i);
             vx_u4 v = *at;
+            if (x.hidden) {
+                const uint32_t b = i / (D * 4), e = i / 4 % D, j = i % 4 ^ vx_v_swizzle(e);  // j: slots 8 j .. 8 j + 7 of row e
+                const uint32_t base = vx_chunk_base(ch, x.chunk + b);
+                const int pt = x.have >> b & 1u ? place_in(last_t, base) : -1, pl = place_in((int)ch.low, base), ps = place_in(sinks, base);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int p = 16 * (k >> 2) + 4 * (int)j + (k & 3);
-                if ((p > pt) | ((p < pl) & (p >= ps))) v[k / 2] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
+                for (int k = 0; k < 8; ++k) {
+                    const int p = 16 * (k >> 2) + 4 * (int)j + (k & 3);
+                    if ((p > pt) | ((p < pl) & (p >= ps))) v[k / 2] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
+                }
+                *at = v;
             }
-            *at = v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) found |= (v[k] & (E::kExp | E::kExp << 16)) + (E::kOne | E::kOne << 16);  // all ones carry
+        }
+        if (found & 0x80008000u) s_found = x.chunk + 1;
+        vx_barrier();
+        if (*(volatile uint32_t*)&s_found != x.chunk + 1) return;
+        for (uint32_t i = threadIdx.x; i < 2 * D * 32; i += kPromptThreads) {
+            uint16_t* h = (uint16_t*)vb + i;
+            if ((*h & E::kExp) == E::kExp) *h = 0;
         }
         vx_barrier();
     };
@@ -777,7 +799,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
                 begin(i);
                 const uint8_t *from1 = source(i + 1), *from2 = source(i + 2);
                 const Step after = step_of(i + 2);
-                if (now.hidden) clear(now, buf);
+                if (now.mixed) settle(now, buf);
                 __builtin_amdgcn_s_setprio(1);  // before the other workgroup's waves that stage or take maxima: 479 -> 470 us
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
@@ -813,7 +835,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
                     load_k(from1, buf ^ 1, j);
                     load_v(from1, buf ^ 1, j);
                 }
-                if (now.hidden) clear(now, buf);
+                if (now.mixed) settle(now, buf);
                 scores(s[0], 0, buf);
                 scores(s[1], 1, buf);
                 bound(s, now);
@@ -825,6 +847,29 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
         vx_wait_loads<0>();  // nothing may land in LDS that is another workgroup's by then
     }
 
+    if (n_steps && *(volatile uint32_t*)&s_found) {  // infinities and NaN that settle took out, value by value from the pages
+#pragma unroll 1
+        for (uint32_t i = 0; i < n_steps; ++i) {
+            if (i == 0 || i - first >= 32) look_up(i);
+            const Step x = step_of(i);
+            if (!x.mixed) continue;
+#pragma unroll 1
+            for (int j = 0; j < 64; ++j) {
+                if (!(x.have >> j / 32 & 1u)) continue;
+                const int at = (int)(2 * (i - first)) + j / 32, p = (int)vx_chunk_base(ch, x.chunk + j / 32) + (j & 31);
+                const uint32_t lo32 = (uint32_t)__builtin_amdgcn_readlane((int)place_lo, at), hi32 = (uint32_t)__builtin_amdgcn_readlane((int)place_hi, at);
+                const uint16_t* v = (const uint16_t*)(a.c.pool + ((uint64_t)hi32 << 32 | lo32) + v_from_k) + vx_vslot(j & 31) + 4 * grp * 32;
+                if (p > t || (p < low && p >= sinks)) continue;
+#pragma unroll
+                for (int n = 0; n < NM; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const uint16_t h = v[(32 * n + 8 * (r >> 2) + (r & 3)) * 32];
+                        if ((h & E::kExp) == E::kExp) o[n][r] += (float)__builtin_bit_cast(typename E::elt, h);
+                    }
+            }
+        }
+    }
     l = vx_sum_pair(l);
     if (t < 0) {
         if (mine && a.splits > 1 && grp == 0) a.part_ml[2 * (((size_t)row * a.q.heads + head) * a.splits + blockIdx.y) + 1] = -1.0f;
