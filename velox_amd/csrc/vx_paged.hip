@@ -47,41 +47,49 @@ __device__ __forceinline__ uint32_t vx_units(const VxRopeTable& t, uint32_t d) {
     constexpr uint32_t V = VxVec<T>::V;
     return (t.interleaved ? t.rot : t.rot / 2) / V + (d - t.rot) / V;
 }
-// Unit u of the head at x turned by the row's cos / sin table cs, V values at a time given to put(first element,
-// values).
-template <class T, class Put>
-__device__ __forceinline__ void vx_turn_unit(const VxRopeTable& t, const T* x, uint32_t u, const float2* cs, Put put) {
-    constexpr uint32_t V = VxVec<T>::V;
-    const uint32_t half = t.rot / 2, pair_units = (t.interleaved ? t.rot : half) / V;
-    float y[V];
-    if (u >= pair_units) {
-        const uint32_t e = t.rot + (u - pair_units) * V;
-        const VxVec<T> a = *(const VxVec<T>*)(x + e);
-#pragma unroll
-        for (uint32_t i = 0; i < V; ++i) y[i] = (float)a.v[i];
-        put(e, y);
-    } else if (t.interleaved) {
-        const VxVec<T> a = *(const VxVec<T>*)(x + u * V);
-#pragma unroll
-        for (uint32_t i = 0; i < V; i += 2) {
-            const float2 r = vx_rotate((float)a.v[i], (float)a.v[i + 1], cs[u * (V / 2) + i / 2]);
-            y[i] = r.x;
-            y[i + 1] = r.y;
-        }
-        put(u * V, y);
-    } else {
-        const VxVec<T> a = *(const VxVec<T>*)(x + u * V), b = *(const VxVec<T>*)(x + half + u * V);
-        float z[V];
-#pragma unroll
-        for (uint32_t i = 0; i < V; ++i) {
-            const float2 r = vx_rotate((float)a.v[i], (float)b.v[i], cs[u * V + i]);
-            y[i] = r.x;
-            z[i] = r.y;
-        }
-        put(u * V, y);
-        put(half + u * V, z);
+// Unit u of a head: what load reads of the values at x, and turn hands on, turned by the row's cos / sin table cs, V
+// values at a time as put(first element, values).
+template <class T>
+struct VxUnit {
+    static constexpr uint32_t V = VxVec<T>::V;
+    VxVec<T> a, b;  // b: the second half's values of half-layout pairs
+    __device__ __forceinline__ void load(const VxRopeTable& t, const T* x, uint32_t u) {
+        const uint32_t half = t.rot / 2, pair_units = (t.interleaved ? t.rot : half) / V;
+        const uint32_t e = u < pair_units ? u * V : t.rot + (u - pair_units) * V;
+        a = *(const VxVec<T>*)(x + e);
+        if (!t.interleaved && u < pair_units) b = *(const VxVec<T>*)(x + half + e);
     }
-}
+    template <class Put>
+    __device__ __forceinline__ void turn(const VxRopeTable& t, uint32_t u, const float2* cs, Put put) const {
+        const uint32_t half = t.rot / 2, pair_units = (t.interleaved ? t.rot : half) / V;
+        float y[V];
+        if (u >= pair_units) {
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) y[i] = (float)a.v[i];
+            put(t.rot + (u - pair_units) * V, y);
+        } else if (t.interleaved) {
+#pragma unroll
+            for (uint32_t i = 0; i < V; i += 2) {
+                const float2 r = vx_rotate((float)a.v[i], (float)a.v[i + 1], cs[u * (V / 2) + i / 2]);
+                y[i] = r.x;
+                y[i + 1] = r.y;
+            }
+            put(u * V, y);
+        } else {
+            float z[V];
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) {
+                const float2 r = vx_rotate((float)a.v[i], (float)b.v[i], cs[u * V + i]);
+                y[i] = r.x;
+                z[i] = r.y;
+            }
+            put(u * V, y);
+            put(half + u * V, z);
+        }
+    }
+};
+constexpr int kUnitsAhead = 4;  // units a thread requests before it turns the first
+
 template <class O, int V>
 __device__ __forceinline__ void vx_put(O* to, const float* y) {
     struct alignas(V * sizeof(O)) Out {
@@ -102,25 +110,31 @@ __global__ __launch_bounds__(kRopeThreads) void vx_rope_vec_kernel(VxRopeTable t
     constexpr int V = VxVec<T>::V;
     __shared__ float2 cs[kRopeThreads > 2 * kVxMaxRopePairs ? kRopeThreads : 2 * kVxMaxRopePairs];
     const uint32_t half = t.rot / 2, row0 = blockIdx.x * per, n = min(per, n_rows - row0);  // n * half <= 256
+    const uint32_t units = vx_units<T>(t, d), total = n * x.heads;
+    const uint32_t step = units < kRopeThreads ? kRopeThreads / units : 1;  // heads at a time; a thread keeps its unit
+    VxUnit<T> v[kUnitsAhead];
+    const auto load = [&](uint32_t u, uint32_t i) {
+#pragma unroll
+        for (int k = 0; k < kUnitsAhead; ++k) {
+            const uint32_t j = i + k * step, w = j / x.heads, h = j % x.heads;
+            if (j < total) v[k].load(t, (const T*)x.data + (size_t)(row0 + w) * x.rs + (size_t)h * x.hs, u);
+        }
+    };
+    const uint32_t u0 = threadIdx.x % units, i0 = threadIdx.x / units < step ? threadIdx.x / units : total;
+    load(u0, i0);  // on its way while the angles are formed
     for (uint32_t i = threadIdx.x; i < n * half; i += kRopeThreads) cs[i] = vx_turn(t, i % half, positions[row0 + i / half]);
     __syncthreads();
-    const uint32_t units = vx_units<T>(t, d), step = kRopeThreads / units;  // a thread keeps its unit
-    if (step) {
-        const uint32_t u = threadIdx.x % units;
-        if (threadIdx.x / units >= step) return;
-        for (uint32_t i = threadIdx.x / units; i < n * x.heads; i += step) {
-            const uint32_t w = i / x.heads, h = i % x.heads;
-            T* to = (T*)o.data + (size_t)(row0 + w) * o.rs + (size_t)h * o.hs;
-            vx_turn_unit<T>(t, (const T*)x.data + (size_t)(row0 + w) * x.rs + (size_t)h * x.hs, u, cs + w * half,
-                            [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
+    for (uint32_t u = u0; u < units; u += kRopeThreads) {  // (once, unless a head has more units than threads)
+        if (u != u0) load(u, i0);
+        for (uint32_t i = i0; i < total; i += kUnitsAhead * step) {
+            if (i != i0) load(u, i);
+#pragma unroll
+            for (int k = 0; k < kUnitsAhead; ++k) {
+                const uint32_t j = i + k * step, w = j / x.heads, h = j % x.heads;
+                T* to = (T*)o.data + (size_t)(row0 + w) * o.rs + (size_t)h * o.hs;
+                if (j < total) v[k].turn(t, u, cs + w * half, [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
+            }
         }
-        return;
-    }
-    for (uint32_t i = threadIdx.x; i < n * x.heads * units; i += kRopeThreads) {
-        const uint32_t w = i / units / x.heads, h = i / units % x.heads;
-        T* to = (T*)o.data + (size_t)(row0 + w) * o.rs + (size_t)h * o.hs;
-        vx_turn_unit<T>(t, (const T*)x.data + (size_t)(row0 + w) * x.rs + (size_t)h * x.hs, i % units, cs + w * half,
-                        [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
     }
 }
 
@@ -203,11 +217,11 @@ __device__ __forceinline__ bool vx_find_block(const VxAppendArgs& a, uint32_t it
 // ---- append: workgroups (x) take a 32-position block (a V block of the pages, up to 32 rows) of a sequence each;
 // y deals its heads ----
 struct VxBlock {
-    uint32_t row0, n, i0;  // rows row0 .. row0 + n at places i0 .. of the block
+    uint32_t row0, n, i0, pos;  // rows row0 .. row0 + n at places i0 .. of the block, positions pos ..
     uint32_t in_page;      // the block's place in its page
     uint16_t *k, *v;       // the page's K and V; NULL: no page
 };
-__device__ __forceinline__ bool vx_block(const VxRopeTable& t, const VxAppendArgs& a, VxBlock& b, float2 (*cs)[kVxMaxRopePairs / 2]) {
+__device__ __forceinline__ bool vx_block(const VxAppendArgs& a, VxBlock& b) {
     uint32_t seq, blk;
     if (!vx_find_block(a, blockIdx.x, seq, blk)) return false;
     const VxSpan r = vx_span(a.q_start, a.c.lens, a.n_rows, seq);
@@ -216,17 +230,22 @@ __device__ __forceinline__ bool vx_block(const VxRopeTable& t, const VxAppendArg
     b.i0 = (uint32_t)((from > p0 ? from : p0) - p0);
     b.n = (uint32_t)((end < p0 + 32 ? end : p0 + 32) - p0) - b.i0;
     b.row0 = r.lo + (uint32_t)(p0 + b.i0 - r.pos0);
-    const uint32_t half = t.rot / 2;
+    b.pos = (uint32_t)(p0 + b.i0);
     const uint64_t pi = (uint64_t)p0 / a.c.page_size;
     uint32_t page = kVxNoPage;
     if (pi < a.c.max_pages) page = a.c.table[(size_t)seq * a.c.table_stride + pi];
-    for (uint32_t i = threadIdx.x; i < b.n * half; i += 256) cs[i / half][i % half] = vx_turn(t, i % half, (uint32_t)(p0 + b.i0 + i / half));
     const bool have = page < a.c.n_pages;
     b.k = have ? (uint16_t*)(a.c.pool + (size_t)page * a.c.page_bytes) : nullptr;
     b.v = have ? b.k + (size_t)a.c.hkv * a.c.page_size * a.c.d : nullptr;
     b.in_page = (uint32_t)((uint64_t)p0 % a.c.page_size);
-    __syncthreads();
     return true;
+}
+// cos and sin of the block's rows w0 .. w1.
+__device__ __forceinline__ void vx_angles(const VxRopeTable& t, const VxBlock& b, uint32_t w0, uint32_t w1,
+                                          float2 (*cs)[kVxMaxRopePairs / 2]) {
+    const uint32_t half = t.rot / 2;
+    for (uint32_t i = threadIdx.x; i < (w1 - w0) * half; i += 256) cs[w0 + i / half][i % half] = vx_turn(t, i % half, b.pos + w0 + i / half);
+    __syncthreads();
 }
 
 // T: the rows' type, C: the cache's. K and q by units of 16 bytes; V by 8 dimensions of the 8 positions that share
@@ -236,23 +255,40 @@ __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxApp
     constexpr int V = VxVec<T>::V;
     __shared__ float2 cs[32][kVxMaxRopePairs / 2];
     VxBlock b;
-    if (!vx_block(t, a, b, cs)) return;
+    if (!vx_block(a, b)) return;
     const uint32_t d = a.c.d, hkv = a.c.hkv, hq = a.q.data ? a.q.heads : 0, heads = hq + hkv;
     const uint32_t units = vx_units<T>(t, d), step = 256 / units;  // d <= 128: at most 32 units
     const uint32_t u = threadIdx.x % units, mine = threadIdx.x / units;
-    if (mine < step)
-        for (uint32_t i = blockIdx.y * step + mine; i < b.n * heads; i += gridDim.y * step) {
-            const uint32_t w = i / heads, h = i % heads;
+    // the workgroups share the block's (row, head) pairs out in runs, so that each forms its own rows' angles only
+    const uint32_t all = b.n * heads, from = all * blockIdx.y / gridDim.y, total = all * (blockIdx.y + 1) / gridDim.y;
+    const uint32_t i0 = mine < step ? from + mine : total;
+    VxUnit<T> v[kUnitsAhead];
+    const auto load = [&](uint32_t i) {
+#pragma unroll
+        for (int k = 0; k < kUnitsAhead; ++k) {
+            const uint32_t j = i + k * step, w = j / heads, h = j % heads;
+            const T* x = h < hq ? (const T*)a.q.data + (size_t)(b.row0 + w) * a.q.rs + (size_t)h * a.q.hs
+                                : (const T*)a.k.data + (size_t)(b.row0 + w) * a.k.rs + (size_t)(h - hq) * a.k.hs;
+            if (j < total) v[k].load(t, x, u);
+        }
+    };
+    load(i0);  // on its way while the angles are formed
+    vx_angles(t, b, from / heads, (total + heads - 1) / heads, cs);
+    for (uint32_t i = i0; i < total; i += kUnitsAhead * step) {
+        if (i != i0) load(i);
+#pragma unroll
+        for (int k = 0; k < kUnitsAhead; ++k) {
+            const uint32_t j = i + k * step, w = j / heads, h = j % heads;
+            if (j >= total) continue;
             if (h < hq) {
                 T* to = (T*)a.qo.data + (size_t)(b.row0 + w) * a.qo.rs + (size_t)h * a.qo.hs;
-                vx_turn_unit<T>(t, (const T*)a.q.data + (size_t)(b.row0 + w) * a.q.rs + (size_t)h * a.q.hs, u, cs[w],
-                                [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
+                v[k].turn(t, u, cs[w], [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
             } else if (b.k) {
                 C* to = (C*)b.k + ((size_t)(h - hq) * a.c.page_size + b.in_page + b.i0 + w) * d;
-                vx_turn_unit<T>(t, (const T*)a.k.data + (size_t)(b.row0 + w) * a.k.rs + (size_t)(h - hq) * a.k.hs, u, cs[w],
-                                [&](uint32_t e, const float* y) { vx_put<C, V>(to + e, y); });
+                v[k].turn(t, u, cs[w], [&](uint32_t e, const float* y) { vx_put<C, V>(to + e, y); });
             }
         }
+    }
     if (!b.v) return;
     const uint32_t groups = d / 8;
     // from the last workgroup of the block on: the first ones have rows left over
@@ -299,7 +335,8 @@ __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxApp
 __global__ __launch_bounds__(256) void vx_append_rows_kernel(VxRopeTable t, VxAppendArgs a) {
     __shared__ float2 cs[32][kVxMaxRopePairs / 2];
     VxBlock b;
-    if (!vx_block(t, a, b, cs)) return;
+    if (!vx_block(a, b)) return;
+    vx_angles(t, b, 0, b.n, cs);
     const uint32_t half = t.rot / 2, d = a.c.d, hkv = a.c.hkv, hq = a.q.data ? a.q.heads : 0, heads = hq + 2 * hkv;
     const uint32_t units = half + (d - t.rot);
     for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < b.n * heads * units; i += gridDim.y * 256) {
@@ -654,9 +691,7 @@ hipError_t vx_launch_rope_append(const VxRopeTable& t, const VxAppendArgs& a, hi
     // a sequence's rows touch at most rows / 32 + 2 blocks
     const uint64_t bound = (uint64_t)a.n_rows / 32 + 2ull * a.c.n_seqs;
     const uint32_t blocks = (uint32_t)(bound < a.n_rows ? bound : a.n_rows);
-    // every workgroup of a block computes its angles again: no more of them than fill the GPU
-    const uint32_t y = blocks >= 512 ? 1 : blocks >= 256 ? 2 : blocks >= 128 ? 4 : 8;
-    const dim3 grid(blocks, y);
+    const dim3 grid(blocks, 8);
     const bool vec = (!a.q.data || (vx_vec_rows(a.q) && vx_vec_rows(a.qo) && a.q.dtype == a.k.dtype)) && vx_vec_rows(a.k) &&
                      vx_vec_rows(a.v) && a.k.dtype == a.v.dtype && vx_vec_pairs(t, a.k.dtype, a.c.d);
     if (!vec) vx_append_rows_kernel<<<grid, 256, 0, st>>>(t, a);
