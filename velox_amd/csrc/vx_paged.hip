@@ -42,6 +42,19 @@ struct alignas(16) VxVec {
     static constexpr int V = 16 / sizeof(T);
     T v[V];
 };
+// 16 bytes (or 8) with the non-temporal hint (NT) or without.
+template <bool NT, class V>
+__device__ __forceinline__ V vx_get(const V* p) {
+    typedef uint32_t W __attribute__((ext_vector_type(sizeof(V) / 4)));
+    if constexpr (NT) return __builtin_bit_cast(V, __builtin_nontemporal_load((const W*)p));
+    else return *p;
+}
+template <bool NT, class V>
+__device__ __forceinline__ void vx_set(V* p, const V& v) {
+    typedef uint32_t W __attribute__((ext_vector_type(sizeof(V) / 4)));
+    if constexpr (NT) __builtin_nontemporal_store(__builtin_bit_cast(W, v), (W*)p);
+    else *p = v;
+}
 template <class T>
 __device__ __forceinline__ uint32_t vx_units(const VxRopeTable& t, uint32_t d) {
     constexpr uint32_t V = VxVec<T>::V;
@@ -49,15 +62,15 @@ __device__ __forceinline__ uint32_t vx_units(const VxRopeTable& t, uint32_t d) {
 }
 // Unit u of a head: what load reads of the values at x, and turn hands on, turned by the row's cos / sin table cs, V
 // values at a time as put(first element, values).
-template <class T>
+template <class T, bool NT>
 struct VxUnit {
     static constexpr uint32_t V = VxVec<T>::V;
     VxVec<T> a, b;  // b: the second half's values of half-layout pairs
     __device__ __forceinline__ void load(const VxRopeTable& t, const T* x, uint32_t u) {
         const uint32_t half = t.rot / 2, pair_units = (t.interleaved ? t.rot : half) / V;
         const uint32_t e = u < pair_units ? u * V : t.rot + (u - pair_units) * V;
-        a = *(const VxVec<T>*)(x + e);
-        if (!t.interleaved && u < pair_units) b = *(const VxVec<T>*)(x + half + e);
+        a = vx_get<NT>((const VxVec<T>*)(x + e));
+        if (!t.interleaved && u < pair_units) b = vx_get<NT>((const VxVec<T>*)(x + half + e));
     }
     template <class Put>
     __device__ __forceinline__ void turn(const VxRopeTable& t, uint32_t u, const float2* cs, Put put) const {
@@ -90,21 +103,22 @@ struct VxUnit {
 };
 constexpr int kUnitsAhead = 4;  // units a thread requests before it turns the first
 
-template <class O, int V>
+template <bool NT, class O, int V>
 __device__ __forceinline__ void vx_put(O* to, const float* y) {
     struct alignas(V * sizeof(O)) Out {
         O v[V];
     } o;
 #pragma unroll
     for (int i = 0; i < V; ++i) o.v[i] = (O)y[i];
-    *(Out*)to = o;
+    vx_set<NT>((Out*)to, o);
 }
 
 // ---- rotation of rows: a workgroup takes kRows rows, whose cos / sin all heads share through LDS ----
-// Bound by its bytes: 4001 rows of 64 heads of 128 (fp16, 131 MB moved) take @@ us (@@ TB/s).
+// Bound by its bytes: 4001 rows of 64 heads of 128 (fp16, 131 MB moved, cold) take 24 us (5.4 TB/s; a copy of as much
+// 26 us).
 constexpr int kRopeThreads = 256;
 
-template <class T>
+template <class T, bool NT>
 __global__ __launch_bounds__(kRopeThreads) void vx_rope_vec_kernel(VxRopeTable t, VxRowsView x, VxRowsView o, uint32_t n_rows,
                                                                    uint32_t d, const uint32_t* __restrict__ positions, uint32_t per) {
     constexpr int V = VxVec<T>::V;
@@ -112,7 +126,7 @@ __global__ __launch_bounds__(kRopeThreads) void vx_rope_vec_kernel(VxRopeTable t
     const uint32_t half = t.rot / 2, row0 = blockIdx.x * per, n = min(per, n_rows - row0);  // n * half <= 256
     const uint32_t units = vx_units<T>(t, d), total = n * x.heads;
     const uint32_t step = units < kRopeThreads ? kRopeThreads / units : 1;  // heads at a time; a thread keeps its unit
-    VxUnit<T> v[kUnitsAhead];
+    VxUnit<T, false> v[kUnitsAhead];
     const auto load = [&](uint32_t u, uint32_t i) {
 #pragma unroll
         for (int k = 0; k < kUnitsAhead; ++k) {
@@ -132,7 +146,7 @@ __global__ __launch_bounds__(kRopeThreads) void vx_rope_vec_kernel(VxRopeTable t
             for (int k = 0; k < kUnitsAhead; ++k) {
                 const uint32_t j = i + k * step, w = j / x.heads, h = j % x.heads;
                 T* to = (T*)o.data + (size_t)(row0 + w) * o.rs + (size_t)h * o.hs;
-                if (j < total) v[k].turn(t, u, cs + w * half, [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
+                if (j < total) v[k].turn(t, u, cs + w * half, [&](uint32_t e, const float* y) { vx_put<NT, T, V>(to + e, y); });
             }
         }
     }
@@ -178,67 +192,69 @@ __device__ __forceinline__ VxSpan vx_span(const uint32_t* q_start, const uint32_
     return r;
 }
 
-// The sequence and index within it of 32-position block `item` of the batch, blocks counted over the sequences
-// in order; false behind the last. Every wave walks the sequences 64 at a time.
-__device__ __forceinline__ bool vx_find_block(const VxAppendArgs& a, uint32_t item, uint32_t& seq, uint32_t& blk) {
-    const uint32_t lane = threadIdx.x & 63u;
-    if (!a.q_start) {
-        seq = item;
-        blk = 0;
-        return a.c.lens[item] > 0;
-    }
-    uint32_t base = 0;
-    for (uint32_t s0 = 0; s0 < a.c.n_seqs; s0 += 64) {
-        const uint32_t s = s0 + lane;
-        uint32_t n = 0;
-        if (s < a.c.n_seqs) {
-            const VxSpan r = vx_span(a.q_start, a.c.lens, a.n_rows, s);
-            const int64_t end = r.pos0 + (r.hi - r.lo), from = r.pos0 > 0 ? r.pos0 : 0;
-            if (end > from) n = (uint32_t)(((end + 31) >> 5) - (from >> 5));
-        }
-        uint32_t upto = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t v = __shfl_up(upto, o);
-            if (lane >= (uint32_t)o) upto += v;
-        }
-        const uint64_t hit = __ballot(item < base + upto);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            seq = s0 + (uint32_t)l;
-            blk = item - base - (uint32_t)(__shfl(upto, l) - __shfl(n, l));
-            return true;
-        }
-        base += __shfl(upto, 63);
-    }
-    return false;
-}
-
 // ---- append: workgroups (x) take a 32-position block (a V block of the pages, up to 32 rows) of a sequence each;
 // y deals its heads ----
 struct VxBlock {
     uint32_t row0, n, i0, pos;  // rows row0 .. row0 + n at places i0 .. of the block, positions pos ..
-    uint32_t in_page;      // the block's place in its page
-    uint16_t *k, *v;       // the page's K and V; NULL: no page
+    uint32_t in_page, page;     // the block's place in its page; no page: >= n_pages
 };
-__device__ __forceinline__ bool vx_block(const VxAppendArgs& a, VxBlock& b) {
-    uint32_t seq, blk;
-    if (!vx_find_block(a, blockIdx.x, seq, blk)) return false;
-    const VxSpan r = vx_span(a.q_start, a.c.lens, a.n_rows, seq);
+// Block `item` of the batch, blocks counted over the sequences in order; false behind the last. Every wave walks the
+// sequences 64 at a time.
+__device__ __forceinline__ bool vx_block(const VxAppendArgs& a, uint32_t item, VxBlock& b) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t seq = item, blk = 0;
+    VxSpan r;
+    if (!a.q_start) {
+        r = vx_span(a.q_start, a.c.lens, a.n_rows, item);
+        if (r.pos0 < 0) return false;
+    } else {
+        uint32_t base = 0;
+        bool found = false;
+        for (uint32_t s0 = 0; s0 < a.c.n_seqs && !found; s0 += 64) {
+            const uint32_t s = s0 + lane;
+            uint32_t n = 0;
+            VxSpan mine = {0, 0, 0};
+            if (s < a.c.n_seqs) {
+                mine = vx_span(a.q_start, a.c.lens, a.n_rows, s);
+                const int64_t end = mine.pos0 + (mine.hi - mine.lo), from = mine.pos0 > 0 ? mine.pos0 : 0;
+                if (end > from) n = (uint32_t)(((end + 31) >> 5) - (from >> 5));
+            }
+            uint32_t upto = n;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t v = __shfl_up(upto, o);
+                if (lane >= (uint32_t)o) upto += v;
+            }
+            const uint64_t hit = __ballot(item < base + upto);
+            if (hit) {
+                const int l = __builtin_ctzll(hit);
+                const auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+                seq = s0 + (uint32_t)l;
+                blk = item - base - (of(upto) - of(n));
+                r.lo = of(mine.lo);
+                r.hi = of(mine.hi);
+                r.pos0 = (int64_t)((uint64_t)of((uint32_t)(mine.pos0 >> 32)) << 32 | of((uint32_t)mine.pos0));
+                found = true;
+            }
+            base += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        }
+        if (!found) return false;
+    }
     const int64_t from = r.pos0 > 0 ? r.pos0 : 0, end = r.pos0 + (r.hi - r.lo);
     const int64_t p0 = ((from >> 5) + blk) << 5;  // the block's first position
+    const uint64_t pi = (uint64_t)p0 / a.c.page_size;
+    b.page = kVxNoPage;
+    if (pi < a.c.max_pages) b.page = a.c.table[(size_t)seq * a.c.table_stride + pi];
     b.i0 = (uint32_t)((from > p0 ? from : p0) - p0);
     b.n = (uint32_t)((end < p0 + 32 ? end : p0 + 32) - p0) - b.i0;
     b.row0 = r.lo + (uint32_t)(p0 + b.i0 - r.pos0);
     b.pos = (uint32_t)(p0 + b.i0);
-    const uint64_t pi = (uint64_t)p0 / a.c.page_size;
-    uint32_t page = kVxNoPage;
-    if (pi < a.c.max_pages) page = a.c.table[(size_t)seq * a.c.table_stride + pi];
-    const bool have = page < a.c.n_pages;
-    b.k = have ? (uint16_t*)(a.c.pool + (size_t)page * a.c.page_bytes) : nullptr;
-    b.v = have ? b.k + (size_t)a.c.hkv * a.c.page_size * a.c.d : nullptr;
     b.in_page = (uint32_t)((uint64_t)p0 % a.c.page_size);
     return true;
+}
+// The block's page: its K, V behind; NULL: none.
+__device__ __forceinline__ uint16_t* vx_page(const VxAppendArgs& a, const VxBlock& b) {
+    return b.page < a.c.n_pages ? (uint16_t*)(a.c.pool + (size_t)b.page * a.c.page_bytes) : nullptr;
 }
 // cos and sin of the block's rows w0 .. w1.
 __device__ __forceinline__ void vx_angles(const VxRopeTable& t, const VxBlock& b, uint32_t w0, uint32_t w1,
@@ -250,19 +266,19 @@ __device__ __forceinline__ void vx_angles(const VxRopeTable& t, const VxBlock& b
 
 // T: the rows' type, C: the cache's. K and q by units of 16 bytes; V by 8 dimensions of the 8 positions that share
 // 16 bytes of a V block, transposed in registers, so that whole blocks leave as whole lines.
-template <class T, class C>
+template <class T, class C, bool NT>
 __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxAppendArgs a) {
     constexpr int V = VxVec<T>::V;
     __shared__ float2 cs[32][kVxMaxRopePairs / 2];
     VxBlock b;
-    if (!vx_block(a, b)) return;
+    if (!vx_block(a, blockIdx.x, b)) return;
     const uint32_t d = a.c.d, hkv = a.c.hkv, hq = a.q.data ? a.q.heads : 0, heads = hq + hkv;
     const uint32_t units = vx_units<T>(t, d), step = 256 / units;  // d <= 128: at most 32 units
     const uint32_t u = threadIdx.x % units, mine = threadIdx.x / units;
     // the workgroups share the block's (row, head) pairs out in runs, so that each forms its own rows' angles only
     const uint32_t all = b.n * heads, from = all * blockIdx.y / gridDim.y, total = all * (blockIdx.y + 1) / gridDim.y;
     const uint32_t i0 = mine < step ? from + mine : total;
-    VxUnit<T> v[kUnitsAhead];
+    VxUnit<T, NT> v[kUnitsAhead];
     const auto load = [&](uint32_t i) {
 #pragma unroll
         for (int k = 0; k < kUnitsAhead; ++k) {
@@ -274,6 +290,7 @@ __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxApp
     };
     load(i0);  // on its way while the angles are formed
     vx_angles(t, b, from / heads, (total + heads - 1) / heads, cs);
+    uint16_t* const page = vx_page(a, b);
     for (uint32_t i = i0; i < total; i += kUnitsAhead * step) {
         if (i != i0) load(i);
 #pragma unroll
@@ -282,17 +299,17 @@ __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxApp
             if (j >= total) continue;
             if (h < hq) {
                 T* to = (T*)a.qo.data + (size_t)(b.row0 + w) * a.qo.rs + (size_t)h * a.qo.hs;
-                v[k].turn(t, u, cs[w], [&](uint32_t e, const float* y) { vx_put<T, V>(to + e, y); });
-            } else if (b.k) {
-                C* to = (C*)b.k + ((size_t)(h - hq) * a.c.page_size + b.in_page + b.i0 + w) * d;
-                v[k].turn(t, u, cs[w], [&](uint32_t e, const float* y) { vx_put<C, V>(to + e, y); });
+                v[k].turn(t, u, cs[w], [&](uint32_t e, const float* y) { vx_put<NT, T, V>(to + e, y); });
+            } else if (page) {
+                C* to = (C*)page + ((size_t)(h - hq) * a.c.page_size + b.in_page + b.i0 + w) * d;
+                v[k].turn(t, u, cs[w], [&](uint32_t e, const float* y) { vx_put<NT, C, V>(to + e, y); });
             }
         }
     }
-    if (!b.v) return;
-    const uint32_t groups = d / 8;
-    // from the last workgroup of the block on: the first ones have rows left over
-    for (uint32_t i = (gridDim.y - 1 - blockIdx.y) * 256 + threadIdx.x; i < hkv * groups * 4; i += gridDim.y * 256) {
+    if (!page) return;
+    const uint32_t groups = d / 8, pieces = hkv * groups * 4;  // a head's pieces lie in one run: whole rows, whole blocks
+    const uint32_t v_to = pieces * (blockIdx.y + 1) / gridDim.y;
+    for (uint32_t i = pieces * blockIdx.y / gridDim.y + threadIdx.x; i < v_to; i += 256) {
         const uint32_t e0 = i % groups * 8, j = i / groups % 4, h = i / groups / 4;  // slots 8 j .. 8 j + 7 of 8 dimensions
         C x[8][8];
         uint32_t there = 0;
@@ -310,7 +327,7 @@ __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxApp
                 }
             }
         }
-        C* to = (C*)b.v + ((size_t)h * a.c.page_size + b.in_page) * d + e0 * 32 + 8 * j;
+        C* to = (C*)page + ((size_t)(hkv + h) * a.c.page_size + b.in_page) * d + e0 * 32 + 8 * j;
         if (there == 255u) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -335,8 +352,10 @@ __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxApp
 __global__ __launch_bounds__(256) void vx_append_rows_kernel(VxRopeTable t, VxAppendArgs a) {
     __shared__ float2 cs[32][kVxMaxRopePairs / 2];
     VxBlock b;
-    if (!vx_block(a, b)) return;
+    if (!vx_block(a, blockIdx.x, b)) return;
     vx_angles(t, b, 0, b.n, cs);
+    uint16_t* const kp = vx_page(a, b);
+    uint16_t* const vp = kp + (size_t)a.c.hkv * a.c.page_size * a.c.d;
     const uint32_t half = t.rot / 2, d = a.c.d, hkv = a.c.hkv, hq = a.q.data ? a.q.heads : 0, heads = hq + 2 * hkv;
     const uint32_t units = half + (d - t.rot);
     for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < b.n * heads * units; i += gridDim.y * 256) {
@@ -357,12 +376,12 @@ __global__ __launch_bounds__(256) void vx_append_rows_kernel(VxRopeTable t, VxAp
             const size_t ob = (size_t)(b.row0 + w) * a.qo.rs + (size_t)hh * a.qo.hs;
             vx_store(a.qo.data, ob + e0, a.qo.dtype, y0);
             if (pair) vx_store(a.qo.data, ob + e1, a.qo.dtype, y1);
-        } else if (b.k && h < hq + hkv) {
-            uint16_t* to = b.k + ((size_t)hh * a.c.page_size + b.in_page + b.i0 + w) * d;
+        } else if (kp && h < hq + hkv) {
+            uint16_t* to = kp + ((size_t)hh * a.c.page_size + b.in_page + b.i0 + w) * d;
             vx_store(to, e0, a.c.dtype, y0);
             if (pair) vx_store(to, e1, a.c.dtype, y1);
-        } else if (b.k) {
-            uint16_t* to = b.v + ((size_t)hh * (a.c.page_size / 32) + b.in_page / 32) * d * 32;
+        } else if (kp) {
+            uint16_t* to = vp + ((size_t)hh * (a.c.page_size / 32) + b.in_page / 32) * d * 32;
             const uint32_t slot = vx_vslot(b.i0 + w);
             vx_store(to, (size_t)e0 * 32 + slot, a.c.dtype, y0);
             if (pair) vx_store(to, (size_t)e1 * 32 + slot, a.c.dtype, y1);
@@ -656,6 +675,11 @@ uint32_t copy_grid(const VxPages& p, uint64_t moves) {
 
 }  // namespace
 
+// Rows of more bytes than the XCDs' L2 caches hold go past them (non-temporal): what reads them next finds them in
+// memory anyway. 4001 rows of 64 heads of 128 (fp16, 131 MB moved, cold) 31.1 -> 24.3 us by non-temporal stores
+// (loads made it 30.9); 8300 rows of Llama-3-8B's q, k and v (204 MB) 63 -> 47 us by both.
+static constexpr uint64_t kStreamBytes = 32ull << 20;
+
 // Whether 16-byte loads and stores fit rows of type elements.
 static bool vx_vec_rows(const VxRowsView& r) {
     const uint32_t v = r.dtype == VELOX_DT_F32 ? 4 : 8;
@@ -672,9 +696,11 @@ hipError_t vx_launch_rope_rows(const VxRopeTable& t, const VxRowsView& x, const 
         // a thread for every angle where the rows fill the GPU several times over, one row a workgroup below
         const uint32_t most = 2 * kRopeThreads / t.rot, share = n_rows / 1024, per = share < 1 ? 1 : share < most ? share : most;
         const uint32_t grid = (n_rows + per - 1) / per;
-        if (x.dtype == VELOX_DT_F32) vx_rope_vec_kernel<float><<<grid, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions, per);
-        else if (x.dtype == VELOX_DT_F16) vx_rope_vec_kernel<_Float16><<<grid, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions, per);
-        else vx_rope_vec_kernel<__bf16><<<grid, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions, per);
+        const bool nt = (uint64_t)n_rows * x.heads * d * (x.dtype == VELOX_DT_F32 ? 4 : 2) > kStreamBytes;
+        const auto go = [&](auto kernel) { kernel<<<grid, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions, per); };
+        if (x.dtype == VELOX_DT_F32) go(nt ? vx_rope_vec_kernel<float, true> : vx_rope_vec_kernel<float, false>);
+        else if (x.dtype == VELOX_DT_F16) go(nt ? vx_rope_vec_kernel<_Float16, true> : vx_rope_vec_kernel<_Float16, false>);
+        else go(nt ? vx_rope_vec_kernel<__bf16, true> : vx_rope_vec_kernel<__bf16, false>);
     } else {
         vx_rope_rows_kernel<<<n_rows, kRopeThreads, 0, st>>>(t, x, out, n_rows, d, positions);
     }
@@ -683,8 +709,10 @@ hipError_t vx_launch_rope_rows(const VxRopeTable& t, const VxRowsView& x, const 
 
 template <class T>
 static void vx_append_vec(const VxRopeTable& t, const VxAppendArgs& a, dim3 grid, hipStream_t st) {
-    if (a.c.dtype == VELOX_DT_F16) vx_append_vec_kernel<T, _Float16><<<grid, 256, 0, st>>>(t, a);
-    else vx_append_vec_kernel<T, __bf16><<<grid, 256, 0, st>>>(t, a);
+    const bool nt = (uint64_t)a.n_rows * ((a.q.data ? a.q.heads : 0) + 2 * a.c.hkv) * a.c.d * sizeof(T) > kStreamBytes;
+    const auto go = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(t, a); };
+    if (a.c.dtype == VELOX_DT_F16) go(nt ? vx_append_vec_kernel<T, _Float16, true> : vx_append_vec_kernel<T, _Float16, false>);
+    else go(nt ? vx_append_vec_kernel<T, __bf16, true> : vx_append_vec_kernel<T, __bf16, false>);
 }
 
 hipError_t vx_launch_rope_append(const VxRopeTable& t, const VxAppendArgs& a, hipStream_t st) {
