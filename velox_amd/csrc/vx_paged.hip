@@ -424,57 +424,100 @@ __global__ void vx_pages_reset_kernel(VxPages p) {
     for (size_t i = i0; i < kVxPagesHead; i += step) p.scratch[i] = 0;
 }
 
-// One workgroup: who needs what (a thread per sequence), the lowest free pages (a scan of refs that ends when
-// it has enough), then a thread per page given out.
+// Which of the eight pages from `first` on are free, as bits; the loads are in flight until used.
+struct VxRefs8 {
+    uint4 r[2];
+    uint32_t n;  // pages there are
+    __device__ __forceinline__ void load(const VxPages& p, uint32_t first) {
+        n = first < p.n_pages ? min(8u, p.n_pages - first) : 0u;
+        if (n == 8) {
+            r[0] = *(const uint4*)(p.refs + first);
+            r[1] = *(const uint4*)(p.refs + first + 4);
+        } else {
+            uint32_t* w = (uint32_t*)r;
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) w[k] = k < n ? p.refs[first + k] : 1u;
+        }
+    }
+    __device__ __forceinline__ uint32_t free() const {
+        return (uint32_t)(r[0].x == 0) | (uint32_t)(r[0].y == 0) << 1 | (uint32_t)(r[0].z == 0) << 2 | (uint32_t)(r[0].w == 0) << 3 |
+               (uint32_t)(r[1].x == 0) << 4 | (uint32_t)(r[1].y == 0) << 5 | (uint32_t)(r[1].z == 0) << 6 | (uint32_t)(r[1].w == 0) << 7;
+    }
+};
+
+// One workgroup: who needs what (a thread per sequence, or four), the lowest free pages (a scan of refs that ends
+// when it has enough), then a thread per page given out. What bounds it is the chain of dependent loads -- length,
+// last page, its count -- and a dozen barriers: 64 sequences and 1000 pages take 7 us, so the scan's first pages are
+// requested at the start, and the pages found stay in LDS.
+constexpr uint32_t kPerThread = kVxMaxPagedSeqs / kPageThreads;
+constexpr uint32_t kListed = 4096;  // pages found that LDS holds; the rest lie in the scratch memory
+
 __global__ __launch_bounds__(kPageThreads) void vx_pages_extend_kernel(VxPages p, const uint32_t* __restrict__ add) {
     __shared__ uint32_t s_upto[kVxMaxPagedSeqs];  // pages given to sequences up to this one, itself included
     __shared__ uint32_t s_old[kVxMaxPagedSeqs];   // pages it had; bit 31: its last one is copied
     __shared__ uint32_t s_spot[kVxMaxPagedSeqs];  // the shared last page it would write
+    __shared__ uint32_t s_list[kListed];
     __shared__ uint32_t s_moves, s_granted, s_refused;
     const uint32_t tid = threadIdx.x, n = p.n_seqs, per = (n + kPageThreads - 1) / kPageThreads;
     const uint32_t a0 = min(tid * per, n), a1 = min(a0 + per, n);
     uint32_t* src = p.scratch + kVxPagesHead;
     uint32_t* dst = src + vx_pages_moves(p.n_seqs, p.n_pages);
     uint32_t* list = dst + vx_pages_moves(p.n_seqs, p.n_pages);
+    VxRefs8 refs;
+    refs.load(p, tid * 8);
+    uint32_t len[kPerThread], grow[kPerThread], refs_of[kPerThread];
+#pragma unroll
+    for (uint32_t k = 0; k < kPerThread; ++k) {
+        const bool is = a0 + k < a1;
+        len[k] = is ? p.lens[a0 + k] : 0u;
+        grow[k] = is ? add[a0 + k] : 0u;
+    }
     if (tid == 0) s_moves = s_granted = s_refused = 0;
-    const auto pages_of = [&](uint64_t len) { return (len + p.page_size - 1) / p.page_size; };
-    const auto fits_in = [&](uint64_t len, uint64_t grow) {
-        return grow && pages_of(len + grow) <= p.max_pages && len + grow < 0x80000000ull;
-    };
+    const auto pages_of = [&](uint64_t x) { return (uint32_t)((x + p.page_size - 1) / p.page_size); };
+    uint32_t fits = 0;
     int any = 0;
-    for (uint32_t s = a0; s < a1; ++s) {
-        const uint64_t len = p.lens[s], grow = add[s], old = pages_of(len);
-        const bool fits = fits_in(len, grow);
+#pragma unroll
+    for (uint32_t k = 0; k < kPerThread; ++k) {
+        const uint32_t s = a0 + k;
+        refs_of[k] = 0;
+        if (s >= a1) continue;
+        const uint64_t now = (uint64_t)len[k] + grow[k];
+        const bool ok = grow[k] && now < 0x80000000ull && (now + p.page_size - 1) / p.page_size <= p.max_pages;
+        const uint32_t old = ok ? pages_of(len[k]) : 0u;
         uint32_t spot = kVxNoPage;
-        if (fits && len % p.page_size) {
+        if (ok && len[k] % p.page_size) {
             const uint32_t last = p.table[(size_t)s * p.table_stride + old - 1];
-            if (last < p.n_pages && p.refs[last] > 1) spot = last;
+            if (last < p.n_pages) refs_of[k] = p.refs[last];
+            if (refs_of[k] > 1) spot = last;
         }
         s_spot[s] = spot;
-        s_old[s] = (uint32_t)(fits ? old : 0);
+        s_old[s] = old;
+        fits |= (uint32_t)ok << k;
         any |= spot != kVxNoPage;
     }
     any = __syncthreads_or(any);
     uint32_t mine = 0;
-    for (uint32_t s = a0; s < a1; ++s) {
-        const uint64_t len = p.lens[s], grow = add[s];
-        const bool fits = fits_in(len, grow);
-        uint32_t need = fits ? (uint32_t)(pages_of(len + grow) - pages_of(len)) : 0;
-        const uint32_t spot = any ? s_spot[s] : kVxNoPage;
-        if (spot != kVxNoPage) {
-            uint32_t same = 0;
-            bool later = false;
-            for (uint32_t j = 0; j < n; ++j) {
-                const bool eq = s_spot[j] == spot;
-                same += eq;
-                later |= eq && j > s;
-            }
-            if (later || same != p.refs[spot]) {  // else it is the last of all its holders and keeps the page
-                s_old[s] |= 0x80000000u;
-                ++need;
+#pragma unroll
+    for (uint32_t k = 0; k < kPerThread; ++k) {
+        const uint32_t s = a0 + k;
+        if (s >= a1) continue;
+        if (fits >> k & 1) {
+            mine += pages_of((uint64_t)len[k] + grow[k]) - pages_of(len[k]);
+            const uint32_t spot = s_spot[s];
+            if (any && spot != kVxNoPage) {
+                uint32_t same = 0;
+                bool later = false;
+                for (uint32_t j = 0; j < n; ++j) {
+                    const bool eq = s_spot[j] == spot;
+                    same += eq;
+                    later |= eq && j > s;
+                }
+                if (later || same != refs_of[k]) {  // else it is the last of all its holders and keeps the page
+                    s_old[s] |= 0x80000000u;
+                    ++mine;
+                }
             }
         }
-        mine += need;
         s_upto[s] = mine;  // within this thread's sequences, for now
     }
     uint32_t total;
@@ -483,34 +526,35 @@ __global__ __launch_bounds__(kPageThreads) void vx_pages_extend_kernel(VxPages p
     // the lowest free pages
     uint32_t found = 0;
     for (uint32_t base = 0; base < p.n_pages && found < total; base += kPageThreads * 8) {
-        uint32_t free = 0;
-        const uint32_t first = base + tid * 8;
-        for (uint32_t k = 0; k < 8 && first + k < p.n_pages; ++k) free |= (p.refs[first + k] == 0) << k;
-        uint32_t got;
+        if (base) refs.load(p, base + tid * 8);
+        uint32_t free = refs.free(), got;
         uint32_t rank = found + vx_scan(__popc(free), got);
-        for (; free; free &= free - 1, ++rank)
-            if (rank < total) list[rank] = first + __builtin_ctz(free);
+        for (; free; free &= free - 1, ++rank) {
+            if (rank >= total) break;
+            const uint32_t page = base + tid * 8 + __builtin_ctz(free);
+            if (rank < kListed) s_list[rank] = page;
+            else list[rank] = page;
+        }
         found += got;
     }
     __syncthreads();
+    const auto listed = [&](uint32_t rank) { return rank < kListed ? s_list[rank] : list[rank]; };
     // sequences in order until the pages run out; the refused are then the last that extend
-    for (uint32_t s = a0; s < a1; ++s) {
-        const uint64_t len = p.lens[s], grow = add[s];
-        if (!grow) continue;
-        const bool fits = pages_of(len + grow) <= p.max_pages;
-        if (!fits || s_upto[s] > found) {
+#pragma unroll
+    for (uint32_t k = 0; k < kPerThread; ++k) {
+        const uint32_t s = a0 + k;
+        if (s >= a1 || !grow[k]) continue;
+        if (!(fits >> k & 1) || s_upto[s] > found) {
             atomicAdd(&s_refused, 1u);
             continue;
         }
         atomicMax(&s_granted, s_upto[s]);
-        p.lens[s] = (uint32_t)(len + grow);
+        p.lens[s] = len[k] + grow[k];
         if (s_old[s] >> 31) {
-            const uint32_t old = s_old[s] & 0x7FFFFFFFu, from = s_spot[s];
-            const uint32_t to = list[s ? s_upto[s - 1] : 0u];
-            const uint32_t m = atomicAdd(&s_moves, 1u);
+            const uint32_t from = s_spot[s], to = listed(s ? s_upto[s - 1] : 0u), m = atomicAdd(&s_moves, 1u);
             src[m] = from;
             dst[m] = to;
-            p.table[(size_t)s * p.table_stride + old - 1] = to;
+            p.table[(size_t)s * p.table_stride + (s_old[s] & 0x7FFFFFFFu) - 1] = to;
             p.refs[to] = 1;
             atomicSub(&p.refs[from], 1u);
         }
@@ -525,8 +569,9 @@ __global__ __launch_bounds__(kPageThreads) void vx_pages_extend_kernel(VxPages p
         }
         const uint32_t copied = s_old[lo] >> 31, k = r - (lo ? s_upto[lo - 1] : 0u);
         if (k < copied) continue;  // written above
-        p.table[(size_t)lo * p.table_stride + (s_old[lo] & 0x7FFFFFFFu) + k - copied] = list[r];
-        p.refs[list[r]] = 1;
+        const uint32_t page = listed(r);
+        p.table[(size_t)lo * p.table_stride + (s_old[lo] & 0x7FFFFFFFu) + k - copied] = page;
+        p.refs[page] = 1;
     }
     if (tid == 0) {
         p.scratch[0] = s_refused;
@@ -555,29 +600,31 @@ __global__ __launch_bounds__(256) void vx_pages_copy_kernel(VxPages p) { vx_copy
 
 // A workgroup takes a few columns of the table: all its entries are read into LDS before one is written, so
 // that every sequence takes its parent's old pages whatever the order. References change by the difference;
-// the sums do not depend on the order of the atomics. Workgroup 0 does the lengths.
+// the sums do not depend on the order of the atomics. The last workgroup does the lengths.
 constexpr uint32_t kForkWords = 16384;
-__global__ __launch_bounds__(256) void vx_pages_fork_kernel(VxPages p, const uint32_t* __restrict__ from, uint32_t cols) {
+constexpr int kForkThreads = 512;
+__global__ __launch_bounds__(kForkThreads) void vx_pages_fork_kernel(VxPages p, const uint32_t* __restrict__ from, uint32_t cols) {
     __shared__ uint32_t old[kForkWords];
-    const uint32_t n = p.n_seqs, c0 = blockIdx.x * cols, nc = min(cols, p.max_pages - c0);
-    for (uint32_t i = threadIdx.x; i < n * nc; i += 256) old[i] = p.table[(size_t)(i / nc) * p.table_stride + c0 + i % nc];
+    const uint32_t n = p.n_seqs;
+    if (blockIdx.x == gridDim.x - 1) {
+        for (uint32_t s = threadIdx.x; s < n; s += kForkThreads) old[s] = p.lens[s];
+        __syncthreads();
+        for (uint32_t s = threadIdx.x; s < n; s += kForkThreads) {
+            const uint32_t f = from[s], len = f < n ? old[f] : 0u;
+            if (len != old[s]) p.lens[s] = len;
+        }
+        return;
+    }
+    const uint32_t c0 = blockIdx.x * cols, nc = min(cols, p.max_pages - c0);
+    for (uint32_t i = threadIdx.x; i < n * nc; i += kForkThreads) old[i] = p.table[(size_t)(i / nc) * p.table_stride + c0 + i % nc];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n * nc; i += 256) {
+    for (uint32_t i = threadIdx.x; i < n * nc; i += kForkThreads) {
         const uint32_t s = i / nc, c = i % nc, f = from[s];
         const uint32_t was = old[i], now = f < n ? old[f * nc + c] : kVxNoPage;
         if (was == now) continue;
         p.table[(size_t)s * p.table_stride + c0 + c] = now;
         if (now < p.n_pages) atomicAdd(&p.refs[now], 1u);
         if (was < p.n_pages) atomicSub(&p.refs[was], 1u);
-    }
-    if (blockIdx.x == 0) {
-        __syncthreads();
-        for (uint32_t s = threadIdx.x; s < n; s += 256) old[s] = p.lens[s];
-        __syncthreads();
-        for (uint32_t s = threadIdx.x; s < n; s += 256) {
-            const uint32_t f = from[s], len = f < n ? old[f] : 0u;
-            if (len != old[s]) p.lens[s] = len;
-        }
     }
 }
 
@@ -619,18 +666,20 @@ __global__ __launch_bounds__(kPageThreads) void vx_pages_plan_kernel(VxPages p) 
     uint32_t* dst = src + vx_pages_moves(p.n_seqs, p.n_pages);
     uint32_t* map = dst + vx_pages_moves(p.n_seqs, p.n_pages);
     uint32_t live = 0, total;
-    for (uint32_t i = tid; i < p.n_pages; i += kPageThreads) live += p.refs[i] != 0;
+    VxRefs8 refs;
+    for (uint32_t base = 0; base < p.n_pages; base += kPageThreads * 8) {
+        refs.load(p, base + tid * 8);
+        live += refs.n - __popc(refs.free());
+    }
     vx_scan(live, total);
     uint32_t holes = 0, moved = 0;
     for (uint32_t base = 0; base < p.n_pages; base += kPageThreads * 8) {
-        uint32_t hole = 0, move = 0;
         const uint32_t first = base + tid * 8;
-        for (uint32_t k = 0; k < 8 && first + k < p.n_pages; ++k) {
-            const bool is = p.refs[first + k] != 0;
-            if (first + k < total) hole |= (uint32_t)!is << k;
-            else if (is) move |= 1u << k;
-            else map[first + k] = kVxNoPage;
-        }
+        if (p.n_pages > kPageThreads * 8) refs.load(p, first);
+        const uint32_t free = refs.free(), there = (1u << refs.n) - 1u;
+        const uint32_t front = first >= total ? 0u : total - first >= 8 ? 255u : (1u << (total - first)) - 1u;  // of the first L pages
+        uint32_t hole = free & front, move = ~free & there & ~front;
+        for (uint32_t dead = free & ~front; dead; dead &= dead - 1) map[first + __builtin_ctz(dead)] = kVxNoPage;
         // at most 8192 of either in a tile: both counts in one scan
         uint32_t got;
         const uint32_t at = vx_scan(__popc(hole) | __popc(move) << 16, got);
@@ -742,8 +791,11 @@ hipError_t vx_launch_pages_extend(const VxPages& p, const uint32_t* add, hipStre
 }
 
 hipError_t vx_launch_pages_fork(const VxPages& p, const uint32_t* src, hipStream_t st) {
-    const uint32_t most = kForkWords / p.n_seqs, cols = most < p.max_pages ? most : p.max_pages;
-    vx_pages_fork_kernel<<<(p.max_pages + cols - 1) / cols, 256, 0, st>>>(p, src, cols);
+    // about 2048 entries a workgroup, in runs of four columns at least (n_seqs <= 4096: they fit)
+    uint32_t cols = 2048 / p.n_seqs;
+    if (cols < 4) cols = 4;
+    if (cols > p.max_pages) cols = p.max_pages;
+    vx_pages_fork_kernel<<<(p.max_pages + cols - 1) / cols + 1, kForkThreads, 0, st>>>(p, src, cols);
     return hipGetLastError();
 }
 
