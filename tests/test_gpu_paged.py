@@ -89,7 +89,7 @@ class Filled:
             g = h // (hq // self.hkv)
             x = q[:, h].double()
             s = torch.where(seen, x @ k[:, g].T * scale, -math.inf)
-            big = torch.where(seen, x.abs() @ k[:, g].abs().T * scale, 0.0).amax(1, keepdim=True) if n else torch.zeros(rows, 1, device="cuda", dtype=torch.float64)
+            big = torch.where(seen, x.abs() @ k[:, g].abs().T * abs(scale), 0.0).amax(1, keepdim=True) if n else torch.zeros(rows, 1, device="cuda", dtype=torch.float64)
             any_ = seen.any(1, keepdim=True) if n else torch.zeros(rows, 1, dtype=torch.bool, device="cuda")
             p = torch.where(any_, torch.softmax(torch.where(any_, s, 0.0), 1), 0.0) if n else s
             o = p @ v[:, g] if n else torch.zeros(rows, d, dtype=torch.float64, device="cuda")
@@ -151,6 +151,44 @@ def test_token_attention_output_types_strides_and_scale(out):
         f.check(odd[s:s + 1], o[s:s + 1], s, s, 0, 0, False)
 
 
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"), ("bf16", "f16")])
+def test_attention_in_place_at_any_alignment_with_a_negative_scale(q, kv):
+    lens, start = [70, 33], [0, 40, 45]
+    f = Filled(lens, 2, 64, 32, kv)
+    flat = torch.randn(45 * 6 * 65 + 1, generator=gen(4), device="cuda").to(T[q])
+    for shift in (0, 1):
+        x = flat[shift:shift + 45 * 6 * 65].unflatten(0, (45, 6, 65))[:, :, :64]
+        for scale in (0.2, -0.2):
+            room = flat.clone()
+            y = room[shift:shift + 45 * 6 * 65].unflatten(0, (45, 6, 65))[:, :, :64]
+            assert paged.prompt_attention(f.cache, 0, y, ints(start), scale=scale, out=y) is y
+            for s in range(2):
+                f.check(x[start[s]:start[s + 1]], y[start[s]:start[s + 1]], s, 0, 0, 0, q == kv, scale=scale)
+            assert torch.equal(room[:shift], flat[:shift])
+            y = room[shift:shift + 45 * 6 * 65].unflatten(0, (45, 6, 65))[:, :, :64]
+            y.copy_(x)
+            assert paged.attention(f.cache, 0, y[:2], scale=scale, out=y[:2]).data_ptr() == y.data_ptr()
+            for s in range(2):
+                f.check(x[s:s + 1], y[s:s + 1], s, 0, 0, 0, q == kv, scale=scale)
+
+
+def test_weights_far_below_the_largest():
+    """One position holds most of the weight, thousands of others 2^-20 of it each: fp16 weights would lose bits."""
+    n, d = 8000, 64
+    for q, kv in (("f16", "f16"), ("f32", "f16"), ("bf16", "bf16")):
+        f = Filled([n], 1, d, 32, kv)
+        f.pool[0].view(-1, 2, 32 * d)[:, 0] = 0
+        for s, k in enumerate(f.k):
+            k.zero_()
+        number, r = int(f.table[0, 40 // 32]), 40 % 32
+        f.pool[0, number, r * d] = 8.0
+        f.k[0][40, 0, 0] = 8.0
+        x = torch.zeros(3, 2, d, device="cuda").to(T[q])
+        x[:, :, 0] = 20 * math.log(2)  # times 8 / 8
+        f.check(x[:1], paged.attention(f.cache, 0, x[:1]), 0, 0, 0, 0, q == kv)
+        f.check(x, paged.prompt_attention(f.cache, 0, x, ints([0, 3])), 0, 0, 0, 0, q == kv)
+
+
 def test_token_attention_large_values():
     """Scores of several hundred: the weights fall to nothing but for a few."""
     f = Filled([900, 40], 1, 128, 32, "bf16", amp=30.0)
@@ -183,10 +221,19 @@ def test_positions_without_a_page_are_left_out(q, kv, value):
 def test_lengths_past_the_table_are_left_out():
     f = Filled([64], 2, 64, 32, "bf16")
     n = f.table.shape[1] * 32
-    f.cache.lens.fill_(n + 1000)
     x = queries(1, 4, 2, 64, "f32")
-    out = paged.attention(f.cache, 0, x)
-    f.check(x, out, 0, 0, 0, 0, False)
+    for more in (1000, 2 ** 31 - 1 - n):
+        f.cache.lens.fill_(n + more)
+        f.check(x, paged.attention(f.cache, 0, x), 0, 0, 0, 0, False)
+        f.check(x, paged.prompt_attention(f.cache, 0, x, ints([0, 1])), 0, 0, 0, 0, False)
+        assert (paged.attention(f.cache, 0, x, window=500) == 0).all()
+        assert (paged.prompt_attention(f.cache, 0, x, ints([0, 1]), window=500) == 0).all()
+        f.lens[0] = 40  # of a window that lies behind the table the sinks are left
+        k, v = f.k[0], f.v[0]
+        f.k[0], f.v[0] = k[:40], v[:40]
+        f.check(x, paged.attention(f.cache, 0, x, window=500, sinks=40), 0, 0, 0, 0, False)
+        f.check(x, paged.prompt_attention(f.cache, 0, x, ints([0, 1]), window=500, sinks=40), 0, 0, 0, 0, False)
+        f.lens[0], f.k[0], f.v[0] = 64, k, v
 
 
 @pytest.mark.parametrize("hq,hkv,d,page,q,kv", [(9, 3, 64, 32, "f32", "f16"), (8, 2, 128, 64, "bf16", "bf16"), (28, 4, 128, 96, "f16", "f16"),

@@ -579,7 +579,8 @@ __global__ __launch_bounds__(kPageThreads) void vx_pages_extend_kernel(VxPages p
     }
 }
 
-// Copies the moves' pages of every layer. Work items of 16 KiB, dealt over the grid.
+// Copies the moves' pages of every layer. Work items of 16 KiB, dealt over the grid; past the caches (48 pages in 28
+// layers, 227 MB moved: a fork and an extend 69 -> 64 us; 2.5 GB moved by a compaction 532 -> 524 us, 4.9 TB/s).
 constexpr uint32_t kMoveItem = 16384;
 __device__ __forceinline__ void vx_copy_moves(const VxPages& p, uint32_t wg, uint32_t n_wgs) {
     const uint32_t moves = p.scratch[2];
@@ -593,7 +594,7 @@ __device__ __forceinline__ void vx_copy_moves(const VxPages& p, uint32_t wg, uin
         const uint32_t bytes = (uint32_t)min((uint64_t)kMoveItem, p.page_bytes - (uint64_t)part * kMoveItem);
         const uint4* f = (const uint4*)(base + (size_t)src[m] * p.page_bytes);
         uint4* t = (uint4*)(base + (size_t)dst[m] * p.page_bytes);
-        for (uint32_t k = threadIdx.x; k < bytes / 16; k += blockDim.x) t[k] = f[k];
+        for (uint32_t k = threadIdx.x; k < bytes / 16; k += blockDim.x) vx_set<true>(t + k, vx_get<true>(f + k));
     }
 }
 __global__ __launch_bounds__(256) void vx_pages_copy_kernel(VxPages p) { vx_copy_moves(p, blockIdx.x, gridDim.x); }

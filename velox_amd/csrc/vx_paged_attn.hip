@@ -87,6 +87,7 @@ __device__ __forceinline__ void vx_store4(void* p, size_t i, uint32_t dtype, vx_
 struct VxBf16 {
     typedef __bf16 elt;
     static constexpr uint32_t kExp = 0x7F80u, kOne = 0x0080u;  // the exponent's bits, and the lowest of them
+    static constexpr float kUp = 0.0f, kUpTerms = 0.0f;         // the weights are taken times 2^kUp (kUpTerms: in the token form)
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ float sum2(v2 a, float c) { return __builtin_amdgcn_fdot2_f32_bf16(a, v2{(__bf16)1.0f, (__bf16)1.0f}, c, false); }
@@ -96,6 +97,8 @@ struct VxBf16 {
 struct VxF16 {
     typedef _Float16 elt;
     static constexpr uint32_t kExp = 0x7C00u, kOne = 0x0400u;
+    // fp16 weights lose bits below 2^-14 and are 0 below 2^-25: they are moved up as far as the largest allows
+    static constexpr float kUp = 7.0f, kUpTerms = 14.0f;
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ float sum2(v2 a, float c) { return __builtin_amdgcn_fdot2(a, v2{(_Float16)1.0f, (_Float16)1.0f}, c, false); }
@@ -113,14 +116,16 @@ struct VxChunks {
 __device__ __forceinline__ int64_t vx_low(int64_t t, uint32_t window) {
     return window && t + 1 > (int64_t)window ? t + 1 - (int64_t)window : 0;
 }
-__device__ __forceinline__ VxChunks vx_chunks(int64_t first, int64_t last, uint32_t window, uint32_t sinks) {
+// cap: positions the table has entries for; the walk ends there, however long the sequence says it is.
+__device__ __forceinline__ VxChunks vx_chunks(int64_t first, int64_t last, uint32_t window, uint32_t sinks, uint64_t cap) {
     VxChunks c;
     c.t = last;
     c.sinks = sinks;
     c.low = vx_low(first, window);
     c.low_chunk = (uint32_t)(c.low >> 5);
-    c.sink = min((uint32_t)((min((int64_t)sinks, c.low) + 31) >> 5), c.low_chunk);
-    c.n = last < 0 ? 0 : c.sink + (uint32_t)(last >> 5) - c.low_chunk + 1;
+    const uint32_t end = (uint32_t)((min((uint64_t)(last + 1), cap) + 31) >> 5);  // chunks in all, the hidden ones too
+    c.sink = min(min((uint32_t)((min((int64_t)sinks, c.low) + 31) >> 5), c.low_chunk), end);
+    c.n = last < 0 ? 0 : c.sink + (end > c.low_chunk ? end - c.low_chunk : 0u);
     return c;
 }
 __device__ __forceinline__ uint32_t vx_chunk_base(const VxChunks& c, uint32_t i) {
@@ -161,7 +166,8 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
 #pragma unroll
         for (int c = 0; c < NC; ++c) raw[c].read(a.q.data, (size_t)seq * a.q.rs + (size_t)(h0 + col) * a.q.hs + 32 * c + 8 * grp, a.q.dtype);
     }
-    const VxChunks ch = vx_chunks((int64_t)a.c.lens[seq] - 1, (int64_t)a.c.lens[seq] - 1, a.window, a.sinks);
+    const int64_t t = (int64_t)a.c.lens[seq] - 1;
+    const VxChunks ch = vx_chunks(t, t, a.window, a.sinks, (uint64_t)a.c.max_pages * a.c.page_size);
     const uint32_t per = (ch.n + a.splits - 1) / a.splits;
     const uint32_t c0 = min(split * per, ch.n), c1 = min(c0 + per, ch.n);
     const uint32_t* table = a.c.table + (size_t)seq * a.c.table_stride;
@@ -280,13 +286,13 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
-        const float r = __builtin_amdgcn_exp2f(m - ref);
+        const float r = __builtin_amdgcn_exp2f(m - ref), from = ref - E::kUpTerms;
         m = mn;
         v8 pf[PT];
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float p = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - ref);
+            const float p = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - from);
             sum += p;
             float rest = p;
 #pragma unroll
@@ -523,7 +529,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     VxRowTile rt;
     if (!vx_find_tile(a, tiles - 1 - blockIdx.x / a.c.hkv, G, rt)) return;
     const uint32_t r0 = rt.tile * kPromptRows, r1 = min(r0 + kPromptRows, rt.rows * G);  // the workgroup's pairs
-    const VxChunks ch = vx_chunks(rt.pos0 + r0 / G, rt.pos0 + (r1 - 1) / G, a.window, a.sinks);
+    const VxChunks ch = vx_chunks(rt.pos0 + r0 / G, rt.pos0 + (r1 - 1) / G, a.window, a.sinks,
+                                  (uint64_t)a.c.max_pages * a.c.page_size);
     const uint32_t per = ((ch.n + a.splits - 1) / a.splits + 1) & ~1u;
     const uint32_t c0 = min(blockIdx.y * per, ch.n), c1 = min(c0 + per, ch.n);
     const uint32_t* table = a.c.table + (size_t)rt.seq * a.c.table_stride;
@@ -745,7 +752,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     // by is the sum of what it was made of.
     const auto add = [&](const vx_f16& s, int b, uint32_t buf) {
         const unsigned char* vb = lds + 4 * kChunk + buf * (2 * kChunk) + b * kChunk;
-        const float ref = m == -INFINITY ? 0.0f : m;
+        const float ref = (m == -INFINITY ? 0.0f : m) - E::kUp;
         v8 pf[PT][2];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -936,10 +943,9 @@ hipError_t vx_launch_paged_attention(const VxPagedAttnArgs& a, hipStream_t st) {
 // Splits of the prompt form: where the row tiles alone leave CUs empty, the positions are split until there are two
 // workgroups for each, into parts of 512 positions at least. Rows for a workgroup on every CU are not split: four
 // chunks of 380 to 500 rows behind 4000 positions of Qwen2.5-7B take 171 us and 69 for the join as two splits.
-uint32_t vx_paged_prompt_splits(const VxPagedView& c, uint32_t heads, uint32_t n_rows, uint32_t max_rows, uint32_t max_len) {
+uint32_t vx_paged_prompt_splits(const VxPagedView& c, uint32_t heads, uint32_t n_rows, uint32_t span) {
     const uint64_t g = heads / c.hkv, tiles = ((uint64_t)n_rows * g + kPromptRows - 1) / kPromptRows * c.hkv;
-    (void)max_rows;
-    const uint64_t want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles, most = max_len / 512;
+    const uint64_t want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles, most = span / 512;
     const uint64_t s = want < most ? want : most;
     return s < 1 ? 1 : s > 64 ? 64 : (uint32_t)s;
 }

@@ -256,7 +256,8 @@ int velox_hip_paged_prompt_attention_bytes(const VeloxHipPagedCache* c, uint32_t
         *bytes = 0;
         return VELOX_HIP_OK;
     }
-    const uint32_t s = vx_paged_prompt_splits(view(c, 0), heads, n_rows, max_rows ? max_rows : n_rows, max_positions(c, max_len));
+    const uint32_t s = vx_paged_prompt_splits(view(c, 0), heads, n_rows, max_positions(c, max_len));
+    (void)max_rows;  // bounds the part of a window that the call plans by, which is never more
     *bytes = part_bytes(n_rows, heads, s, c->head_dim);
     return VELOX_HIP_OK;
 }
@@ -277,7 +278,10 @@ int velox_hip_paged_prompt_attention(const VeloxHipPagedCache* c, uint32_t layer
     a.window = mask.window;
     a.sinks = mask.sinks;
     a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt((float)c->head_dim);
-    a.splits = vx_paged_prompt_splits(a.c, q->heads, n_rows, max_rows ? max_rows : n_rows, max_positions(c, max_len));
+    uint32_t span = max_positions(c, max_len);
+    const uint64_t seen = (uint64_t)mask.window + mask.sinks + (max_rows && max_rows < n_rows ? max_rows : n_rows) + 64u;
+    if (mask.window && seen < span) span = (uint32_t)seen;
+    a.splits = vx_paged_prompt_splits(a.c, q->heads, n_rows, span);
     const uint64_t need = part_bytes(n_rows, q->heads, a.splits, c->head_dim);
     if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need)) return VELOX_HIP_EINVAL;
     a.part_o = (float*)workspace;
