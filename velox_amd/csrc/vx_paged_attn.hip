@@ -919,10 +919,13 @@ hipError_t launch_prompt(const VxPagedAttnArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// Splits of the token form: workgroups for about two rounds of the GPU (a sequence's own length decides how many
-// chunks a split has, so unequal sequences even out), each with a chunk at least for every wave.
+// Splits of the token form: workgroups for one round of the GPU (two a CU; a sequence's own length decides how many
+// chunks a split has, so unequal sequences even out), each with a chunk at least for every wave; none for up to 192 KB
+// of K and V of a head. One SmolLM sequence of 600 positions takes 7.5 us unsplit and 7.0 in two launches replayed
+// from a graph (at 400 6.7 and 6.7, at 1100 10.6 and 6.9), and a launch less is 2.5 us of an eager caller's time.
 uint32_t vx_paged_attn_splits(const VxPagedView& c, uint32_t heads, uint32_t rows, uint32_t max_len) {
-    const uint32_t units = rows * c.hkv * ((heads / c.hkv + 15) / 16), chunks = (max_len + 31) / 32;
+    const uint32_t units = rows * c.hkv * ((heads / c.hkv + 15) / 16), chunks = max_len / 32 + (max_len % 32 != 0);
+    if ((uint64_t)chunks * 32 * c.d * 4 <= 192u << 10) return 1;
     const uint32_t want = (512 + units - 1) / units, most = (chunks + kTokenWaves - 1) / kTokenWaves;
     const uint32_t s = want < most ? want : most;
     return s < 1 ? 1 : s > 64 ? 64 : s;
