@@ -46,6 +46,10 @@ def _call(fn, index: int, *args) -> None:
         L.check(rc, fn.__name__)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _words(t: torch.Tensor, n: int, device: torch.device, what: str) -> int:
     """The address of an int32 vector of n elements (n < 0: any length)."""
     if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
@@ -205,7 +209,7 @@ def rope(turn: Rope, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor
     device = _gpu(x, "x")
     _need(bool(turn.handle), "rope: the handle is closed")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=device)
+        out = _like(x)
     xr, n = _rows(x, device, "x")
     o, _ = _rows(out, device, "out")
     _need(out.shape == x.shape and out.dtype == x.dtype, "out: the shape and type of x are wanted")
@@ -227,9 +231,9 @@ def rope_append(cache: PagedCache, layer: int, turn: Rope | None, q: torch.Tenso
     _need(vn == n, "k and v: as many rows of each are wanted")
     qr = qo = None
     if q is not None:
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
         qr, qn = _rows(q, device, "q", 0, d)
+        if q_out is None:
+            q_out = _like(q)
         qo, on = _rows(q_out, device, "q_out", qr.heads, d)
         _need(qn == n and on == n, "q and q_out: as many rows as k are wanted")
     else:
@@ -263,7 +267,7 @@ def attention(cache: PagedCache, layer: int, q: torch.Tensor, *, window: int = 0
     qr, n = _rows(q, device, "q", 0, cache.head_dim)
     _need(n == cache.n_seqs, f"q: {cache.n_seqs} rows are wanted")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = _like(q)
     o, on = _rows(out, device, "out", qr.heads, cache.head_dim)
     _need(on == n, "out: as many rows as q are wanted")
     if workspace is None:
@@ -282,7 +286,7 @@ def prompt_attention(cache: PagedCache, layer: int, q: torch.Tensor, q_start: to
     _need(layer >= 0 and max_len >= 0 and max_rows >= 0, "layer, max_rows and max_len have to be at least 0")
     qr, n = _rows(q, device, "q", 0, cache.head_dim)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = _like(q)
     o, on = _rows(out, device, "out", qr.heads, cache.head_dim)
     _need(on == n, "out: as many rows as q are wanted")
     start = _words(q_start, cache.n_seqs + 1, device, "q_start")
