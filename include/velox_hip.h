@@ -446,7 +446,8 @@ int velox_hip_paged_bytes(const VeloxHipPagedCache* c, uint64_t* page_bytes, uin
                           uint64_t* table_bytes, uint64_t* refs_bytes, uint64_t* scratch_bytes);
 
 /* Activation rows: element e of head h of row r at data[r * row_stride + h * head_stride + e] (strides in
- * elements; slices of fused q/k/v rows are such rows). Any alignment of the element type. */
+ * elements; slices of fused q/k/v rows are such rows). Any alignment of the element type. A call takes fewer than
+ * 2^24 rows. */
 typedef struct VeloxHipRows {
     void* data;
     uint32_t dtype;         /* VELOX_DT_F32, _F16 or _BF16 */
@@ -501,7 +502,7 @@ int velox_hip_rope_append(const VeloxHipPagedCache* c, uint32_t layer, const Vel
  * o = sum_j softmax_j(scale q . k_j) v_j over the positions j that the row at position t sees: j <= t and
  * (window == 0, or j > t - window, or j < sinks). Head h reads KV head h / (heads / num_kv_heads). A row that
  * sees nothing gives 0. scale 0: 1 / sqrt(head_dim). q and out: any element types (q of another type than the
- * cache's is not rounded to it); out may be q. What positions that a row does not see hold, infinities and NaN
+ * cache's is not rounded to it); out may be q (other overlaps are not allowed). What positions that a row does not see hold, infinities and NaN
  * among it, does not matter to the row. A row that sees an infinity or NaN gets no number where it enters.
  *
  * paged_attention: row s is the newest position of sequence s (t = lens[s] - 1), s < n_seqs. Long caches are
@@ -510,8 +511,10 @@ int velox_hip_rope_append(const VeloxHipPagedCache* c, uint32_t layer, const Vel
  * bounds, enough for every mask (may be 0 bytes: NULL), 16-byte aligned.
  *
  * paged_prompt_attention: the rows of a ragged batch as in velox_hip_rope_append; every row sees what its own
- * position allows. max_rows: an upper bound of a sequence's rows that the split is planned by (0: n_rows). Rows
- * behind the last sequence, and in front of position 0, are left as they were. */
+ * position allows. max_rows: an upper bound of a sequence's rows that the split is planned by (0: n_rows).
+ * workspace: velox_hip_paged_prompt_attention_bytes of the same cache, heads and bounds, enough for every mask and for
+ * up to the n_rows it was asked for (may be 0 bytes: NULL), 16-byte aligned. Rows behind the last sequence, and in
+ * front of position 0, are left as they were. */
 typedef struct VeloxHipAttnMask {
     uint32_t window, sinks;
 } VeloxHipAttnMask;

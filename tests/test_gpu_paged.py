@@ -774,6 +774,15 @@ def test_a_captured_step_crosses_pages():
     assert a.lens.tolist() == [70, 104, 70]
 
 
+def test_a_prompt_workspace_serves_fewer_rows():
+    f = Filled([2100], 2, 64, 64, "bf16")
+    space = f.cache.prompt_workspace(8, total_rows=900)
+    for n in (900, 300, 33, 1):
+        q, start = queries(n, 8, 2, 64, "bf16"), ints([0, n])
+        got = paged.prompt_attention(f.cache, 0, q, start, workspace=space)
+        assert torch.equal(got, paged.prompt_attention(f.cache, 0, q, start))
+
+
 def test_calls_run_on_the_current_stream():
     f = Filled([500, 90], 2, 64, 32, "bf16")
     x = torch.zeros(2, 4, 64, device="cuda")

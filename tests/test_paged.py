@@ -105,6 +105,35 @@ def test_workspace_grows_with_its_bounds(hiplib):
         last = n.value
 
 
+@pytest.mark.parametrize("heads, hkv", [(4, 2), (32, 8), (28, 4), (9, 3), (128, 1), (300, 1), (8, 8)])
+def test_prompt_workspace_grows_with_its_rows(hiplib, heads, hkv):
+    """Fewer rows are split more, yet the size for a number of rows is enough for any smaller one; the largest of
+    the sizes that the numbers up to it need."""
+    d = desc(num_kv_heads=hkv, n_seqs=1, max_pages=500, table_stride=500, n_pages=500, num_layers=1, layer_stride=0)
+
+    def size(n):
+        v = C.c_uint64()
+        assert hiplib.velox_hip_paged_prompt_attention_bytes(C.byref(d), heads, n, 0, 0, C.byref(v)) == 0
+        return v.value
+
+    last = 0
+    for n in list(range(1, 700)) + [1000, 2048, 4096, 8192, 100000, (1 << 24) - 1]:
+        assert size(n) >= last
+        last = size(n)
+    assert size(1) and last == size(200000)
+
+
+def test_refuses_too_many_rows(hiplib):
+    from velox_amd.paged import Rope
+
+    d, turn, n = desc(), Rope(64), C.c_uint64()
+    for many in (1 << 24, (1 << 32) - 1):
+        assert prompt(hiplib, d, n=many) == L.EINVAL
+        assert append(hiplib, d, n=many) == L.EINVAL
+        assert hiplib.velox_hip_rope_rows(turn.handle, C.byref(rows()), C.byref(rows()), many, 64, P, None) == L.EINVAL
+        assert hiplib.velox_hip_paged_prompt_attention_bytes(C.byref(d), 4, many, 0, 0, C.byref(n)) == L.EINVAL
+
+
 def test_refuses_append_arguments(hiplib):
     d = desc()
     for kw in (dict(layer=2), dict(k=rows(3)), dict(v=rows(1)), dict(q=rows(4)), dict(qo=rows(4)), dict(q=rows(4), qo=rows(3)),
@@ -155,6 +184,22 @@ def test_rope_frequencies(hiplib):
         assert all(x / 32 * (1 - 1e-12) <= y <= x * (1 + 1e-12) for x, y in zip(f0, f))
         assert f[0] == f0[0] or r == 2
     assert Rope(64, scaling="yarn", factor=4, original_len=4096, amplitude=1.0).frequencies()[1] == 1.0
+
+
+@pytest.mark.parametrize("r, theta, length, low, high", [(128, 1e6, 4096, 0, 0), (64, 1e4, 32768, 0, 0), (64, 1e4, 4096, 2.0, 16.0),
+                                                       (18, 5e5, 100, 0, 0), (128, 1e4, 5, 0, 0)])
+def test_yarn_frequencies(r, theta, length, low, high):
+    from velox_amd.paged import Rope
+
+    turn = Rope(r, theta=theta, scaling="yarn", factor=16, original_len=length, low_turns=low, high_turns=high)
+    got, _ = turn.frequencies()
+    # the pair that turns n times within the length: theta^(-2 j / r) length = 2 pi n, solved for j
+    pair = lambda n: r * math.log(length / (2 * math.pi * n)) / (2 * math.log(theta))  # noqa: E731
+    a, b = max(math.floor(pair(high or 32)), 0), min(math.ceil(pair(low or 1)), r - 1)
+    for j, y in enumerate(got):
+        f = theta ** (-2 * j / r)
+        ramp = 0.0 if j <= a else 1.0 if j >= b else (j - a) / (b - a)
+        assert y == pytest.approx((1 - ramp) * f + ramp * f / 16, rel=1e-12)
 
 
 def test_refuses_rope_configurations(hiplib):

@@ -6,6 +6,8 @@
 
 constexpr uint32_t kVxNoPage = VELOX_HIP_NO_PAGE;
 constexpr uint32_t kVxMaxRopePairs = 128;   // rot_dim <= 256
+constexpr uint32_t kVxMaxRows = (1u << 24) - 1u;  // a launch has fewer than 2^32 threads, 256 of them for a row at most
+constexpr uint32_t kVxPromptRows = 128;     // (row, head) pairs of a workgroup of the prompt attention
 constexpr uint32_t kVxMaxPagedSeqs = 4096;  // the extend kernel keeps a few words per sequence in LDS
 
 // One layer of a cache.

@@ -138,6 +138,9 @@ __device__ __forceinline__ uint32_t vx_chunk_base(const VxChunks& c, uint32_t i)
 // head size 128) in registers while the next one's are on their way. q of another type than the cache's enters as
 // QT terms of the cache's type whose sum keeps fp32's precision (three of bf16; two of fp16, of which each
 // head's largest value is brought to 2^13 first, so that the second term stays in range), the weights as PT.
+// Bound by the bytes of K and V where there are many: 4 sequences of 91000 to 131000 positions of Llama-3-8B's heads 293 us
+// (6.7 TB/s); by latency (lengths, table, first chunk, the join) below: 32 sequences of 600 to 2100 positions of
+// Qwen2.5-7B's heads (90 MB) 21.7 us, one SmolLM sequence of 700 8.6 us. Four waves: eight or two took as long.
 // Non-temporal loads (NT) where the caches cannot hold the K and V anyway: Llama-3-8B's heads, 4 sequences of 91000 to
 // 131000 positions 330 -> 292 us (5.9 -> 6.7 TB/s); 32 sequences of Qwen2.5-7B (90 MB, in the memory-side cache from
 // one call to the next) 21.8 us without, 23.6 with.
@@ -365,7 +368,8 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
     }
 }
 
-// Joins a row's splits: a workgroup per (row, head), each of its waves over a quarter of the splits. Of a prompt's
+// Joins a row's splits: a workgroup per (row, head), each of its waves over a quarter of the splits (3.9 us for 32 rows of
+// 28 heads, 4.1 with one wave for all of them; a launch's latency). Of a prompt's
 // rows, those behind the last sequence and those in front of position 0 (their sums say -1) are passed over.
 template <int D>
 __global__ __launch_bounds__(256) void vx_paged_join_kernel(VxPagedAttnArgs a) {
@@ -437,9 +441,14 @@ hipError_t launch_token(const VxPagedAttnArgs& a, bool nt, hipStream_t st) {
 // the weights are the B operand of O^T = V^T P^T without leaving their lanes: the K row that scores row
 // 16 t + 8 a + 4 g + b is position 16 a + 8 t + 4 g + b of the chunk (two bits swapped), which puts position
 // order into the order of the pages' V blocks.
+// Bound by the matrix cores and what shares their issue slots: 8192 rows of Llama-3-8B's heads through a window of 4096
+// take 393 us (1050 TFLOP/s of the visible pairs) with the matrix cores busy in 54 % of the clocks, at 1.8 GHz; four chunks
+// of 380 to 500 rows behind 4000 positions of Qwen2.5-7B's heads 123 us (890 TFLOP/s). 64 pairs a wave (616 us), 8 or 2
+// waves a workgroup (523, 729 against 471 then) were slower.
 constexpr int kPromptWaves = 4;
 constexpr int kPromptThreads = 64 * kPromptWaves;
-constexpr int kPromptRows = 32 * kPromptWaves;
+constexpr int kPromptRows = kVxPromptRows;
+static_assert(kPromptRows == 32 * kPromptWaves, "each wave has 32 pairs");
 
 template <int N>
 __device__ __forceinline__ void vx_wait_loads() {
@@ -911,7 +920,7 @@ hipError_t launch_prompt(const VxPagedAttnArgs& a, hipStream_t st) {
     uint64_t tiles = (uint64_t)a.n_rows * G / kPromptRows + a.c.n_seqs;
     const uint64_t most = (uint64_t)a.n_rows * ((G + kPromptRows - 1) / kPromptRows + 1);
     if (tiles > most) tiles = most;
-    if (tiles * a.c.hkv > 0x7FFFFFFFull) return hipErrorInvalidValue;
+    if (tiles * a.c.hkv > kVxMaxRows) return hipErrorInvalidValue;  // threads of a launch
     vx_paged_prompt_kernel<E, D, QT, PT><<<dim3((uint32_t)(tiles * a.c.hkv), a.splits), kPromptThreads, 0, st>>>(a, (uint32_t)tiles);
     const hipError_t e = hipGetLastError();
     return e != hipSuccess || a.splits == 1 ? e : launch_join(a, st);

@@ -179,7 +179,7 @@ int velox_hip_rope_frequencies(const VeloxHipRope* r, double* freq, double* ampl
 int velox_hip_rope_rows(const VeloxHipRope* r, const VeloxHipRows* x, const VeloxHipRows* out, uint32_t n_rows,
                         uint32_t head_dim, const uint32_t* d_positions, hipStream_t st) {
     if (!r || !rows_ok(x) || !rows_ok(out) || x->dtype != out->dtype || x->heads != out->heads || head_dim > 65536u ||
-        r->cfg.rot_dim > head_dim)
+        r->cfg.rot_dim > head_dim || n_rows > kVxMaxRows)
         return VELOX_HIP_EINVAL;
     if (x->data == out->data && (x->row_stride != out->row_stride || x->head_stride != out->head_stride)) return VELOX_HIP_EINVAL;
     if (!n_rows) return VELOX_HIP_OK;
@@ -199,7 +199,7 @@ int velox_hip_rope_append(const VeloxHipPagedCache* c, uint32_t layer, const Vel
     if (q && q->data == q_out->data && (q->row_stride != q_out->row_stride || q->head_stride != q_out->head_stride))
         return VELOX_HIP_EINVAL;
     if (!d_q_start && n_rows > c->n_seqs) return VELOX_HIP_EINVAL;
-    if (d_q_start && !aligned(d_q_start, 4)) return VELOX_HIP_EINVAL;
+    if ((d_q_start && !aligned(d_q_start, 4)) || n_rows > kVxMaxRows) return VELOX_HIP_EINVAL;
     if (!n_rows) return VELOX_HIP_OK;
     VxAppendArgs a;
     std::memset(&a, 0, sizeof(a));
@@ -256,9 +256,24 @@ int velox_hip_paged_prompt_attention_bytes(const VeloxHipPagedCache* c, uint32_t
         *bytes = 0;
         return VELOX_HIP_OK;
     }
-    const uint32_t s = vx_paged_prompt_splits(view(c, 0), heads, n_rows, max_positions(c, max_len));
     (void)max_rows;  // bounds the part of a window that the call plans by, which is never more
-    *bytes = part_bytes(n_rows, heads, s, c->head_dim);
+    if (n_rows > kVxMaxRows) return VELOX_HIP_EINVAL;
+    // Fewer rows are split more: the largest need of up to n_rows rows. It is that of rows that just fill their tiles,
+    // or of n_rows.
+    const VxPagedView v = view(c, 0);
+    const uint32_t g = heads / c->num_kv_heads, span = max_positions(c, max_len);
+    uint64_t most = 0;
+    for (uint32_t tiles = 1; ; ++tiles) {
+        const uint64_t fill = (uint64_t)tiles * kVxPromptRows / g;
+        const uint32_t rows = fill < n_rows ? (uint32_t)fill : n_rows;
+        if (rows) {
+            const uint32_t s = vx_paged_prompt_splits(v, heads, rows, span);
+            const uint64_t need = part_bytes(rows, heads, s, c->head_dim);
+            if (need > most) most = need;
+            if (rows == n_rows || s == 1) break;
+        }
+    }
+    *bytes = most;
     return VELOX_HIP_OK;
 }
 
@@ -266,7 +281,7 @@ int velox_hip_paged_prompt_attention(const VeloxHipPagedCache* c, uint32_t layer
                                      const VeloxHipRows* out, const uint32_t* d_q_start, uint32_t n_rows,
                                      VeloxHipAttnMask mask, float scale, uint32_t max_rows, uint32_t max_len,
                                      void* workspace, uint64_t workspace_bytes, hipStream_t st) {
-    if (!attn_ok(c, layer, q, out, scale) || !d_q_start || !aligned(d_q_start, 4) || n_rows > 0x7FFFFFFFu) return VELOX_HIP_EINVAL;
+    if (!attn_ok(c, layer, q, out, scale) || !d_q_start || !aligned(d_q_start, 4) || n_rows > kVxMaxRows) return VELOX_HIP_EINVAL;
     if (!n_rows) return VELOX_HIP_OK;
     VxPagedAttnArgs a;
     std::memset(&a, 0, sizeof(a));

@@ -166,7 +166,7 @@ class PagedCache:
         return torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
 
     def prompt_workspace(self, heads: int, *, total_rows: int, max_rows: int = 0, max_len: int = 0) -> torch.Tensor | None:
-        """What prompt_attention() needs with these bounds (None: nothing)."""
+        """What prompt_attention() needs for up to total_rows rows with these bounds (None: nothing)."""
         n = C.c_uint64()
         L.check(self.lib.velox_hip_paged_prompt_attention_bytes(self._ref, heads, total_rows, max_rows, max_len, C.byref(n)),
                 "paged_prompt_attention_bytes")
