@@ -444,7 +444,8 @@ hipError_t launch_token(const VxPagedAttnArgs& a, bool nt, hipStream_t st) {
 // Bound by the matrix cores and what shares their issue slots: 8192 rows of Llama-3-8B's heads through a window of 4096
 // take 393 us (1050 TFLOP/s of the visible pairs) with the matrix cores busy in 54 % of the clocks, at 1.8 GHz; four chunks
 // of 380 to 500 rows behind 4000 positions of Qwen2.5-7B's heads 123 us (890 TFLOP/s). 64 pairs a wave (616 us), 8 or 2
-// waves a workgroup (523, 729 against 471 then) were slower.
+// waves a workgroup (523, 729 against 471 then) were slower; written orders of products, exponentials and LDS reads took
+// as long (391 to 396 us), so the chip's power is what holds it.
 constexpr int kPromptWaves = 4;
 constexpr int kPromptThreads = 64 * kPromptWaves;
 constexpr int kPromptRows = kVxPromptRows;
