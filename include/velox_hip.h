@@ -491,8 +491,8 @@ int velox_hip_rope_rows(const VeloxHipRope* r, const VeloxHipRows* x, const Velo
                         uint32_t head_dim, const uint32_t* d_positions, hipStream_t stream);
 /* The new rows of a layer: q turned into q_out, k turned and v into the pages (rounded to the cache's type).
  * Rows d_q_start[s] .. d_q_start[s + 1] are sequence s's, its last one at position lens[s] - 1 (d_q_start NULL:
- * row s is sequence s's, n_rows <= n_seqs). Rows behind the last sequence, and rows in front of position 0, are
- * left as they were. rope NULL: no rotation. q and q_out may both be NULL, or the same rows. No two sequences
+ * row s is sequence s's, n_rows <= n_seqs). Rows of no sequence (in front of the first, behind the last), and rows in
+ * front of position 0, are left as they were. rope NULL: no rotation. q and q_out may both be NULL, or the same rows. No two sequences
  * may write the same page (velox_hip_pages_extend sees to it). */
 int velox_hip_rope_append(const VeloxHipPagedCache* c, uint32_t layer, const VeloxHipRope* rope, const VeloxHipRows* q,
                           const VeloxHipRows* k, const VeloxHipRows* v, const VeloxHipRows* q_out,
@@ -513,8 +513,8 @@ int velox_hip_rope_append(const VeloxHipPagedCache* c, uint32_t layer, const Vel
  * paged_prompt_attention: the rows of a ragged batch as in velox_hip_rope_append; every row sees what its own
  * position allows. max_rows: an upper bound of a sequence's rows that the split is planned by (0: n_rows).
  * workspace: velox_hip_paged_prompt_attention_bytes of the same cache, heads and bounds, enough for every mask and for
- * up to the n_rows it was asked for (may be 0 bytes: NULL), 16-byte aligned. Rows behind the last sequence, and in
- * front of position 0, are left as they were. */
+ * up to the n_rows it was asked for (may be 0 bytes: NULL), 16-byte aligned. Rows of no sequence, and in front of
+ * position 0, are left as they were. */
 typedef struct VeloxHipAttnMask {
     uint32_t window, sinks;
 } VeloxHipAttnMask;

@@ -274,6 +274,21 @@ def test_prompt_rows_in_front_of_position_0_stay():
     f.check(x[6:], out[6:], 0, 6, 0, 0, True)
 
 
+@pytest.mark.parametrize("lens", [(9000, 7000), (40, 30)], ids=["split", "whole"])
+def test_prompt_rows_of_no_sequence_stay(lens):
+    f = Filled(lens, 2, 64, 32, "bf16")
+    x = queries(20, 4, 2, 64, "bf16")
+    out = torch.full((20, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    space = f.cache.prompt_workspace(4, total_rows=20)
+    assert (space is None) == (lens[0] < 1000)
+    if space is not None:
+        space.zero_()
+    paged.prompt_attention(f.cache, 0, x, ints([3, 8, 15]), out=out, workspace=space)
+    assert (out[:3] == 7).all() and (out[15:] == 7).all()
+    f.check(x[3:8], out[3:8], 0, 0, 0, 0, True)
+    f.check(x[8:15], out[8:15], 1, 0, 0, 0, True)
+
+
 @pytest.mark.parametrize("q,kv", [("bf16", "bf16"), ("f32", "bf16"), ("f16", "f16"), ("f32", "f16")])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 def test_rows_do_not_see_what_later_or_left_positions_hold(q, kv, value):
@@ -772,6 +787,58 @@ def test_a_captured_step_crosses_pages():
         torch.cuda.synchronize()
         assert torch.equal(out, out2) and torch.equal(a.table, b.table) and torch.equal(a.lens, b.lens) and torch.equal(a.refs, b.refs)
     assert a.lens.tolist() == [70, 104, 70]
+
+
+def test_captured_page_operations_and_prompts():
+    """A serving turn (free, prompts, fork, trim, compact) in one graph, replayed with other inputs and eager work
+    between, against the same turns run eagerly on a second cache."""
+    hq, hkv, d, page, n, window = 4, 2, 64, 32, 4, 50
+
+    def make():
+        # 40 pages of 32 positions: parts of 512 at least are split off, so that the workspace is used
+        c = paged.PagedCache(120, n, 40, page_size=page, num_kv_heads=hkv, head_dim=d, n_layers=2)
+        c.extend(ints([700, 5, 64, 200]))
+        c.pool.copy_(torch.randn(c.pool.shape, generator=gen(5), device="cuda"))
+        return c
+
+    a, b = make(), make()
+    turn = paged.Rope(d)
+    x = torch.zeros(20, hq + 2 * hkv, d, device="cuda")
+    rows, start, src, gone = ints([5, 0, 9, 1]), ints([0, 5, 5, 14, 15]), ints([0, 1, 2, 3]), ints([-1, -1])
+    q, out = torch.zeros(20, hq, d, device="cuda"), torch.zeros(20, hq, d, device="cuda")
+    space = a.prompt_workspace(hq, total_rows=20)
+    assert space is not None
+
+    def step(c, q, out):
+        c.free(gone)
+        c.fork(src)
+        c.extend(rows)
+        for layer in range(2):
+            paged.rope_append(c, layer, turn, x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], q, q_start=start)
+            paged.prompt_attention(c, layer, q, start, sinks=4, window=window * layer, out=out, workspace=space)
+        c.trim(700)
+        c.compact()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        step(a, q, out)
+    torch.cuda.current_stream().wait_stream(side)
+    q2, out2 = torch.zeros_like(q), torch.zeros_like(out)
+    for i, (s, g) in enumerate([([0, 1, 2, 3], [-1, -1]), ([0, 0, 2, 2], [-1, -1]), ([0, 1, 0, 3], [1, 1]), ([3, 1, 2, -1], [-1, 2]),
+                                ([0, 2, 2, 0], [7, -1]), ([0, 1, 2, 3], [0, 2])]):
+        x.copy_(torch.randn(x.shape, generator=gen(100 + i), device="cuda"))
+        src.copy_(ints(s))
+        gone.copy_(ints(g))
+        graph.replay()
+        torch.cuda.synchronize()
+        step(b, q2, out2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, out2) and torch.equal(q, q2)
+        for u, w in ((a.table, b.table), (a.lens, b.lens), (a.refs, b.refs), (a.pool, b.pool)):
+            assert torch.equal(u, w)
+        assert a.status() == b.status()
 
 
 def test_a_prompt_workspace_serves_fewer_rows():

@@ -370,7 +370,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
 
 // Joins a row's splits: a workgroup per (row, head), each of its waves over a quarter of the splits (3.9 us for 32 rows of
 // 28 heads, 4.1 with one wave for all of them; a launch's latency). Of a prompt's
-// rows, those behind the last sequence and those in front of position 0 (their sums say -1) are passed over.
+// rows, those of no sequence and those in front of position 0 (their sums say -1) are passed over.
 template <int D>
 __global__ __launch_bounds__(256) void vx_paged_join_kernel(VxPagedAttnArgs a) {
     constexpr int N = D / 64;
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(256) void vx_paged_join_kernel(VxPagedAttnArgs a) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t row = blockIdx.x / a.q.heads, h = blockIdx.x % a.q.heads;
     const float* ml = a.part_ml + 2 * (size_t)blockIdx.x * a.splits;
-    if (a.q_start && (row >= a.q_start[a.c.n_seqs] || ml[1] < 0.0f)) return;
+    if (a.q_start && (row < a.q_start[0] || row >= a.q_start[a.c.n_seqs] || ml[1] < 0.0f)) return;
     const float* po = a.part_o + (size_t)blockIdx.x * a.splits * D + lane * N;
     const uint32_t per = (a.splits + 3) / 4, s0 = min(wave * per, a.splits), s1 = min(s0 + per, a.splits);
     float v[16][N];  // per <= 16; requested before the weights are known

@@ -281,7 +281,7 @@ def prompt_attention(cache: PagedCache, layer: int, q: torch.Tensor, q_start: to
                      scale: float = 0.0, max_rows: int = 0, max_len: int = 0, out: torch.Tensor | None = None,
                      workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of a ragged batch's rows, q [row][q head][head size]; sequence s has rows q_start[s] .. q_start[s + 1],
-    the last of them its newest position. Rows behind the last sequence are not written."""
+    the last of them its newest position. Rows of no sequence are not written."""
     device = cache.device
     _need(layer >= 0 and max_len >= 0 and max_rows >= 0, "layer, max_rows and max_len have to be at least 0")
     qr, n = _rows(q, device, "q", 0, cache.head_dim)
