@@ -29,11 +29,18 @@ typedef uint32_t vx_u4 __attribute__((ext_vector_type(4)));
 // Eight elements as they lie in memory, at any alignment, to be widened once they are there.
 struct VxEight {
     vx_u4 w[2];
-    __device__ __forceinline__ void read(const void* p, size_t i, uint32_t dtype) {
-        if (dtype == VELOX_DT_F32) __builtin_memcpy(w, (const float*)p + i, 32);
-        else __builtin_memcpy(w, (const uint16_t*)p + i, 16);
-    }
 };
+// N of them, `step` elements apart from element i on. HALF: no fp32. One branch for all, so that no read waits for another.
+template <bool HALF, int N>
+__device__ __forceinline__ void vx_request(VxEight (&raw)[N], const void* p, size_t i, uint32_t step, uint32_t dtype) {
+    if (!HALF && dtype == VELOX_DT_F32) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) __builtin_memcpy(raw[c].w, (const float*)p + i + step * c, 32);
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) __builtin_memcpy(raw[c].w, (const uint16_t*)p + i + step * c, 16);
+    }
+}
 template <int N>
 __device__ __forceinline__ void vx_widen(const VxEight (&raw)[N], uint32_t dtype, float (&x)[N][8]) {
     if (dtype == VELOX_DT_F32) {
@@ -138,17 +145,13 @@ __device__ __forceinline__ uint32_t vx_chunk_base(const VxChunks& c, uint32_t i)
 // head size 128) in registers while the next one's are on their way. q of another type than the cache's enters as
 // QT terms of the cache's type whose sum keeps fp32's precision (three of bf16; two of fp16, of which each
 // head's largest value is brought to 2^13 first, so that the second term stays in range), the weights as PT.
-// Bound by the bytes of K and V where there are many: 4 sequences of 91000 to 131000 positions of Llama-3-8B's heads 293 us
+// Bound by the bytes of K and V where there are many: 4 sequences of 91000 to 131000 positions of Llama-3-8B's heads 292 us
 // (6.7 TB/s); by latency (lengths, table, first chunk, the join) below: 32 sequences of 600 to 2100 positions of
-// Qwen2.5-7B's heads (90 MB) 21.7 us, one SmolLM sequence of 700 8.6 us. Four waves: eight or two took as long.
+// Qwen2.5-7B's heads (90 MB) 20.2 us, one SmolLM sequence of 700 7.5 us (21.7 and 8.6 while the waits for a chunk were
+// waits for the next one too). Four waves: eight were slower (25.4 against 22.9 us for 32 sequences of 1500).
 // Non-temporal loads (NT) where the caches cannot hold the K and V anyway: Llama-3-8B's heads, 4 sequences of 91000 to
 // 131000 positions 330 -> 292 us (5.9 -> 6.7 TB/s); 32 sequences of Qwen2.5-7B (90 MB, in the memory-side cache from
 // one call to the next) 21.8 us without, 23.6 with.
-template <bool NT, class V>
-__device__ __forceinline__ V vx_read(const V* p) {
-    if constexpr (NT) return __builtin_nontemporal_load(p);
-    else return *p;
-}
 constexpr uint64_t kTokenCached = 256ull << 20;  // bytes of the memory-side cache
 constexpr int kTokenWaves = 4;
 constexpr int kTokenThreads = 64 * kTokenWaves;
@@ -159,17 +162,15 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
     typedef typename E::v8 v8;
     __shared__ __attribute__((aligned(16))) float s_o[kTokenWaves * 16 * OP];
     __shared__ float s_m[kTokenWaves * 16], s_l[kTokenWaves * 16];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, grp = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t col = lane & 15u, grp = lane >> 4;
     const uint32_t G = a.q.heads / a.c.hkv, ng = (G + 15) / 16;
     const uint32_t kvh = blockIdx.y / ng, g0 = blockIdx.y % ng * 16, gn = min(16u, G - g0);
     const uint32_t seq = blockIdx.z, split = blockIdx.x, h0 = kvh * G + g0;
     // q: column col is head h0 + col. The requests go out first; the first chunk's follow before q is widened.
     VxEight raw[NC] = {};
-    if (col < gn) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) raw[c].read(a.q.data, (size_t)seq * a.q.rs + (size_t)(h0 + col) * a.q.hs + 32 * c + 8 * grp, a.q.dtype);
-    }
-    const int64_t t = (int64_t)a.c.lens[seq] - 1;
+    if (col < gn) vx_request<QT == 1>(raw, a.q.data, (size_t)seq * a.q.rs + (size_t)(h0 + col) * a.q.hs + 8 * grp, 32, a.q.dtype);
+    const int64_t t = (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)a.c.lens[seq]) - 1;
     const VxChunks ch = vx_chunks(t, t, a.window, a.sinks, (uint64_t)a.c.max_pages * a.c.page_size);
     const uint32_t per = (ch.n + a.splits - 1) / a.splits;
     const uint32_t c0 = min(split * per, ch.n), c1 = min(c0 + per, ch.n);
@@ -186,6 +187,8 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
             places = base - j * a.c.page_size;
             if (j < a.c.max_pages) pages = table[j];
         }
+        // waited for here: at every later use the wait would be for all that is on its way by then, the next chunk too
+        asm volatile("" : "+v"(pages));
     };
     look_up(0);
 
@@ -193,16 +196,23 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
         v8 k[2][NC], v[NB];
     };
     const uint32_t n_mine = c1 > c0 + wave ? (c1 - c0 - wave + kTokenWaves - 1) / kTokenWaves : 0;
+    // this lane's bytes of a chunk's K and V. Buffer loads: a uniform base, one offset a lane for all of them, and nothing
+    // (0) is read of a page that is not there
+    const uint32_t k_at = (col * D + 8 * grp) * 2, v_at = (col * 32 + 8 * grp) * 2;
     const auto load = [&](Chunk& x, uint32_t page, uint32_t place) {
-        const uint16_t* kp = (const uint16_t*)(a.c.pool + (size_t)(page < a.c.n_pages ? page : 0u) * a.c.page_bytes);
-        const uint16_t* vp = kp + ((size_t)a.c.hkv * a.c.page_size + (size_t)kvh * a.c.page_size + place) * D;
-        kp += ((size_t)kvh * a.c.page_size + place) * D;
+        const bool have = page < a.c.n_pages;
+        uint8_t* kp = a.c.pool + (size_t)(have ? page : 0u) * a.c.page_bytes + ((size_t)kvh * a.c.page_size + place) * (D * 2);
+        const int bytes = have ? 64 * D : 0;
+        const auto kr = __builtin_amdgcn_make_buffer_rsrc(kp, (short)0, bytes, 0x00020000);
+        const auto vr = __builtin_amdgcn_make_buffer_rsrc(kp + (size_t)a.c.hkv * a.c.page_size * (D * 2), (short)0, bytes, 0x00020000);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) x.k[b][c] = vx_read<NT>((const v8*)(kp + (16 * b + col) * D + 32 * c + 8 * grp));
+            for (int c = 0; c < NC; ++c) x.k[b][c] = __builtin_bit_cast(v8, __builtin_amdgcn_raw_buffer_load_b128(kr, k_at + 64 * c, b * 32 * D, NT ? 2 : 0));
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) x.v[nb] = vx_read<NT>((const v8*)(vp + (16 * nb + col) * 32 + 8 * grp));
+        for (int nb = 0; nb < NB; ++nb)
+            x.v[nb] = __builtin_bit_cast(v8, __builtin_amdgcn_raw_buffer_load_b128(vr, v_at + nb % 4 * 1024, nb / 4 * 4096, NT ? 2 : 0));
+        __builtin_amdgcn_sched_barrier(0);  // requested before the chunk at hand is multiplied
     };
     const auto page_of = [&](uint32_t k) { return (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(k & 63u)); };
     const auto place_of = [&](uint32_t k) { return (uint32_t)__builtin_amdgcn_readlane((int)places, (int)(k & 63u)); };
@@ -253,7 +263,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
     for (int nb = 0; nb < NB; ++nb) o[nb] = vx_f4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
     const auto use = [&](Chunk& x, uint32_t page, uint32_t base) {
-        if (page >= a.c.n_pages) return;
+        const bool have = page < a.c.n_pages;
         vx_f4 s[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -264,14 +274,14 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
                 for (int c = 0; c < NC; ++c) s[b] = E::mfma(x.k[b][c], qf[t][c], s[b]);
             s[b] *= to_log2;
         }
-        if ((int64_t)base < ch.low || (int64_t)base + 31 > ch.t) {  // some positions are hidden: their places may hold anything
+        if (!have || (int64_t)base < ch.low || (int64_t)base + 31 > ch.t) {  // some positions are hidden: their places may hold anything
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 uint32_t keep[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int64_t p = (int64_t)base + 16 * b + 4 * grp + r;
-                    const bool seen = p <= ch.t && (p >= ch.low || p < (int64_t)ch.sinks);
+                    const bool seen = have & (p <= ch.t) & ((p >= ch.low) | (p < (int64_t)ch.sinks));
                     if (!seen) s[b][r] = -INFINITY;
                     keep[r] = seen ? 0xFFFFu : 0u;
                 }
@@ -315,20 +325,19 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) o[nb] = E::mfma(x.v[nb], pf[t], o[nb]);
     };
-    for (uint32_t k = 0; k < n_mine; k += 2) {
-        if (k + 1 < n_mine) {
-            py = page_of(k + 1);
-            load(y, py, place_of(k + 1));
-        }
+    // Chunk k + 2 is requested whether there is one or not (then nothing is read): behind a branch the wait for chunk
+    // k + 1 would be one for it as well.
+    uint32_t k = 0;
+    for (; k + 2 <= n_mine; k += 2) {
+        py = page_of(k + 1);
+        load(y, py, place_of(k + 1));
         use(x, px, base_of(k));
-        if (k + 1 >= n_mine) break;
-        if (k + 2 < n_mine) {
-            if (((k + 2) & 63u) == 0) look_up(k + 2);
-            px = page_of(k + 2);
-            load(x, px, place_of(k + 2));
-        }
+        if (((k + 2) & 63u) == 0) look_up(k + 2);
+        px = page_of(k + 2);
+        load(x, px, place_of(k + 2));
         use(y, py, base_of(k + 1));
     }
+    if (k < n_mine) use(x, px, base_of(k));
 
     // the waves' (m, l, o) meet
     l += __shfl_xor(l, 16);
@@ -557,10 +566,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
 
     // q is requested before the table and the first K, and brought into its operands behind them
     VxEight raw[NK] = {};
-    if (mine) {
-#pragma unroll
-        for (int c = 0; c < NK; ++c) raw[c].read(a.q.data, (size_t)row * a.q.rs + (size_t)head * a.q.hs + 16 * c + 8 * grp, a.q.dtype);
-    }
+    if (mine) vx_request<QT == 1>(raw, a.q.data, (size_t)row * a.q.rs + (size_t)head * a.q.hs + 8 * grp, 16, a.q.dtype);
 
     // where the K of the next 64 chunks lies in the pool, one a lane, and which of them have a page (page 0 stands in
     // for the others, and for chunks past the last)
@@ -929,16 +935,27 @@ hipError_t launch_prompt(const VxPagedAttnArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// Splits of the token form: workgroups for one round of the GPU (two a CU; a sequence's own length decides how many
-// chunks a split has, so unequal sequences even out), each with a chunk at least for every wave; none for up to 192 KB
-// of K and V of a head. One SmolLM sequence of 600 positions takes 7.5 us unsplit and 7.0 in two launches replayed
-// from a graph (at 400 6.7 and 6.7, at 1100 10.6 and 6.9), and a launch less is 2.5 us of an eager caller's time.
+// Splits of the token form. What a CU has to do is its last workgroup's end: rounds / splits of a sequence's K and V of a
+// head, rounds = workgroups / 256 CUs, at 16 us per MB (62 GB/s); lengths differ, which more rounds even out (0.3 of
+// one). A round's start costs 1 us, the join 4. 24 sequences of 3000 positions, 4 KV heads of 128: 37.0 us with 3 splits
+// (288 workgroups), 32.6 with 6 (576), 29.2 with 8 (768), 31.2 with 11 (1056); 64 of 1000: 23.6 unsplit (256), 28.3 with 2.
+// A split has a chunk at least for every wave (one sequence of 2000 positions 8.2 us, with two chunks a wave 9.6).
 uint32_t vx_paged_attn_splits(const VxPagedView& c, uint32_t heads, uint32_t rows, uint32_t max_len) {
     const uint32_t units = rows * c.hkv * ((heads / c.hkv + 15) / 16), chunks = max_len / 32 + (max_len % 32 != 0);
-    if ((uint64_t)chunks * 32 * c.d * 4 <= 192u << 10) return 1;
-    const uint32_t want = (512 + units - 1) / units, most = (chunks + kTokenWaves - 1) / kTokenWaves;
-    const uint32_t s = want < most ? want : most;
-    return s < 1 ? 1 : s > 64 ? 64 : s;
+    const uint32_t most = (chunks + kTokenWaves - 1) / kTokenWaves, rounds0 = (units + 255) / 256;
+    const double whole = 16e-6 * max_len * c.d * 4;
+    const auto cost = [&](uint32_t rounds, uint32_t s) { return whole * (rounds + 0.3) / s + rounds; };
+    double best = cost(rounds0, 1);
+    uint32_t splits = 1;
+    for (uint32_t r = rounds0; r <= rounds0 + 8; ++r) {
+        uint32_t s = 256 * r / units;  // the most of so many rounds
+        if (s > most) s = most;
+        if (s > 64) s = 64;
+        if (s <= splits) continue;
+        const double t = cost((units * s + 255) / 256, s) + 4.0;
+        if (t < best) best = t, splits = s;
+    }
+    return splits;
 }
 
 hipError_t vx_launch_paged_attention(const VxPagedAttnArgs& a, hipStream_t st) {

@@ -242,6 +242,8 @@ int velox_hip_paged_attention(const VeloxHipPagedCache* c, uint32_t layer, const
     if (mask.window && (uint64_t)mask.window + mask.sinks + 64u < span) span = mask.window + mask.sinks + 64u;
     a.span = span;
     a.splits = vx_paged_attn_splits(a.c, q->heads, c->n_seqs, span);
+    const uint32_t planned = vx_paged_attn_splits(a.c, q->heads, c->n_seqs, max_positions(c, max_len));  // the workspace's
+    if (a.splits > planned) a.splits = planned;
     const uint64_t need = part_bytes(c->n_seqs, q->heads, a.splits, c->head_dim);
     if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need)) return VELOX_HIP_EINVAL;
     a.part_o = (float*)workspace;
