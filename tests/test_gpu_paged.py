@@ -498,6 +498,31 @@ def test_append_one_row_each_without_rotation_and_without_pages():
     assert torch.equal(f.pool[0, same].view(torch.int16), before[0, same].view(torch.int16))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_append_many_sequences_of_few_rows(dtype, ragged):
+    """130 sequences at once give, bit for bit, what 13 batches of ten give."""
+    n, hq, hkv, d, page = 130, 6, 2, 128, 32
+    rng = np.random.default_rng(3)
+    count = rng.integers(0, 4, n) if ragged else np.ones(n, int)
+    a = paged.PagedCache(n * 4, n, 4, page_size=page, num_kv_heads=hkv, head_dim=d)
+    a.extend(ints(rng.integers(1, 60, n).tolist()))
+    a.extend(ints(count.tolist()))
+    b = torch.zeros_like(a.pool)
+    start = np.concatenate([[0], np.cumsum(count)])
+    x = torch.randn(int(start[-1]), hq + 2 * hkv, d, generator=gen(4), device="cuda").to(dtype)
+    q, k, v = x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:]
+    turn = paged.Rope(d, layout="interleaved" if ragged else "half")
+    out = paged.rope_append(a, 0, turn, q, k, v, q_start=ints(start.tolist()) if ragged else None)
+    parts = []
+    for s in range(0, n, 10):
+        c = paged.PagedCache.over(b, a.table[s:s + 10], a.lens[s:s + 10], page_size=page, num_kv_heads=hkv, head_dim=d)
+        r = slice(int(start[s]), int(start[s + 10]))
+        own = ints((start[s:s + 11] - start[s]).tolist()) if ragged else None
+        parts.append(paged.rope_append(c, 0, turn, q[r], k[r], v[r], q_start=own))
+    assert torch.equal(out, torch.cat(parts)) and torch.equal(a.pool, b)
+
+
 def test_append_more_rows_than_positions_leaves_the_front_ones():
     f = Filled([3], 1, 64, 32, "bf16")
     x = torch.randn(10, 4, 64, device="cuda")

@@ -65,6 +65,15 @@ struct VxPages {
 constexpr uint32_t kVxPagesHead = 64;
 VX_HD uint32_t vx_pages_moves(uint32_t n_seqs, uint32_t n_pages) { return n_seqs > n_pages ? n_seqs : n_pages; }
 
+#ifdef __HIP_DEVICE_COMPILE__
+// A word at a uniform address that no kernel in flight writes, by a scalar load: it waits for no vector load.
+__device__ __forceinline__ uint32_t vx_word(const uint32_t* p) {
+    return *(const __attribute__((address_space(4))) uint32_t*)(uintptr_t)p;
+}
+#else
+__device__ uint32_t vx_word(const uint32_t* p);
+#endif
+
 hipError_t vx_launch_rope_rows(const VxRopeTable& t, const VxRowsView& x, const VxRowsView& out, uint32_t n_rows,
                                uint32_t d, const uint32_t* positions, hipStream_t st);
 hipError_t vx_launch_rope_append(const VxRopeTable& t, const VxAppendArgs& a, hipStream_t st);

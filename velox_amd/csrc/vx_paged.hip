@@ -19,13 +19,14 @@ __device__ __forceinline__ void vx_store(void* p, size_t i, uint32_t dtype, floa
 // cos and sin of position * f_j, times the amplitude. The angle is position * f_j / 2 pi turns in 64 bits (a
 // product in 32 would be off by 2^-24 of a position's whole angle: 0.06 rad at position 10^6); its fraction of
 // a turn, at most one half, is exact to 2^-25 in fp32.
-__device__ __forceinline__ float2 vx_turn(const VxRopeTable& t, uint32_t j, uint32_t pos) {
-    const double turns = (double)pos * t.turns[j];
+__device__ __forceinline__ float2 vx_turn_of(const VxRopeTable& t, double freq, uint32_t pos) {
+    const double turns = (double)pos * freq;
     const float f = (float)(turns - rint(turns));
     float s, c;
     sincospif(2.0f * f, &s, &c);
     return make_float2(c * t.amp, s * t.amp);
 }
+__device__ __forceinline__ float2 vx_turn(const VxRopeTable& t, uint32_t j, uint32_t pos) { return vx_turn_of(t, t.turns[j], pos); }
 
 // A pair turned by cs = (cos, sin); the same roundings wherever it is done (the empty statement keeps the values in
 // fp32: a product, a sum and the conversion to fp16 would become one instruction in some places and not in others).
@@ -66,11 +67,18 @@ template <class T, bool NT>
 struct VxUnit {
     static constexpr uint32_t V = VxVec<T>::V;
     VxVec<T> a, b;  // b: the second half's values of half-layout pairs
+    // SAME: as many loads in every lane (a unit that has no b reads a's place), so that no branch stands between the loads
+    // of several units.
+    template <bool SAME>
     __device__ __forceinline__ void load(const VxRopeTable& t, const T* x, uint32_t u) {
         const uint32_t half = t.rot / 2, pair_units = (t.interleaved ? t.rot : half) / V;
         const uint32_t e = u < pair_units ? u * V : t.rot + (u - pair_units) * V;
         a = vx_get<NT>((const VxVec<T>*)(x + e));
-        if (!t.interleaved && u < pair_units) b = vx_get<NT>((const VxVec<T>*)(x + half + e));
+        if constexpr (SAME) {
+            if (!t.interleaved) b = vx_get<NT>((const VxVec<T>*)(x + (u < pair_units ? half + e : e)));
+        } else if (!t.interleaved && u < pair_units) {
+            b = vx_get<NT>((const VxVec<T>*)(x + half + e));
+        }
     }
     template <class Put>
     __device__ __forceinline__ void turn(const VxRopeTable& t, uint32_t u, const float2* cs, Put put) const {
@@ -131,7 +139,7 @@ __global__ __launch_bounds__(kRopeThreads) void vx_rope_vec_kernel(VxRopeTable t
 #pragma unroll
         for (int k = 0; k < kUnitsAhead; ++k) {
             const uint32_t j = i + k * step, w = j / x.heads, h = j % x.heads;
-            if (j < total) v[k].load(t, (const T*)x.data + (size_t)(row0 + w) * x.rs + (size_t)h * x.hs, u);
+            if (j < total) v[k].template load<false>(t, (const T*)x.data + (size_t)(row0 + w) * x.rs + (size_t)h * x.hs, u);
         }
     };
     const uint32_t u0 = threadIdx.x % units, i0 = threadIdx.x / units < step ? threadIdx.x / units : total;
@@ -197,16 +205,18 @@ __device__ __forceinline__ VxSpan vx_span(const uint32_t* q_start, const uint32_
 struct VxBlock {
     uint32_t row0, n, i0, pos;  // rows row0 .. row0 + n at places i0 .. of the block, positions pos ..
     uint32_t in_page, page;     // the block's place in its page; no page: >= n_pages
+    uint32_t seq;
 };
 // Block `item` of the batch, blocks counted over the sequences in order; false behind the last. Every wave walks the
-// sequences 64 at a time.
+// sequences 64 at a time. One row each (no q_start): which row it is does not wait for the length; the rest is
+// vx_block_place's.
 __device__ __forceinline__ bool vx_block(const VxAppendArgs& a, uint32_t item, VxBlock& b) {
     const uint32_t lane = threadIdx.x & 63u;
     uint32_t seq = item, blk = 0;
     VxSpan r;
     if (!a.q_start) {
-        r = vx_span(a.q_start, a.c.lens, a.n_rows, item);
-        if (r.pos0 < 0) return false;
+        b = VxBlock{item, 1, 0, 0, 0, kVxNoPage, item};
+        return true;
     } else {
         uint32_t base = 0;
         bool found = false;
@@ -242,31 +252,43 @@ __device__ __forceinline__ bool vx_block(const VxAppendArgs& a, uint32_t item, V
     }
     const int64_t from = r.pos0 > 0 ? r.pos0 : 0, end = r.pos0 + (r.hi - r.lo);
     const int64_t p0 = ((from >> 5) + blk) << 5;  // the block's first position
-    const uint64_t pi = (uint64_t)p0 / a.c.page_size;
+    const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+    const uint32_t i0 = (uint32_t)((from > p0 ? from : p0) - p0), n = (uint32_t)((end < p0 + 32 ? end : p0 + 32) - p0) - i0;
+    b = VxBlock{uniform(r.lo + (uint32_t)(p0 + i0 - r.pos0)), uniform(n), uniform(i0), uniform((uint32_t)p0 + i0), 0, kVxNoPage, uniform(seq)};
+    return true;
+}
+// The block's position (one row each: the length's last) and page; false: in front of position 0.
+__device__ __forceinline__ bool vx_block_place(const VxAppendArgs& a, VxBlock& b) {
+    if (!a.q_start) {
+        const uint32_t len = vx_word(a.c.lens + b.seq);
+        if (!len) return false;
+        b.pos = len - 1;
+        b.i0 = b.pos & 31u;
+    }
+    const uint32_t p0 = b.pos - b.i0, pi = p0 / a.c.page_size;
     b.page = kVxNoPage;
-    if (pi < a.c.max_pages) b.page = a.c.table[(size_t)seq * a.c.table_stride + pi];
-    b.i0 = (uint32_t)((from > p0 ? from : p0) - p0);
-    b.n = (uint32_t)((end < p0 + 32 ? end : p0 + 32) - p0) - b.i0;
-    b.row0 = r.lo + (uint32_t)(p0 + b.i0 - r.pos0);
-    b.pos = (uint32_t)(p0 + b.i0);
-    b.in_page = (uint32_t)((uint64_t)p0 % a.c.page_size);
+    if (pi < a.c.max_pages) b.page = vx_word(a.c.table + (size_t)b.seq * a.c.table_stride + pi);
+    b.in_page = p0 - pi * a.c.page_size;
     return true;
 }
 // The block's page: its K, V behind; NULL: none.
 __device__ __forceinline__ uint16_t* vx_page(const VxAppendArgs& a, const VxBlock& b) {
     return b.page < a.c.n_pages ? (uint16_t*)(a.c.pool + (size_t)b.page * a.c.page_bytes) : nullptr;
 }
-// cos and sin of the block's rows w0 .. w1.
-__device__ __forceinline__ void vx_angles(const VxRopeTable& t, const VxBlock& b, uint32_t w0, uint32_t w1,
+// cos and sin of the block's rows w0 .. w1; freq: t.turns[threadIdx.x % half], where there are pairs.
+__device__ __forceinline__ void vx_angles(const VxRopeTable& t, const VxBlock& b, uint32_t w0, uint32_t w1, double freq,
                                           float2 (*cs)[kVxMaxRopePairs / 2]) {
-    const uint32_t half = t.rot / 2;
-    for (uint32_t i = threadIdx.x; i < (w1 - w0) * half; i += 256) cs[w0 + i / half][i % half] = vx_turn(t, i % half, b.pos + w0 + i / half);
+    const uint32_t half = t.rot / 2, n = (w1 - w0) * half;
+    if (threadIdx.x < n) cs[w0 + threadIdx.x / half][threadIdx.x % half] = vx_turn_of(t, freq, b.pos + w0 + threadIdx.x / half);
+    for (uint32_t i = threadIdx.x + 256; i < n; i += 256) cs[w0 + i / half][i % half] = vx_turn(t, i % half, b.pos + w0 + i / half);
     __syncthreads();
 }
 
-// Bound by its bytes: 8540 rows of Llama-3-8B's q, k and v (bf16, 210 MB moved) take 47 us (4.5 TB/s), one row each of 32
-// sequences of Qwen2.5-7B 5 us (latency). T: the rows' type, C: the cache's. K and q by units of 16 bytes; V by 8 dimensions of the 8 positions that share
-// 16 bytes of a V block, transposed in registers, so that whole blocks leave as whole lines.
+// Bound by its bytes: 8540 rows of Llama-3-8B's q, k and v (bf16, 210 MB moved) take 43 us (4.8 TB/s), one row each of 32
+// sequences of Qwen2.5-7B 3.8 us, a launch and the length, the page number and a line behind each other (47 and 4.6 us
+// while branches around the loads made them wait for each other). T: the rows' type, C: the cache's. K and q by units
+// of 16 bytes; V by 8 dimensions of the 8 positions that share 16 bytes of a V block, transposed in registers, so that
+// whole blocks leave as whole lines.
 template <class T, class C, bool NT>
 __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxAppendArgs a) {
     constexpr int V = VxVec<T>::V;
@@ -280,20 +302,63 @@ __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxApp
     const uint32_t all = b.n * heads, from = all * blockIdx.y / gridDim.y, total = all * (blockIdx.y + 1) / gridDim.y;
     const uint32_t i0 = mine < step ? from + mine : total;
     VxUnit<T, NT> v[kUnitsAhead];
-    const auto load = [&](uint32_t i) {
+    // pinned: the compiler would otherwise choose between their addresses and read them lane by lane, between the loads
+    typedef const T __attribute__((address_space(1)))* Global;
+    Global qp = (Global)a.q.data, kp = (Global)a.k.data;
+    uint64_t qrs = a.q.rs, qhs = a.q.hs, krs = a.k.rs, khs = a.k.hs;
+    asm volatile("" : "+s"(qp), "+s"(kp), "+s"(qrs), "+s"(qhs), "+s"(krs), "+s"(khs));
+    const auto load = [&](uint32_t base, uint32_t i) {  // base: i of the first thread
 #pragma unroll
         for (int k = 0; k < kUnitsAhead; ++k) {
-            const uint32_t j = i + k * step, w = j / heads, h = j % heads;
-            const T* x = h < hq ? (const T*)a.q.data + (size_t)(b.row0 + w) * a.q.rs + (size_t)h * a.q.hs
-                                : (const T*)a.k.data + (size_t)(b.row0 + w) * a.k.rs + (size_t)(h - hq) * a.k.hs;
-            if (j < total) v[k].load(t, x, u);
+            if (base + k * step >= total) continue;
+            const uint32_t j = min(i + k * step, total - 1), w = j / heads, h = j % heads;
+            const bool is_q = h < hq;
+            const Global x = (is_q ? qp : kp) + (size_t)(b.row0 + w) * (is_q ? qrs : krs) + (size_t)(is_q ? h : h - hq) * (is_q ? qhs : khs);
+            v[k].template load<true>(t, (const T*)x, u);
         }
     };
-    load(i0);  // on its way while the angles are formed
-    vx_angles(t, b, from / heads, (total + heads - 1) / heads, cs);
+    const double freq = t.rot ? t.turns[threadIdx.x % (t.rot / 2)] : 0.0;
+    load(from, i0);  // on its way while the block is placed, V moved and the angles formed
+    if (!vx_block_place(a, b)) return;
     uint16_t* const page = vx_page(a, b);
-    for (uint32_t i = i0; i < total; i += kUnitsAhead * step) {
-        if (i != i0) load(i);
+    const uint32_t groups = d / 8, pieces = page ? hkv * groups * 4 : 0;  // a head's pieces lie in one run: whole rows, whole blocks
+    const uint32_t v_to = pieces * (blockIdx.y + 1) / gridDim.y;
+    for (uint32_t i = pieces * blockIdx.y / gridDim.y + 255 - threadIdx.x; i < v_to; i += 256) {  // the last threads first: with few rows the others turn
+        const uint32_t e0 = i % groups * 8, j = i / groups % 4, h = i / groups / 4;  // slots 8 j .. 8 j + 7 of 8 dimensions
+        VxVec<T> y[8][8 / V];  // all requested before one is looked at
+        uint32_t there = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t p = 16 * (k >> 2) + 4 * j + (k & 3);  // the position of slot 8 j + k
+            const uint32_t w = min(max(p, b.i0) - b.i0, b.n - 1);  // of slots without a row another's (a branch would be a wait)
+            there |= (uint32_t)(p - b.i0 < b.n) << k;
+            const T* from = (const T*)a.v.data + (size_t)(b.row0 + w) * a.v.rs + (size_t)h * a.v.hs + e0;
+#pragma unroll
+            for (int q = 0; q < 8 / V; ++q) y[k][q] = ((const VxVec<T>*)from)[q];
+        }
+        const auto x = [&](int k, int e) { return (C)(float)y[k][e / V].v[e % V]; };
+        C* to = (C*)page + ((size_t)(hkv + h) * a.c.page_size + b.in_page) * d + e0 * 32 + 8 * j;
+        if (there == 255u) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                struct alignas(16) Out {
+                    C v[8];
+                } o;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) o.v[k] = x(k, e);
+                *(Out*)(to + e * 32) = o;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (there >> k & 1)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) to[e * 32 + k] = x(k, e);
+        }
+    }
+    vx_angles(t, b, from / heads, (total + heads - 1) / heads, freq, cs);
+    for (uint32_t base = from, i = i0; base < total; base += kUnitsAhead * step, i += kUnitsAhead * step) {
+        if (base != from) load(base, i);
 #pragma unroll
         for (int k = 0; k < kUnitsAhead; ++k) {
             const uint32_t j = i + k * step, w = j / heads, h = j % heads;
@@ -307,54 +372,14 @@ __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxApp
             }
         }
     }
-    if (!page) return;
-    const uint32_t groups = d / 8, pieces = hkv * groups * 4;  // a head's pieces lie in one run: whole rows, whole blocks
-    const uint32_t v_to = pieces * (blockIdx.y + 1) / gridDim.y;
-    for (uint32_t i = pieces * blockIdx.y / gridDim.y + threadIdx.x; i < v_to; i += 256) {
-        const uint32_t e0 = i % groups * 8, j = i / groups % 4, h = i / groups / 4;  // slots 8 j .. 8 j + 7 of 8 dimensions
-        C x[8][8];
-        uint32_t there = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t p = 16 * (k >> 2) + 4 * j + (k & 3);  // the position of slot 8 j + k
-            if (p - b.i0 < b.n) {
-                there |= 1u << k;
-                const T* from = (const T*)a.v.data + (size_t)(b.row0 + p - b.i0) * a.v.rs + (size_t)h * a.v.hs + e0;
-#pragma unroll
-                for (int q = 0; q < 8 / V; ++q) {
-                    const VxVec<T> y = ((const VxVec<T>*)from)[q];
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[k][q * V + e] = (C)(float)y.v[e];
-                }
-            }
-        }
-        C* to = (C*)page + ((size_t)(hkv + h) * a.c.page_size + b.in_page) * d + e0 * 32 + 8 * j;
-        if (there == 255u) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                struct alignas(16) Out {
-                    C v[8];
-                } o;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) o.v[k] = x[k][e];
-                *(Out*)(to + e * 32) = o;
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (there >> k & 1)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) to[e * 32 + k] = x[k][e];
-        }
-    }
 }
 
 // The same value by value, for rows of several types or without 16-byte alignment, and pairs that do not fill vectors.
 __global__ __launch_bounds__(256) void vx_append_rows_kernel(VxRopeTable t, VxAppendArgs a) {
     __shared__ float2 cs[32][kVxMaxRopePairs / 2];
     VxBlock b;
-    if (!vx_block(a, blockIdx.x, b)) return;
-    vx_angles(t, b, 0, b.n, cs);
+    if (!vx_block(a, blockIdx.x, b) || !vx_block_place(a, b)) return;
+    vx_angles(t, b, 0, b.n, t.rot ? t.turns[threadIdx.x % (t.rot / 2)] : 0.0, cs);
     uint16_t* const kp = vx_page(a, b);
     uint16_t* const vp = kp + (size_t)a.c.hkv * a.c.page_size * a.c.d;
     const uint32_t half = t.rot / 2, d = a.c.d, hkv = a.c.hkv, hq = a.q.data ? a.q.heads : 0, heads = hq + 2 * hkv;
@@ -770,7 +795,9 @@ hipError_t vx_launch_rope_append(const VxRopeTable& t, const VxAppendArgs& a, hi
     // a sequence's rows touch at most rows / 32 + 2 blocks
     const uint64_t bound = (uint64_t)a.n_rows / 32 + 2ull * a.c.n_seqs;
     const uint32_t blocks = (uint32_t)(bound < a.n_rows ? bound : a.n_rows);
-    const dim3 grid(blocks, 8);
+    // Heads are shared out over 8 workgroups of a block; over 2 where there are many blocks of few rows (one row each of 512
+    // sequences of Qwen2.5-7B 15.5 us by 8, 8.3 by 2; of 8 sequences 3.6 and 3.8; prompts of 8540 rows 43.6 and 51.6).
+    const dim3 grid(blocks, blocks > 64 && a.n_rows < 4 * (uint64_t)blocks ? 2 : 8);
     const bool vec = (!a.q.data || (vx_vec_rows(a.q) && vx_vec_rows(a.qo) && a.q.dtype == a.k.dtype)) && vx_vec_rows(a.k) &&
                      vx_vec_rows(a.v) && a.k.dtype == a.v.dtype && vx_vec_pairs(t, a.k.dtype, a.c.d);
     if (!vec) vx_append_rows_kernel<<<grid, 256, 0, st>>>(t, a);

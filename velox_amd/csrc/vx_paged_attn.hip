@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
     // q: column col is head h0 + col. The requests go out first; the first chunk's follow before q is widened.
     VxEight raw[NC] = {};
     if (col < gn) vx_request<QT == 1>(raw, a.q.data, (size_t)seq * a.q.rs + (size_t)(h0 + col) * a.q.hs + 8 * grp, 32, a.q.dtype);
-    const int64_t t = (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)a.c.lens[seq]) - 1;
+    const int64_t t = (int64_t)vx_word(a.c.lens + seq) - 1;
     const VxChunks ch = vx_chunks(t, t, a.window, a.sinks, (uint64_t)a.c.max_pages * a.c.page_size);
     const uint32_t per = (ch.n + a.splits - 1) / a.splits;
     const uint32_t c0 = min(split * per, ch.n), c1 = min(c0 + per, ch.n);
