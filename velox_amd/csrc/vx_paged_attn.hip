@@ -147,7 +147,7 @@ __device__ __forceinline__ uint32_t vx_chunk_base(const VxChunks& c, uint32_t i)
 // head's largest value is brought to 2^13 first, so that the second term stays in range), the weights as PT.
 // Bound by the bytes of K and V where there are many: 4 sequences of 91000 to 131000 positions of Llama-3-8B's heads 292 us
 // (6.7 TB/s); by latency (lengths, table, first chunk, the join) below: 32 sequences of 600 to 2100 positions of
-// Qwen2.5-7B's heads (90 MB) 20.2 us, one SmolLM sequence of 700 7.5 us (21.7 and 8.6 while the waits for a chunk were
+// Qwen2.5-7B's heads (90 MB) 20.1 us, one SmolLM sequence of 700 7.5 us (21.7 and 8.6 while the waits for a chunk were
 // waits for the next one too). Four waves: eight were slower (25.4 against 22.9 us for 32 sequences of 1500).
 // Non-temporal loads (NT) where the caches cannot hold the K and V anyway: Llama-3-8B's heads, 4 sequences of 91000 to
 // 131000 positions 330 -> 292 us (5.9 -> 6.7 TB/s); 32 sequences of Qwen2.5-7B (90 MB, in the memory-side cache from
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
     // q: column col is head h0 + col. The requests go out first; the first chunk's follow before q is widened.
     VxEight raw[NC] = {};
     if (col < gn) vx_request<QT == 1>(raw, a.q.data, (size_t)seq * a.q.rs + (size_t)(h0 + col) * a.q.hs + 8 * grp, 32, a.q.dtype);
-    const int64_t t = (int64_t)vx_word(a.c.lens + seq) - 1;
+    const int64_t t = (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)a.c.lens[seq]) - 1;
     const VxChunks ch = vx_chunks(t, t, a.window, a.sinks, (uint64_t)a.c.max_pages * a.c.page_size);
     const uint32_t per = (ch.n + a.splits - 1) / a.splits;
     const uint32_t c0 = min(split * per, ch.n), c1 = min(c0 + per, ch.n);
@@ -377,28 +377,28 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
     }
 }
 
-// Joins a row's splits: a workgroup per (row, head), each of its waves over a quarter of the splits (3.9 us for 32 rows of
-// 28 heads, 4.1 with one wave for all of them; a launch's latency). Of a prompt's
+// Joins a row's splits: a workgroup per (row, head), each of its waves over a quarter of the splits (2.7 to 4 us for
+// 32 rows of 28 heads, a launch's latency; maxima and sums are requested first: they are joined while the rest arrives). Of a prompt's
 // rows, those of no sequence and those in front of position 0 (their sums say -1) are passed over.
 template <int D>
 __global__ __launch_bounds__(256) void vx_paged_join_kernel(VxPagedAttnArgs a) {
     constexpr int N = D / 64;
     __shared__ float s_acc[4][D];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t row = blockIdx.x / a.q.heads, h = blockIdx.x % a.q.heads;
     const float* ml = a.part_ml + 2 * (size_t)blockIdx.x * a.splits;
-    if (a.q_start && (row < a.q_start[0] || row >= a.q_start[a.c.n_seqs] || ml[1] < 0.0f)) return;
+    float m = -INFINITY, sum = 0.0f;
+    if (lane < a.splits) {  // at most 64; first, so that they are joined while the sums arrive
+        m = ml[2 * lane];
+        sum = ml[2 * lane + 1];
+    }
+    if (a.q_start && (row < vx_word(a.q_start) || row >= vx_word(a.q_start + a.c.n_seqs) || ml[1] < 0.0f)) return;
     const float* po = a.part_o + (size_t)blockIdx.x * a.splits * D + lane * N;
     const uint32_t per = (a.splits + 3) / 4, s0 = min(wave * per, a.splits), s1 = min(s0 + per, a.splits);
     float v[16][N];  // per <= 16; requested before the weights are known
 #pragma unroll
     for (int i = 0; i < 16; ++i)
         if (s0 + i < s1) __builtin_memcpy(v[i], po + (size_t)(s0 + i) * D, 4 * N);
-    float m = -INFINITY, sum = 0.0f;
-    if (lane < a.splits) {  // at most 64
-        m = ml[2 * lane];
-        sum = ml[2 * lane + 1];
-    }
     float top = m;
 #pragma unroll
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
