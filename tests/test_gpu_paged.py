@@ -265,6 +265,27 @@ def test_prompt_attention_few_rows_behind_a_long_context():
                 f.check(x[start[s]:start[s + 1]], out[start[s]:start[s + 1]], s, 0, window, sinks, q == "bf16")
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows, n", [(1100, 8000), (2000, 2100), (40, 1700), (9, 40000)])
+def test_prompt_attention_in_few_and_many_splits(d, rows, n):
+    f = Filled([n], 2, d, 64, "bf16")
+    x = queries(rows, 4, 2, d, "bf16")
+    space = f.cache.prompt_workspace(4, total_rows=rows)
+    assert space is not None
+    out = paged.prompt_attention(f.cache, 0, x, ints([0, rows]), workspace=space)
+    f.check(x, out, 0, 0, 0, 0, True)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens", [[2000] * 6, [1000] * 40, [30000, 7], [3000] * 30])
+def test_token_attention_in_few_and_many_splits(d, lens):
+    f = Filled(lens, 2, d, 64, "bf16")
+    x = queries(len(lens), 4, 2, d, "f32")
+    out = paged.attention(f.cache, 0, x)
+    for s in range(len(lens)):
+        f.check(x[s:s + 1], out[s:s + 1], s, 0, 0, 0, False)
+
+
 def test_prompt_rows_in_front_of_position_0_stay():
     f = Filled([4], 2, 64, 32, "bf16")
     x = queries(10, 4, 2, 64, "bf16")

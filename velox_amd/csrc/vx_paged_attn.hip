@@ -377,35 +377,40 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
     }
 }
 
-// Joins a row's splits: a workgroup per (row, head), each of its waves over a quarter of the splits (2.7 to 4 us for
-// 32 rows of 28 heads, a launch's latency; maxima and sums are requested first: they are joined while the rest arrives). Of a prompt's
+// Joins a row's splits: W waves for a (row, head), each over its part of the splits: one where there are few splits or many
+// rows, which then take few workgroups and no barrier (2000 prompt rows of SmolLM in 3 splits, both kernels, 29 us by one,
+// 43 by four), else four (4 sequences of 2000 positions of Llama-3-8B in 8 splits 9.9 us, by one 10.3). A launch's
+// latency where there are few. Maxima and sums are requested first: they are joined while the rest arrives. Of a prompt's
 // rows, those of no sequence and those in front of position 0 (their sums say -1) are passed over.
-template <int D>
-__global__ __launch_bounds__(256) void vx_paged_join_kernel(VxPagedAttnArgs a) {
+template <int D, int W>
+__global__ __launch_bounds__(256) void vx_paged_join_kernel(VxPagedAttnArgs a, uint32_t items) {
     constexpr int N = D / 64;
-    __shared__ float s_acc[4][D];
+    __shared__ float s_acc[W == 4 ? 4 : 1][D];
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t row = blockIdx.x / a.q.heads, h = blockIdx.x % a.q.heads;
-    const float* ml = a.part_ml + 2 * (size_t)blockIdx.x * a.splits;
+    const uint32_t item = W == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
+    if (item >= items) return;
+    const uint32_t row = item / a.q.heads, h = item % a.q.heads;
+    const float* ml = a.part_ml + 2 * (size_t)item * a.splits;
     float m = -INFINITY, sum = 0.0f;
-    if (lane < a.splits) {  // at most 64; first, so that they are joined while the sums arrive
+    if (lane < a.splits) {  // at most 64 (W 1: 16)
         m = ml[2 * lane];
         sum = ml[2 * lane + 1];
     }
     if (a.q_start && (row < vx_word(a.q_start) || row >= vx_word(a.q_start + a.c.n_seqs) || ml[1] < 0.0f)) return;
-    const float* po = a.part_o + (size_t)blockIdx.x * a.splits * D + lane * N;
-    const uint32_t per = (a.splits + 3) / 4, s0 = min(wave * per, a.splits), s1 = min(s0 + per, a.splits);
+    const float* po = a.part_o + (size_t)item * a.splits * D + lane * N;
+    const uint32_t per = (a.splits + W - 1) / W, s0 = W == 4 ? min(wave * per, a.splits) : 0u, s1 = min(s0 + per, a.splits);
     float v[16][N];  // per <= 16; requested before the weights are known
 #pragma unroll
     for (int i = 0; i < 16; ++i)
         if (s0 + i < s1) __builtin_memcpy(v[i], po + (size_t)(s0 + i) * D, 4 * N);
     float top = m;
 #pragma unroll
-    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    for (int x = W == 4 ? 32 : 8; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
     sum *= f;
 #pragma unroll
-    for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+    for (int x = W == 4 ? 32 : 8; x; x >>= 1) sum += __shfl_xor(sum, x);
+    sum = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sum)));
     float acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0f;
@@ -416,19 +421,25 @@ __global__ __launch_bounds__(256) void vx_paged_join_kernel(VxPagedAttnArgs a) {
 #pragma unroll
             for (int e = 0; e < N; ++e) acc[e] += w * v[i][e];
         }
-#pragma unroll
-    for (int e = 0; e < N; ++e) s_acc[wave][lane * N + e] = acc[e];
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < D; e += 256) {
-        const float o = (s_acc[0][e] + s_acc[1][e]) + (s_acc[2][e] + s_acc[3][e]);
+    const auto put = [&](uint32_t e, float o) {
         vx_store(a.out.data, (size_t)row * a.out.rs + (size_t)h * a.out.hs + e, a.out.dtype, sum != 0.0f ? o / sum : 0.0f);
+    };
+    if constexpr (W == 4) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) s_acc[wave][lane * N + e] = acc[e];
+        __syncthreads();
+        for (uint32_t e = threadIdx.x; e < D; e += 256) put(e, (s_acc[0][e] + s_acc[1][e]) + (s_acc[2][e] + s_acc[3][e]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) put(lane * N + e, acc[e]);
     }
 }
 
 hipError_t launch_join(const VxPagedAttnArgs& a, hipStream_t st) {
-    const uint64_t items = (uint64_t)a.n_rows * a.q.heads;
-    if (a.c.d == 64) vx_paged_join_kernel<64><<<(uint32_t)items, 256, 0, st>>>(a);
-    else vx_paged_join_kernel<128><<<(uint32_t)items, 256, 0, st>>>(a);
+    const uint32_t items = a.n_rows * a.q.heads;
+    const auto go = [&](auto kernel, uint32_t grid) { kernel<<<grid, 256, 0, st>>>(a, items); };
+    if (a.splits > 16 || (a.splits > 4 && items < 4096)) go(a.c.d == 64 ? vx_paged_join_kernel<64, 4> : vx_paged_join_kernel<128, 4>, items);
+    else go(a.c.d == 64 ? vx_paged_join_kernel<64, 1> : vx_paged_join_kernel<128, 1>, (items + 3) / 4);
     return hipGetLastError();
 }
 
@@ -541,6 +552,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kBuf];  // K of two steps, V of two steps
     __shared__ uint32_t s_found;  // settle: 1 + the first chunk of the last step with infinities or NaN, else 0
     if (threadIdx.x == 0) s_found = 0;
+    // read anew, as LDS: a generic read would wait for the loads in flight too
+    const auto found_now = [&] { return *(volatile __attribute__((address_space(3))) uint32_t*)&s_found; };
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t col = lane & 31u, grp = lane >> 5;
     const uint32_t G = a.q.heads / a.c.hkv, kvh = blockIdx.x % a.c.hkv;
@@ -757,7 +770,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
         }
         if (found & 0x80008000u) s_found = x.chunk + 1;
         vx_barrier();
-        if (*(volatile uint32_t*)&s_found != x.chunk + 1) return;
+        if (found_now() != x.chunk + 1) return;
         for (uint32_t i = threadIdx.x; i < 2 * D * 32; i += kPromptThreads) {
             uint16_t* h = (uint16_t*)vb + i;
             if ((*h & E::kExp) == E::kExp) *h = 0;
@@ -870,7 +883,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
         vx_wait_loads<0>();  // nothing may land in LDS that is another workgroup's by then
     }
 
-    if (n_steps && *(volatile uint32_t*)&s_found) {  // infinities and NaN that settle took out, value by value from the pages
+    if (n_steps && found_now()) {  // infinities and NaN that settle took out, value by value from the pages
 #pragma unroll 1
         for (uint32_t i = 0; i < n_steps; ++i) {
             if (i == 0 || i - first >= 32) look_up(i);
