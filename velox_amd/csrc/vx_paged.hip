@@ -473,9 +473,10 @@ struct VxRefs8 {
 
 // One workgroup: who needs what (a thread per sequence, or four), the lowest free pages (a scan of refs that ends
 // when it has enough), then a thread per page given out. What bounds it is the chain of dependent loads -- length,
-// last page, its count -- and a dozen barriers: 8 sequences take 6 us, 64 that share pages 9 us, so the scan's first pages are
-// requested at the start, and the pages found stay in LDS.
+// last page, its count -- and a dozen barriers: 8 sequences take 6.2 us, 64 that share pages 8.8 us, so the scan's first
+// pages are requested at the start, and the pages found stay in LDS.
 constexpr uint32_t kPerThread = kVxMaxPagedSeqs / kPageThreads;
+constexpr uint32_t kLooked = 64;
 constexpr uint32_t kListed = 4096;  // pages found that LDS holds; the rest lie in the scratch memory
 
 __global__ __launch_bounds__(kPageThreads) void vx_pages_extend_kernel(VxPages p, const uint32_t* __restrict__ add) {
@@ -522,6 +523,28 @@ __global__ __launch_bounds__(kPageThreads) void vx_pages_extend_kernel(VxPages p
         any |= spot != kVxNoPage;
     }
     any = __syncthreads_or(any);
+    // how many write into a shared page, and the last of them: among few sequences each looks at all the others (8: 6.2 us,
+    // by counting 7.3), else they are counted in the moves' memory, a word a page (4096 that share by twos, launches and
+    // copies included: 39 us, by looking 584; 200: 16 and 20)
+    const bool counted = any && n > kLooked;
+    if (counted) {
+#pragma unroll
+        for (uint32_t k = 0; k < kPerThread; ++k)
+            if (a0 + k < a1 && s_spot[a0 + k] != kVxNoPage) {
+                __hip_atomic_store(src + s_spot[a0 + k], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(dst + s_spot[a0 + k], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // there before anyone counts: a barrier alone waits for LDS only
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < kPerThread; ++k)
+            if (a0 + k < a1 && s_spot[a0 + k] != kVxNoPage) {
+                atomicAdd(src + s_spot[a0 + k], 1u);
+                atomicMax(dst + s_spot[a0 + k], a0 + k);
+            }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
     uint32_t mine = 0;
 #pragma unroll
     for (uint32_t k = 0; k < kPerThread; ++k) {
@@ -531,14 +554,17 @@ __global__ __launch_bounds__(kPageThreads) void vx_pages_extend_kernel(VxPages p
             mine += pages_of((uint64_t)len[k] + grow[k]) - pages_of(len[k]);
             const uint32_t spot = s_spot[s];
             if (any && spot != kVxNoPage) {
-                uint32_t same = 0;
-                bool later = false;
-                for (uint32_t j = 0; j < n; ++j) {
-                    const bool eq = s_spot[j] == spot;
-                    same += eq;
-                    later |= eq && j > s;
+                uint32_t same = 0, last = 0;
+                if (counted) {
+                    same = __hip_atomic_load(src + spot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    last = __hip_atomic_load(dst + spot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
-                if (later || same != refs_of[k]) {  // else it is the last of all its holders and keeps the page
+                for (uint32_t j = 0; j < n && !counted; ++j)
+                    if (s_spot[j] == spot) {
+                        ++same;
+                        last = j;
+                    }
+                if (last != s || same != refs_of[k]) {  // else it is the last of all its holders and keeps the page
                     s_old[s] |= 0x80000000u;
                     ++mine;
                 }
