@@ -46,8 +46,11 @@ def _call(fn, index: int, *args) -> None:
         L.check(rc, fn.__name__)
 
 
-def _like(t: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
+def _like(t: torch.Tensor, r: L.Rows, dim: int) -> tuple[torch.Tensor, L.Rows]:
+    """A new tensor of t's shape and type, and its rows; r: t's."""
+    out = torch.empty_like(t, memory_format=torch.contiguous_format)
+    h = r.heads
+    return out, L.Rows(out.data_ptr(), r.dtype, h, h * dim, dim)
 
 
 def _words(t: torch.Tensor, n: int, device: torch.device, what: str) -> int:
@@ -208,11 +211,12 @@ def rope(turn: Rope, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor
     """x [row][head][element] turned by positions (int32 [row]); out: x itself, or a tensor of its shape and type."""
     device = _gpu(x, "x")
     _need(bool(turn.handle), "rope: the handle is closed")
-    if out is None:
-        out = _like(x)
     xr, n = _rows(x, device, "x")
-    o, _ = _rows(out, device, "out")
-    _need(out.shape == x.shape and out.dtype == x.dtype, "out: the shape and type of x are wanted")
+    if out is None:
+        out, o = _like(x, xr, x.shape[2])
+    else:
+        o, _ = _rows(out, device, "out")
+        _need(out.shape == x.shape and out.dtype == x.dtype, "out: the shape and type of x are wanted")
     at = _words(positions, n, device, "positions")
     if x.numel():
         _call(turn.lib.velox_hip_rope_rows, device.index, turn.handle, xr, o, n, x.shape[2], at)
@@ -233,8 +237,10 @@ def rope_append(cache: PagedCache, layer: int, turn: Rope | None, q: torch.Tenso
     if q is not None:
         qr, qn = _rows(q, device, "q", 0, d)
         if q_out is None:
-            q_out = _like(q)
-        qo, on = _rows(q_out, device, "q_out", qr.heads, d)
+            on = qn
+            q_out, qo = _like(q, qr, d)
+        else:
+            qo, on = _rows(q_out, device, "q_out", qr.heads, d)
         _need(qn == n and on == n, "q and q_out: as many rows as k are wanted")
     else:
         _need(q_out is None, "q_out without q")
@@ -245,7 +251,12 @@ def rope_append(cache: PagedCache, layer: int, turn: Rope | None, q: torch.Tenso
     return q_out
 
 
+_WHOLE = L.AttnMask(0, 0)
+
+
 def _mask(window: int, sinks: int) -> L.AttnMask:
+    if window == 0 and sinks >= 0:
+        return _WHOLE  # sinks do nothing without a window
     _need(window >= 0 and sinks >= 0, "window and sinks have to be at least 0")
     return L.AttnMask(min(window, 0xFFFFFFFF), min(sinks, 0xFFFFFFFF))
 
@@ -267,9 +278,10 @@ def attention(cache: PagedCache, layer: int, q: torch.Tensor, *, window: int = 0
     qr, n = _rows(q, device, "q", 0, cache.head_dim)
     _need(n == cache.n_seqs, f"q: {cache.n_seqs} rows are wanted")
     if out is None:
-        out = _like(q)
-    o, on = _rows(out, device, "out", qr.heads, cache.head_dim)
-    _need(on == n, "out: as many rows as q are wanted")
+        out, o = _like(q, qr, cache.head_dim)
+    else:
+        o, on = _rows(out, device, "out", qr.heads, cache.head_dim)
+        _need(on == n, "out: as many rows as q are wanted")
     if workspace is None:
         workspace = cache.attention_workspace(qr.heads, max_len=max_len)
     space, size = _space(workspace, device)
@@ -286,9 +298,10 @@ def prompt_attention(cache: PagedCache, layer: int, q: torch.Tensor, q_start: to
     _need(layer >= 0 and max_len >= 0 and max_rows >= 0, "layer, max_rows and max_len have to be at least 0")
     qr, n = _rows(q, device, "q", 0, cache.head_dim)
     if out is None:
-        out = _like(q)
-    o, on = _rows(out, device, "out", qr.heads, cache.head_dim)
-    _need(on == n, "out: as many rows as q are wanted")
+        out, o = _like(q, qr, cache.head_dim)
+    else:
+        o, on = _rows(out, device, "out", qr.heads, cache.head_dim)
+        _need(on == n, "out: as many rows as q are wanted")
     start = _words(q_start, cache.n_seqs + 1, device, "q_start")
     if n == 0:
         return out
