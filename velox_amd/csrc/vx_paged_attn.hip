@@ -147,7 +147,7 @@ __device__ __forceinline__ uint32_t vx_chunk_base(const VxChunks& c, uint32_t i)
 // head's largest value is brought to 2^13 first, so that the second term stays in range), the weights as PT.
 // Bound by the bytes of K and V where there are many: 4 sequences of 91000 to 131000 positions of Llama-3-8B's heads 292 us
 // (6.7 TB/s); by latency (lengths, table, first chunk, the join) below: 32 sequences of 600 to 2100 positions of
-// Qwen2.5-7B's heads (90 MB) 20.1 us, one SmolLM sequence of 700 7.5 us (21.7 and 8.6 while the waits for a chunk were
+// Qwen2.5-7B's heads (90 MB) 19.6 us, one SmolLM sequence of 700 7.5 us (21.7 and 8.6 while the waits for a chunk were
 // waits for the next one too). Four waves: eight were slower (25.4 against 22.9 us for 32 sequences of 1500).
 // Non-temporal loads (NT) where the caches cannot hold the K and V anyway: Llama-3-8B's heads, 4 sequences of 91000 to
 // 131000 positions 330 -> 292 us (5.9 -> 6.7 TB/s); 32 sequences of Qwen2.5-7B (90 MB, in the memory-side cache from
@@ -462,10 +462,10 @@ hipError_t launch_token(const VxPagedAttnArgs& a, bool nt, hipStream_t st) {
 // 16 t + 8 a + 4 g + b is position 16 a + 8 t + 4 g + b of the chunk (two bits swapped), which puts position
 // order into the order of the pages' V blocks.
 // Bound by the matrix cores and what shares their issue slots: 8192 rows of Llama-3-8B's heads through a window of 4096
-// take 393 us (1050 TFLOP/s of the visible pairs) with the matrix cores busy in 54 % of the clocks, at 1.8 GHz; four chunks
-// of 380 to 500 rows behind 4000 positions of Qwen2.5-7B's heads 123 us (890 TFLOP/s). 64 pairs a wave (616 us), 8 or 2
+// take 388 to 404 us (1020 to 1060 TFLOP/s of the visible pairs) with the matrix cores busy in 54 % of the clocks, at 1.8 GHz; four chunks
+// of 380 to 500 rows behind 4000 positions of Qwen2.5-7B's heads 124 us (880 TFLOP/s). 64 pairs a wave (616 us), 8 or 2
 // waves a workgroup (523, 729 against 471 then) were slower; written orders of products, exponentials and LDS reads took
-// as long (391 to 396 us), so the chip's power is what holds it.
+// as long (391 to 396 us).
 constexpr int kPromptWaves = 4;
 constexpr int kPromptThreads = 64 * kPromptWaves;
 constexpr int kPromptRows = kVxPromptRows;
