@@ -985,7 +985,8 @@ hipError_t vx_launch_paged_attention(const VxPagedAttnArgs& a, hipStream_t st) {
 
 // Splits of the prompt form: where the row tiles alone leave CUs empty, the positions are split until there are two
 // workgroups for each, into parts of 512 positions at least. Rows for a workgroup on every CU are not split: four
-// chunks of 380 to 500 rows behind 4000 positions of Qwen2.5-7B take 171 us and 69 for the join as two splits.
+// chunks of 400 rows behind 4000 positions take 121 us (Qwen2.5-7B) and 127 (Llama-3-8B), as two splits 129 and 150; 2000
+// rows 51 and 53, as two splits 67 and 73. Below that it pays: 2000 rows of SmolLM (141 workgroups) 29 us in three.
 uint32_t vx_paged_prompt_splits(const VxPagedView& c, uint32_t heads, uint32_t n_rows, uint32_t span) {
     const uint64_t g = heads / c.hkv, tiles = ((uint64_t)n_rows * g + kPromptRows - 1) / kPromptRows * c.hkv;
     const uint64_t want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles, most = span / 512;
