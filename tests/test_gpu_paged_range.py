@@ -1,0 +1,55 @@
+"""The paged cache's operators at the sizes that only long or many rows reach, and to the precision that they state,
+against plain float64 computations of the same inputs (tolerances: test_gpu_paged.py's, with the weights' rounding given).
+"""
+import math
+
+import pytest
+import torch
+
+from velox_amd import paged
+from test_gpu_paged import T, Filled, half_step, ints, queries
+
+pytestmark = pytest.mark.gpu
+
+
+def near(f, q, out, seq, weights, window=0, sinks=0, scale=None, small=0.0):
+    """Rows q of sequence seq, the last one its newest position. weights: how far a softmax weight may be off, relative
+    to itself; small: and relative to the row's largest."""
+    n, rows, d = f.lens[seq], q.shape[0], f.d
+    scale = scale or 1 / math.sqrt(d)
+    t = torch.arange(n - rows, n, device="cuda").unsqueeze(1)
+    j = torch.arange(n, device="cuda").unsqueeze(0)
+    hidden = j > t
+    if window:
+        hidden |= (j <= t - window) & (j >= sinks)
+    u, ou = half_step(torch.float32), half_step(out.dtype)
+    for h in range(q.shape[1]):
+        g = h // (q.shape[1] // f.hkv)
+        x, k, v = q[:, h].double(), f.k[seq][:, g].double(), f.v[seq][:, g].double()
+        big = (x.abs() @ k.abs().T * abs(scale)).masked_fill_(hidden, 0.0).amax(1, keepdim=True)
+        p = torch.softmax((x @ k.T * scale).masked_fill_(hidden, -math.inf), 1)
+        o, a = p @ v, p @ v.abs()
+        c = 2 * ((d + 8) * u * big + 2 ** -22 * big) + weights + (n + 64) * u
+        tol = ou * o.abs() * (1 + c) + (c * a + small * n * v.abs().amax()) * (1 + ou) + 1e-30
+        bad = ~((out[:, h].double() - o).abs() <= tol)
+        assert not bad.any(), (seq, h, int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 4)])
+def test_weights_are_held_in_two_terms(t, d, window, sinks):
+    """q of the cache's type, an fp32 output: two terms leave u^2 of a weight (of fp16 weights, times 2^7 against a
+    maximum that is at most 2^8 too low, no less than 2^-25 of that), one would leave u."""
+    lens, rows = [40, 33, 2, 700, 6000], [40, 33, 2, 200, 5]
+    start = [sum(rows[:i]) for i in range(len(rows) + 1)]
+    f = Filled(lens, 2, d, 32, t)
+    x = queries(start[-1], 6, 2, d, t)
+    weights, small = half_step(T[t]) ** 2, 2.0 ** -32 if t == "f16" else 0.0
+    out = torch.empty(start[-1], 6, d, device="cuda")
+    paged.prompt_attention(f.cache, 0, x, ints(start), window=window, sinks=sinks, out=out)
+    last = ints(start[1:]).long() - 1
+    one = paged.attention(f.cache, 0, x[last], window=window, sinks=sinks, out=torch.empty(len(lens), 6, d, device="cuda"))
+    for s in range(len(lens)):
+        near(f, x[start[s]:start[s + 1]], out[start[s]:start[s + 1]], s, weights, window, sinks, small=small)
+        near(f, x[last[s]:last[s] + 1], one[s:s + 1], s, weights, window, sinks, small=small)

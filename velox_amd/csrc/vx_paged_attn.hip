@@ -96,8 +96,6 @@ struct VxBf16 {
     static constexpr uint32_t kExp = 0x7F80u, kOne = 0x0080u;  // the exponent's bits, and the lowest of them
     static constexpr float kUp = 0.0f, kUpTerms = 0.0f;         // the weights are taken times 2^kUp (kUpTerms: in the token form)
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
-    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
-    static __device__ __forceinline__ float sum2(v2 a, float c) { return __builtin_amdgcn_fdot2_f32_bf16(a, v2{(__bf16)1.0f, (__bf16)1.0f}, c, false); }
     static __device__ __forceinline__ vx_f4 mfma(v8 a, v8 b, vx_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ vx_f16 mfma(v8 a, v8 b, vx_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -107,8 +105,6 @@ struct VxF16 {
     // fp16 weights lose bits below 2^-14 and are 0 below 2^-25: they are moved up as far as the largest allows
     static constexpr float kUp = 7.0f, kUpTerms = 14.0f;
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
-    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-    static __device__ __forceinline__ float sum2(v2 a, float c) { return __builtin_amdgcn_fdot2(a, v2{(_Float16)1.0f, (_Float16)1.0f}, c, false); }
     static __device__ __forceinline__ vx_f4 mfma(v8 a, v8 b, vx_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ vx_f16 mfma(v8 a, v8 b, vx_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
@@ -461,9 +457,12 @@ hipError_t launch_token(const VxPagedAttnArgs& a, bool nt, hipStream_t st) {
 // the weights are the B operand of O^T = V^T P^T without leaving their lanes: the K row that scores row
 // 16 t + 8 a + 4 g + b is position 16 a + 8 t + 4 g + b of the chunk (two bits swapped), which puts position
 // order into the order of the pages' V blocks.
+// The weights enter as PT terms of the cache's type (q of that type: two, as in the token form), so that they are off by
+// 2^-16 (bf16) or 2^-22 (fp16) and the output by its own rounding only. One term made half as many products of the
+// weights, 404 and 127 us below, but a bf16 output's error against 64 bits was 1.3 times that rounding.
 // Bound by the matrix cores and what shares their issue slots: 8192 rows of Llama-3-8B's heads through a window of 4096
-// take 388 to 404 us (1020 to 1060 TFLOP/s of the visible pairs) with the matrix cores busy in 54 % of the clocks, at 1.8 GHz; four chunks
-// of 380 to 500 rows behind 4000 positions of Qwen2.5-7B's heads 124 us (880 TFLOP/s). 64 pairs a wave (616 us), 8 or 2
+// take 555 us (740 TFLOP/s of the visible pairs, 1110 with the second terms' products); four chunks of 392 to 500 rows
+// behind 4000 positions of Qwen2.5-7B's heads 179 us. Before the second term 64 pairs a wave (616 us), 8 or 2
 // waves a workgroup (523, 729 against 471 then) were slower; written orders of products, exponentials and LDS reads took
 // as long (391 to 396 us).
 constexpr int kPromptWaves = 4;
@@ -777,8 +776,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
         }
         vx_barrier();
     };
-    // o += V^T P^T of a chunk. Weights of one term are summed as they are rounded, two by two: what the row is divided
-    // by is the sum of what it was made of.
+    // o += V^T P^T of a chunk, the weights as PT terms, never one: rounded once to bf16 (2^-8) or fp16 (2^-11) they would
+    // cost the output as much as its own rounding.
     const auto add = [&](const vx_f16& s, int b, uint32_t buf) {
         const unsigned char* vb = lds + 4 * kChunk + buf * (2 * kChunk) + b * kChunk;
         const float ref = (m == -INFINITY ? 0.0f : m) - E::kUp;
@@ -786,7 +785,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], to_log2, -ref));
-            if constexpr (PT > 1) l += p;
+            l += p;
             float rest = p;
 #pragma unroll
             for (int u = 0; u < PT; ++u) {
@@ -794,10 +793,6 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
                 pf[u][r >> 3][r & 7] = v;
                 rest -= (float)v;
             }
-        }
-        if constexpr (PT == 1) {
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) l = E::sum2(typename E::v2{pf[0][r >> 3][r & 7], pf[0][r >> 3][(r & 7) + 1]}, l);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -997,9 +992,9 @@ uint32_t vx_paged_prompt_splits(const VxPagedView& c, uint32_t heads, uint32_t n
 hipError_t vx_launch_paged_prompt(const VxPagedAttnArgs& a, hipStream_t st) {
     const bool same = a.q.dtype == a.c.dtype, bf16 = a.c.dtype == VELOX_DT_BF16;
     if (a.c.d == 64) {
-        if (bf16) return same ? launch_prompt<VxBf16, 64, 1, 1>(a, st) : launch_prompt<VxBf16, 64, 3, 3>(a, st);
-        return same ? launch_prompt<VxF16, 64, 1, 1>(a, st) : launch_prompt<VxF16, 64, 2, 2>(a, st);
+        if (bf16) return same ? launch_prompt<VxBf16, 64, 1, 2>(a, st) : launch_prompt<VxBf16, 64, 3, 3>(a, st);
+        return same ? launch_prompt<VxF16, 64, 1, 2>(a, st) : launch_prompt<VxF16, 64, 2, 2>(a, st);
     }
-    if (bf16) return same ? launch_prompt<VxBf16, 128, 1, 1>(a, st) : launch_prompt<VxBf16, 128, 3, 3>(a, st);
-    return same ? launch_prompt<VxF16, 128, 1, 1>(a, st) : launch_prompt<VxF16, 128, 2, 2>(a, st);
+    if (bf16) return same ? launch_prompt<VxBf16, 128, 1, 2>(a, st) : launch_prompt<VxBf16, 128, 3, 3>(a, st);
+    return same ? launch_prompt<VxF16, 128, 1, 2>(a, st) : launch_prompt<VxF16, 128, 2, 2>(a, st);
 }
