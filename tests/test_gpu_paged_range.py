@@ -53,3 +53,25 @@ def test_weights_are_held_in_two_terms(t, d, window, sinks):
     for s in range(len(lens)):
         near(f, x[start[s]:start[s + 1]], out[start[s]:start[s + 1]], s, weights, window, sinks, small=small)
         near(f, x[last[s]:last[s] + 1], one[s:s + 1], s, weights, window, sinks, small=small)
+
+
+def test_calls_refuse_tensors_that_require_a_gradient():
+    f = Filled([64, 3], 2, 64, 32, "bf16")
+    c, turn = f.cache, paged.Rope(64)
+    x = torch.randn(2, 4, 64, device="cuda")
+    g = x.clone().requires_grad_()
+    calls = [lambda g: paged.attention(c, 0, g), lambda g: paged.attention(c, 0, x, out=g), lambda g: paged.prompt_attention(c, 0, g, ints([0, 1, 2])),
+             lambda g: paged.rope(turn, g, ints([0, 1])), lambda g: paged.rope_append(c, 0, turn, g, x[:, :2], x[:, 2:]),
+             lambda g: paged.rope_append(c, 0, turn, x, g[:, :2], x[:, 2:]), lambda g: paged.rope_append(c, 0, turn, x, x[:, :2], g[:, 2:])]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call(g)
+    pool = torch.zeros_like(f.pool).requires_grad_()
+    over = lambda: paged.PagedCache.over(pool, f.table, f.cache.lens, page_size=32, num_kv_heads=2, head_dim=64)  # noqa: E731
+    with pytest.raises(ValueError, match="gradient"):
+        over()
+    with torch.no_grad():
+        over()
+        assert torch.equal(paged.rope(turn, g, ints([0, 1])), paged.rope(turn, x, ints([0, 1])))
+        for call in calls:
+            call(g)

@@ -254,3 +254,21 @@ def test_python_calls_refuse_cpu_tensors():
         paged.Rope(64, layout="other")
     with pytest.raises(RuntimeError):
         paged.Rope(63)
+
+
+def test_rows_that_require_a_gradient_are_refused():
+    """No gradient would reach them: an error, not a result without a graph."""
+    import torch
+
+    from velox_amd import paged
+
+    cpu = torch.device("cpu")
+    x = torch.zeros(2, 3, 64, requires_grad=True)
+    for t in (x, x * 2, (x * 2)[:, :2]):
+        with pytest.raises(ValueError, match="gradient"):
+            paged._rows(t, cpu, "x")
+        with torch.no_grad():
+            assert paged._rows(t, cpu, "x")[1] == 2
+        with torch.inference_mode():
+            assert paged._rows(t, cpu, "x")[1] == 2
+        assert paged._rows(t.detach(), cpu, "x")[1] == 2

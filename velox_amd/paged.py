@@ -3,7 +3,8 @@
 Thin calls of the C ABI (include/velox_hip.h, "paged KV cache"): a call checks types, shapes and devices
 (ValueError), launches on the current stream of the cache's device and returns without waiting; a status other
 than 0 raises as everywhere in this package. Tensors of whole numbers are int32 and hold the C ABI's unsigned
-values: -1 is VELOX_HIP_NO_PAGE / VELOX_HIP_NO_SEQ. Calls can be captured into a graph once `out` and
+values: -1 is VELOX_HIP_NO_PAGE / VELOX_HIP_NO_SEQ. The operators have no backward pass: with gradients enabled, tensors
+that require one are refused. Calls can be captured into a graph once `out` and
 `workspace` are given. There is no CPU fallback.
 """
 from __future__ import annotations
@@ -28,6 +29,11 @@ _stream = torch._C._cuda_getCurrentRawStream
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
+
+
+def _no_gradient(t: torch.Tensor, what: str) -> None:
+    _need(not (t.requires_grad and torch.is_grad_enabled()),
+          f"{what}: requires a gradient, and none is formed here (detach it, or call under torch.no_grad())")
 
 
 def _gpu(t: torch.Tensor, what: str) -> torch.device:
@@ -67,6 +73,8 @@ def _rows(t: torch.Tensor, device: torch.device, what: str, heads: int = 0, dim:
     code = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
     if code is None or t.device != device or t.dim() != 3:
         raise ValueError(f"{what}: a float32, float16 or bfloat16 tensor [row][head][element] on {device} is wanted")
+    if t.requires_grad:
+        _no_gradient(t, what)
     n, h, d = t.shape
     if (heads and h != heads) or (dim and d != dim):
         raise ValueError(f"{what}: heads and head size {heads, dim} are wanted, got {h, d}")
@@ -102,6 +110,7 @@ class PagedCache:
 
     def _bind(self, pool, table, lens, page_size, num_kv_heads, head_dim, refs) -> None:
         device = _gpu(pool, "pool")
+        _no_gradient(pool, "pool")
         _need(pool.dim() == 3 and pool.dtype in (torch.float16, torch.bfloat16), "pool: float16 or bfloat16 [layer][page][element]")
         n_layers, n_pages, elements = pool.shape
         _need(elements == 2 * num_kv_heads * page_size * head_dim, "pool: a page holds 2 * KV heads * page size * head size elements")
