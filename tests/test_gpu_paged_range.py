@@ -75,3 +75,17 @@ def test_calls_refuse_tensors_that_require_a_gradient():
         assert torch.equal(paged.rope(turn, g, ints([0, 1])), paged.rope(turn, x, ints([0, 1])))
         for call in calls:
             call(g)
+
+
+@pytest.mark.parametrize("hq,hkv,d,t", [(8, 2, 64, "f32"), (16, 8, 128, "bf16")])
+def test_short_rows_of_many_sequences(hq, hkv, d, t):
+    """The bound on a sequence's rows decides the splits and nothing else, also where it is too low."""
+    lens, rows = [600 + 37 * i for i in range(40)], [2 + i * 5 % 7 for i in range(40)]
+    start = [sum(rows[:i]) for i in range(41)]
+    f = Filled(lens, hkv, d, 64, "bf16")
+    x = queries(start[-1], hq, hkv, d, t)
+    for max_rows in (0, 8, 1):
+        space = f.cache.prompt_workspace(hq, total_rows=start[-1], max_rows=max_rows, max_len=lens[-1])
+        out = paged.prompt_attention(f.cache, 0, x, ints(start), max_rows=max_rows, max_len=lens[-1], workspace=space)
+        for s in range(40):
+            near(f, x[start[s]:start[s + 1]], out[start[s]:start[s + 1]], s, 2 ** -16 if t == "bf16" else 2 ** -20)

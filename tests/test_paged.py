@@ -272,3 +272,34 @@ def test_rows_that_require_a_gradient_are_refused():
         with torch.inference_mode():
             assert paged._rows(t, cpu, "x")[1] == 2
         assert paged._rows(t.detach(), cpu, "x")[1] == 2
+
+
+def prompt_bytes(lib, d, heads, n, max_rows, max_len=0):
+    v = C.c_uint64()
+    assert lib.velox_hip_paged_prompt_attention_bytes(C.byref(d), heads, n, max_rows, max_len, C.byref(v)) == 0
+    return v.value
+
+
+def test_short_rows_of_many_sequences_are_not_split(hiplib):
+    """Every sequence has workgroups of its own, a KV head each: where those are 512 at least nothing is split."""
+    d = desc(num_kv_heads=8, head_dim=128, n_seqs=80, max_pages=64, table_stride=64, n_pages=4096, page_size=64, num_layers=1)
+    for m in (0, 1, 2, 3, 4, 8, 100, 256, 300):
+        most = 0
+        for n in range(1, 400):
+            tiles = 8 * -(-n * 4 // 128)  # of 128 (row, head) pairs
+            splits = max(1, min(-(-512 // tiles) if tiles < 256 else 1, 4096 // 512))
+            if m and 8 * -(-n // m) >= 512:
+                splits = 1
+            most = max(most, n * 32 * splits * (128 + 2) * 4 if splits > 1 else 0)
+            assert prompt_bytes(hiplib, d, 32, n, m) == most, (n, m)
+
+
+@pytest.mark.parametrize("heads, hkv", [(4, 2), (28, 4), (9, 3), (300, 1)])
+@pytest.mark.parametrize("max_rows", [1, 5, 64])
+def test_prompt_workspace_of_short_rows_grows_with_them(hiplib, heads, hkv, max_rows):
+    d = desc(num_kv_heads=hkv, n_seqs=4096, max_pages=500, table_stride=500, n_pages=500, num_layers=1, layer_stride=0)
+    last = 0
+    for n in list(range(1, 400)) + [1000, 2048, 4096, 100000]:
+        size = prompt_bytes(hiplib, d, heads, n, max_rows)
+        assert last <= size <= prompt_bytes(hiplib, d, heads, n, 0)
+        last = size

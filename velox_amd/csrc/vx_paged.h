@@ -79,7 +79,8 @@ hipError_t vx_launch_rope_rows(const VxRopeTable& t, const VxRowsView& x, const 
 hipError_t vx_launch_rope_append(const VxRopeTable& t, const VxAppendArgs& a, hipStream_t st);
 uint32_t vx_paged_attn_splits(const VxPagedView& c, uint32_t heads, uint32_t rows, uint32_t max_len);
 hipError_t vx_launch_paged_attention(const VxPagedAttnArgs& a, hipStream_t st);
-uint32_t vx_paged_prompt_splits(const VxPagedView& c, uint32_t heads, uint32_t n_rows, uint32_t span);
+uint32_t vx_paged_prompt_split_rows(const VxPagedView& c, uint32_t max_rows);  // the most rows that are split
+uint32_t vx_paged_prompt_splits(const VxPagedView& c, uint32_t heads, uint32_t n_rows, uint32_t max_rows, uint32_t span);
 hipError_t vx_launch_paged_prompt(const VxPagedAttnArgs& a, hipStream_t st);
 
 hipError_t vx_launch_pages_reset(const VxPages& p, hipStream_t st);

@@ -982,7 +982,17 @@ hipError_t vx_launch_paged_attention(const VxPagedAttnArgs& a, hipStream_t st) {
 // workgroups for each, into parts of 512 positions at least. Rows for a workgroup on every CU are not split: four
 // chunks of 400 rows behind 4000 positions take 121 us (Qwen2.5-7B) and 127 (Llama-3-8B), as two splits 129 and 150; 2000
 // rows 51 and 53, as two splits 67 and 73. Below that it pays: 2000 rows of SmolLM (141 workgroups) 29 us in three.
-uint32_t vx_paged_prompt_splits(const VxPagedView& c, uint32_t heads, uint32_t n_rows, uint32_t span) {
+// Every sequence has tiles of its own: rows of at most max_rows a sequence are that many sequences at least, and with two
+// workgroups for each CU from them alone nothing is split (64 sequences of 4 rows behind 4096 positions, Llama-3-8B:
+// 512 workgroups 210 us, in eight splits 247; 128 behind 2000, Qwen2.5-7B: 107 and 129; fp32 rows 317 and 340, 162
+// and 176). With fewer it pays still, though the tiles are more than the rows fill: 64 of 4 rows, Qwen2.5-7B, fp32 rows,
+// 256 workgroups 190 us, in eight splits 175.
+uint32_t vx_paged_prompt_split_rows(const VxPagedView& c, uint32_t max_rows) {
+    const uint64_t rows = max_rows ? (uint64_t)max_rows * (511 / c.hkv) : kVxMaxRows;
+    return rows < kVxMaxRows ? (uint32_t)rows : kVxMaxRows;
+}
+uint32_t vx_paged_prompt_splits(const VxPagedView& c, uint32_t heads, uint32_t n_rows, uint32_t max_rows, uint32_t span) {
+    if (n_rows > vx_paged_prompt_split_rows(c, max_rows)) return 1;
     const uint64_t g = heads / c.hkv, tiles = ((uint64_t)n_rows * g + kPromptRows - 1) / kPromptRows * c.hkv;
     const uint64_t want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles, most = span / 512;
     const uint64_t s = want < most ? want : most;

@@ -254,25 +254,25 @@ int velox_hip_paged_attention(const VeloxHipPagedCache* c, uint32_t layer, const
 int velox_hip_paged_prompt_attention_bytes(const VeloxHipPagedCache* c, uint32_t heads, uint32_t n_rows, uint32_t max_rows,
                                            uint32_t max_len, uint64_t* bytes) {
     if (!shape_ok(c) || !bytes || !heads || heads > 65535u || heads % c->num_kv_heads) return VELOX_HIP_EINVAL;
-    if (n_rows == 0) {
+    if (n_rows > kVxMaxRows) return VELOX_HIP_EINVAL;
+    // Fewer rows are split more: the largest need of up to n_rows rows. It is that of rows that just fill their tiles, or
+    // of as many as are split at all. A window shortens a call's span, which splits less.
+    const VxPagedView v = view(c, 0);
+    const uint32_t g = heads / c->num_kv_heads, span = max_positions(c, max_len), split_rows = vx_paged_prompt_split_rows(v, max_rows);
+    const uint32_t last = n_rows < split_rows ? n_rows : split_rows;
+    uint64_t most = 0;
+    if (!last) {
         *bytes = 0;
         return VELOX_HIP_OK;
     }
-    (void)max_rows;  // bounds the part of a window that the call plans by, which is never more
-    if (n_rows > kVxMaxRows) return VELOX_HIP_EINVAL;
-    // Fewer rows are split more: the largest need of up to n_rows rows. It is that of rows that just fill their tiles,
-    // or of n_rows.
-    const VxPagedView v = view(c, 0);
-    const uint32_t g = heads / c->num_kv_heads, span = max_positions(c, max_len);
-    uint64_t most = 0;
     for (uint32_t tiles = 1; ; ++tiles) {
         const uint64_t fill = (uint64_t)tiles * kVxPromptRows / g;
-        const uint32_t rows = fill < n_rows ? (uint32_t)fill : n_rows;
+        const uint32_t rows = fill < last ? (uint32_t)fill : last;
         if (rows) {
-            const uint32_t s = vx_paged_prompt_splits(v, heads, rows, span);
+            const uint32_t s = vx_paged_prompt_splits(v, heads, rows, max_rows, span);
             const uint64_t need = part_bytes(rows, heads, s, c->head_dim);
             if (need > most) most = need;
-            if (rows == n_rows || s == 1) break;
+            if (rows == last || s == 1) break;
         }
     }
     *bytes = most;
@@ -298,7 +298,7 @@ int velox_hip_paged_prompt_attention(const VeloxHipPagedCache* c, uint32_t layer
     uint32_t span = max_positions(c, max_len);
     const uint64_t seen = (uint64_t)mask.window + mask.sinks + (max_rows && max_rows < n_rows ? max_rows : n_rows) + 64u;
     if (mask.window && seen < span) span = (uint32_t)seen;
-    a.splits = vx_paged_prompt_splits(a.c, q->heads, n_rows, span);
+    a.splits = vx_paged_prompt_splits(a.c, q->heads, n_rows, max_rows, span);
     const uint64_t need = part_bytes(n_rows, q->heads, a.splits, c->head_dim);
     if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need)) return VELOX_HIP_EINVAL;
     a.part_o = (float*)workspace;
