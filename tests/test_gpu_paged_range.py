@@ -89,3 +89,15 @@ def test_short_rows_of_many_sequences(hq, hkv, d, t):
         out = paged.prompt_attention(f.cache, 0, x, ints(start), max_rows=max_rows, max_len=lens[-1], workspace=space)
         for s in range(40):
             near(f, x[start[s]:start[s + 1]], out[start[s]:start[s + 1]], s, 2 ** -16 if t == "bf16" else 2 ** -20)
+
+
+def test_calls_refuse_numbers_past_32_bits():
+    f = Filled([64, 3], 2, 64, 32, "bf16")
+    c, x, wrap = f.cache, torch.randn(2, 4, 64, device="cuda"), 1 << 32
+    for call in (lambda: paged.attention(c, wrap, x), lambda: paged.attention(c, 0, x, max_len=wrap), lambda: c.attention_workspace(wrap + 4),
+                 lambda: c.attention_workspace(4, max_len=wrap + 1), lambda: paged.prompt_attention(c, wrap, x, ints([0, 1, 2])),
+                 lambda: paged.prompt_attention(c, 0, x, ints([0, 1, 2]), max_rows=wrap + 1), lambda: c.prompt_workspace(4, total_rows=wrap + 2),
+                 lambda: c.prompt_workspace(4, total_rows=-1), lambda: paged.prompt_attention(c, 0, x, ints([0, 1, 2]), max_len=wrap),
+                 lambda: paged.rope_append(c, wrap, None, x, x[:, :2], x[:, 2:])):
+        with pytest.raises(ValueError):
+            call()

@@ -303,3 +303,17 @@ def test_prompt_workspace_of_short_rows_grows_with_them(hiplib, heads, hkv, max_
         size = prompt_bytes(hiplib, d, heads, n, max_rows)
         assert last <= size <= prompt_bytes(hiplib, d, heads, n, 0)
         last = size
+
+
+def test_numbers_past_32_bits_are_refused():
+    """ctypes takes a number modulo 2^32: layer 2^32 would be layer 0."""
+    import torch
+
+    from velox_amd import paged
+
+    cpu = torch.device("cpu")
+    for call in (lambda: paged.Rope((1 << 32) + 64), lambda: paged.Rope(64, scaling="yarn", factor=2.0, original_len=(1 << 32) + 4096),
+                 lambda: paged.Rope(64, original_len=-1), lambda: paged._rows(torch.zeros(1, 1, 2).expand((1 << 32) + 1, 1, 2), cpu, "x")):
+        with pytest.raises(ValueError):
+            call()
+    assert paged._rows(torch.zeros(1, 1, 2).expand(1 << 20, 1, 2), cpu, "x")[1] == 1 << 20

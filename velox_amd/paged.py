@@ -31,6 +31,13 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _numbers(what: str, *values: int) -> None:
+    """Whole numbers that the C ABI's 32 bits hold: ctypes would take others modulo 2^32."""
+    for v in values:
+        if not 0 <= v <= 0xFFFFFFFF:
+            raise ValueError(f"{what}: whole numbers of [0, 2^32) are wanted, got {v}")
+
+
 def _no_gradient(t: torch.Tensor, what: str) -> None:
     _need(not (t.requires_grad and torch.is_grad_enabled()),
           f"{what}: requires a gradient, and none is formed here (detach it, or call under torch.no_grad())")
@@ -76,6 +83,8 @@ def _rows(t: torch.Tensor, device: torch.device, what: str, heads: int = 0, dim:
     if t.requires_grad:
         _no_gradient(t, what)
     n, h, d = t.shape
+    if (n | h | d) >> 32:
+        _numbers(what, n, h, d)
     if (heads and h != heads) or (dim and d != dim):
         raise ValueError(f"{what}: heads and head size {heads, dim} are wanted, got {h, d}")
     rs, hs, es = t.stride()
@@ -122,6 +131,7 @@ class PagedCache:
         self.n_seqs, self.max_pages = table.shape
         self.pool, self.table, self.lens, self.refs = pool, table, lens, refs
         stride = table.stride(0) if self.n_seqs > 1 else self.max_pages
+        _numbers("table", self.max_pages, stride)
         d = L.PagedCacheDesc(pool.data_ptr(), pool.stride(0) * 2, _DTYPES[pool.dtype], n_layers, num_kv_heads, head_dim, n_pages,
                              page_size, self.n_seqs, self.max_pages, stride, 0, table.data_ptr(),
                              _words(lens, self.n_seqs, device, "lens"), None, None)
@@ -153,7 +163,9 @@ class PagedCache:
 
     def free(self, seqs: torch.Tensor) -> None:
         """The sequences listed (int32) are empty."""
-        self._pages("free", _words(seqs, -1, self.device, "seqs"), seqs.numel())
+        listed = _words(seqs, -1, self.device, "seqs")
+        _numbers("seqs", seqs.numel())
+        self._pages("free", listed, seqs.numel())
 
     def trim(self, window: int, sinks: int = 0) -> None:
         """Frees the whole pages that no later row of a window sees."""
@@ -174,12 +186,14 @@ class PagedCache:
     def attention_workspace(self, heads: int, *, max_len: int = 0) -> torch.Tensor | None:
         """What attention() needs with these bounds, whatever its mask (None: nothing)."""
         n = C.c_uint64()
+        _numbers("heads and max_len", heads, max_len)
         L.check(self.lib.velox_hip_paged_attention_bytes(self._ref, heads, max_len, C.byref(n)), "paged_attention_bytes")
         return torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
 
     def prompt_workspace(self, heads: int, *, total_rows: int, max_rows: int = 0, max_len: int = 0) -> torch.Tensor | None:
         """What prompt_attention() needs for up to total_rows rows with these bounds (None: nothing)."""
         n = C.c_uint64()
+        _numbers("heads, total_rows, max_rows and max_len", heads, total_rows, max_rows, max_len)
         L.check(self.lib.velox_hip_paged_prompt_attention_bytes(self._ref, heads, total_rows, max_rows, max_len, C.byref(n)),
                 "paged_prompt_attention_bytes")
         return torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
@@ -191,7 +205,8 @@ class Rope:
     def __init__(self, rot_dim: int, *, theta: float = 10000.0, layout: str = "half", scaling: str = "none", factor: float = 1.0,
                  original_len: int = 0, low_turns: float = 0.0, high_turns: float = 0.0, amplitude: float = 0.0):
         _need(layout in _LAYOUTS and scaling in _SCALINGS, f"layout is one of {tuple(_LAYOUTS)}, scaling one of {tuple(_SCALINGS)}")
-        _need(rot_dim > 0 and original_len >= 0, "rot_dim has to be positive")
+        _need(rot_dim > 0, "rot_dim has to be positive")
+        _numbers("rot_dim and original_len", rot_dim, original_len)
         self.lib = L.load()
         self.handle = C.c_void_p()
         self.rot_dim = rot_dim
@@ -238,7 +253,7 @@ def rope_append(cache: PagedCache, layer: int, turn: Rope | None, q: torch.Tenso
     q_start (int32 [sequences + 1]) gives the sequences' rows; None: row s is sequence s's."""
     device, d = cache.device, cache.head_dim
     _need(turn is None or bool(turn.handle), "rope_append: the handle is closed")
-    _need(layer >= 0, "layer has to be at least 0")
+    _numbers("layer", layer)
     kr, n = _rows(k, device, "k", cache.num_kv_heads, d)
     vr, vn = _rows(v, device, "v", cache.num_kv_heads, d)
     _need(vn == n, "k and v: as many rows of each are wanted")
@@ -283,7 +298,7 @@ def attention(cache: PagedCache, layer: int, q: torch.Tensor, *, window: int = 0
     """Attention of every sequence's newest position: q [sequence][q head][head size], already in the cache.
     max_len bounds lens for planning; workspace: cache.attention_workspace of the same bounds (None: made here)."""
     device = cache.device
-    _need(layer >= 0 and max_len >= 0, "layer and max_len have to be at least 0")
+    _numbers("layer and max_len", layer, max_len)
     qr, n = _rows(q, device, "q", 0, cache.head_dim)
     _need(n == cache.n_seqs, f"q: {cache.n_seqs} rows are wanted")
     if out is None:
@@ -304,7 +319,7 @@ def prompt_attention(cache: PagedCache, layer: int, q: torch.Tensor, q_start: to
     """Attention of a ragged batch's rows, q [row][q head][head size]; sequence s has rows q_start[s] .. q_start[s + 1],
     the last of them its newest position. Rows of no sequence are not written."""
     device = cache.device
-    _need(layer >= 0 and max_len >= 0 and max_rows >= 0, "layer, max_rows and max_len have to be at least 0")
+    _numbers("layer, max_rows and max_len", layer, max_rows, max_len)
     qr, n = _rows(q, device, "q", 0, cache.head_dim)
     if out is None:
         out, o = _like(q, qr, cache.head_dim)
