@@ -101,3 +101,18 @@ def test_calls_refuse_numbers_past_32_bits():
                  lambda: paged.rope_append(c, wrap, None, x, x[:, :2], x[:, 2:])):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("q,kv", [("f32", "f16"), ("bf16", "f16"), ("f16", "f16"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("amp,scale", [(1e-30, 1e-20), (1.0, 1e-43), (1e-30, -1e-12)])
+def test_scales_next_to_nothing(q, kv, amp, scale):
+    """Scores that vanish leave the mean of what a row sees."""
+    f = Filled([300, 70], 2, 64, 32, kv)
+    x = (queries(120, 4, 2, 64, "f32") * amp).to(T[q])
+    out = torch.empty(120, 4, 64, device="cuda")
+    paged.prompt_attention(f.cache, 0, x, ints([0, 70, 120]), scale=scale, window=100, sinks=3, out=out)
+    one = paged.attention(f.cache, 0, x[:2], scale=scale, window=100, sinks=3, out=torch.empty(2, 4, 64, device="cuda"))
+    weights = half_step(T[kv]) ** 2 + 2 ** -20
+    for s, (lo, hi) in enumerate(((0, 70), (70, 120))):
+        near(f, x[lo:hi], out[lo:hi], s, weights, 100, 3, scale=scale, small=2.0 ** -32)
+        near(f, x[s:s + 1], one[s:s + 1], s, weights, 100, 3, scale=scale, small=2.0 ** -32)

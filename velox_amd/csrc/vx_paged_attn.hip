@@ -662,7 +662,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
                 big = vx_max_pair(big);
                 const int e = vx_to_2_14(big);
                 by = ldexpf(by, e);
-                to_log2 = ldexpf(to_log2, -e);
+                // never 0, times which a hidden score's infinity is NaN (the products stay below 2^38: at 2^-126 they are nothing)
+                to_log2 = fmaxf(ldexpf(to_log2, -e), 0x1p-126f);
             }
 #pragma unroll
             for (int c = 0; c < NK; ++c)
