@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from velox_amd import paged
-from test_gpu_paged import T, Filled, half_step, ints, queries
+from test_gpu_paged import SLOT, T, Filled, close_turn, gen, half_step, ints, queries, turned
+from test_gpu_paged import test_append as check_append
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +117,79 @@ def test_scales_next_to_nothing(q, kv, amp, scale):
     for s, (lo, hi) in enumerate(((0, 70), (70, 120))):
         near(f, x[lo:hi], out[lo:hi], s, weights, 100, 3, scale=scale, small=2.0 ** -32)
         near(f, x[s:s + 1], one[s:s + 1], s, weights, 100, 3, scale=scale, small=2.0 ** -32)
+
+
+@pytest.mark.parametrize("hq,hkv,d,q,kv", [(32, 8, 128, "bf16", "bf16"), (16, 8, 128, "f32", "f16"), (16, 8, 128, "f32", "bf16"), (24, 8, 64, "f16", "f16"),
+                                           (16, 8, 64, "f32", "bf16")])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (3000, 70)])
+def test_long_prompt_behind_a_long_context(hq, hkv, d, q, kv, window, sinks):
+    """Workgroups that walk 2500 to 4600 positions whole: their pages are looked up several times."""
+    n, rows = 4637, 2101
+    f = Filled([n], hkv, d, 64, kv)
+    assert f.cache.prompt_workspace(hq, total_rows=rows) is not None and -(-rows * (hq // hkv) // 128) * hkv >= 256  # not split
+    x = queries(rows, hq, hkv, d, q)
+    near(f, x, paged.prompt_attention(f.cache, 0, x, ints([0, rows]), window=window, sinks=sinks), 0,
+         half_step(T[kv]) ** 2 if q == kv else 2 ** -20, window, sinks, small=2.0 ** -32)
+
+
+@pytest.mark.parametrize("q,kv", [("bf16", "bf16"), ("f32", "bf16"), ("f16", "f16"), ("f32", "f16")])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv,n,rows,where,window,sinks", [(32, 8, 4637, 2101, 4600, 0, 0), (32, 8, 4637, 2101, 3000, 1500, 3), (32, 8, 4637, 2101, 5, 3000, 9),
+                                                              (2, 1, 1700, 40, 1690, 0, 0), (2, 1, 9000, 90, 3, 4000, 5)],
+                         ids=["late", "window", "sink", "split", "split-sink"])
+def test_infinities_in_long_walks_and_splits(d, q, kv, hq, hkv, n, rows, where, window, sinks):
+    """What is no number in V reaches the rows that see its position, far along a walk and in one of several splits."""
+    f = Filled([n], hkv, d, 64, kv)
+    x = queries(rows, hq, hkv, d, q)
+    space = f.cache.prompt_workspace(hq, total_rows=rows)
+    assert space is not None  # (of 2101 rows: for fewer)
+    t = torch.arange(n - rows, n, device="cuda")
+    sees = (t >= where) & ((t < where + window) | (where < sinks) if window else True)
+    assert sees.any() and (window or not sees.all())
+    h, e, r = hkv - 1, d - 3, where % 64
+    cell = f.pool[0, int(f.table[0, where // 64])][hkv * 64 * d:].view(hkv, 2, d, 32)
+    g = hq // hkv
+    for value in (math.nan, math.inf, -math.inf):
+        cell[h, r // 32, e, int(SLOT[r % 32])] = value
+        out = paged.prompt_attention(f.cache, 0, x, ints([0, rows]), window=window, sinks=sinks, workspace=space)
+        assert torch.equal(torch.isfinite(out[:, h * g:, e]), ~sees.view(-1, 1).expand(rows, g))
+        out[:, h * g:, e] = 0
+        assert torch.isfinite(out).all()
+    f.v[0][:, h, e] = 0  # that dimension is looked at above
+    near(f, x, out, 0, half_step(T[kv]) ** 2 if q == kv else 2 ** -20, window, sinks, small=2.0 ** -32)
+
+
+@pytest.mark.parametrize("q", ["f32", "bf16"])
+def test_token_attention_past_the_caches(q):
+    """K and V of more than 256 MiB: loads that leave nothing in the caches."""
+    f = Filled([70011], 8, 128, 256, "bf16")
+    assert f.table.shape[1] * 256 * 8 * 128 * 4 > 256 << 20
+    x = queries(1, 16, 8, 128, q)
+    out = torch.empty(1, 16, 128, device="cuda")
+    near(f, x, paged.attention(f.cache, 0, x, out=out), 0, 2 ** -16 if q == "bf16" else 2 ** -20)
+    near(f, x, paged.attention(f.cache, 0, x, window=69000, sinks=33, out=out), 0, 2 ** -16 if q == "bf16" else 2 ** -20, 69000, 33)
+
+
+@pytest.mark.parametrize("rows,heads", [(2049, 70), (4001, 70), (4001, 3)])
+@pytest.mark.parametrize("layout,rot", [("half", 128), ("interleaved", 128), ("half", 64), ("interleaved", 64)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_rope_of_many_rows(rows, heads, layout, rot, dtype):
+    """Several rows a workgroup and fewer in the last one, more heads than are requested at once, and more bytes than the caches."""
+    x = torch.randn(rows, heads, 128, generator=gen(rows), device="cuda").to(T[dtype])
+    at = torch.randint(0, 2 ** 31 - 1, (rows,), generator=gen(5), device="cuda", dtype=torch.int32)
+    turn = paged.Rope(rot, theta=5e5, layout=layout)
+    want, size = turned(x, at, turn, layout == "interleaved")
+    got = paged.rope(turn, x, at)
+    close_turn(got, want, size, T[dtype])
+    paged.rope(turn, x, at, out=x)
+    assert torch.equal(x, got)
+
+
+@pytest.mark.parametrize("hq,hkv,q,kv,rows,layout", [(32, 8, "bf16", "bf16", [2700, 33, 70], "half"), (64, 8, "f32", "bf16", [800, 1, 70], "half"),
+                                                     (64, 8, "f16", "f16", [1600, 33, 70], "interleaved"), (32, 8, "f32", "f16", [1300, 1, 75], "interleaved"),
+                                                     (64, 8, "bf16", "bf16", [70, 33, 1], "half"), (32, 8, "f32", "bf16", [70, 33, 1], "half")])
+def test_append_of_many_heads_and_bytes(hq, hkv, q, kv, rows, layout):
+    """More heads than a thread requests at once, and rows past the caches; blocks of fewer than 32 rows among them."""
+    if rows[0] > 70:
+        assert (sum(rows) + 3) * (hq + 2 * hkv) * 128 * T[q].itemsize > 32 << 20
+    check_append(hq, hkv, 128, 64, 128, layout, q, kv, rows, [17, 5, 64])
