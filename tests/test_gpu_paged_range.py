@@ -193,3 +193,40 @@ def test_append_of_many_heads_and_bytes(hq, hkv, q, kv, rows, layout):
     if rows[0] > 70:
         assert (sum(rows) + 3) * (hq + 2 * hkv) * 128 * T[q].itemsize > 32 << 20
     check_append(hq, hkv, 128, 64, 128, layout, q, kv, rows, [17, 5, 64])
+
+
+def test_a_captured_step_of_split_token_attention():
+    """A decode step whose attention is split and joined, in a graph that is replayed with eager steps on a second cache
+    between, against those."""
+    hq, hkv, d = 4, 2, 64
+
+    def make():
+        c = paged.PagedCache(160, 3, 64, page_size=32, num_kv_heads=hkv, head_dim=d)
+        c.extend(ints([1500, 2, 700]))
+        c.pool.copy_(torch.randn(c.pool.shape, generator=gen(5), device="cuda"))
+        return c
+
+    a, b = make(), make()
+    turn, one = paged.Rope(d), ints([1, 1, 1])
+    x = torch.zeros(3, hq + 2 * hkv, d, device="cuda")
+    sets = [(torch.empty(3, hq, d, device="cuda"), torch.empty(3, hq, d, device="cuda"), a.attention_workspace(hq)) for _ in range(2)]
+    assert sets[0][2] is not None
+
+    def step(c, q, out, space):
+        c.extend(one)
+        paged.rope_append(c, 0, turn, x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], q)
+        paged.attention(c, 0, q, out=out, workspace=space)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        step(a, *sets[0])
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(40):
+        x.copy_(torch.randn(x.shape, generator=gen(100 + i), device="cuda"))
+        sets[0][2].fill_(255 if i % 2 else 0)  # nothing of an earlier call is needed: all bits set are NaN
+        graph.replay()
+        step(b, *sets[1])
+        torch.cuda.synchronize()
+        assert torch.isfinite(sets[0][1]).all() and torch.equal(sets[0][1], sets[1][1]) and torch.equal(a.lens, b.lens)

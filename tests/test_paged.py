@@ -317,3 +317,15 @@ def test_numbers_past_32_bits_are_refused():
         with pytest.raises(ValueError):
             call()
     assert paged._rows(torch.zeros(1, 1, 2).expand(1 << 20, 1, 2), cpu, "x")[1] == 1 << 20
+
+
+def test_refuses_a_workspace_that_a_long_cache_needs_and_is_not_given(hiplib):
+    d = desc(n_seqs=1, max_pages=5000, table_stride=5000, n_pages=5000, num_layers=1)
+    n = C.c_uint64()
+    assert hiplib.velox_hip_paged_attention_bytes(C.byref(d), 4, 0, C.byref(n)) == 0 and n.value
+    for space, size in ((None, n.value), (P, n.value - 1), (P + 4, n.value)):
+        assert attention(hiplib, d, max_len=0, space=space, size=size) == L.EINVAL
+    assert hiplib.velox_hip_paged_prompt_attention_bytes(C.byref(d), 4, 7, 0, 0, C.byref(n)) == 0 and n.value
+    for space, size in ((None, n.value), (P, n.value - 1), (P + 4, n.value)):
+        assert hiplib.velox_hip_paged_prompt_attention(C.byref(d), 0, C.byref(rows()), C.byref(rows()), P, 7, L.AttnMask(0, 0), 0.0, 0, 0, space,
+                                                       size, None) == L.EINVAL
