@@ -504,7 +504,7 @@ int velox_hip_rope_append(const VeloxHipPagedCache* c, uint32_t layer, const Vel
  * sees nothing gives 0. scale 0: 1 / sqrt(head_dim). q and out: any element types (q of another type than the
  * cache's is not rounded to it); out may be q (other overlaps are not allowed). Scores and sums are fp32; the weights (softmax's
  * numerators) enter the products in 16 bits over bf16 pages where q is bf16 too, in 24 where it is not, in 22 over fp16
- * pages. What positions that a row does not see hold, infinities and NaN among it, does not matter to the row. A row that sees an infinity or NaN gets no number where it enters.
+ * pages (there q of another type too, no finer than 2^-38 of its head's largest value). What positions that a row does not see hold, infinities and NaN among it, does not matter to the row. A row that sees an infinity or NaN gets no number where it enters.
  *
  * paged_attention: row s is the newest position of sequence s (t = lens[s] - 1), s < n_seqs. Long caches are
  * split over workgroups and joined. max_len: an upper bound of lens that the split is planned by (0: max_pages *

@@ -160,7 +160,9 @@ __global__ __launch_bounds__(kRopeThreads) void vx_rope_vec_kernel(VxRopeTable t
     }
 }
 
-// The same value by value, for rows without 16-byte alignment and pairs that do not fill vectors.
+// The same value by value, for rows without 16-byte alignment and pairs that do not fill vectors. Bound by its loads of one
+// value each: 4001 rows of 64 heads of 128 in bf16 44 us at an odd address, 84 with 18 or 34 of 128 turned (by vectors 22;
+// the bytes at a copy's rate 27).
 __global__ __launch_bounds__(kRopeThreads) void vx_rope_rows_kernel(VxRopeTable t, VxRowsView x, VxRowsView o, uint32_t n_rows,
                                                                     uint32_t d, const uint32_t* __restrict__ positions) {
     __shared__ float2 cs[kVxMaxRopePairs];
@@ -208,7 +210,8 @@ struct VxBlock {
     uint32_t seq;
 };
 // Block `item` of the batch, blocks counted over the sequences in order; false behind the last. Every wave walks the
-// sequences 64 at a time. One row each (no q_start): which row it is does not wait for the length; the rest is
+// sequences 64 at a time (one row each of 64, 512 and 4096 sequences, Qwen2.5-7B's heads, 5.3, 11.5 and 167 us; without
+// q_start, hence without the walk, 4.6, 8.3 and 49). One row each (no q_start): which row it is does not wait for the length; the rest is
 // vx_block_place's.
 __device__ __forceinline__ bool vx_block(const VxAppendArgs& a, uint32_t item, VxBlock& b) {
     const uint32_t lane = threadIdx.x & 63u;
@@ -284,7 +287,7 @@ __device__ __forceinline__ void vx_angles(const VxRopeTable& t, const VxBlock& b
     __syncthreads();
 }
 
-// Bound by its bytes: 8540 rows of Llama-3-8B's q, k and v (bf16, 210 MB moved) take 43 us (4.8 TB/s), one row each of 32
+// Bound by its bytes: 8531 rows of Llama-3-8B's q, k and v (bf16, 210 MB moved) take 43 us (4.8 TB/s), one row each of 32
 // sequences of Qwen2.5-7B 3.8 us, a launch and the length, the page number and a line behind each other (47 and 4.6 us
 // while branches around the loads made them wait for each other). T: the rows' type, C: the cache's. K and q by units
 // of 16 bytes; V by 8 dimensions of the 8 positions that share 16 bytes of a V block, transposed in registers, so that
@@ -374,7 +377,9 @@ __global__ __launch_bounds__(256) void vx_append_vec_kernel(VxRopeTable t, VxApp
     }
 }
 
-// The same value by value, for rows of several types or without 16-byte alignment, and pairs that do not fill vectors.
+// The same value by value, for rows of several types or without 16-byte alignment, and pairs that do not fill vectors. 8500
+// rows of Llama-3-8B's q, k and v in bf16 take 182 us at odd addresses, 244 with 34 of 128 turned (by vectors 43); fp32 q
+// beside bf16 k and v 310 us (348 MB, 71 at a copy's rate).
 __global__ __launch_bounds__(256) void vx_append_rows_kernel(VxRopeTable t, VxAppendArgs a) {
     __shared__ float2 cs[32][kVxMaxRopePairs / 2];
     VxBlock b;
@@ -779,7 +784,7 @@ uint32_t copy_grid(const VxPages& p, uint64_t moves) {
 
 // Rows of more bytes than the XCDs' L2 caches hold go past them (non-temporal): what reads them next finds them in
 // memory anyway. 4001 rows of 64 heads of 128 (fp16, 131 MB moved, cold) 31.1 -> 24.3 us by non-temporal stores
-// (loads made it 30.9); 8540 rows of Llama-3-8B's q, k and v (210 MB) 63 -> 47 us by both.
+// (loads made it 30.9); 8531 rows of Llama-3-8B's q, k and v (210 MB) 63 -> 47 us by both.
 static constexpr uint64_t kStreamBytes = 32ull << 20;
 
 // Whether 16-byte loads and stores fit rows of type elements.
@@ -822,7 +827,7 @@ hipError_t vx_launch_rope_append(const VxRopeTable& t, const VxAppendArgs& a, hi
     const uint64_t bound = (uint64_t)a.n_rows / 32 + 2ull * a.c.n_seqs;
     const uint32_t blocks = (uint32_t)(bound < a.n_rows ? bound : a.n_rows);
     // Heads are shared out over 8 workgroups of a block; over 2 where there are many blocks of few rows (one row each of 512
-    // sequences of Qwen2.5-7B 15.5 us by 8, 8.3 by 2; of 8 sequences 3.6 and 3.8; prompts of 8540 rows 43.6 and 51.6).
+    // sequences of Qwen2.5-7B 15.5 us by 8, 8.3 by 2; of 8 sequences 3.6 and 3.8; prompts of 8531 rows 43.6 and 51.6).
     const dim3 grid(blocks, blocks > 64 && a.n_rows < 4 * (uint64_t)blocks ? 2 : 8);
     const bool vec = (!a.q.data || (vx_vec_rows(a.q) && vx_vec_rows(a.qo) && a.q.dtype == a.k.dtype)) && vx_vec_rows(a.k) &&
                      vx_vec_rows(a.v) && a.k.dtype == a.v.dtype && vx_vec_pairs(t, a.k.dtype, a.c.d);

@@ -141,11 +141,12 @@ __device__ __forceinline__ uint32_t vx_chunk_base(const VxChunks& c, uint32_t i)
 // head size 128) in registers while the next one's are on their way. q of another type than the cache's enters as
 // QT terms of the cache's type whose sum keeps fp32's precision (three of bf16; two of fp16, of which each
 // head's largest value is brought to 2^13 first, so that the second term stays in range), the weights as PT.
-// Bound by the bytes of K and V where there are many: 4 sequences of 91000 to 131000 positions of Llama-3-8B's heads 292 us
+// Bound by the bytes of K and V where there are many: 4 sequences of 107243 to 131000 positions of Llama-3-8B's heads 292 us
 // (6.7 TB/s); by latency (lengths, table, first chunk, the join) below: 32 sequences of 600 to 2100 positions of
 // Qwen2.5-7B's heads (90 MB) 19.6 us, one SmolLM sequence of 700 7.5 us (21.7 and 8.6 while the waits for a chunk were
-// waits for the next one too). Four waves: eight were slower (25.4 against 22.9 us for 32 sequences of 1500).
-// Non-temporal loads (NT) where the caches cannot hold the K and V anyway: Llama-3-8B's heads, 4 sequences of 91000 to
+// waits for the next one too). Four waves: eight were slower where the GPU is full (25.4 against 22.9 us for 32 sequences
+// of 1500); with few workgroups more waves were not tried.
+// Non-temporal loads (NT) where the caches cannot hold the K and V anyway: Llama-3-8B's heads, 4 sequences of 107243 to
 // 131000 positions 330 -> 292 us (5.9 -> 6.7 TB/s); 32 sequences of Qwen2.5-7B (90 MB, in the memory-side cache from
 // one call to the next) 21.8 us without, 23.6 with.
 constexpr uint64_t kTokenCached = 256ull << 20;  // bytes of the memory-side cache
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void vx_paged_token_kernel(VxPage
 }
 
 // Joins a row's splits: W waves for a (row, head), each over its part of the splits: one where there are few splits or many
-// rows, which then take few workgroups and no barrier (2000 prompt rows of SmolLM in 3 splits, both kernels, 29 us by one,
+// rows, which then take few workgroups and no barrier (2000 prompt rows of SmolLM in 3 splits, both kernels, with weights of one term, 29 us by one,
 // 43 by four), else four (4 sequences of 2000 positions of Llama-3-8B in 8 splits 9.9 us, by one 10.3). A launch's
 // latency where there are few. Maxima and sums are requested first: they are joined while the rest arrives. Of a prompt's
 // rows, those of no sequence and those in front of position 0 (their sums say -1) are passed over.
@@ -459,10 +460,11 @@ hipError_t launch_token(const VxPagedAttnArgs& a, bool nt, hipStream_t st) {
 // order into the order of the pages' V blocks.
 // The weights enter as PT terms of the cache's type (q of that type: two, as in the token form), so that they are off by
 // 2^-16 (bf16) or 2^-22 (fp16) and the output by its own rounding only. One term made half as many products of the
-// weights, 404 and 127 us below, but a bf16 output's error against 64 bits was 1.3 times that rounding.
+// weights, 1.38 times as fast, but a bf16 output's error against 64 bits was 1.3 times that rounding.
 // Bound by the matrix cores and what shares their issue slots: 8192 rows of Llama-3-8B's heads through a window of 4096
-// take 555 us (740 TFLOP/s of the visible pairs, 1110 with the second terms' products); four chunks of 392 to 500 rows
-// behind 4000 positions of Qwen2.5-7B's heads 179 us. Before the second term 64 pairs a wave (616 us), 8 or 2
+// take 550 to 607 us by the box (680 to 750 TFLOP/s of the visible pairs, half as much again with the second terms'
+// products; the matrix cores busy in 58 % of the clocks, at 1.8 GHz); four chunks of 392 to 500 rows
+// behind 4000 positions of Qwen2.5-7B's heads 177 to 190 us. Before the second term 64 pairs a wave (616 us), 8 or 2
 // waves a workgroup (523, 729 against 471 then) were slower; written orders of products, exponentials and LDS reads took
 // as long (391 to 396 us).
 constexpr int kPromptWaves = 4;
@@ -495,7 +497,9 @@ __device__ __forceinline__ float vx_sum_pair(float v) {
     return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
 }
 
-// Row tile `item` (counted over the sequences in order): its sequence, its index there, and the sequence's rows.
+// Row tile `item` (counted over the sequences in order): its sequence, its index there, and the sequence's rows. Every
+// workgroup scans the sequences in front of its own, 64 at a time: one row each of 64, 512 and 4096 sequences of 20 positions
+// (Qwen2.5-7B's heads) 10, 47 and 770 us, by the token form 5, 20 and 150.
 struct VxRowTile {
     uint32_t seq, tile, lo, rows;
     int64_t pos0;  // position of row lo
@@ -808,7 +812,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void vx_paged_prompt_kernel(VxPa
     // The walk, a step of two chunks at a time: while step i's weights are formed and added, the scores of step
     // i + 1 are multiplied and the loads of what follows go out between the products (issued in one go they held a
     // wave up for 1800 of a step's 4500 clocks). LDS: K of steps i + 1 and i + 2, V of steps i and i + 1, each in two
-    // buffers. With q in several terms the registers hold one step's scores only (PIPE false).
+    // buffers. With q in several terms the next step's scores are not multiplied ahead (PIPE false): at head size 128 the
+    // registers do not hold them (240 and 255 of 256 are taken); at 64 (158 and 186) they would, which was not tried.
     if (n_steps) {
         Step now = step_of(0), next = now;
         Scores s;
@@ -980,9 +985,11 @@ hipError_t vx_launch_paged_attention(const VxPagedAttnArgs& a, hipStream_t st) {
 }
 
 // Splits of the prompt form: where the row tiles alone leave CUs empty, the positions are split until there are two
-// workgroups for each, into parts of 512 positions at least. Rows for a workgroup on every CU are not split: four
-// chunks of 400 rows behind 4000 positions take 121 us (Qwen2.5-7B) and 127 (Llama-3-8B), as two splits 129 and 150; 2000
-// rows 51 and 53, as two splits 67 and 73. Below that it pays: 2000 rows of SmolLM (141 workgroups) 29 us in three.
+// workgroups for each, into parts of 512 positions at least. Rows for a workgroup on every CU are not split, as equal parts
+// of every tile's positions with every row joined: four chunks of 400 rows behind 4000 positions take 168 us (Qwen2.5-7B)
+// and 175 (Llama-3-8B), as two splits 172 and 199; 2000 rows 68 and 69, as two splits 79 and 83 (fp32 rows 297 and 307,
+// 274 and 327; 108 and 110, 113 and 125). Below that it pays: 2000 rows of SmolLM (141 workgroups) 33 us in three, 39 whole.
+// Causal tiles have unequal walks, and cutting the long ones alone was not tried.
 // Every sequence has tiles of its own: rows of at most max_rows a sequence are that many sequences at least, and with two
 // workgroups for each CU from them alone nothing is split (64 sequences of 4 rows behind 4096 positions, Llama-3-8B:
 // 512 workgroups 210 us, in eight splits 247; 128 behind 2000, Qwen2.5-7B: 107 and 129; fp32 rows 317 and 340, 162
