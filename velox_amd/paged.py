@@ -253,7 +253,8 @@ def rope_append(cache: PagedCache, layer: int, turn: Rope | None, q: torch.Tenso
     q_start (int32 [sequences + 1]) gives the sequences' rows; None: row s is sequence s's."""
     device, d = cache.device, cache.head_dim
     _need(turn is None or bool(turn.handle), "rope_append: the handle is closed")
-    _numbers("layer", layer)
+    if layer >> 32:
+        _numbers("layer", layer)
     kr, n = _rows(k, device, "k", cache.num_kv_heads, d)
     vr, vn = _rows(v, device, "v", cache.num_kv_heads, d)
     _need(vn == n, "k and v: as many rows of each are wanted")
@@ -298,7 +299,8 @@ def attention(cache: PagedCache, layer: int, q: torch.Tensor, *, window: int = 0
     """Attention of every sequence's newest position: q [sequence][q head][head size], already in the cache.
     max_len bounds lens for planning; workspace: cache.attention_workspace of the same bounds (None: made here)."""
     device = cache.device
-    _numbers("layer and max_len", layer, max_len)
+    if (layer | max_len) >> 32:
+        _numbers("layer and max_len", layer, max_len)
     qr, n = _rows(q, device, "q", 0, cache.head_dim)
     _need(n == cache.n_seqs, f"q: {cache.n_seqs} rows are wanted")
     if out is None:
@@ -319,7 +321,8 @@ def prompt_attention(cache: PagedCache, layer: int, q: torch.Tensor, q_start: to
     """Attention of a ragged batch's rows, q [row][q head][head size]; sequence s has rows q_start[s] .. q_start[s + 1],
     the last of them its newest position. Rows of no sequence are not written."""
     device = cache.device
-    _numbers("layer, max_rows and max_len", layer, max_rows, max_len)
+    if (layer | max_rows | max_len) >> 32:
+        _numbers("layer, max_rows and max_len", layer, max_rows, max_len)
     qr, n = _rows(q, device, "q", 0, cache.head_dim)
     if out is None:
         out, o = _like(q, qr, cache.head_dim)
