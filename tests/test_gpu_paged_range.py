@@ -230,3 +230,79 @@ def test_a_captured_step_of_split_token_attention():
         step(b, *sets[1])
         torch.cuda.synchronize()
         assert torch.isfinite(sets[0][1]).all() and torch.equal(sets[0][1], sets[1][1]) and torch.equal(a.lens, b.lens)
+
+
+@pytest.mark.parametrize("d,rot", [(2048, 256), (1040, 256), (4099, 34)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rope_of_wide_heads(d, rot, layout, dtype):
+    """Heads of more units than a workgroup has threads."""
+    x = torch.randn(7, 3, d, generator=gen(d), device="cuda").to(T[dtype])
+    at, turn = ints([0, 1, 5, 100, 4096, 99999, 2 ** 31 - 1]), paged.Rope(rot, theta=5e5, layout=layout)
+    want, size = turned(x, at, turn, layout == "interleaved")
+    got = paged.rope(turn, x, at)
+    close_turn(got, want, size, T[dtype])
+    assert torch.equal(paged.rope(turn, x, at, out=x), got)
+
+
+@pytest.mark.parametrize("q,k,v,kv", [("f32", "bf16", "bf16", "bf16"), ("bf16", "f32", "f16", "f16"), ("f16", "f16", "f32", "bf16")])
+@pytest.mark.parametrize("odd", [0, 1])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_append_of_mixed_types_at_any_address(q, k, v, kv, odd, ragged):
+    """Each of q, k and v by itself against the same rows in one type, whose roundings come last."""
+    n, hq, hkv, d = 6, 5, 2, 64
+    rows = [3, 0, 40, 1, 7, 2] if ragged else [1] * 5  # one row each of the first five of six sequences
+    start = [sum(rows[:i]) for i in range(len(rows) + 1)]
+    f = Filled([70, 33, 90, 1, 64, 128], hkv, d, 32, kv)
+    turn, total = paged.Rope(d, layout="interleaved" if odd else "half"), start[-1]
+
+    def made(heads, dtype, seed):
+        room = torch.empty(total * heads * d + 1, dtype=T[dtype], device="cuda")
+        x = room[odd:odd + total * heads * d].view(total, heads, d)
+        return x.copy_(torch.randn(total, heads, d, generator=gen(seed), device="cuda"))
+
+    xq, xk, xv = made(hq, q, 1), made(hkv, k, 2), made(hkv, v, 3)
+    at = ints(start) if ragged else None
+    pool = f.pool.clone()
+    out = paged.rope_append(f.cache, 0, turn, xq, xk, xv, q_start=at)
+    got = f.pool.clone()
+    f.pool.copy_(pool)
+    wide = paged.rope_append(f.cache, 0, turn, xq.float(), xk.float(), xv.float(), q_start=at)
+    assert out.dtype == T[q] and torch.equal(out, wide.to(T[q])) and torch.equal(got.view(torch.int16), f.pool.view(torch.int16))
+    assert not torch.equal(f.pool.view(torch.int16), pool.view(torch.int16))
+
+
+@pytest.mark.parametrize("q,kv", [("bf16", "bf16"), ("f32", "f16")])
+def test_prompts_in_place_of_split_rows_and_of_many_heads(q, kv):
+    weights = half_step(T[kv]) ** 2 if q == kv else 2 ** -20
+    for hq, hkv, n, rows in ((4, 2, 3000, 50), (300, 1, 90, 40), (300, 1, 2500, 3)):
+        f = Filled([n], hkv, 64, 32, kv)
+        x = queries(rows, hq, hkv, 64, q)
+        y = x.clone()
+        assert (f.cache.prompt_workspace(hq, total_rows=rows) is None) == (n < 1000)
+        assert paged.prompt_attention(f.cache, 0, y, ints([0, rows]), out=y) is y
+        near(f, x, y, 0, weights, small=2.0 ** -32)
+        one = x[-1:].clone()
+        paged.attention(f.cache, 0, one, out=one)
+        near(f, x[-1:], one, 0, weights, small=2.0 ** -32)
+
+
+def test_layers_of_a_larger_pool():
+    """A cache over every second layer and the first pages of a pool, in the rows of a wider table."""
+    hkv, d, page = 2, 64, 32
+    f = Filled([100, 40], hkv, d, page, "bf16")
+    n_pages = f.pool.shape[1]
+    pool = torch.full((5, n_pages + 3, f.pool.shape[2]), float("nan"), dtype=torch.bfloat16, device="cuda")
+    pool[2, :n_pages] = f.pool[0]
+    table = torch.full((2, 11), -1, dtype=torch.int32, device="cuda")
+    table[:, 3:3 + f.table.shape[1]] = f.table
+    c = paged.PagedCache.over(pool[::2, :n_pages], table[:, 3:8], f.cache.lens, page_size=page, num_kv_heads=hkv, head_dim=d)
+    x = queries(30, 4, hkv, d, "f32")
+    for out, rows in ((paged.prompt_attention(c, 1, x, ints([0, 20, 30])), ((0, 20), (20, 30))), (paged.attention(c, 1, x[:2]), ((0, 1), (1, 2)))):
+        for s, (lo, hi) in enumerate(rows):
+            near(f, x[lo:hi], out[lo:hi], s, 2 ** -20)
+    before = pool.clone()
+    paged.rope_append(c, 2, None, None, x[:2, :2], x[:2, 2:])
+    same = torch.ones(5, n_pages + 3, dtype=torch.bool, device="cuda")
+    same[4, table[:, 3:8].max(1).values.new_tensor([int(f.table[0, 3]), int(f.table[1, 1])]).long()] = False
+    assert torch.equal(pool[same].view(torch.int16), before[same].view(torch.int16)) and not torch.equal(pool[4].view(torch.int16), before[4].view(torch.int16))
