@@ -306,3 +306,17 @@ def test_layers_of_a_larger_pool():
     same = torch.ones(5, n_pages + 3, dtype=torch.bool, device="cuda")
     same[4, table[:, 3:8].max(1).values.new_tensor([int(f.table[0, 3]), int(f.table[1, 1])]).long()] = False
     assert torch.equal(pool[same].view(torch.int16), before[same].view(torch.int16)) and not torch.equal(pool[4].view(torch.int16), before[4].view(torch.int16))
+
+
+def test_in_place_rows_lie_as_q_does():
+    f = Filled([40, 7], 2, 64, 32, "bf16")
+    x = queries(2, 4, 2, 64, "f32")
+    flat = x.as_strided((2, 4, 64), (256, 64, 1))
+    for call in (lambda: paged.attention(f.cache, 0, x, out=flat), lambda: paged.prompt_attention(f.cache, 0, x, ints([0, 1, 2]), out=flat)):
+        with pytest.raises(RuntimeError):
+            call()
+    f = Filled([40], 2, 64, 32, "bf16")
+    for run in (lambda a, o: paged.attention(f.cache, 0, a, out=o), lambda a, o: paged.prompt_attention(f.cache, 0, a, ints([0, 1]), out=o)):
+        y = x[:1].clone()
+        run(y, y.as_strided((1, 4, 64), (1000, 64, 1)))  # of one row there is no stride
+        near(f, x[:1], y, 0, 2 ** -20)

@@ -329,3 +329,11 @@ def test_refuses_a_workspace_that_a_long_cache_needs_and_is_not_given(hiplib):
     for space, size in ((None, n.value), (P, n.value - 1), (P + 4, n.value)):
         assert hiplib.velox_hip_paged_prompt_attention(C.byref(d), 0, C.byref(rows()), C.byref(rows()), P, 7, L.AttnMask(0, 0), 0.0, 0, 0, space,
                                                        size, None) == L.EINVAL
+
+
+def test_attention_refuses_rows_at_one_address_that_lie_otherwise(hiplib):
+    """out may be q; other rows from the same address on would be written while q's are read."""
+    d = desc()
+    for out in (rows(rs=512), rows(hs=128), rows(dtype=L.DT_BF16)):
+        assert attention(hiplib, d, out=out) == L.EINVAL
+        assert prompt(hiplib, d, out=out) == L.EINVAL

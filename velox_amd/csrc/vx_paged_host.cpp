@@ -77,8 +77,12 @@ uint64_t part_bytes(uint32_t rows, uint32_t heads, uint32_t splits, uint32_t d) 
     return splits > 1 ? (uint64_t)rows * heads * splits * (d + 2u) * 4u : 0;
 }
 
-bool attn_ok(const VeloxHipPagedCache* c, uint32_t layer, const VeloxHipRows* q, const VeloxHipRows* out, float scale) {
+// out is q, or memory of its own: rows at one address have to lie alike.
+bool attn_ok(const VeloxHipPagedCache* c, uint32_t layer, const VeloxHipRows* q, const VeloxHipRows* out, uint32_t n_rows, float scale) {
     if (!shape_ok(c) || !layers_ok(c) || !table_ok(c) || layer >= c->num_layers || !rows_ok(q) || !rows_ok(out)) return false;
+    if (q->data == out->data && (elt(q->dtype) != elt(out->dtype) || (n_rows > 1 && q->row_stride != out->row_stride) ||
+                                 (q->heads > 1 && q->head_stride != out->head_stride)))
+        return false;
     return q->heads == out->heads && q->heads % c->num_kv_heads == 0 && std::isfinite(scale);
 }
 
@@ -227,7 +231,7 @@ int velox_hip_paged_attention_bytes(const VeloxHipPagedCache* c, uint32_t heads,
 int velox_hip_paged_attention(const VeloxHipPagedCache* c, uint32_t layer, const VeloxHipRows* q, const VeloxHipRows* out,
                               VeloxHipAttnMask mask, float scale, uint32_t max_len, void* workspace,
                               uint64_t workspace_bytes, hipStream_t st) {
-    if (!attn_ok(c, layer, q, out, scale)) return VELOX_HIP_EINVAL;
+    if (!attn_ok(c, layer, q, out, c ? c->n_seqs : 0, scale)) return VELOX_HIP_EINVAL;
     VxPagedAttnArgs a;
     std::memset(&a, 0, sizeof(a));
     a.c = view(c, layer);
@@ -283,7 +287,7 @@ int velox_hip_paged_prompt_attention(const VeloxHipPagedCache* c, uint32_t layer
                                      const VeloxHipRows* out, const uint32_t* d_q_start, uint32_t n_rows,
                                      VeloxHipAttnMask mask, float scale, uint32_t max_rows, uint32_t max_len,
                                      void* workspace, uint64_t workspace_bytes, hipStream_t st) {
-    if (!attn_ok(c, layer, q, out, scale) || !d_q_start || !aligned(d_q_start, 4) || n_rows > kVxMaxRows) return VELOX_HIP_EINVAL;
+    if (!attn_ok(c, layer, q, out, n_rows, scale) || !d_q_start || !aligned(d_q_start, 4) || n_rows > kVxMaxRows) return VELOX_HIP_EINVAL;
     if (!n_rows) return VELOX_HIP_OK;
     VxPagedAttnArgs a;
     std::memset(&a, 0, sizeof(a));
