@@ -199,7 +199,7 @@ def prepare(case, seed):
 
 def _held(x):
     """Rows in whole numbers (as fp32) and their scales."""
-    scale = x.abs().amax(-1, keepdim=True) / 127
+    scale = (x.abs().amax(-1, keepdim=True).double() / 127).float()  # rounded once
     codes = torch.where(scale > 0, x.double() / scale.double(), 0.0).round_()  # to the nearest of exact quotients
     return codes.float(), scale
 
@@ -323,7 +323,7 @@ def run(s):
 def _exact_rows(x):
     """(whole numbers, scale) of every row, in float64; the scale is a 32-bit number by definition."""
     top = x.float().abs().max(dim=1).values
-    scale = (top / 127.0).double()
+    scale = (top.double() / 127.0).float().double()
     return torch.where(scale.unsqueeze(1) == 0, 0.0, torch.round(x.double() / scale.unsqueeze(1))), scale
 
 
