@@ -562,6 +562,99 @@ int velox_hip_pages_trim(const VeloxHipPagedCache* c, uint32_t window, uint32_t 
 int velox_hip_pages_compact(const VeloxHipPagedCache* c, hipStream_t stream);
 int velox_hip_pages_status(const VeloxHipPagedCache* c, uint32_t* refused, uint32_t* free_pages, hipStream_t stream);
 
+/* ---- 8-bit integer products (no counterpart in the reference, whose weights are fp32, fp16, 4 bits or fp8) ----
+ * Weights and activations in whole numbers of [-128, 127] with one fp32 scale for each weight row (output channel) and
+ * each activation row (token). As the paged cache's, every entry point checks its arguments (EINVAL), launches on `stream`
+ * with the stream's device current, allocates nothing, does not synchronize and can be captured into a hipGraph; a call's
+ * workspace is the call's own until the stream has passed it. Rows are VeloxHipRows with heads 1 (head_stride is not
+ * looked at).
+ *
+ * A row in 8 bits: scale = max |x| / 127 in fp32, codes x / scale to the nearest whole number (ties to even) of the exact
+ * quotient. A row of zeros (or whose scale would be below the least normal number) has scale 0 and codes 0; a row with an
+ * infinity or NaN has scale NaN and codes 0, so that its products are NaN and other rows' are not touched. */
+#define VELOX_HIP_INT8_MAX_K 131072u  /* sums of k products stay below 2^31 */
+typedef struct VeloxHipInt8Matrix {
+    void* codes;            /* velox_hip_int8_layout's code_bytes, 16-byte aligned */
+    float* scales;          /* scale_bytes, 16-byte aligned */
+    uint32_t n, k;          /* rows (paired: n / 2 gate rows, then their up rows) and columns of a matrix */
+    uint32_t count;         /* matrices of that shape (experts); a plain product takes 1; <= 1024 */
+    uint32_t paired;        /* 1: SwiGLU over gate and up rows; n is even */
+} VeloxHipInt8Matrix;
+/* The laid-out sizes of a matrix (its pointers are not looked at): 16-row tiles (paired: gate tile u at 2u, up tile u at
+ * 2u + 1) x 64 columns of 1 KiB, lane l of a tile holding columns 16 (l / 16) .. + 15 of row l % 16, k filled up to a
+ * multiple of 128 and rows to whole tiles with zeros; scales in the tiles' row order. Either output may be NULL. */
+int velox_hip_int8_layout(const VeloxHipInt8Matrix* m, uint64_t* code_bytes, uint64_t* scale_bytes);
+/* Matrices [first, first + number) from device memory: codes [number][n][k] by strides (bytes), scales [number][n] by a
+ * stride (elements) and next to each other in a matrix. */
+int velox_hip_int8_pack(const VeloxHipInt8Matrix* m, uint32_t first, uint32_t number, const int8_t* d_codes,
+                        uint64_t matrix_stride, uint64_t row_stride, const float* d_scales, uint64_t scale_stride,
+                        hipStream_t stream);
+
+typedef struct VeloxHipInt8Rows {
+    int8_t* codes;          /* row r at codes + r * row_stride; 16-byte aligned */
+    float* scales;          /* [rows] */
+    uint64_t row_stride;    /* bytes: a multiple of 128, at least k filled up to one */
+} VeloxHipInt8Rows;
+/* n_rows rows of k values in 8 bits (bytes behind k, up to the next multiple of 128, are 0). */
+int velox_hip_int8_quantize(const VeloxHipRows* x, uint32_t n_rows, uint32_t k, const VeloxHipInt8Rows* out,
+                            hipStream_t stream);
+/* y[r][n] = (sum_k c[r][k] w[n][k]) scale[n] scale[r], the sum exact, the scales' products in fp32; then
+ * VELOX_GEMV_STORE: out = y (+ bias[n]); VELOX_GEMV_RESIDUAL: out = residual + y (+ bias[n]) (residual may be out itself:
+ * the same data and stride; other overlaps are not allowed); VELOX_GEMV_SWIGLU (a paired matrix, and only that):
+ * out[r][j] = silu(gate_j) up_j. fp32 throughout, rounded once to out's type. The rows come as x, quantized on the way
+ * (workspace: velox_hip_int8_product_bytes, 16-byte aligned), or as q, already in 8 bits (no workspace); the other is
+ * NULL. m->count is 1. Fewer than 2^24 rows. */
+int velox_hip_int8_product_bytes(const VeloxHipInt8Matrix* m, uint32_t n_rows, uint64_t* bytes);
+int velox_hip_int8_product(const VeloxHipInt8Matrix* m, const VeloxHipRows* x, const VeloxHipInt8Rows* q, uint32_t n_rows,
+                           const float* d_bias, const VeloxHipRows* residual, const VeloxHipRows* out, int mode,
+                           void* workspace, uint64_t workspace_bytes, hipStream_t stream);
+
+/* ---- experts (the reference's velox_cuda_moe_gate_topk / _dispatch_topk, src/codegen.rs:2112-2211) ----
+ * route: of n_experts experts the top_k with the largest choice values, in descending order, equal ones by index.
+ *   score: SOFTMAX exp(x_e) / sum over the row, SIGMOID 1 / (1 + exp(-x_e)); choice value: score + bias[e] (d_bias NULL: 0).
+ *   With groups > 1 (groups of n_experts / groups neighbours) only the experts of the top_groups groups with the largest
+ *   marks take part, a group's mark being the LARGEST of its choice values or the sum of its TWO largest (equal marks by
+ *   index). weights[r][j] = scale * score, divided by the row's sum of chosen scores first with renormalize (0 where that
+ *   sum is 0). Scores are formed and compared in 64 bits (softmax without a bias and with LARGEST marks by the logits
+ *   themselves), so that nearly equal ones keep their order. A logit of -infinity or NaN takes its expert out of the row
+ *   and of the softmax's sum, a bias that is not finite takes it out of every row; a logit of +infinity counts as the
+ *   largest finite number. Where fewer than
+ *   top_k experts are left, the rest of ids is VELOX_HIP_NO_EXPERT and of weights 0: a row of -infinity is padding. */
+#define VELOX_HIP_NO_EXPERT 0xFFFFFFFFu
+#define VELOX_ROUTE_SOFTMAX 0u
+#define VELOX_ROUTE_SIGMOID 1u
+#define VELOX_GROUP_LARGEST 0u
+#define VELOX_GROUP_TWO 1u
+typedef struct VeloxHipRouteConfig {
+    uint32_t n_experts, top_k;   /* 1..1024, 1..64; top_k <= n_experts / groups * top_groups */
+    uint32_t scores;             /* VELOX_ROUTE_* */
+    uint32_t groups, top_groups; /* 1..64, a divisor of n_experts; 1..groups */
+    uint32_t group_by;           /* VELOX_GROUP_* */
+    uint32_t renormalize;        /* 0 or 1 */
+    float scale;                 /* finite */
+} VeloxHipRouteConfig;
+/* logits [n_rows][n_experts] (heads 1), ids and weights [n_rows][top_k]. Fewer than 2^24 rows. */
+int velox_hip_expert_route(const VeloxHipRouteConfig* cfg, const VeloxHipRows* logits, const float* d_bias, uint32_t n_rows,
+                           uint32_t* d_ids, float* d_weights, hipStream_t stream);
+/* The n_slots slots of d_ids (row r, place j: slot r * top_k + j) in the order of their experts first .. first + count - 1,
+ * an expert's slots in their own order: d_order[offsets[e] .. offsets[e + 1]) are expert first + e's, d_offsets has count + 1
+ * entries. Slots of other ids are left out; d_order behind the last offset is VELOX_HIP_NO_EXPERT. n_slots <= 2^20,
+ * count <= 1024; workspace: velox_hip_expert_group_bytes (may be 0 bytes: NULL), 16-byte aligned. */
+int velox_hip_expert_group_bytes(uint32_t n_slots, uint32_t count, uint64_t* bytes);
+int velox_hip_expert_group(const uint32_t* d_ids, uint32_t n_slots, uint32_t first, uint32_t count, uint32_t* d_order,
+                           uint32_t* d_offsets, void* workspace, uint64_t workspace_bytes, hipStream_t stream);
+/* out[r] = residual[r] (NULL: 0) + sum over j of weights[r][j] down_e(h), h = silu(gate_e(x[r])) up_e(x[r]), e = ids[r][j]
+ * - first. gate_up (paired, n = 2 inner, k = hidden) and down (n = hidden, k = inner) hold the experts first .. first +
+ * count - 1; other ids (VELOX_HIP_NO_EXPERT, experts that live elsewhere) add nothing, a row may name an expert twice. x and
+ * h enter the products in 8 bits (h from fp32), sums are fp32 in the order of j, rounded once to out's type. out may be x or the residual (the same data and stride). n_rows * top_k <= 2^20; workspace:
+ * velox_hip_expert_ffn_bytes of the same matrices, enough for up to n_rows rows of any types, 16-byte aligned. */
+int velox_hip_expert_ffn_bytes(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Matrix* down, uint32_t n_rows,
+                               uint32_t top_k, uint64_t* bytes);
+int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Matrix* down, uint32_t first,
+                         const VeloxHipRows* x, const uint32_t* d_ids, const float* d_weights, uint32_t n_rows, uint32_t top_k,
+                         const VeloxHipRows* residual, const VeloxHipRows* out, void* workspace, uint64_t workspace_bytes,
+                         hipStream_t stream);
+
 /* ---- runner (velox_cuda_runner.cu:327-726 flow: plan, alloc, load, capture, prefill, decode) ---- */
 typedef struct VeloxHipRunOptions {
     const char* model;       /* builtin config name (unless model_file or weights_path is given) */

@@ -140,6 +140,27 @@ class AttnMask(C.Structure):
     _fields_ = [("window", C.c_uint32), ("sinks", C.c_uint32)]
 
 
+NO_EXPERT = 0xFFFFFFFF
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+GROUP_LARGEST, GROUP_TWO = 0, 1
+
+
+class Int8MatrixDesc(C.Structure):
+    """VeloxHipInt8Matrix: laid-out 8-bit matrices of one shape."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("n", C.c_uint32), ("k", C.c_uint32), ("count", C.c_uint32),
+                ("paired", C.c_uint32)]
+
+
+class Int8RowsDesc(C.Structure):
+    """VeloxHipInt8Rows: activation rows in 8 bits."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("row_stride", C.c_uint64)]
+
+
+class RouteConfig(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("n_experts", "top_k", "scores", "groups", "top_groups", "group_by", "renormalize")] + \
+               [("scale", C.c_float)]
+
+
 MLA_Q_A, MLA_Q_B, MLA_KV_A, MLA_KV_B, MLA_O, MLA_NORM, MLA_Q_A_NORM, MLA_KV_A_NORM = range(1, 9)
 
 
@@ -273,6 +294,18 @@ _SIGS = {
     "velox_hip_pages_trim": (_I, [C.POINTER(PagedCacheDesc), _U32, _U32, _P]),
     "velox_hip_pages_compact": (_I, [C.POINTER(PagedCacheDesc), _P]),
     "velox_hip_pages_status": (_I, [C.POINTER(PagedCacheDesc), C.POINTER(_U32), C.POINTER(_U32), _P]),
+    "velox_hip_int8_layout": (_I, [C.POINTER(Int8MatrixDesc), C.POINTER(_U64), C.POINTER(_U64)]),
+    "velox_hip_int8_pack": (_I, [C.POINTER(Int8MatrixDesc), _U32, _U32, _P, _U64, _U64, _P, _U64, _P]),
+    "velox_hip_int8_quantize": (_I, [C.POINTER(Rows), _U32, _U32, C.POINTER(Int8RowsDesc), _P]),
+    "velox_hip_int8_product_bytes": (_I, [C.POINTER(Int8MatrixDesc), _U32, C.POINTER(_U64)]),
+    "velox_hip_int8_product": (_I, [C.POINTER(Int8MatrixDesc), C.POINTER(Rows), C.POINTER(Int8RowsDesc), _U32, _P, C.POINTER(Rows),
+                                    C.POINTER(Rows), _I, _P, _U64, _P]),
+    "velox_hip_expert_route": (_I, [C.POINTER(RouteConfig), C.POINTER(Rows), _P, _U32, _P, _P, _P]),
+    "velox_hip_expert_group_bytes": (_I, [_U32, _U32, C.POINTER(_U64)]),
+    "velox_hip_expert_group": (_I, [_P, _U32, _U32, _U32, _P, _P, _P, _U64, _P]),
+    "velox_hip_expert_ffn_bytes": (_I, [C.POINTER(Int8MatrixDesc), C.POINTER(Int8MatrixDesc), _U32, _U32, C.POINTER(_U64)]),
+    "velox_hip_expert_ffn": (_I, [C.POINTER(Int8MatrixDesc), C.POINTER(Int8MatrixDesc), _U32, C.POINTER(Rows), _P, _P, _U32, _U32,
+                                  C.POINTER(Rows), C.POINTER(Rows), _P, _U64, _P]),
     "velox_hip_arena_check": (_I, [C.POINTER(Arena), C.POINTER(ModelConfig)]),
     "velox_hip_record_error": (None, [_I]),
     "velox_hip_decode": (None, [C.POINTER(Arena), _U32, C.c_size_t, _U64, _P]),
