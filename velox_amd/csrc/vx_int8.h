@@ -47,11 +47,12 @@ struct VxI8Args {
     uint32_t n_rows;           // plain products
     VxGrouped g;               // HIDDEN, SLOT
     uint32_t top;              // HIDDEN: position p reads row order[p] / top of a
-    uint32_t max_items;
+    uint32_t max_items, item_rows;
     const float* bias;         // STORE
     VxI8View res, out;         // STORE (res.data NULL: none), SWIGLU
+    uint32_t vec;              // 1: res and out rows begin at whole multiples of four elements
     float* part;               // HIDDEN: h of position p at part + p * part_stride; SLOT: the answer of slot s at s
-    uint64_t part_stride;      // elements
+    uint64_t part_stride;      // elements, a multiple of 4
 };
 
 struct VxRouteArgs {

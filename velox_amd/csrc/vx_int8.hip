@@ -4,6 +4,17 @@
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+template <int V>
+struct vx_int {
+    static constexpr int value = V;
+};
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void vx_each(F f) {  // f(vx_int<0>) .. f(vx_int<N - 1>)
+    if constexpr (I < N) {
+        f(vx_int<I>{});
+        vx_each<N, I + 1>(f);
+    }
+}
 
 __device__ __forceinline__ float vx_load(const void* p, size_t i, uint32_t dtype) {
     if (dtype == VELOX_DT_F32) return ((const float*)p)[i];
@@ -16,6 +27,61 @@ __device__ __forceinline__ void vx_store(void* p, size_t i, uint32_t dtype, floa
     else if (dtype == VELOX_DT_F16) ((_Float16*)p)[i] = (_Float16)v;
     else ((__bf16*)p)[i] = (__bf16)v;
 }
+
+// Four neighbouring values of a row at element i as fp32, and back (rounded once); VEC: at whole 16- or 8-byte places.
+template <bool VEC>
+__device__ __forceinline__ float4 vx_load4(const void* p, size_t i, uint32_t dtype, uint32_t left) {
+    float4 v = make_float4(0, 0, 0, 0);
+    if (VEC && left >= 4u) {
+        if (dtype == VELOX_DT_F32) return *(const float4*)((const float*)p + i);
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+        const uint2 w = *(const uint2*)((const uint16_t*)p + i);
+        if (dtype == VELOX_DT_F16) {
+            const h4 h = __builtin_bit_cast(h4, w);
+            return make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
+        }
+        const b4 b = __builtin_bit_cast(b4, w);
+        return make_float4((float)b[0], (float)b[1], (float)b[2], (float)b[3]);
+    }
+    if (left > 0u) v.x = vx_load(p, i, dtype);
+    if (left > 1u) v.y = vx_load(p, i + 1u, dtype);
+    if (left > 2u) v.z = vx_load(p, i + 2u, dtype);
+    if (left > 3u) v.w = vx_load(p, i + 3u, dtype);
+    return v;
+}
+template <bool VEC>
+__device__ __forceinline__ void vx_store4(void* p, size_t i, uint32_t dtype, uint32_t left, float4 v) {
+    if (VEC && left >= 4u) {
+        if (dtype == VELOX_DT_F32) {
+            *(float4*)((float*)p + i) = v;
+            return;
+        }
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+        if (dtype == VELOX_DT_F16) *(h4*)((uint16_t*)p + i) = h4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+        else *(b4*)((uint16_t*)p + i) = b4{(__bf16)v.x, (__bf16)v.y, (__bf16)v.z, (__bf16)v.w};
+        return;
+    }
+    if (left > 0u) vx_store(p, i, dtype, v.x);
+    if (left > 1u) vx_store(p, i + 1u, dtype, v.y);
+    if (left > 2u) vx_store(p, i + 2u, dtype, v.z);
+    if (left > 3u) vx_store(p, i + 3u, dtype, v.w);
+}
+// Outputs n .. n + 3 of row r (of `cols` in a row), y their products with the bias: the residual added, stored.
+template <bool VEC>
+__device__ __forceinline__ void vx_finish(const VxI8Args& a, size_t r, uint32_t n, uint32_t cols, float4 y) {
+    const uint32_t left = cols - n;
+    if (a.res.data) {
+        const float4 v = vx_load4<VEC>(a.res.data, r * a.res.rs + n, a.res.dtype, left);
+        y.x += v.x;
+        y.y += v.y;
+        y.z += v.z;
+        y.w += v.w;
+    }
+    vx_store4<VEC>(a.out.data, r * a.out.rs + n, a.out.dtype, left, y);
+}
+__device__ __forceinline__ float vx_swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
 // ---- weights ----
 __global__ __launch_bounds__(256) void vx_i8_pack_kernel(VxI8Mat m, uint32_t first, const int8_t* __restrict__ src, uint64_t ms,
@@ -119,37 +185,325 @@ __global__ __launch_bounds__(256) void vx_i8_kernel(VxI8Args a, uint32_t row0, u
     }
     if (!live) return;
     const float s = a.a.scales[row];
-    const float* ws = a.w.scales + (uint64_t)e * a.w.n_tiles * 16u + 16u * t0 + 4u * (lane >> 4);
-    if constexpr (EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN) {
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const float gate = (float)acc0[i] * ws[i] * s, up = (float)acc1[i] * ws[16u + i] * s;
-            const float h = gate / (1.0f + expf(-gate)) * up;
-            const uint32_t j = 8u * t0 + 4u * (lane >> 4) + i;
-            if (j < a.w.n / 2u) {
-                if constexpr (EPI == VX_I8_HIDDEN) a.part[(size_t)p * a.part_stride + j] = h;
-                else vx_store(a.out.data, (size_t)p * a.out.rs + j, a.out.dtype, h);
+    const float* ws = a.w.scales + ((uint64_t)e * a.w.n_tiles + t0) * 16u + 4u * (lane >> 4);
+    const auto scaled = [&](const v4i& acc, const float* w) {
+        return make_float4((float)acc[0] * w[0] * s, (float)acc[1] * w[1] * s, (float)acc[2] * w[2] * s, (float)acc[3] * w[3] * s);
+    };
+    const auto put = [&](uint32_t n, uint32_t cols, float4 y) {
+        if (n >= cols) return;
+        if constexpr (EPI == VX_I8_STORE) {
+            if (a.bias) {
+                const float4 b = vx_load4<false>(a.bias, n, VELOX_DT_F32, cols - n);
+                y = make_float4(y.x + b.x, y.y + b.y, y.z + b.z, y.w + b.w);
             }
         }
+        if constexpr (kGrouped) *(float4*)(a.part + (size_t)(EPI == VX_I8_SLOT ? slot : p) * a.part_stride + n) = y;  // (rows of whole float4)
+        else if (a.vec) vx_finish<true>(a, p, n, cols, y);
+        else vx_finish<false>(a, p, n, cols, y);
+    };
+    if constexpr (EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN) {
+        const float4 g = scaled(acc0, ws), u = scaled(acc1, ws + 16);
+        put(8u * t0 + 4u * (lane >> 4), a.w.n / 2u, make_float4(vx_swiglu(g.x, u.x), vx_swiglu(g.y, u.y), vx_swiglu(g.z, u.z), vx_swiglu(g.w, u.w)));
     } else {
+        put(16u * t0 + 4u * (lane >> 4), a.w.n, scaled(acc0, ws));
+        if (two) put(16u * (t0 + 1u) + 4u * (lane >> 4), a.w.n, scaled(acc1, ws + 16));
+    }
+}
+
+// ---- products of many rows: tiles through LDS ----
+// A workgroup of WN x WM waves takes 32 WN FN weight rows by 32 WM FM activation rows, a wave 32 FN by 32 FM of them on
+// v_mfma_i32_32x32x32_i8 (D[n = 8 (i / 4) + 4 (lane / 32) + i % 4][row = lane % 32]). 128 columns of both go straight to LDS at
+// a time, two stages; a column quarter's operands are read while the one before is multiplied, and the barrier between
+// two stages stands in front of the last quarter's products, behind which everything of the stage is in registers.
+// Weights lie in LDS as in memory (1 KiB tiles, operand reads of 256 neighbouring bytes); of an activation row's eight
+// 16-byte units, unit u lies at u ^ (row % 8), so that eight rows' reads of one unit meet all banks.
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+// 16 bytes a lane from memory to lds + 16 lane.
+__device__ __forceinline__ void vx_to_lds(uint32_t lds, const void* from, uint32_t off) {
+    const uint64_t v = (uint64_t)(uintptr_t)from;  // (a scalar operand, wherever the compiler formed it)
+    const uint64_t base = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
+}
+__device__ __forceinline__ void vx_to_lds(uint32_t lds, const void* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "m0", "memory");
+}
+
+// What a lane of the wave wrote to LDS is what the others read behind this.
+__device__ __forceinline__ void vx_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Workgroup b of `total`: the b / 8-th of XCD b % 8 (workgroups are dealt out in turn), each XCD taking a run of neighbours.
+__device__ __forceinline__ uint32_t vx_xcd_run(uint32_t b, uint32_t total) {
+    const uint32_t x = b & 7u, i = b >> 3, q = total >> 3, r = total & 7u;
+    return x * q + (x < r ? x : r) + i;
+}
+
+template <int WN, int WM, int FN, int FM, int EPI>
+__global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, uint32_t row0, uint32_t n_blocks, uint32_t m_blocks) {
+    constexpr int W = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, STAGE = (TN + TM) * 128;
+    constexpr bool kGrouped = EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };  // (quotients are formed in vector registers)
+    uint32_t nb, e = 0, first, end = a.n_rows;
+    if constexpr (kGrouped) {
+        const uint32_t total = uniform(*a.g.n_items) * n_blocks;
+        if (blockIdx.x >= total) return;
+        const uint32_t id = vx_xcd_run(blockIdx.x, total);
+        const uint2 it = a.g.items[id / n_blocks];
+        nb = uniform(id % n_blocks);
+        e = uniform(it.x);
+        first = uniform(it.y);
+        end = uniform(a.g.offsets[e + 1u]);
+    } else {
+        // patches of up to 4 row blocks by all weight blocks, the rows first
+        const uint32_t id = vx_xcd_run(blockIdx.x, n_blocks * m_blocks), patch = id / (4u * n_blocks);
+        const uint32_t high = m_blocks - 4u * patch < 4u ? m_blocks - 4u * patch : 4u, in = id - patch * 4u * n_blocks;
+        nb = uniform(in / high);
+        first = uniform(row0 + (4u * patch + in % high) * TM);
+    }
+    const uint32_t wn = wave / WM, wm = wave % WM;
+    const uint32_t steps = a.w.k_tiles / 2u, tile0 = nb * (TN / 16);
+
+    // where this wave's share of a stage comes from: weight tiles (two pieces of 1 KiB each), groups of 8 rows
+    constexpr int PW = TN / 16 / W, PA = TM / 8 / W;
+    const uint8_t* pw[PW];
+    const uint8_t* pa[PA];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
 #pragma unroll
-        for (uint32_t t = 0; t < 2u; ++t) {
-            if (t && !two) break;
+    for (int j = 0; j < PW; ++j) {
+        const uint32_t t = tile0 + wave * PW + j;
+        pw[j] = (const uint8_t*)a.w.codes + ((uint64_t)e * a.w.n_tiles + (t < a.w.n_tiles ? t : a.w.n_tiles - 1u)) * a.w.k_tiles * 1024u;
+    }
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t n = 16u * (t0 + t) + 4u * (lane >> 4) + i;
-                if (n >= a.w.n) continue;
-                float y = (float)(t ? acc1 : acc0)[i] * ws[16u * t + i] * s;
-                if constexpr (EPI == VX_I8_SLOT) {
-                    a.part[(size_t)slot * a.part_stride + n] = y;
-                } else {
-                    if (a.bias) y += a.bias[n];
-                    if (a.res.data) y += vx_load(a.res.data, (size_t)p * a.res.rs + n, a.res.dtype);
-                    vx_store(a.out.data, (size_t)p * a.out.rs + n, a.out.dtype, y);
-                }
-            }
+    for (int j = 0; j < PA; ++j) {
+        const uint32_t p = first + (wave * PA + j) * 8u + (lane >> 3);
+        uint32_t row = p < end ? p : end - 1u;
+        if constexpr (EPI == VX_I8_HIDDEN) row = a.g.order[row] / a.top;
+        pa[j] = (const uint8_t*)a.a.codes + (uint64_t)row * a.a.rs + (((lane & 7u) ^ (lane >> 3)) * 16u);
+    }
+    // piece j of this wave's share of a stage into LDS, its pointer moved on
+    auto fetch = [&](auto j_, uint32_t stage) {
+        constexpr int j = decltype(j_)::value;
+        const uint32_t base = lds0 + stage * STAGE;
+        if constexpr (j < PW) {
+            vx_to_lds(base + (wave * PW + j) * 2048u, pw[j], lane * 16u);
+            vx_to_lds(base + (wave * PW + j) * 2048u + 1024u, pw[j] + 1024, lane * 16u);
+            pw[j] += 2048;
+        } else {
+            vx_to_lds(base + TN * 128 + (wave * PA + j - PW) * 1024u, pa[j - PW]);
+            pa[j - PW] += 128;
+        }
+    };
+    auto fetch_all = [&](uint32_t stage) { vx_each<PW + PA>([&](auto j) { fetch(j, stage); }); };
+    // operands of column quarter s: the weights' by tile, the rows' by their unit's place
+    const uint32_t w_at = wn * FN * 4096u + ((lane >> 4) & 1u) * 2048u + (lane >> 5) * 256u + (lane & 15u) * 16u;
+    uint32_t a_at[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) a_at[s] = TN * 128u + (wm * FM * 32u + (lane & 31u)) * 128u + (((2u * s + (lane >> 5)) ^ (lane & 7u)) * 16u);
+    // what the epilogue needs: outputs 4 (lane % LANES) .. + 3 of the wave's, the rows lane % 32 of its blocks
+    constexpr bool kSwiglu = EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN;
+    constexpr int ROW = 32 * FN + 4, LANES = (kSwiglu ? 16 : 32) * FN / 4, AT_ONCE = 64 / LANES;
+    const uint32_t cols = kSwiglu ? a.w.n / 2u : a.w.n, col0 = (tile0 * 16u + wn * FN * 32u) / (kSwiglu ? 2u : 1u);
+    float4 w0 = make_float4(0, 0, 0, 0), w1 = w0;
+    float row_scale[FM];
+    uint32_t row_slot[FM];
+    {
+        const uint32_t c = 4u * (lane % LANES), at = tile0 * 16u + wn * FN * 32u + (kSwiglu ? c / 16u * 32u + c % 16u : c);
+        const float* ws = a.w.scales + (uint64_t)e * a.w.n_tiles * 16u + at;
+        if (at < a.w.n_tiles * 16u) {
+            w0 = *(const float4*)ws;
+            if constexpr (kSwiglu) w1 = *(const float4*)(ws + 16);
+        }
+        if constexpr (EPI == VX_I8_STORE) {
+            if (a.bias && at < a.w.n) w1 = vx_load4<false>(a.bias, at, VELOX_DT_F32, a.w.n - at);
+        }
+#pragma unroll
+        for (int m = 0; m < FM; ++m) {
+            const uint32_t p = first + (wm * FM + m) * 32u + (lane & 31u), at_p = p < end ? p : end - 1u;
+            row_slot[m] = at_p;
+            if constexpr (kGrouped) row_slot[m] = a.g.order[at_p];
+            row_scale[m] = a.a.scales[EPI == VX_I8_HIDDEN ? row_slot[m] / a.top : at_p];
         }
     }
+    v4i fw[2][FN], fa[2][FM];
+    v16i acc[FN][FM];
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[n][m][i] = 0;
+
+    // operand r of quarter s: the first of the weights', the rows', the other weights'
+    auto read = [&](auto s_, auto r_, uint32_t stage, auto to_) {
+        constexpr int s = decltype(s_)::value, r = decltype(r_)::value, to = decltype(to_)::value;
+        const uint8_t* base = lds + stage * STAGE;
+        if constexpr (r >= 1 && r <= FM) fa[to][r - 1] = *(const v4i*)(base + a_at[s] + (r - 1) * 4096);
+        else fw[to][r ? r - FM : 0] = *(const v4i*)(base + w_at + (r ? r - FM : 0) * 4096 + (s >> 1) * 1024 + (s & 1) * 512);
+    };
+    // The products of the operands in set `from`; between them the next quarter's reads and (LO <= j < HI) the pieces of a
+    // stage's fetch. The order is fixed: left to itself the compiler puts the reads together and waits for them.
+    auto quarter = [&](auto from_, auto next_, uint32_t stage, auto lo_, auto hi_, uint32_t into) {
+        constexpr int from = decltype(from_)::value, next = decltype(next_)::value, LO = decltype(lo_)::value, HI = decltype(hi_)::value;
+        constexpr int P = FN * FM, R = FN + FM;
+        vx_each<P>([&](auto i_) {
+            constexpr int i = decltype(i_)::value, n = i / FM, m = i % FM;
+            if constexpr (next >= 0) {
+                constexpr int r0 = i * R / P, r1 = (i + 1) * R / P;
+                if constexpr (r1 > r0) read(vx_int<(next >= 0 ? next : 0)>{}, vx_int<r0>{}, stage, vx_int<from ^ 1>{});
+                if constexpr (r1 > r0 + 1) read(vx_int<(next >= 0 ? next : 0)>{}, vx_int<r0 + 1>{}, stage, vx_int<from ^ 1>{});
+            }
+            constexpr int d0 = LO + i * (HI - LO) / P, d1 = LO + (i + 1) * (HI - LO) / P;
+            if constexpr (d1 > d0) fetch(vx_int<d0>{}, into);
+            if constexpr (d1 > d0 + 1) fetch(vx_int<d0 + 1>{}, into);
+            if constexpr (d1 > d0 + 2) fetch(vx_int<d0 + 2>{}, into);
+            acc[n][m] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[from][n], fa[from][m], acc[n][m], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto ready = [&] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    constexpr int HALF = (PW + PA) / 2;
+
+    // Step i reads stage i % 2. In its last quarter and the next step's first, stage i + 2's pieces come; behind the
+    // last step's there are none left, the steps' last pieces come again in their place (and are not read).
+    fetch_all(0);
+    ready();
+    vx_each<FN + FM>([&](auto r) { read(vx_int<0>{}, r, 0, vx_int<0>{}); });
+    if (steps > 1u) vx_each<HALF>([&](auto j) { fetch(j, 1); });
+    for (uint32_t i = 0; i + 1u < steps; ++i) {
+        const uint32_t st = i & 1u;
+        quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<HALF>{}, vx_int<PW + PA>{}, st ^ 1u);
+        quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+        quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+        ready();
+        if (i + 2u == steps) {
+#pragma unroll
+            for (int j = 0; j < HALF; ++j) {
+                if (j < PW) pw[j] -= 2048;
+                else pa[j - PW] -= 128;
+            }
+        }
+        quarter(vx_int<1>{}, vx_int<0>{}, st ^ 1u, vx_int<0>{}, vx_int<HALF>{}, st);
+    }
+    const uint32_t st = (steps - 1u) & 1u;
+    quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+    quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+    quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+    quarter(vx_int<1>{}, vx_int<-1>{}, 0, vx_int<0>{}, vx_int<0>{}, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing may come into LDS behind the workgroup's end)
+
+    // Epilogue, one block of 32 rows at a time: the sums go through LDS, where the lane of row lane % 32 writes those of n =
+    // 8 q + 4 (lane / 32) + 0 .. 3 of every weight block; a row's outputs are then formed by neighbouring lanes, four each, and
+    // leave in whole lines. Rolled loops: code that runs once comes through the instruction cache at memory's pace (with the
+    // scales applied in front of LDS and everything unrolled a launch took 60 us more).
+    static_assert(W * 32 * ROW * 4 <= 2 * STAGE, "the epilogue's rows lie in the stages");
+    int* mine = (int*)lds + wave * 32 * ROW;
+    asm volatile("s_barrier" ::: "memory");
+    const uint32_t n = col0 + 4u * (lane % LANES);
+#pragma unroll 1
+    for (int m = 0; m < FM; ++m) {
+        vx_each<FM>([&](auto m_) {
+            constexpr int mm = decltype(m_)::value;
+            if (m == mm) {
+#pragma unroll
+                for (int b = 0; b < FN; ++b)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *(v4i*)(mine + (lane & 31u) * ROW + 32 * b + 8 * q + 4u * (lane >> 5)) = v4i{acc[b][mm][4 * q], acc[b][mm][4 * q + 1], acc[b][mm][4 * q + 2], acc[b][mm][4 * q + 3]};
+            }
+        });
+        float s = row_scale[0];
+        uint32_t slot = row_slot[0];
+#pragma unroll
+        for (int j = 1; j < FM; ++j) {
+            s = m == j ? row_scale[j] : s;
+            slot = m == j ? row_slot[j] : slot;
+        }
+        vx_wave_sync();
+        const uint32_t p0 = first + (wm * FM + m) * 32u;
+        // DT: an element type (rows of whole vectors), or 3: any type and place
+        const auto leave = [&](auto dt_, auto res_) {
+            constexpr uint32_t DT = decltype(dt_)::value;
+            constexpr bool RES = decltype(res_)::value != 0;
+            constexpr int PASSES = 32 / AT_ONCE, TOGETHER = DT < 3u && PASSES > 4 ? 4 : 1;
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += AT_ONCE * TOGETHER) {
+                float4 y[TOGETHER], res[TOGETHER];
+                uint32_t to[TOGETHER];
+                bool live[TOGETHER];
+#pragma unroll
+                for (int j = 0; j < TOGETHER; ++j) {
+                    const uint32_t in = r0 + j * AT_ONCE + lane / LANES;
+                    live[j] = p0 + in < end && n < cols;
+                    to[j] = EPI == VX_I8_SLOT ? (uint32_t)__shfl((int)slot, (int)in) : p0 + in;
+                    if constexpr (RES && DT < 3u) {
+                        if (live[j]) res[j] = vx_load4<true>(a.res.data, (size_t)to[j] * a.res.rs + n, DT, cols - n);
+                    }
+                    const float sr = __shfl(s, (int)in);
+                    const int* at = mine + in * ROW;
+                    if constexpr (kSwiglu) {
+                        const uint32_t c = 4u * (lane % LANES), b = c / 16u * 32u + c % 16u;
+                        const v4i g = *(const v4i*)(at + b), u = *(const v4i*)(at + b + 16u);
+                        y[j] = make_float4(vx_swiglu((float)g[0] * w0.x * sr, (float)u[0] * w1.x * sr), vx_swiglu((float)g[1] * w0.y * sr, (float)u[1] * w1.y * sr),
+                                           vx_swiglu((float)g[2] * w0.z * sr, (float)u[2] * w1.z * sr), vx_swiglu((float)g[3] * w0.w * sr, (float)u[3] * w1.w * sr));
+                    } else {
+                        const v4i c = *(const v4i*)(at + 4u * (lane % LANES));
+                        y[j] = make_float4((float)c[0] * w0.x * sr, (float)c[1] * w0.y * sr, (float)c[2] * w0.z * sr, (float)c[3] * w0.w * sr);
+                        if constexpr (EPI == VX_I8_STORE) {
+                            if (a.bias) y[j] = make_float4(y[j].x + w1.x, y[j].y + w1.y, y[j].z + w1.z, y[j].w + w1.w);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < TOGETHER; ++j) {
+                    if (!live[j]) continue;
+                    if constexpr (kGrouped) {
+                        *(float4*)(a.part + (size_t)to[j] * a.part_stride + n) = y[j];  // (rows of whole float4)
+                    } else if constexpr (DT < 3u) {
+                        if constexpr (RES) y[j] = make_float4(y[j].x + res[j].x, y[j].y + res[j].y, y[j].z + res[j].z, y[j].w + res[j].w);
+                        vx_store4<true>(a.out.data, (size_t)to[j] * a.out.rs + n, DT, cols - n, y[j]);
+                    } else {
+                        vx_finish<false>(a, to[j], n, cols, y[j]);
+                    }
+                }
+            }
+        };
+        if constexpr (kGrouped) {
+            leave(vx_int<VELOX_DT_F32>{}, vx_int<0>{});
+        } else {
+            const bool res = EPI == VX_I8_STORE && a.res.data;
+            if (!a.vec || (res && a.res.dtype != a.out.dtype)) leave(vx_int<3>{}, vx_int<0>{});
+            else if (a.out.dtype == VELOX_DT_F32) res ? leave(vx_int<0>{}, vx_int<1>{}) : leave(vx_int<0>{}, vx_int<0>{});
+            else if (a.out.dtype == VELOX_DT_F16) res ? leave(vx_int<1>{}, vx_int<1>{}) : leave(vx_int<1>{}, vx_int<0>{});
+            else res ? leave(vx_int<2>{}, vx_int<1>{}) : leave(vx_int<2>{}, vx_int<0>{});
+        }
+        vx_wave_sync();
+    }
+}
+
+constexpr uint32_t kTileStep = 1u << 20;  // rows of a launch
+
+template <int WN, int WM, int FN, int FM, int EPI>
+hipError_t vx_i8_tile_launch(const VxI8Args& a, hipStream_t st) {
+    constexpr uint32_t TN = 32 * WN * FN, TM = 32 * WM * FM, lds = 2 * (TN + TM) * 128;
+    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_tile_kernel<WN, WM, FN, FM, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (set != hipSuccess) return set;
+    const uint32_t n_blocks = (a.w.n_tiles * 16u + TN - 1u) / TN;
+    if (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) {
+        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, EPI>), dim3(a.max_items * n_blocks), dim3(64 * WN * WM), lds, st, a, 0u, n_blocks, 0u);
+        return hipGetLastError();
+    }
+    for (uint32_t r = 0; r < a.n_rows; r += kTileStep) {
+        const uint32_t rows = a.n_rows - r < kTileStep ? a.n_rows - r : kTileStep, m_blocks = (rows + TM - 1u) / TM;
+        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, EPI>), dim3(n_blocks * m_blocks), dim3(64 * WN * WM), lds, st, a, r, n_blocks, m_blocks);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
 }
 
 template <int EPI>
@@ -185,14 +539,29 @@ hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k,
     return hipGetLastError();
 }
 
-uint32_t vx_i8_item_rows(uint32_t, uint32_t) { return 16u; }
+// Positions of a block of a grouped product: tiles of 128 once an expert has 32 on average (4096 rows of 8 in 256 experts, 64 of
+// them here: 2590 us by 16 -> 1171 by 128; 32 rows: 288 -> 302).
+uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count) { return slots >= 32u * count ? 128u : 16u; }
 
+// The tile kernel from 65 rows on (8192 x 8192, rows already in 8 bits: 64 rows 44 -> 42 us, 128 49 -> 43, 300 109 -> 43),
+// its 256 x 256 form where those tiles come to two rounds of the CUs (8192 rows of 8192 x 8192: 554 -> 471 us, of 8192 x 29568:
+// 1893 -> 1553; 2048 rows of 4096 x 4096, half a round: 40 -> 54).
+template <int EPI>
+hipError_t vx_i8_choose(const VxI8Args& a, hipStream_t st) {
+    if constexpr (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) {
+        if (a.item_rows == 128u) return vx_i8_tile_launch<2, 2, 2, 2, EPI>(a, st);
+    } else if (a.n_rows > 64u) {
+        if ((uint64_t)((a.w.n_tiles + 15u) / 16u) * ((a.n_rows + 255u) / 256u) >= 512u) return vx_i8_tile_launch<2, 2, 4, 4, EPI>(a, st);
+        return vx_i8_tile_launch<2, 2, 2, 2, EPI>(a, st);
+    }
+    return vx_i8_launch<EPI>(a, st);
+}
 hipError_t vx_launch_i8_product(const VxI8Args& a, int epi, hipStream_t st) {
     switch (epi) {
-        case VX_I8_STORE: return vx_i8_launch<VX_I8_STORE>(a, st);
-        case VX_I8_SWIGLU: return vx_i8_launch<VX_I8_SWIGLU>(a, st);
-        case VX_I8_HIDDEN: return vx_i8_launch<VX_I8_HIDDEN>(a, st);
-        case VX_I8_SLOT: return vx_i8_launch<VX_I8_SLOT>(a, st);
+        case VX_I8_STORE: return vx_i8_choose<VX_I8_STORE>(a, st);
+        case VX_I8_SWIGLU: return vx_i8_choose<VX_I8_SWIGLU>(a, st);
+        case VX_I8_HIDDEN: return vx_i8_choose<VX_I8_HIDDEN>(a, st);
+        case VX_I8_SLOT: return vx_i8_choose<VX_I8_SLOT>(a, st);
         default: return hipErrorInvalidValue;
     }
 }

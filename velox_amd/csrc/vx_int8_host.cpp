@@ -44,6 +44,9 @@ bool same_or_apart(const VeloxHipRows* a, const VeloxHipRows* b, uint32_t n_rows
     return a->data != b->data || (elt(a->dtype) == elt(b->dtype) && (n_rows <= 1u || a->row_stride == b->row_stride));
 }
 
+// Every row begins at a whole multiple of four elements.
+bool whole(const VeloxHipRows* r) { return aligned(r->data, 4u * elt(r->dtype)) && r->row_stride % 4u == 0; }
+
 // A workspace's regions, each from a multiple of 256 bytes on.
 struct Space {
     uint8_t* base;
@@ -166,6 +169,7 @@ int velox_hip_int8_product(const VeloxHipInt8Matrix* m, const VeloxHipRows* x, c
     a.bias = d_bias;
     if (residual) a.res = view(residual);
     a.out = view(out);
+    a.vec = whole(out) && (!residual || whole(residual));
     return (int)vx_launch_i8_product(a, m->paired ? VX_I8_SWIGLU : VX_I8_STORE, st);
 }
 
@@ -257,6 +261,7 @@ int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Ma
     a.g = VxGrouped{f.order, f.offsets, f.items, f.n_items};
     a.top = top_k;
     a.max_items = max_items(slots, gu.count, g.item_rows);
+    a.item_rows = g.item_rows;
     a.part = f.hidden;
     a.part_stride = f.hidden_stride;
     if (e == hipSuccess) e = vx_launch_i8_product(a, VX_I8_HIDDEN, st);
