@@ -1,19 +1,7 @@
 // vx_experts.hip -- the choice of experts, the grouping of rows by expert, the sum of the experts' answers.
-#include "vx_int8.h"
+#include "vx_int8_dev.h"
 
 namespace {
-
-__device__ __forceinline__ float vx_load(const void* p, size_t i, uint32_t dtype) {
-    if (dtype == VELOX_DT_F32) return ((const float*)p)[i];
-    if (dtype == VELOX_DT_F16) return (float)((const _Float16*)p)[i];
-    return (float)((const __bf16*)p)[i];
-}
-// The fp32 value rounded once (to nearest even) to the element type.
-__device__ __forceinline__ void vx_store(void* p, size_t i, uint32_t dtype, float v) {
-    if (dtype == VELOX_DT_F32) ((float*)p)[i] = v;
-    else if (dtype == VELOX_DT_F16) ((_Float16*)p)[i] = (_Float16)v;
-    else ((__bf16*)p)[i] = (__bf16)v;
-}
 
 // ---- routing ----
 constexpr uint32_t kRouteItems = kVxI8MaxCount / 64u;  // experts of a lane at most
@@ -138,156 +126,199 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
 }
 
 // ---- grouping: a stable counting sort of the slots by expert ----
-constexpr uint32_t kGroupWaves = 4, kGroupRun = 512, kGroupSlots = kGroupWaves * kGroupRun;  // a wave's, a workgroup's slots
+// A workgroup takes kGroupSlots slots, a wave kGroupRun neighbours of them. Slots of one expert within a wave find each other by
+// ballots of their keys' bits, so that ranks follow the slots' order; waves' and workgroups' counts are summed in order.
+// Several workgroups count first (their counts through memory), then place; one does both at once.
+constexpr uint32_t kGroupWaves = 4, kGroupRun = 256, kGroupSlots = kGroupWaves * kGroupRun, kGroupSteps = kGroupRun / 64u;
+constexpr uint32_t kGroupThreads = 64u * kGroupWaves;
 
-// The expert of slot i of a run (count: none of ours).
-__device__ __forceinline__ uint32_t vx_key(const VxGroupArgs& a, uint32_t i) {
-    if (i >= a.n_slots) return a.count;
-    const uint32_t e = a.ids[i] - a.first;
-    return e < a.count ? e : a.count;
+// A wave's keys: slot run + 64 i + lane's expert, or a.count (none of ours).
+struct VxKeys {
+    uint32_t key[kGroupSteps];
+    uint32_t steps;  // those with slots
+};
+__device__ __forceinline__ VxKeys vx_keys(const VxGroupArgs& a, uint32_t run) {
+    const uint32_t lane = threadIdx.x & 63u;
+    VxKeys k;
+    k.steps = run < a.n_slots ? (a.n_slots - run + 63u) / 64u : 0u;
+    k.steps = k.steps < kGroupSteps ? k.steps : kGroupSteps;
+#pragma unroll
+    for (uint32_t i = 0; i < kGroupSteps; ++i) {
+        const uint32_t slot = run + 64u * i + lane, e = slot < a.n_slots ? a.ids[slot] - a.first : a.count;
+        k.key[i] = e < a.count ? e : a.count;
+    }
+    return k;
 }
 // The lanes of the wave whose key is this lane's.
-__device__ __forceinline__ uint64_t vx_peers(uint32_t key) {
+__device__ __forceinline__ uint64_t vx_peers(uint32_t key, uint32_t bits) {
     uint64_t m = ~0ull;
-#pragma unroll
-    for (int b = 0; b < 11; ++b) {
-        const uint64_t v = __ballot(key >> b & 1u);
-        m &= key >> b & 1u ? v : ~v;
+    for (uint32_t b = 0; b < bits; ++b) {
+        const bool mine = key >> b & 1u;
+        const uint64_t v = __ballot(mine);
+        m &= mine ? v : ~v;
     }
     return m;
 }
-// What a lane of the wave wrote to LDS is what the others read behind this.
-__device__ __forceinline__ void vx_wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
 // How many slots of each expert every wave's run holds: tally[wave][count + 1].
-__device__ __forceinline__ void vx_tally(const VxGroupArgs& a, uint32_t block, uint32_t* tally) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n = a.count + 1u;
-    for (uint32_t i = threadIdx.x; i < kGroupWaves * n; i += 64u * kGroupWaves) tally[i] = 0;
-    __syncthreads();
-    const uint32_t run = block * kGroupSlots + wave * kGroupRun;
-    for (uint32_t i = 0; i < kGroupRun; i += 64u) {
-        const uint32_t key = vx_key(a, run + i + lane);
-        const uint64_t peers = vx_peers(key);
-        if (lane == (uint32_t)__builtin_ctzll(peers)) tally[wave * n + key] += (uint32_t)__popcll(peers);
+__device__ __forceinline__ void vx_tally(const VxGroupArgs& a, const VxKeys& k, uint32_t* tally) {
+    const uint32_t lane = threadIdx.x & 63u, n = a.count + 1u;
+    uint32_t* mine = tally + (threadIdx.x >> 6) * n;
+    for (uint32_t i = lane; i < n; i += 64u) mine[i] = 0;
+    vx_wave_sync();
+#pragma unroll
+    for (uint32_t i = 0; i < kGroupSteps; ++i) {
+        if (i >= k.steps) break;
+        const uint64_t peers = vx_peers(k.key[i], a.key_bits);
+        if (lane == (uint32_t)__builtin_ctzll(peers)) mine[k.key[i]] += (uint32_t)__popcll(peers);
         vx_wave_sync();
     }
     __syncthreads();
 }
-__global__ __launch_bounds__(64 * kGroupWaves) void vx_group_count_kernel(VxGroupArgs a) {
+__global__ __launch_bounds__(kGroupThreads) void vx_group_count_kernel(VxGroupArgs a) {
     __shared__ uint32_t tally[kGroupWaves * (kVxI8MaxCount + 1u)];
-    vx_tally(a, blockIdx.x, tally);
-    for (uint32_t e = threadIdx.x; e < a.count; e += 64u * kGroupWaves) {
+    vx_tally(a, vx_keys(a, blockIdx.x * kGroupSlots + (threadIdx.x >> 6) * kGroupRun), tally);
+    for (uint32_t e = threadIdx.x; e < a.count; e += kGroupThreads) {
         uint32_t n = 0;
+#pragma unroll
         for (uint32_t w = 0; w < kGroupWaves; ++w) n += tally[w * (a.count + 1u) + e];
         a.hist[(size_t)blockIdx.x * a.count + e] = n;
     }
 }
-// Exclusive sums of v over the workgroup's threads, the total in `total`; room: kGroupWaves words.
-__device__ __forceinline__ uint32_t vx_scan(uint32_t v, uint32_t* room, uint32_t& total) {
+// Exclusive sums of u and v (the latter below 2^32) over the workgroup's threads, and the totals; room: 2 kGroupWaves words.
+__device__ __forceinline__ uint2 vx_scan(uint2 v, uint32_t* room, uint2& total) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint32_t s = v;
+    uint2 s = v;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t o = __shfl_up(s, off);
-        if (lane >= (uint32_t)off) s += o;
+        const uint32_t x = __shfl_up(s.x, off), y = __shfl_up(s.y, off);
+        if (lane >= (uint32_t)off) {
+            s.x += x;
+            s.y += y;
+        }
     }
-    if (lane == 63u) room[wave] = s;
+    if (lane == 63u) {
+        room[2u * wave] = s.x;
+        room[2u * wave + 1u] = s.y;
+    }
     __syncthreads();
-    uint32_t before = 0;
-    total = 0;
+    uint2 before = make_uint2(0, 0);
+    total = before;
+#pragma unroll
     for (uint32_t w = 0; w < kGroupWaves; ++w) {
-        if (w < wave) before += room[w];
-        total += room[w];
+        if (w < wave) before = make_uint2(before.x + room[2u * w], before.y + room[2u * w + 1u]);
+        total = make_uint2(total.x + room[2u * w], total.y + room[2u * w + 1u]);
     }
-    __syncthreads();
-    return before + s - v;
+    return make_uint2(before.x + s.x - v.x, before.y + s.y - v.y);
 }
-__global__ __launch_bounds__(64 * kGroupWaves) void vx_group_place_kernel(VxGroupArgs a) {
+// PER: experts of a thread, neighbours.
+template <uint32_t PER>
+__global__ __launch_bounds__(kGroupThreads) void vx_group_place_kernel(VxGroupArgs a) {
     __shared__ uint32_t tally[kGroupWaves * (kVxI8MaxCount + 1u)];
-    __shared__ uint32_t room[kGroupWaves];
-    constexpr uint32_t T = 64u * kGroupWaves, PER = kVxI8MaxCount / T;
+    __shared__ uint32_t room[2u * kGroupWaves];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n = a.count + 1u, block = blockIdx.x, blocks = gridDim.x;
-    vx_tally(a, block, tally);
-    // thread t: experts PER t .. + PER - 1
-    uint32_t mine[PER], front[PER], sum = 0;
+    const uint32_t run = block * kGroupSlots + wave * kGroupRun;
+    const VxKeys k = vx_keys(a, run);
+    uint32_t mine[PER], front[PER];
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
         const uint32_t e = threadIdx.x * PER + j;
         mine[j] = front[j] = 0;
-        if (e < a.count) {
-            if (blocks == 1u) {
-                for (uint32_t w = 0; w < kGroupWaves; ++w) mine[j] += tally[w * n + e];
-            } else {
-                for (uint32_t b = 0; b < blocks; ++b) {
-                    const uint32_t c = a.hist[(size_t)b * a.count + e];
-                    if (b < block) front[j] += c;
-                    mine[j] += c;
-                }
+        if (blocks > 1u && e < a.count) {
+#pragma unroll 16
+            for (uint32_t b = 0; b < blocks; ++b) {
+                const uint32_t c = a.hist[(size_t)b * a.count + e];
+                front[j] += b < block ? c : 0u;
+                mine[j] += c;
             }
         }
-        sum += mine[j];
     }
-    uint32_t total;
-    uint32_t at = vx_scan(sum, room, total);
-    uint32_t items = 0;
+    vx_tally(a, k, tally);
+    uint2 sum = make_uint2(0, 0);  // slots and blocks of a grouped product
 #pragma unroll
-    for (uint32_t j = 0; j < PER; ++j) items += (mine[j] + a.item_rows - 1u) / a.item_rows;
-    uint32_t n_items;
-    uint32_t item = vx_scan(items, room, n_items);
+    for (uint32_t j = 0; j < PER; ++j) {
+        const uint32_t e = threadIdx.x * PER + j;
+        if (blocks == 1u && e < a.count) {
+#pragma unroll
+            for (uint32_t w = 0; w < kGroupWaves; ++w) mine[j] += tally[w * n + e];
+        }
+        sum.x += mine[j];
+        sum.y += (mine[j] + a.item_rows - 1u) / a.item_rows;
+    }
+    uint2 total, at = vx_scan(sum, room, total);
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
         const uint32_t e = threadIdx.x * PER + j;
         if (e < a.count) {
             if (block == 0) {
-                a.offsets[e] = at;
+                a.offsets[e] = at.x;
                 if (a.items)
-                    for (uint32_t p = 0; p < mine[j]; p += a.item_rows) a.items[item++] = make_uint2(e, at + p);
+                    for (uint32_t p = 0; p < mine[j]; p += a.item_rows) a.items[at.y++] = make_uint2(e, at.x + p);
             }
-            // each wave's first place of the expert
-            uint32_t place = at + front[j];
+            uint32_t place = at.x + front[j];  // each wave's first place of the expert
+#pragma unroll
             for (uint32_t w = 0; w < kGroupWaves; ++w) {
                 const uint32_t c = tally[w * n + e];
                 tally[w * n + e] = place;
                 place += c;
             }
         }
-        at += mine[j];
+        at.x += mine[j];
     }
     if (block == 0 && threadIdx.x == 0) {
-        a.offsets[a.count] = total;
-        if (a.items) *a.n_items = n_items;
+        a.offsets[a.count] = total.x;
+        if (a.items) *a.n_items = total.y;
     }
     __syncthreads();
-    const uint32_t run = block * kGroupSlots + wave * kGroupRun;
-    for (uint32_t i = 0; i < kGroupRun; i += 64u) {
-        const uint32_t slot = run + i + lane, key = vx_key(a, slot);
-        const uint64_t peers = vx_peers(key);
-        const uint32_t rank = (uint32_t)__popcll(peers & ((1ull << lane) - 1ull));
+    uint32_t* places = tally + wave * n;
+#pragma unroll
+    for (uint32_t i = 0; i < kGroupSteps; ++i) {
+        if (i >= k.steps) break;
+        const uint32_t key = k.key[i];
+        const uint64_t peers = vx_peers(key, a.key_bits);
+        const uint32_t rank = (uint32_t)__popcll(peers & ((1ull << lane) - 1ull)), place = places[key];
+        vx_wave_sync();
         if (key < a.count) {
-            const uint32_t place = tally[wave * n + key];
-            a.order[place + rank] = slot;
-            vx_wave_sync();
-            if (rank == 0) tally[wave * n + key] = place + (uint32_t)__popcll(peers);
+            a.order[place + rank] = run + 64u * i + lane;
+            if (rank == 0) places[key] = place + (uint32_t)__popcll(peers);
         }
         vx_wave_sync();
     }
-    for (uint32_t p = total + block * T + threadIdx.x; p < a.n_slots; p += blocks * T) a.order[p] = kVxNoExpert;
+    for (uint32_t p = total.x + block * kGroupThreads + threadIdx.x; p < a.n_slots; p += blocks * kGroupThreads) a.order[p] = kVxNoExpert;
 }
 
 // ---- the sum of a row's experts ----
-__global__ __launch_bounds__(256) void vx_combine_kernel(VxCombineArgs a) {
-    const uint32_t r = blockIdx.x;
-    for (uint32_t c = threadIdx.x; c < a.n; c += 256u) {
-        float y = a.res.data ? vx_load(a.res.data, (size_t)r * a.res.rs + c, a.res.dtype) : 0.0f;
-        float sum = 0.0f;
-        for (uint32_t j = 0; j < a.top; ++j) {
-            const size_t slot = (size_t)r * a.top + j;
-            if (a.ids[slot] - a.first < a.count) sum = __builtin_fmaf(a.weights[slot], a.part[slot * a.part_stride + c], sum);
+// A workgroup takes 1024 outputs of a row, a thread four. Lane j of a wave looks at the row's slot j; the slots of our
+// experts are then added in order, four of their answers on the way at a time.
+constexpr uint32_t kCombineCols = 1024u;
+template <bool VEC>
+__global__ __launch_bounds__(256) void vx_combine_kernel(VxCombineArgs a, uint32_t blocks) {
+    const uint32_t r = blockIdx.x / blocks, c = blockIdx.x % blocks * kCombineCols + 4u * threadIdx.x, lane = threadIdx.x & 63u;
+    const size_t slot0 = (size_t)r * a.top;
+    const bool mine = lane < a.top && a.ids[slot0 + lane] - a.first < a.count;
+    const float w = mine ? a.weights[slot0 + lane] : 0.0f;
+    uint64_t left = __ballot(mine);
+    if (c >= a.n) return;
+    float4 res = make_float4(0, 0, 0, 0);
+    if (a.res.data) res = vx_load4<VEC>(a.res.data, (size_t)r * a.res.rs + c, a.res.dtype, a.n - c);
+    const float* part = a.part + slot0 * a.part_stride + c;
+    float4 sum = make_float4(0, 0, 0, 0);
+    while (left) {
+        float4 v[4];
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t at = left ? (uint32_t)__builtin_ctzll(left) : 0u;
+            f[j] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), (int)at));
+            v[j] = make_float4(0, 0, 0, 0);
+            if (left) v[j] = *(const float4*)(part + at * a.part_stride);
+            else f[j] = 0.0f;
+            left &= left - 1u;
         }
-        vx_store(a.out.data, (size_t)r * a.out.rs + c, a.out.dtype, y + sum);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            sum = make_float4(__builtin_fmaf(f[j], v[j].x, sum.x), __builtin_fmaf(f[j], v[j].y, sum.y), __builtin_fmaf(f[j], v[j].z, sum.z), __builtin_fmaf(f[j], v[j].w, sum.w));
     }
+    vx_store4<VEC>(a.out.data, (size_t)r * a.out.rs + c, a.out.dtype, a.n - c, make_float4(res.x + sum.x, res.y + sum.y, res.z + sum.z, res.w + sum.w));
 }
 
 }  // namespace
@@ -302,18 +333,23 @@ hipError_t vx_launch_route(const VxRouteArgs& a, hipStream_t st) {
 
 uint32_t vx_group_blocks(uint32_t n_slots) { return n_slots ? (n_slots + kGroupSlots - 1u) / kGroupSlots : 1u; }
 
-hipError_t vx_launch_group(const VxGroupArgs& a, hipStream_t st) {
+hipError_t vx_launch_group(const VxGroupArgs& args, hipStream_t st) {
+    VxGroupArgs a = args;
+    a.key_bits = 32u - (uint32_t)__builtin_clz(a.count);  // keys 0 .. count
     const uint32_t blocks = vx_group_blocks(a.n_slots);
     if (blocks > 1u) {
-        hipLaunchKernelGGL(vx_group_count_kernel, dim3(blocks), dim3(64 * kGroupWaves), 0, st, a);
+        hipLaunchKernelGGL(vx_group_count_kernel, dim3(blocks), dim3(kGroupThreads), 0, st, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(vx_group_place_kernel, dim3(blocks), dim3(64 * kGroupWaves), 0, st, a);
+    if (a.count <= kGroupThreads) hipLaunchKernelGGL((vx_group_place_kernel<1>), dim3(blocks), dim3(kGroupThreads), 0, st, a);
+    else hipLaunchKernelGGL((vx_group_place_kernel<kVxI8MaxCount / kGroupThreads>), dim3(blocks), dim3(kGroupThreads), 0, st, a);
     return hipGetLastError();
 }
 
 hipError_t vx_launch_combine(const VxCombineArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(vx_combine_kernel, dim3(a.n_rows), dim3(256), 0, st, a);
+    const uint32_t blocks = (a.n + kCombineCols - 1u) / kCombineCols;
+    if (a.vec) hipLaunchKernelGGL((vx_combine_kernel<true>), dim3(a.n_rows * blocks), dim3(256), 0, st, a, blocks);
+    else hipLaunchKernelGGL((vx_combine_kernel<false>), dim3(a.n_rows * blocks), dim3(256), 0, st, a, blocks);
     return hipGetLastError();
 }

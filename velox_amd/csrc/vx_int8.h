@@ -73,6 +73,7 @@ struct VxGroupArgs {
     uint2* items;              // NULL: none
     uint32_t* n_items;
     uint32_t item_rows;
+    uint32_t key_bits;         // set by the launcher
 };
 
 struct VxCombineArgs {
@@ -80,8 +81,9 @@ struct VxCombineArgs {
     const float* weights;
     uint32_t n_rows, top, first, count, n;
     const float* part;         // [slot][part_stride]
-    uint64_t part_stride;
+    uint64_t part_stride;      // a multiple of 4
     VxI8View res, out;
+    uint32_t vec;              // 1: res and out rows begin at whole multiples of four elements
 };
 
 hipError_t vx_launch_i8_pack(const VxI8Mat& m, uint32_t first, uint32_t number, const int8_t* codes, uint64_t ms, uint64_t rs,

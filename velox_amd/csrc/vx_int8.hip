@@ -1,5 +1,5 @@
 // vx_int8.hip -- products of 8-bit integers with a scale for each token and channel.
-#include "vx_int8.h"
+#include "vx_int8_dev.h"
 
 namespace {
 
@@ -16,58 +16,6 @@ __device__ __forceinline__ void vx_each(F f) {  // f(vx_int<0>) .. f(vx_int<N - 
     }
 }
 
-__device__ __forceinline__ float vx_load(const void* p, size_t i, uint32_t dtype) {
-    if (dtype == VELOX_DT_F32) return ((const float*)p)[i];
-    if (dtype == VELOX_DT_F16) return (float)((const _Float16*)p)[i];
-    return (float)((const __bf16*)p)[i];
-}
-// The fp32 value rounded once (to nearest even) to the element type.
-__device__ __forceinline__ void vx_store(void* p, size_t i, uint32_t dtype, float v) {
-    if (dtype == VELOX_DT_F32) ((float*)p)[i] = v;
-    else if (dtype == VELOX_DT_F16) ((_Float16*)p)[i] = (_Float16)v;
-    else ((__bf16*)p)[i] = (__bf16)v;
-}
-
-// Four neighbouring values of a row at element i as fp32, and back (rounded once); VEC: at whole 16- or 8-byte places.
-template <bool VEC>
-__device__ __forceinline__ float4 vx_load4(const void* p, size_t i, uint32_t dtype, uint32_t left) {
-    float4 v = make_float4(0, 0, 0, 0);
-    if (VEC && left >= 4u) {
-        if (dtype == VELOX_DT_F32) return *(const float4*)((const float*)p + i);
-        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-        const uint2 w = *(const uint2*)((const uint16_t*)p + i);
-        if (dtype == VELOX_DT_F16) {
-            const h4 h = __builtin_bit_cast(h4, w);
-            return make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
-        }
-        const b4 b = __builtin_bit_cast(b4, w);
-        return make_float4((float)b[0], (float)b[1], (float)b[2], (float)b[3]);
-    }
-    if (left > 0u) v.x = vx_load(p, i, dtype);
-    if (left > 1u) v.y = vx_load(p, i + 1u, dtype);
-    if (left > 2u) v.z = vx_load(p, i + 2u, dtype);
-    if (left > 3u) v.w = vx_load(p, i + 3u, dtype);
-    return v;
-}
-template <bool VEC>
-__device__ __forceinline__ void vx_store4(void* p, size_t i, uint32_t dtype, uint32_t left, float4 v) {
-    if (VEC && left >= 4u) {
-        if (dtype == VELOX_DT_F32) {
-            *(float4*)((float*)p + i) = v;
-            return;
-        }
-        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-        if (dtype == VELOX_DT_F16) *(h4*)((uint16_t*)p + i) = h4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
-        else *(b4*)((uint16_t*)p + i) = b4{(__bf16)v.x, (__bf16)v.y, (__bf16)v.z, (__bf16)v.w};
-        return;
-    }
-    if (left > 0u) vx_store(p, i, dtype, v.x);
-    if (left > 1u) vx_store(p, i + 1u, dtype, v.y);
-    if (left > 2u) vx_store(p, i + 2u, dtype, v.z);
-    if (left > 3u) vx_store(p, i + 3u, dtype, v.w);
-}
 // Outputs n .. n + 3 of row r (of `cols` in a row), y their products with the bias: the residual added, stored.
 template <bool VEC>
 __device__ __forceinline__ void vx_finish(const VxI8Args& a, size_t r, uint32_t n, uint32_t cols, float4 y) {
@@ -121,93 +69,255 @@ __device__ __forceinline__ int vx_code(float x, float s, float inv) {
     return (int)r;
 }
 
-__global__ __launch_bounds__(256) void vx_i8_quantize_kernel(VxI8View x, uint32_t k, VxI8Rows o, const uint32_t* limit) {
-    __shared__ float red[4];
-    const uint32_t r = blockIdx.x, tid = threadIdx.x, kp = vx_i8_pad(k);
-    if (limit && r >= *limit) return;
-    const size_t base = (size_t)r * x.rs;
-    float top = 0.0f;
-    bool bad = false;
-    for (uint32_t i = tid; i < k; i += 256u) {
-        const float v = fabsf(vx_load(x.data, base + i, x.dtype));
-        bad |= !(v < INFINITY);
-        top = fmaxf(top, v);
-    }
-    if (bad) top = INFINITY;
+// Codes of four values, in the bytes of a word. Where no x * inv is near a half (its error is below 2^-15) rint gives the
+// nearest whole number; else the exact rule above decides.
+__device__ __forceinline__ uint32_t vx_codes(const float* x, float s, float inv) {
+    uint32_t w = 0;
+    float off = 0.0f;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+    for (int i = 0; i < 4; ++i) {
+        const float r = rintf(x[i] * inv);
+        off = fmaxf(off, fabsf(__builtin_fmaf(x[i], inv, -r)));
+        w = __builtin_amdgcn_cvt_pk_u8_f32(r + 128.0f, i, w);
+    }
+    w ^= 0x80808080u;
+    if (off > 0.4999f) {
+        w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= ((uint32_t)vx_code(x[i], s, inv) & 0xFFu) << (8 * i);
+    }
+    return w;
+}
+// A row's scale from the bits of its largest absolute value (those of an infinity or NaN are above any number's).
+struct VxRowScale {
+    float s, inv;
+    bool none;  // codes are 0
+};
+__device__ __forceinline__ VxRowScale vx_row_scale(uint32_t top) {
+    if (top >= 0x7F800000u) return {NAN, 0.0f, true};
+    const float s = __builtin_bit_cast(float, top) / 127.0f;
+    if (s < 1.17549435e-38f) return {0.0f, 0.0f, true};
+    return {s, 1.0f / s, false};
+}
+__device__ __forceinline__ uint32_t vx_size_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
+__device__ __forceinline__ uint32_t vx_max(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// TPR threads take a row, which stays in registers between the search for its largest value and the rounding: NV vectors of
+// 16 bytes each. Bound by the bytes (8192 rows of 29568 bf16: 726 MB).
+template <class T, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void vx_i8_quantize_kernel(VxI8View x, uint32_t n_rows, uint32_t k, VxI8Rows o, const uint32_t* limit) {
+    constexpr int V = 16 / sizeof(T), WG = TPR < 256 ? 256 : TPR, WAVES = TPR / 64;
+    __shared__ uint32_t red[WG / 64];
+    const uint32_t tid = threadIdx.x, t = tid % TPR, r = blockIdx.x * (WG / TPR) + tid / TPR, kp = vx_i8_pad(k);
+    if (limit) n_rows = *limit < n_rows ? *limit : n_rows;
+    if (TPR > 64 ? r >= n_rows : __builtin_amdgcn_readfirstlane((int)r) >= (int)n_rows) return;  // (a wave, or the whole workgroup)
+    struct alignas(16) Vec {
+        T v[V];
+    };
+    const T* from = (const T*)x.data + (size_t)r * x.rs;
+    Vec in[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const uint32_t c = (j * TPR + t) * V;
+        if (c + V <= k) {
+            in[j] = *(const Vec*)(from + c);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) in[j].v[i] = c + i < k ? from[c + i] : (T)0.0f;
+        }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) top = vx_max(top, vx_size_bits((float)in[j].v[i]));
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) top = vx_max(top, (uint32_t)__shfl_xor((int)top, off));
+    if constexpr (TPR > 64) {
+        if ((tid & 63u) == 0) red[tid >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) top = vx_max(top, red[w]);
+    }
+    const VxRowScale q = vx_row_scale(top);
+    int8_t* to = o.codes + (size_t)r * o.rs;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const uint32_t c = (j * TPR + t) * V;
+        if (c >= kp) continue;
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const float f[4] = {(float)in[j].v[4 * i], (float)in[j].v[4 * i + 1], (float)in[j].v[4 * i + 2], (float)in[j].v[4 * i + 3]};
+            w[i] = q.none ? 0u : vx_codes(f, q.s, q.inv);
+        }
+        if constexpr (V == 8) *(uint2*)(to + c) = make_uint2(w[0], w[1]);
+        else *(uint32_t*)(to + c) = w[0];
+    }
+    if (t == 0) o.scales[r] = q.s;
+}
+
+// Rows at other places, or longer than the registers of a workgroup: read twice, value by value.
+__global__ __launch_bounds__(256) void vx_i8_quantize_any_kernel(VxI8View x, uint32_t k, VxI8Rows o) {
+    __shared__ uint32_t red[4];
+    const uint32_t r = blockIdx.x, tid = threadIdx.x, kp = vx_i8_pad(k);
+    const size_t base = (size_t)r * x.rs;
+    uint32_t top = 0;
+    for (uint32_t i = tid; i < k; i += 256u) top = vx_max(top, vx_size_bits(vx_load(x.data, base + i, x.dtype)));
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) top = vx_max(top, (uint32_t)__shfl_xor((int)top, off));
     if ((tid & 63u) == 0) red[tid >> 6] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float s = top / 127.0f;
-    const bool nan = top == INFINITY, none = s < 1.17549435e-38f;
-    const float inv = 1.0f / s;
+    top = vx_max(vx_max(red[0], red[1]), vx_max(red[2], red[3]));
+    const VxRowScale q = vx_row_scale(top);
     int8_t* to = o.codes + (size_t)r * o.rs;
-    for (uint32_t i = tid; i < kp; i += 256u)
-        to[i] = i < k && !nan && !none ? (int8_t)vx_code(vx_load(x.data, base + i, x.dtype), s, inv) : (int8_t)0;
-    if (tid == 0) o.scales[r] = nan ? NAN : none ? 0.0f : s;
+    for (uint32_t i = tid; i < kp; i += 256u) to[i] = i < k && !q.none ? (int8_t)vx_code(vx_load(x.data, base + i, x.dtype), q.s, q.inv) : (int8_t)0;
+    if (tid == 0) o.scales[r] = q.s;
+}
+
+template <class T>
+hipError_t vx_quantize_launch(const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& o, const uint32_t* limit, hipStream_t st) {
+    constexpr uint32_t V = 16 / sizeof(T);
+    const uint32_t vecs = vx_i8_pad(k) / V;  // (the codes behind k are written too)
+#define VX_QUANTIZE(TPR, NV)                                                                                                              \
+    if (vecs <= TPR * NV) {                                                                                                               \
+        constexpr uint32_t wg = TPR < 256 ? 256 : TPR;                                                                                    \
+        hipLaunchKernelGGL((vx_i8_quantize_kernel<T, TPR, NV>), dim3((n_rows + wg / TPR - 1) / (wg / TPR)), dim3(wg), 0, st, x, n_rows, k, o, limit); \
+        return hipGetLastError();                                                                                                         \
+    }
+    VX_QUANTIZE(64, 1)
+    VX_QUANTIZE(64, 2)
+    VX_QUANTIZE(256, 1)
+    VX_QUANTIZE(256, 2)
+    VX_QUANTIZE(256, 4)
+    VX_QUANTIZE(256, 8)
+    VX_QUANTIZE(1024, 4)
+    VX_QUANTIZE(1024, 8)
+    VX_QUANTIZE(1024, 16)
+#undef VX_QUANTIZE
+    return hipErrorInvalidValue;
 }
 
 // ---- products ----
-// One wave: 16 activation rows by two weight tiles (paired: a gate tile and its up tile). The weights are the A operand, so
-// that a lane ends with four neighbouring outputs of one row: D[n = 4 (lane / 16) + i][row = lane % 16].
-template <int EPI>
-__global__ __launch_bounds__(256) void vx_i8_kernel(VxI8Args a, uint32_t row0, uint32_t n_blocks) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t nb = blockIdx.x % n_blocks, item = blockIdx.x / n_blocks;
-    const uint32_t t0 = 2u * (nb * 4u + wave);
-    constexpr bool kGrouped = EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT;
-    uint32_t e = 0, first = row0 + item * 16u, end = a.n_rows;
+// ---- products of few rows: the weights' bytes ----
+// A workgroup of NW waves takes NT weight tiles (paired: gate and up tiles by turns) by 16 MT rows. Its waves deal out the 64-column
+// tiles in turn, so that the weights stream in order, each lane's 16 bytes being its MFMA operand; U tiles are requested
+// while U are multiplied, those behind the last by bounds-checked loads that give zeros. The waves' sums meet in LDS. The
+// weights are the A operand, so that a lane ends with four neighbouring outputs: D[n = 4 (lane / 16) + i][row = lane % 16].
+template <int NT, int MT, int NW, int EPI>
+__global__ __launch_bounds__(64 * NW) void vx_i8_stream_kernel(VxI8Args a, uint32_t n_blocks) {
+    constexpr bool kGrouped = EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT, kSwiglu = EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN;
+    constexpr int U = NT + MT <= 3 ? 4 : 2;
+    __shared__ v4i sums[NW][NT * MT][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+    const uint32_t item = uniform(blockIdx.x / n_blocks), t0 = uniform(blockIdx.x % n_blocks) * NT;
+    uint32_t e = 0, first = item * 16u * MT, end = a.n_rows;
     if constexpr (kGrouped) {
-        if (item >= *a.g.n_items) return;
+        if (item >= uniform(*a.g.n_items)) return;
         const uint2 it = a.g.items[item];
-        e = it.x;
-        first = it.y;
-        end = a.g.offsets[e + 1u];
+        e = uniform(it.x);
+        first = uniform(it.y);
+        end = uniform(a.g.offsets[e + 1u]);
     }
-    if (t0 >= a.w.n_tiles) return;
-    const uint32_t p = first + (lane & 15u);
-    const bool live = p < end;
-    uint32_t slot = p, row = live ? p : first;
-    if constexpr (kGrouped) {
-        slot = a.g.order[live ? p : first];
-        if constexpr (EPI == VX_I8_HIDDEN) row = slot / a.top;
+    const int8_t* x[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const uint32_t p = first + 16u * m + (lane & 15u);
+        uint32_t row = p < end ? p : end - 1u;
+        if constexpr (EPI == VX_I8_HIDDEN) row = a.g.order[row] / a.top;
+        x[m] = a.a.codes + (size_t)row * a.a.rs + 16u * (lane >> 4);
     }
-    const int8_t* x = a.a.codes + (size_t)row * a.a.rs + 16u * (lane >> 4);
-    const bool two = t0 + 1u < a.w.n_tiles;
-    const uint4* w0 = a.w.codes + ((uint64_t)e * a.w.n_tiles + t0) * a.w.k_tiles * 64u + lane;
-    const uint4* w1 = two ? w0 + (uint64_t)a.w.k_tiles * 64u : w0;
-    v4i acc0 = {0, 0, 0, 0}, acc1 = {0, 0, 0, 0};
-    for (uint32_t kt = 0; kt < a.w.k_tiles; ++kt) {
-        const v4i b = *(const v4i*)(x + 64u * kt);
-        acc0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, w0[64u * kt]), b, acc0, 0, 0, 0);
-        acc1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, w1[64u * kt]), b, acc1, 0, 0, 0);
-    }
-    if (!live) return;
-    const float s = a.a.scales[row];
-    const float* ws = a.w.scales + ((uint64_t)e * a.w.n_tiles + t0) * 16u + 4u * (lane >> 4);
-    const auto scaled = [&](const v4i& acc, const float* w) {
-        return make_float4((float)acc[0] * w[0] * s, (float)acc[1] * w[1] * s, (float)acc[2] * w[2] * s, (float)acc[3] * w[3] * s);
+    const uint32_t run = a.w.k_tiles * 1024u;  // bytes of a tile row
+    const uint8_t* w = (const uint8_t*)a.w.codes + ((uint64_t)e * a.w.n_tiles + t0) * run;
+    const uint32_t tiles = a.w.n_tiles - t0 < (uint32_t)NT ? a.w.n_tiles - t0 : (uint32_t)NT;
+    __amdgpu_buffer_rsrc_t rs[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) rs[n] = __builtin_amdgcn_make_buffer_rsrc((void*)(w + (uint64_t)n * run), 0, n < (int)tiles ? (int)run : 0, 0x00020000);
+    struct Set {
+        v4i w[U][NT], x[U][MT];
     };
-    const auto put = [&](uint32_t n, uint32_t cols, float4 y) {
-        if (n >= cols) return;
+    const auto load = [&](Set& s, uint32_t kt) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t k = kt + u * NW, kx = k < a.w.k_tiles ? k : a.w.k_tiles - 1u;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s.w[u][n] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rs[n], (int)(k * 1024u + lane * 16u), 0, 2));
+#pragma unroll
+            for (int m = 0; m < MT; ++m) s.x[u][m] = *(const v4i*)(x[m] + 64u * kx);
+        }
+    };
+    v4i acc[NT][MT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[n][m] = v4i{0, 0, 0, 0};
+    const auto multiply = [&](const Set& s) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[n][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.w[u][n], s.x[u][m], acc[n][m], 0, 0, 0);
+    };
+    Set s0, s1;
+    load(s0, wave);
+    for (uint32_t kt = wave; kt < a.w.k_tiles; kt += 2u * U * NW) {
+        load(s1, kt + U * NW);
+        multiply(s0);
+        load(s0, kt + 2u * U * NW);
+        multiply(s1);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) sums[wave][n * MT + m][lane] = acc[n][m];
+    __syncthreads();
+    // output tiles (paired: of two weight tiles each) by the waves in turn
+    constexpr int OUT = (kSwiglu ? NT / 2 : NT) * MT;
+    const uint32_t cols = kSwiglu ? a.w.n / 2u : a.w.n;
+#pragma unroll 1
+    for (int o = wave; o < OUT; o += NW) {
+        const int n = o / MT, m = o % MT;
+        const uint32_t p = first + 16u * m + (lane & 15u), c = 16u * (t0 / (kSwiglu ? 2u : 1u) + n) + 4u * (lane >> 4);
+        const auto total = [&](int at) {
+            v4i v = sums[0][at][lane];
+#pragma unroll
+            for (int j = 1; j < NW; ++j) v += sums[j][at][lane];
+            return v;
+        };
+        if (p >= end || c >= cols) continue;
+        uint32_t row = p, slot = p;
+        if constexpr (kGrouped) slot = a.g.order[p];
+        if constexpr (EPI == VX_I8_HIDDEN) row = slot / a.top;
+        const float s = a.a.scales[row];
+        const float* ws = a.w.scales + ((uint64_t)e * a.w.n_tiles + t0 + (kSwiglu ? 2 * n : n)) * 16u + 4u * (lane >> 4);
+        const auto scaled = [&](const v4i& v, const float4 f) {
+            return make_float4((float)v[0] * f.x * s, (float)v[1] * f.y * s, (float)v[2] * f.z * s, (float)v[3] * f.w * s);
+        };
+        float4 y = scaled(total((kSwiglu ? 2 * n : n) * MT + m), *(const float4*)ws);
+        if constexpr (kSwiglu) {
+            const float4 u = scaled(total((2 * n + 1) * MT + m), *(const float4*)(ws + 16));
+            y = make_float4(vx_swiglu(y.x, u.x), vx_swiglu(y.y, u.y), vx_swiglu(y.z, u.z), vx_swiglu(y.w, u.w));
+        }
         if constexpr (EPI == VX_I8_STORE) {
             if (a.bias) {
-                const float4 b = vx_load4<false>(a.bias, n, VELOX_DT_F32, cols - n);
+                const float4 b = vx_load4<false>(a.bias, c, VELOX_DT_F32, cols - c);
                 y = make_float4(y.x + b.x, y.y + b.y, y.z + b.z, y.w + b.w);
             }
         }
-        if constexpr (kGrouped) *(float4*)(a.part + (size_t)(EPI == VX_I8_SLOT ? slot : p) * a.part_stride + n) = y;  // (rows of whole float4)
-        else if (a.vec) vx_finish<true>(a, p, n, cols, y);
-        else vx_finish<false>(a, p, n, cols, y);
-    };
-    if constexpr (EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN) {
-        const float4 g = scaled(acc0, ws), u = scaled(acc1, ws + 16);
-        put(8u * t0 + 4u * (lane >> 4), a.w.n / 2u, make_float4(vx_swiglu(g.x, u.x), vx_swiglu(g.y, u.y), vx_swiglu(g.z, u.z), vx_swiglu(g.w, u.w)));
-    } else {
-        put(16u * t0 + 4u * (lane >> 4), a.w.n, scaled(acc0, ws));
-        if (two) put(16u * (t0 + 1u) + 4u * (lane >> 4), a.w.n, scaled(acc1, ws + 16));
+        if constexpr (kGrouped) *(float4*)(a.part + (size_t)(EPI == VX_I8_SLOT ? slot : p) * a.part_stride + c) = y;  // (rows of whole float4)
+        else if (a.vec) vx_finish<true>(a, p, c, cols, y);
+        else vx_finish<false>(a, p, c, cols, y);
     }
+}
+
+template <int NT, int MT, int NW, int EPI>
+hipError_t vx_i8_stream_launch(const VxI8Args& a, hipStream_t st) {
+    const uint32_t n_blocks = (a.w.n_tiles + NT - 1u) / NT;
+    const uint32_t items = EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT ? a.max_items : (a.n_rows + 16u * MT - 1u) / (16u * MT);
+    hipLaunchKernelGGL((vx_i8_stream_kernel<NT, MT, NW, EPI>), dim3(items * n_blocks), dim3(64 * NW), 0, st, a, n_blocks);
+    return hipGetLastError();
 }
 
 // ---- products of many rows: tiles through LDS ----
@@ -229,19 +339,13 @@ __device__ __forceinline__ void vx_to_lds(uint32_t lds, const void* from) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "m0", "memory");
 }
 
-// What a lane of the wave wrote to LDS is what the others read behind this.
-__device__ __forceinline__ void vx_wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Workgroup b of `total`: the b / 8-th of XCD b % 8 (workgroups are dealt out in turn), each XCD taking a run of neighbours.
 __device__ __forceinline__ uint32_t vx_xcd_run(uint32_t b, uint32_t total) {
     const uint32_t x = b & 7u, i = b >> 3, q = total >> 3, r = total & 7u;
     return x * q + (x < r ? x : r) + i;
 }
 
-template <int WN, int WM, int FN, int FM, int EPI>
+template <int WN, int WM, int FN, int FM, int S, int EPI>
 __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, uint32_t row0, uint32_t n_blocks, uint32_t m_blocks) {
     constexpr int W = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, STAGE = (TN + TM) * 128;
     constexpr bool kGrouped = EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT;
@@ -365,42 +469,49 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    auto ready = [&] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    constexpr int HALF = (PW + PA) / 2;
-
-    // Step i reads stage i % 2. In its last quarter and the next step's first, stage i + 2's pieces come; behind the
-    // last step's there are none left, the steps' last pieces come again in their place (and are not read).
-    fetch_all(0);
-    ready();
-    vx_each<FN + FM>([&](auto r) { read(vx_int<0>{}, r, 0, vx_int<0>{}); });
-    if (steps > 1u) vx_each<HALF>([&](auto j) { fetch(j, 1); });
-    for (uint32_t i = 0; i + 1u < steps; ++i) {
-        const uint32_t st = i & 1u;
-        quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<HALF>{}, vx_int<PW + PA>{}, st ^ 1u);
+    constexpr int PIECES = 2 * PW + PA, HALF = (PW + PA) / 2;  // loads of a wave's share of a stage
+    auto ready = [&](auto left_) {  // this wave's loads but the last `left` are in LDS, its reads in registers; then everybody's are
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(left_)::value) : "memory");
+    };
+    uint32_t st = 0;  // stage of step i: i % S
+    const auto behind = [&](uint32_t by) { return st + by < (uint32_t)S ? st + by : st + by - (uint32_t)S; };
+    // Step i: its stage's quarters. Its own place is free once every wave is past the barrier: stage i + S comes there, half in
+    // this step's last quarter (NEXT), half in the next one's first (REST).
+    auto step = [&](auto rest_, auto next_) {
+        constexpr bool REST = decltype(rest_)::value != 0, NEXT = decltype(next_)::value != 0;
+        quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<HALF>{}, vx_int<(REST ? PW + PA : HALF)>{}, behind(S - 1));
         quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
         quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
-        ready();
-        if (i + 2u == steps) {
+        ready(vx_int<(REST ? (S - 2) * PIECES : 0)>{});
+        quarter(vx_int<1>{}, vx_int<0>{}, behind(1), vx_int<0>{}, vx_int<(NEXT ? HALF : 0)>{}, st);
+        st = behind(1);
+    };
 #pragma unroll
-            for (int j = 0; j < HALF; ++j) {
-                if (j < PW) pw[j] -= 2048;
-                else pa[j - PW] -= 128;
-            }
+    for (int j = 0; j < S - 1; ++j)
+        if ((uint32_t)j < steps) vx_each<PW + PA>([&](auto piece) { fetch(piece, j); });
+    if (steps >= (uint32_t)S) ready(vx_int<(S - 2) * PIECES>{});
+    else ready(vx_int<0>{});
+    vx_each<FN + FM>([&](auto r) { read(vx_int<0>{}, r, 0, vx_int<0>{}); });
+    uint32_t i = 0;
+    if (steps >= (uint32_t)S) {
+        vx_each<HALF>([&](auto j) { fetch(j, S - 1); });
+        for (; i + S < steps; ++i) step(vx_int<1>{}, vx_int<1>{});
+        if (S > 1 && i + 1u < steps) {
+            step(vx_int<1>{}, vx_int<0>{});
+            ++i;
         }
-        quarter(vx_int<1>{}, vx_int<0>{}, st ^ 1u, vx_int<0>{}, vx_int<HALF>{}, st);
     }
-    const uint32_t st = (steps - 1u) & 1u;
+    for (; i + 1u < steps; ++i) step(vx_int<0>{}, vx_int<0>{});
     quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
     quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
     quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
     quarter(vx_int<1>{}, vx_int<-1>{}, 0, vx_int<0>{}, vx_int<0>{}, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing may come into LDS behind the workgroup's end)
 
     // Epilogue, one block of 32 rows at a time: the sums go through LDS, where the lane of row lane % 32 writes those of n =
     // 8 q + 4 (lane / 32) + 0 .. 3 of every weight block; a row's outputs are then formed by neighbouring lanes, four each, and
     // leave in whole lines. Rolled loops: code that runs once comes through the instruction cache at memory's pace (with the
     // scales applied in front of LDS and everything unrolled a launch took 60 us more).
-    static_assert(W * 32 * ROW * 4 <= 2 * STAGE, "the epilogue's rows lie in the stages");
+    static_assert(W * 32 * ROW * 4 <= S * STAGE, "the epilogue's rows lie in the stages");
     int* mine = (int*)lds + wave * 32 * ROW;
     asm volatile("s_barrier" ::: "memory");
     const uint32_t n = col0 + 4u * (lane % LANES);
@@ -487,36 +598,19 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
 
 constexpr uint32_t kTileStep = 1u << 20;  // rows of a launch
 
-template <int WN, int WM, int FN, int FM, int EPI>
+template <int WN, int WM, int FN, int FM, int S, int EPI>
 hipError_t vx_i8_tile_launch(const VxI8Args& a, hipStream_t st) {
-    constexpr uint32_t TN = 32 * WN * FN, TM = 32 * WM * FM, lds = 2 * (TN + TM) * 128;
-    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_tile_kernel<WN, WM, FN, FM, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    constexpr uint32_t TN = 32 * WN * FN, TM = 32 * WM * FM, lds = S * (TN + TM) * 128;
+    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_tile_kernel<WN, WM, FN, FM, S, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (set != hipSuccess) return set;
     const uint32_t n_blocks = (a.w.n_tiles * 16u + TN - 1u) / TN;
     if (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) {
-        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, EPI>), dim3(a.max_items * n_blocks), dim3(64 * WN * WM), lds, st, a, 0u, n_blocks, 0u);
+        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, S, EPI>), dim3(a.max_items * n_blocks), dim3(64 * WN * WM), lds, st, a, 0u, n_blocks, 0u);
         return hipGetLastError();
     }
     for (uint32_t r = 0; r < a.n_rows; r += kTileStep) {
         const uint32_t rows = a.n_rows - r < kTileStep ? a.n_rows - r : kTileStep, m_blocks = (rows + TM - 1u) / TM;
-        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, EPI>), dim3(n_blocks * m_blocks), dim3(64 * WN * WM), lds, st, a, r, n_blocks, m_blocks);
-        const hipError_t err = hipGetLastError();
-        if (err != hipSuccess) return err;
-    }
-    return hipSuccess;
-}
-
-template <int EPI>
-hipError_t vx_i8_launch(const VxI8Args& a, hipStream_t st) {
-    const uint32_t n_blocks = (a.w.n_tiles + 7u) / 8u;
-    if (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) {
-        hipLaunchKernelGGL((vx_i8_kernel<EPI>), dim3(a.max_items * n_blocks), dim3(256), 0, st, a, 0u, n_blocks);
-        return hipGetLastError();
-    }
-    const uint32_t step = 16u * ((1u << 23) / n_blocks ? (1u << 23) / n_blocks : 1u);  // a launch has fewer than 2^32 threads
-    for (uint32_t r = 0; r < a.n_rows; r += step) {
-        const uint32_t rows = a.n_rows - r < step ? a.n_rows - r : step;
-        hipLaunchKernelGGL((vx_i8_kernel<EPI>), dim3((rows + 15u) / 16u * n_blocks), dim3(256), 0, st, a, r, n_blocks);
+        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, S, EPI>), dim3(n_blocks * m_blocks), dim3(64 * WN * WM), lds, st, a, r, n_blocks, m_blocks);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
@@ -535,7 +629,14 @@ hipError_t vx_launch_i8_pack(const VxI8Mat& m, uint32_t first, uint32_t number, 
 
 hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& out, const uint32_t* limit,
                                  hipStream_t st) {
-    hipLaunchKernelGGL(vx_i8_quantize_kernel, dim3(n_rows), dim3(256), 0, st, x, k, out, limit);
+    const uint32_t elt = x.dtype == VELOX_DT_F32 ? 4u : 2u;
+    if (((uintptr_t)x.data & 15u) == 0 && x.rs * elt % 16u == 0 && vx_i8_pad(k) * elt <= 1024u * 16u * 16u) {
+        if (x.dtype == VELOX_DT_F32) return vx_quantize_launch<float>(x, n_rows, k, out, limit, st);
+        if (x.dtype == VELOX_DT_F16) return vx_quantize_launch<_Float16>(x, n_rows, k, out, limit, st);
+        return vx_quantize_launch<__bf16>(x, n_rows, k, out, limit, st);
+    }
+    if (limit) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(vx_i8_quantize_any_kernel, dim3(n_rows), dim3(256), 0, st, x, k, out);
     return hipGetLastError();
 }
 
@@ -543,18 +644,25 @@ hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k,
 // them here: 2590 us by 16 -> 1171 by 128; 32 rows: 288 -> 302).
 uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count) { return slots >= 32u * count ? 128u : 16u; }
 
-// The tile kernel from 65 rows on (8192 x 8192, rows already in 8 bits: 64 rows 44 -> 42 us, 128 49 -> 43, 300 109 -> 43),
-// its 256 x 256 form where those tiles come to two rounds of the CUs (8192 rows of 8192 x 8192: 554 -> 471 us, of 8192 x 29568:
+// Up to 16 rows the streaming kernel with one weight tile a workgroup (4096 x 4096, one row: two tiles 6.1 us, one 5.0) or,
+// where more rows share a tile of a large matrix, two (8192 x 8192, 16 rows: 16.1, 14.2); up to 32 rows two or four tiles and eight
+// waves (8192 x 8192: 15.3; 37888 x 3584 paired: two 35.7, four 32.1). From 33 rows on tiles through LDS: 128 x 32 in four stages (64 rows of
+// 8192 x 8192: 18.1, streaming 21.3), from 65 on 128 x 128 (300 rows 109 by 16 -> 43), its 256 x 256 form where those tiles come to two rounds of the CUs (8192 rows of 8192 x 8192: 554 -> 471 us, of 8192 x 29568:
 // 1893 -> 1553; 2048 rows of 4096 x 4096, half a round: 40 -> 54).
 template <int EPI>
 hipError_t vx_i8_choose(const VxI8Args& a, hipStream_t st) {
     if constexpr (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) {
-        if (a.item_rows == 128u) return vx_i8_tile_launch<2, 2, 2, 2, EPI>(a, st);
+        if (a.item_rows == 128u) return vx_i8_tile_launch<2, 2, 2, 2, 2, EPI>(a, st);
     } else if (a.n_rows > 64u) {
-        if ((uint64_t)((a.w.n_tiles + 15u) / 16u) * ((a.n_rows + 255u) / 256u) >= 512u) return vx_i8_tile_launch<2, 2, 4, 4, EPI>(a, st);
-        return vx_i8_tile_launch<2, 2, 2, 2, EPI>(a, st);
+        if ((uint64_t)((a.w.n_tiles + 15u) / 16u) * ((a.n_rows + 255u) / 256u) >= 512u) return vx_i8_tile_launch<2, 2, 4, 4, 2, EPI>(a, st);
+        return vx_i8_tile_launch<2, 2, 2, 2, 2, EPI>(a, st);
     }
-    return vx_i8_launch<EPI>(a, st);
+    constexpr bool one = EPI == VX_I8_STORE || EPI == VX_I8_SLOT;  // (the others take tiles by pairs)
+    if constexpr (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) return vx_i8_stream_launch<2, 1, 4, EPI>(a, st);
+    if (a.n_rows > 32u) return vx_i8_tile_launch<4, 1, 1, 1, 4, EPI>(a, st);
+    if (a.n_rows > 16u) return a.w.n_tiles >= 2048u ? vx_i8_stream_launch<4, 2, 8, EPI>(a, st) : vx_i8_stream_launch<2, 2, 8, EPI>(a, st);
+    if (one && (a.n_rows <= 4u || a.w.n_tiles < 512u)) return vx_i8_stream_launch<one ? 1 : 2, 1, 4, EPI>(a, st);
+    return vx_i8_stream_launch<2, 1, 4, EPI>(a, st);
 }
 hipError_t vx_launch_i8_product(const VxI8Args& a, int epi, hipStream_t st) {
     switch (epi) {

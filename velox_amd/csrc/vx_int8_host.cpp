@@ -285,6 +285,7 @@ int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Ma
     c.part_stride = f.part_stride;
     if (residual) c.res = view(residual);
     c.out = view(out);
+    c.vec = whole(out) && (!residual || whole(residual));
     if (e == hipSuccess) e = vx_launch_combine(c, st);
     return (int)e;
 }
