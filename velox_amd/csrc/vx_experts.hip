@@ -4,125 +4,241 @@
 namespace {
 
 // ---- routing ----
-constexpr uint32_t kRouteItems = kVxI8MaxCount / 64u;  // experts of a lane at most
+// The largest of the wave's values, in every lane's reach as a scalar.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t vx_max_dpp(uint32_t v) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+    return v > o ? v : o;
+}
+__device__ __forceinline__ uint32_t vx_wave_max(uint32_t v) {
+    v = vx_max_dpp<0x111, 0xF>(v);  // from the lanes 1, 2, 4, 8 below in a row of 16, then from the rows below
+    v = vx_max_dpp<0x112, 0xF>(v);
+    v = vx_max_dpp<0x114, 0xF>(v);
+    v = vx_max_dpp<0x118, 0xF>(v);
+    v = vx_max_dpp<0x142, 0xA>(v);
+    v = vx_max_dpp<0x143, 0xC>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// Numbers as unsigned words of the same order (-0 below +0: callers add 0), and back.
+__device__ __forceinline__ uint32_t vx_word_of(float f) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float vx_float_of(uint32_t w) { return __builtin_bit_cast(float, w & 0x80000000u ? w & 0x7FFFFFFFu : ~w); }
+// Whether a is above b for certain, where they are sums of numbers of sizes as and bs, each off by less than 2^-19 (1 + its
+// size): a score in fp32 is off by 22 of its half steps at most (a sum of 1024), its sum with a bias by one more.
+__device__ __forceinline__ bool vx_above(float a, float as, float b, float bs) { return a - b > 1.9073486e-6f * (4.0f + as + bs); }
 
-// One wave per row; lane l holds experts l, l + 64, ... Choice values are 64-bit numbers; an expert that takes no part has
-// -infinity.
+// A row's groups that take part, as a mask, by marks of the choice values in `all` (LDS, one wave's). L lanes a group.
+template <class F>
+__device__ __forceinline__ uint64_t vx_open_groups(const VxRouteArgs& a, const F* all, F* marks, bool& unsure) {
+    const uint32_t lane = threadIdx.x & 63u, size = a.n_experts / a.groups, L = 1u << a.group_lanes, g = lane >> a.group_lanes, sub = lane & (L - 1u);
+    F best = -INFINITY, next = -INFINITY;
+    if (g < a.groups)
+        for (uint32_t j = sub; j < size; j += L) {
+            const F v = all[g * size + j];
+            const F low = best < v ? best : v;
+            next = next > low ? next : low;
+            best = best > v ? best : v;
+        }
+    for (uint32_t off = 1; off < L; off <<= 1) {
+        const F ob = __shfl_xor(best, (int)off), on = __shfl_xor(next, (int)off);
+        const F low = best < ob ? best : ob, high = next > on ? next : on;
+        next = low > high ? low : high;
+        best = best > ob ? best : ob;
+    }
+    const F mark = a.two && next > -INFINITY ? best + next : best;
+    if (sub == 0 && g < a.groups) {
+        marks[g] = mark;
+        if constexpr (sizeof(F) == 4) marks[kVxMaxGroups + g] = fabsf(best) + (a.two && next > -INFINITY ? fabsf(next) : 0.0f);
+    }
+    vx_wave_sync();
+    uint32_t before = 0;  // lane g: the marks in front of group g's
+    const F my = marks[lane < a.groups ? lane : 0u];
+    for (uint32_t j = 0; j < a.groups; ++j) {
+        const F m = marks[j];
+        before += m > my || (m == my && j < lane);
+    }
+    const uint64_t open = __ballot(lane < a.groups && before < a.top_groups);
+    if constexpr (sizeof(F) == 4) {
+        // the last mark that is in and the first that is out have to be apart
+        const uint64_t last = __ballot(lane < a.groups && before == a.top_groups - 1u), out = __ballot(lane < a.groups && before == a.top_groups);
+        if (out) {
+            const int in_at = (int)__builtin_ctzll(last), out_at = (int)__builtin_ctzll(out);
+            unsure = marks[out_at] > -INFINITY && !vx_above(marks[in_at], marks[kVxMaxGroups + in_at], marks[out_at], marks[kVxMaxGroups + out_at]);
+        }
+    }
+    vx_wave_sync();
+    return open;
+}
+
+// One wave per row; lane l holds experts l, l + 64, ... Without a bias the order is the logits'. With one, and for sums of two
+// marks, choice values are first formed in fp32; where two that decide are too near to each other for that (about one row in 300 of 256
+// experts), the row is done again in 64 bits. The largest is found top_k times:
+// by DPP in the wave, its place by ballots. The chosen scores are formed in 64 bits. What bounds it: instructions (256 experts, 8 of
+// them in 4 of 8 groups: about 600 a row).
 template <uint32_t ITEMS>
 __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
-    __shared__ double all[4][ITEMS * 64u];
-    __shared__ double marks[4][kVxMaxGroups];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = blockIdx.x * 4u + wave;
-    const bool live = r < a.n_rows;  // (barriers below: every wave goes on)
-    double score[ITEMS], pick[ITEMS];
-    double top = -INFINITY;
+    __shared__ double room[4][ITEMS * 64u + kVxMaxGroups];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), r = blockIdx.x * 4u + wave;
+    if (r >= a.n_rows) return;  // (waves share nothing)
+    const size_t base = (size_t)r * a.x.rs;
+    float x[ITEMS], bias[ITEMS];
 #pragma unroll
     for (uint32_t i = 0; i < ITEMS; ++i) {
         const uint32_t e = lane + 64u * i;
-        float x = -INFINITY;
-        if (live && e < a.n_experts) x = vx_load(a.x.data, (size_t)r * a.x.rs + e, a.x.dtype);
-        x = x > -INFINITY ? fminf(x, 3.40282347e38f) : -INFINITY;  // (NaN too)
-        score[i] = x;
-        top = fmax(top, score[i]);
+        x[i] = e < a.n_experts ? vx_load(a.x.data, base + e, a.x.dtype) : -INFINITY;
+        bias[i] = a.bias && e < a.n_experts ? a.bias[e] : 0.0f;
     }
-    const bool by_logits = !a.sigmoid && !a.bias && !a.two;
-    if (a.sigmoid) {
+    float top = -INFINITY;
+#pragma unroll
+    for (uint32_t i = 0; i < ITEMS; ++i) {
+        x[i] = x[i] > -INFINITY ? fminf(x[i], 3.40282347e38f) + 0.0f : -INFINITY;  // (NaN too)
+        top = fmaxf(top, x[i]);
+    }
+    if (!a.sigmoid) top = vx_float_of(vx_wave_max(vx_word_of(top)));
+    const auto out = [&](uint32_t i) { return !(x[i] > -INFINITY) || !(fabsf(bias[i]) < INFINITY); };
+    const bool by_logits = !a.bias, marked = a.groups > 1u;
+
+    float pick[ITEMS];
+    bool unsure = false;
+    if (!by_logits || a.two) {
+        constexpr float kLog2e = 1.44269504f;
+        float score[ITEMS], sum = 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < ITEMS; ++i) {
-            const double x = score[i];
-            score[i] = 1.0 / (1.0 + exp(-x));
-            pick[i] = x > -INFINITY ? score[i] : -INFINITY;
+            const float p = __builtin_amdgcn_exp2f((a.sigmoid ? -x[i] : x[i] - top) * kLog2e);
+            score[i] = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + p) : x[i] > -INFINITY ? p : 0.0f;
+            sum += score[i];
         }
+        if (!a.sigmoid) {
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
+            sum = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < ITEMS; ++i) score[i] *= sum;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < ITEMS; ++i) pick[i] = out(i) ? -INFINITY : score[i] + bias[i];
     } else {
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) top = fmax(top, __shfl_xor(top, off));
-        double sum = 0.0;
+        for (uint32_t i = 0; i < ITEMS; ++i) pick[i] = x[i];
+    }
+    uint64_t open = ~0ull;
+    const uint32_t size = a.n_experts / a.groups;
+    if (marked) {
+        float* all = (float*)room[wave];
+#pragma unroll
+        for (uint32_t i = 0; i < ITEMS; ++i) all[lane + 64u * i] = pick[i];
+        vx_wave_sync();
+        open = vx_open_groups<float>(a, all, all + ITEMS * 64u, unsure);
+        unsure = unsure && (!by_logits || a.two);
+    }
+    uint32_t id = kVxNoExpert;  // lane j: the j-th choice
+    if (!unsure) {
+        uint32_t key[ITEMS];
+        const uint32_t none = vx_word_of(-INFINITY);
 #pragma unroll
         for (uint32_t i = 0; i < ITEMS; ++i) {
-            const double x = score[i];
-            score[i] = x > -INFINITY ? exp(x - top) : 0.0;
-            sum += score[i];
-            pick[i] = x;
+            const uint32_t e = lane + 64u * i;
+            float v = by_logits ? x[i] : pick[i] + 0.0f;
+            if (e >= a.n_experts || (marked && !(open >> (e / size) & 1u))) v = -INFINITY;
+            key[i] = vx_word_of(v);
         }
+        float before = 0.0f;
+        for (uint32_t j = 0; j < a.top + (by_logits ? 0u : 1u); ++j) {
+            uint32_t best = key[0];
+#pragma unroll
+            for (uint32_t i = 1; i < ITEMS; ++i) best = best > key[i] ? best : key[i];
+            best = vx_wave_max(best);
+            if (best <= none) break;
+            if (!by_logits) {
+                const float v = vx_float_of(best);
+                unsure = unsure || (j && !vx_above(before, fabsf(before), v, fabsf(v)));
+                before = v;
+                if (j == a.top) break;
+            }
+            uint32_t at = 0;  // the lowest index that has it
+            uint64_t lanes = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < ITEMS; ++i) {
+                const uint64_t m = __ballot(key[i] == best);
+                at = lanes ? at : i;
+                lanes = lanes ? lanes : m;
+            }
+            const uint32_t l = (uint32_t)__builtin_ctzll(lanes);
+#pragma unroll
+            for (uint32_t i = 0; i < ITEMS; ++i) key[i] = i == at && lane == l ? 0u : key[i];
+            id = lane == j ? l + 64u * at : id;
+        }
+    }
+    // 64-bit scores: of what was chosen; of all where the softmax's sum is wanted, or the choice is made again
+    double all_sum = 0.0;
+    const bool whole = !a.sigmoid && (unsure || !a.renorm);
+    const auto exact = [&](float v) { return a.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : v > -INFINITY ? exp((double)v - (double)top) : 0.0; };
+    if (whole) {
+#pragma unroll
+        for (uint32_t i = 0; i < ITEMS; ++i) all_sum += exact(x[i]);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) all_sum += __shfl_xor(all_sum, off);
+    }
+    if (unsure) {
+        double* all = room[wave];
+#pragma unroll 1
+        for (uint32_t i = 0; i < ITEMS; ++i) {
+            float v = x[0], b = bias[0];
+#pragma unroll
+            for (uint32_t q = 1; q < ITEMS; ++q) {
+                v = i == q ? x[q] : v;
+                b = i == q ? bias[q] : b;
+            }
+            const double s = a.sigmoid ? exact(v) : all_sum > 0.0 ? exact(v) / all_sum : 0.0;
+            all[lane + 64u * i] = v > -INFINITY && fabsf(b) < INFINITY ? s + (double)b : -INFINITY;
+        }
+        vx_wave_sync();
+        bool never = false;
+        if (marked) open = vx_open_groups<double>(a, all, all + ITEMS * 64u, never);
+        id = kVxNoExpert;
+        for (uint32_t j = 0; j < a.top; ++j) {
+            double best = -INFINITY;
+            uint32_t at = 0xFFFFFFFFu;
+            for (uint32_t e = lane; e < a.n_experts; e += 64u) {
+                // (without a bias equal scores of different logits keep the logits' order: the largest logit comes first)
+                const double v = marked && !(open >> (e / size) & 1u) ? -INFINITY : by_logits && all[e] > -INFINITY ? (double)vx_load(a.x.data, base + e, a.x.dtype) : all[e];
+                if (v > best) {
+                    best = v;
+                    at = e;
+                }
+            }
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const double ob = __shfl_xor(best, off);
+                const uint32_t oa = __shfl_xor(at, off);
+                if (ob > best || (ob == best && oa < at)) {
+                    best = ob;
+                    at = oa;
+                }
+            }
+            if (at == 0xFFFFFFFFu) break;
+            if ((at & 63u) == lane) all[at] = -INFINITY;
+            if (lane == j) id = at;
+        }
+    }
+    double s = 0.0;
+    if (id != kVxNoExpert) {
+        const float v = vx_load(a.x.data, base + id, a.x.dtype);
+        s = exact(fminf(v, 3.40282347e38f));
+        if (whole) s = all_sum > 0.0 ? s / all_sum : 0.0;
+    }
+    if (a.renorm) {
+        double sum = s;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
-#pragma unroll
-        for (uint32_t i = 0; i < ITEMS; ++i) {
-            score[i] = sum > 0.0 ? score[i] / sum : 0.0;
-            if (!by_logits) pick[i] = pick[i] > -INFINITY ? score[i] : -INFINITY;
-        }
+        s = sum > 0.0 ? s / sum : 0.0;
     }
-    if (a.bias) {
-#pragma unroll
-        for (uint32_t i = 0; i < ITEMS; ++i) {
-            const uint32_t e = lane + 64u * i;
-            const float b = e < a.n_experts ? a.bias[e] : 0.0f;
-            pick[i] = pick[i] > -INFINITY && fabsf(b) < INFINITY ? pick[i] + b : -INFINITY;
-        }
-    }
-    if (a.groups > 1u) {
-#pragma unroll
-        for (uint32_t i = 0; i < ITEMS; ++i) all[wave][lane + 64u * i] = pick[i];
-        __syncthreads();
-        const uint32_t size = a.n_experts / a.groups;
-        double best = -INFINITY, next = -INFINITY;
-        if (lane < a.groups)
-            for (uint32_t j = 0; j < size; ++j) {
-                const double v = all[wave][lane * size + j];
-                next = fmax(next, fmin(best, v));
-                best = fmax(best, v);
-            }
-        const double mark = a.two && next > -INFINITY ? best + next : best;
-        marks[wave][lane] = mark;
-        __syncthreads();
-        uint32_t before = 0;
-        for (uint32_t g = 0; g < a.groups; ++g) {
-            const double m = marks[wave][g];
-            before += m > mark || (m == mark && g < lane);
-        }
-        const uint64_t open = __ballot(lane < a.groups && before < a.top_groups);
-#pragma unroll
-        for (uint32_t i = 0; i < ITEMS; ++i) {
-            const uint32_t e = lane + 64u * i;
-            if (e < a.n_experts && !(open >> (e / size) & 1u)) pick[i] = -INFINITY;
-        }
-    }
-    double mine = 0.0, total = 0.0;  // lane j: the j-th score
-    uint32_t id = kVxNoExpert;
-    for (uint32_t j = 0; j < a.top; ++j) {
-        double best = -INFINITY, s = 0.0;
-        uint32_t at = 0xFFFFFFFFu;
-#pragma unroll
-        for (uint32_t i = 0; i < ITEMS; ++i)
-            if (pick[i] > best) {
-                best = pick[i];
-                s = score[i];
-                at = lane + 64u * i;
-            }
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const double ob = __shfl_xor(best, off), os = __shfl_xor(s, off);
-            const uint32_t oa = __shfl_xor(at, off);
-            if (ob > best || (ob == best && oa < at)) {
-                best = ob;
-                s = os;
-                at = oa;
-            }
-        }
-        if (at == 0xFFFFFFFFu) break;  // (uniform)
-#pragma unroll
-        for (uint32_t i = 0; i < ITEMS; ++i)
-            if (at == lane + 64u * i) pick[i] = -INFINITY;
-        if (lane == j) {
-            id = at;
-            mine = s;
-        }
-        total += s;
-    }
-    if (!live || lane >= a.top) return;
-    if (a.renorm) mine = total > 0.0 ? mine / total : 0.0;
+    if (lane >= a.top) return;
     a.ids[(size_t)r * a.top + lane] = id;
-    a.weights[(size_t)r * a.top + lane] = (float)(mine * a.scale);
+    a.weights[(size_t)r * a.top + lane] = (float)(s * (double)a.scale);
 }
 
 // ---- grouping: a stable counting sort of the slots by expert ----
@@ -323,11 +439,16 @@ __global__ __launch_bounds__(256) void vx_combine_kernel(VxCombineArgs a, uint32
 
 }  // namespace
 
-hipError_t vx_launch_route(const VxRouteArgs& a, hipStream_t st) {
+hipError_t vx_launch_route(const VxRouteArgs& args, hipStream_t st) {
+    VxRouteArgs a = args;
+    a.group_lanes = 0;
+    while ((2u << a.group_lanes) * a.groups <= 64u) ++a.group_lanes;
     const dim3 grid((a.n_rows + 3u) / 4u);
     if (a.n_experts <= 64u) hipLaunchKernelGGL((vx_route_kernel<1>), grid, dim3(256), 0, st, a);
+    else if (a.n_experts <= 128u) hipLaunchKernelGGL((vx_route_kernel<2>), grid, dim3(256), 0, st, a);
     else if (a.n_experts <= 256u) hipLaunchKernelGGL((vx_route_kernel<4>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((vx_route_kernel<kRouteItems>), grid, dim3(256), 0, st, a);
+    else if (a.n_experts <= 512u) hipLaunchKernelGGL((vx_route_kernel<8>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((vx_route_kernel<16>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

@@ -62,6 +62,7 @@ struct VxRouteArgs {
     float scale;
     uint32_t* ids;
     float* weights;
+    uint32_t group_lanes;      // set by the launcher: 2^group_lanes lanes for each group
 };
 
 struct VxGroupArgs {

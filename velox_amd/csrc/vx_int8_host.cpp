@@ -179,6 +179,7 @@ int velox_hip_expert_route(const VeloxHipRouteConfig* cfg, const VeloxHipRows* l
     if (!n_rows) return VELOX_HIP_OK;
     if (!d_ids || !d_weights || !aligned(d_ids, 4) || !aligned(d_weights, 4)) return VELOX_HIP_EINVAL;
     VxRouteArgs a;
+    std::memset(&a, 0, sizeof(a));
     a.x = view(logits);
     a.bias = d_bias;
     a.n_rows = n_rows;
