@@ -48,6 +48,8 @@ struct VxI8Args {
     VxGrouped g;               // HIDDEN, SLOT
     uint32_t top;              // HIDDEN: position p reads row order[p] / top of a
     uint32_t max_items, item_rows;
+    const uint32_t* ids;       // slots one by one: slot s is expert ids[s] - first's, of row s / top
+    uint32_t first;
     const float* bias;         // STORE
     VxI8View res, out;         // STORE (res.data NULL: none), SWIGLU
     uint32_t vec;              // 1: res and out rows begin at whole multiples of four elements
@@ -94,6 +96,13 @@ hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k,
                                  hipStream_t st);
 hipError_t vx_launch_i8_product(const VxI8Args& a, int epi, hipStream_t st);
 uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count);  // positions of a block of a grouped product
+// Few rows, quantized by the workgroups that multiply them: whether x's rows are; plain products, the hidden values of
+// every slot (a.part: [slot]), the experts' answers and their sum.
+bool vx_i8_by_row(const VxI8View& x, uint32_t n_rows, uint32_t k);
+hipError_t vx_launch_i8_row(const VxI8Args& a, const VxI8View& x, int epi, hipStream_t st);
+bool vx_i8_ffn_by_slot(const VxI8View& x, uint32_t n_rows, uint32_t hidden, uint32_t inner);
+hipError_t vx_launch_i8_slots(const VxI8Args& a, const VxI8View& x, hipStream_t st);
+hipError_t vx_launch_i8_answers(const VxI8Args& a, const VxCombineArgs& c, hipStream_t st);
 hipError_t vx_launch_route(const VxRouteArgs& a, hipStream_t st);
 uint32_t vx_group_blocks(uint32_t n_slots);
 hipError_t vx_launch_group(const VxGroupArgs& a, hipStream_t st);

@@ -3,7 +3,6 @@
 
 namespace {
 
-typedef int v4i __attribute__((ext_vector_type(4)));
 template <int V>
 struct vx_int {
     static constexpr int value = V;
@@ -29,7 +28,34 @@ __device__ __forceinline__ void vx_finish(const VxI8Args& a, size_t r, uint32_t 
     }
     vx_store4<VEC>(a.out.data, r * a.out.rs + n, a.out.dtype, left, y);
 }
+// Four sums with the weight rows' scales, the row's scale and (BIAS) the bias: the same roundings in every kernel.
+template <bool BIAS>
+__device__ __forceinline__ float4 vx_scaled(const v4i& c, const float4& w, float s, const float4& b) {
+    float y[4];
+    const float f[4] = {w.x, w.y, w.z, w.w}, d[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float p = (float)c[i] * f[i];
+        y[i] = BIAS ? __builtin_fmaf(p, s, d[i]) : p * s;
+    }
+    return make_float4(y[0], y[1], y[2], y[3]);
+}
 __device__ __forceinline__ float vx_swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+__device__ __forceinline__ float4 vx_swiglu(const v4i& g, const float4& wg, const v4i& u, const float4& wu, float s) {
+    const float4 none = make_float4(0, 0, 0, 0), a = vx_scaled<false>(g, wg, s, none), b = vx_scaled<false>(u, wu, s, none);
+    return make_float4(vx_swiglu(a.x, b.x), vx_swiglu(a.y, b.y), vx_swiglu(a.z, b.z), vx_swiglu(a.w, b.w));
+}
+// Outputs c .. c + 3 of a plain product's row r (of `cols` in a row), from their sums.
+template <bool SWIGLU>
+__device__ __forceinline__ void vx_outputs(const VxI8Args& a, size_t r, uint32_t c, uint32_t cols, const v4i& sum, const v4i& up, const float* ws, float s) {
+    const float4 w = *(const float4*)ws;
+    float4 y;
+    if constexpr (SWIGLU) y = vx_swiglu(sum, w, up, *(const float4*)(ws + 16), s);
+    else if (a.bias) y = vx_scaled<true>(sum, w, s, vx_load4<false>(a.bias, c, VELOX_DT_F32, cols - c));
+    else y = vx_scaled<false>(sum, w, s, w);
+    if (a.vec) vx_finish<true>(a, r, c, cols, y);
+    else vx_finish<false>(a, r, c, cols, y);
+}
 
 // ---- weights ----
 __global__ __launch_bounds__(256) void vx_i8_pack_kernel(VxI8Mat m, uint32_t first, const int8_t* __restrict__ src, uint64_t ms,
@@ -69,25 +95,19 @@ __device__ __forceinline__ int vx_code(float x, float s, float inv) {
     return (int)r;
 }
 
-// Codes of four values, in the bytes of a word. Where no x * inv is near a half (its error is below 2^-15) rint gives the
-// nearest whole number; else the exact rule above decides.
-__device__ __forceinline__ uint32_t vx_codes(const float* x, float s, float inv) {
+// The same of four values, in the bytes of a word, where no x * inv is near a half; `near` says whether one is (rint is
+// right below 0.5 - 2^-15, the error of x * inv).
+__device__ __forceinline__ uint32_t vx_codes(const float* x, float inv, float& near) {
     uint32_t w = 0;
-    float off = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float r = rintf(x[i] * inv);
-        off = fmaxf(off, fabsf(__builtin_fmaf(x[i], inv, -r)));
+        near = fmaxf(near, fabsf(__builtin_fmaf(x[i], inv, -r)));
         w = __builtin_amdgcn_cvt_pk_u8_f32(r + 128.0f, i, w);
     }
-    w ^= 0x80808080u;
-    if (off > 0.4999f) {
-        w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w |= ((uint32_t)vx_code(x[i], s, inv) & 0xFFu) << (8 * i);
-    }
-    return w;
+    return w ^ 0x80808080u;
 }
+constexpr float kVxNear = 0.4999f;
 // A row's scale from the bits of its largest absolute value (those of an infinity or NaN are above any number's).
 struct VxRowScale {
     float s, inv;
@@ -102,103 +122,151 @@ __device__ __forceinline__ VxRowScale vx_row_scale(uint32_t top) {
 __device__ __forceinline__ uint32_t vx_size_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
 __device__ __forceinline__ uint32_t vx_max(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
-// TPR threads take a row, which stays in registers between the search for its largest value and the rounding: NV vectors of
-// 16 bytes each. Bound by the bytes (8192 rows of 29568 bf16: 726 MB).
-template <class T, int TPR, int NV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void vx_i8_quantize_kernel(VxI8View x, uint32_t n_rows, uint32_t k, VxI8Rows o, const uint32_t* limit) {
-    constexpr int V = 16 / sizeof(T), WG = TPR < 256 ? 256 : TPR, WAVES = TPR / 64;
-    __shared__ uint32_t red[WG / 64];
-    const uint32_t tid = threadIdx.x, t = tid % TPR, r = blockIdx.x * (WG / TPR) + tid / TPR, kp = vx_i8_pad(k);
-    if (limit) n_rows = *limit < n_rows ? *limit : n_rows;
-    if (TPR > 64 ? r >= n_rows : __builtin_amdgcn_readfirstlane((int)r) >= (int)n_rows) return;  // (a wave, or the whole workgroup)
+// The largest word of THREADS threads, in each (`red`: a word for each wave).
+template <int THREADS>
+__device__ __forceinline__ uint32_t vx_threads_max(uint32_t v, uint32_t* red) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v = vx_max(v, (uint32_t)__shfl_xor((int)v, off));
+    if constexpr (THREADS > 64) {
+        __syncthreads();  // (what was there has been looked at)
+        if ((threadIdx.x & 63u) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) v = vx_max(v, red[w]);
+    }
+    return v;
+}
+
+// A row of k values (a whole number of 16-byte vectors, so placed) by THREADS threads, t this one's number, as codes at `to`
+// (memory or LDS), k filled up to a multiple of 128; its scale. Up to NV vectors a thread stay in registers between the search
+// for the largest value and the rounding, those behind are read again (MORE). Loads behind the row give 0. Values next to
+// a half, one in 5000, are done again by a rolled loop: little code, which comes through the instruction cache once.
+template <class T, int THREADS, int NV, bool MORE>
+__device__ __forceinline__ float vx_hold_row(const T* from, uint32_t k, uint8_t* to, uint32_t t, uint32_t* red) {
+    constexpr uint32_t V = 16 / sizeof(T), STEP = THREADS * V;
     struct alignas(16) Vec {
         T v[V];
     };
-    const T* from = (const T*)x.data + (size_t)r * x.rs;
+    const uint32_t kp = vx_i8_pad(k);
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, (int)(k * sizeof(T)), 0x00020000);
+    const auto load = [&](uint32_t c) { return __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(c * sizeof(T)), 0, 0)); };
     Vec in[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const uint32_t c = (j * TPR + t) * V;
-        if (c + V <= k) {
-            in[j] = *(const Vec*)(from + c);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) in[j].v[i] = c + i < k ? from[c + i] : (T)0.0f;
-        }
-    }
+    for (uint32_t j = 0; j < NV; ++j) in[j] = load(j * STEP + t * V);
     uint32_t top = 0;
+    const auto look = [&](const Vec& v) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+        for (uint32_t i = 0; i < V; ++i) top = vx_max(top, vx_size_bits((float)v.v[i]));
+    };
 #pragma unroll
-        for (int i = 0; i < V; ++i) top = vx_max(top, vx_size_bits((float)in[j].v[i]));
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) top = vx_max(top, (uint32_t)__shfl_xor((int)top, off));
-    if constexpr (TPR > 64) {
-        if ((tid & 63u) == 0) red[tid >> 6] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) top = vx_max(top, red[w]);
-    }
-    const VxRowScale q = vx_row_scale(top);
-    int8_t* to = o.codes + (size_t)r * o.rs;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const uint32_t c = (j * TPR + t) * V;
-        if (c >= kp) continue;
+    for (uint32_t j = 0; j < NV; ++j) look(in[j]);
+    if constexpr (MORE)
+        for (uint32_t c = NV * STEP + t * V; c < k; c += STEP) look(load(c));
+    const VxRowScale q = vx_row_scale(vx_threads_max<THREADS>(top, red));
+    float near = 0.0f;
+    const auto put = [&](uint32_t c, const Vec& v) {
         uint32_t w[V / 4];
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) {
-            const float f[4] = {(float)in[j].v[4 * i], (float)in[j].v[4 * i + 1], (float)in[j].v[4 * i + 2], (float)in[j].v[4 * i + 3]};
-            w[i] = q.none ? 0u : vx_codes(f, q.s, q.inv);
+        for (uint32_t i = 0; i < V / 4; ++i) {
+            const float f[4] = {(float)v.v[4 * i], (float)v.v[4 * i + 1], (float)v.v[4 * i + 2], (float)v.v[4 * i + 3]};
+            w[i] = vx_codes(f, q.inv, near);
+            w[i] = q.none ? 0u : w[i];
         }
+        if (c >= kp) return;
         if constexpr (V == 8) *(uint2*)(to + c) = make_uint2(w[0], w[1]);
         else *(uint32_t*)(to + c) = w[0];
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j) put(j * STEP + t * V, in[j]);
+    if constexpr (MORE)
+        for (uint32_t c = NV * STEP + t * V; c < kp; c += STEP) put(c, load(c));
+    if (near > kVxNear && !q.none) {
+#pragma unroll 1
+        for (uint32_t c = t * V; c < k; c += STEP) {
+            const Vec v = load(c);
+#pragma unroll 1
+            for (uint32_t i = 0; i < V; ++i) {
+                float f = (float)v.v[0];
+#pragma unroll
+                for (uint32_t j = 1; j < V; ++j) f = i == j ? (float)v.v[j] : f;
+                to[c + i] = (uint8_t)vx_code(f, q.s, q.inv);
+            }
+        }
     }
-    if (t == 0) o.scales[r] = q.s;
+    return q.s;
 }
 
-// Rows at other places, or longer than the registers of a workgroup: read twice, value by value.
-__global__ __launch_bounds__(256) void vx_i8_quantize_any_kernel(VxI8View x, uint32_t k, VxI8Rows o) {
+// Bound by the bytes (8192 rows of 29568 bf16, 726 MB: 138 us).
+template <class T, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void vx_i8_quantize_kernel(VxI8View x, uint32_t n_rows, uint32_t k, VxI8Rows o, const uint32_t* limit) {
+    constexpr int WG = TPR < 256 ? 256 : TPR;
+    __shared__ uint32_t red[WG / 64];
+    const uint32_t r = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * (WG / TPR) + threadIdx.x / TPR)), t = threadIdx.x % TPR;
+    if (limit) n_rows = *limit < n_rows ? *limit : n_rows;
+    if (r >= n_rows) return;  // (a wave that shares nothing, or the workgroup)
+    const float s = vx_hold_row<T, TPR, NV, false>((const T*)x.data + (size_t)r * x.rs, k, (uint8_t*)o.codes + (size_t)r * o.rs, t, red);
+    if (t == 0) o.scales[r] = s;
+}
+
+// Rows at any place and of any length, value by value: NE of them a thread in registers, those behind read twice.
+template <class T, int NE>
+__global__ __launch_bounds__(256) void vx_i8_quantize_any_kernel(VxI8View x, uint32_t k, VxI8Rows o, const uint32_t* limit) {
     __shared__ uint32_t red[4];
     const uint32_t r = blockIdx.x, tid = threadIdx.x, kp = vx_i8_pad(k);
-    const size_t base = (size_t)r * x.rs;
-    uint32_t top = 0;
-    for (uint32_t i = tid; i < k; i += 256u) top = vx_max(top, vx_size_bits(vx_load(x.data, base + i, x.dtype)));
+    if (limit && r >= *limit) return;
+    const T* from = (const T*)x.data + (size_t)r * x.rs;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, (int)(k * sizeof(T)), 0x00020000);
+    const auto load = [&](uint32_t c) -> float {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, (int)(c * 4u), 0, 0));
+        else return (float)__builtin_bit_cast(T, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, (int)(c * 2u), 0, 0));
+    };
+    float in[NE];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) top = vx_max(top, (uint32_t)__shfl_xor((int)top, off));
-    if ((tid & 63u) == 0) red[tid >> 6] = top;
-    __syncthreads();
-    top = vx_max(vx_max(red[0], red[1]), vx_max(red[2], red[3]));
-    const VxRowScale q = vx_row_scale(top);
+    for (uint32_t j = 0; j < NE; ++j) in[j] = load(j * 256u + tid);
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < NE; ++j) top = vx_max(top, vx_size_bits(in[j]));
+#pragma unroll 8
+    for (uint32_t c = NE * 256u + tid; c < k; c += 256u) top = vx_max(top, vx_size_bits(load(c)));
+    const VxRowScale q = vx_row_scale(vx_threads_max<256>(top, red));
     int8_t* to = o.codes + (size_t)r * o.rs;
-    for (uint32_t i = tid; i < kp; i += 256u) to[i] = i < k && !q.none ? (int8_t)vx_code(vx_load(x.data, base + i, x.dtype), q.s, q.inv) : (int8_t)0;
+    const auto put = [&](uint32_t c, float v) {
+        const int code = vx_code(v, q.s, q.inv);
+        if (c < kp) to[c] = q.none ? (int8_t)0 : (int8_t)code;
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < NE; ++j) put(j * 256u + tid, in[j]);
+#pragma unroll 4
+    for (uint32_t c = NE * 256u + tid; c < kp; c += 256u) put(c, load(c));
     if (tid == 0) o.scales[r] = q.s;
 }
 
 template <class T>
 hipError_t vx_quantize_launch(const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& o, const uint32_t* limit, hipStream_t st) {
     constexpr uint32_t V = 16 / sizeof(T);
-    const uint32_t vecs = vx_i8_pad(k) / V;  // (the codes behind k are written too)
+    if (((uintptr_t)x.data & 15u) == 0 && x.rs % V == 0 && k % V == 0 && vx_i8_pad(k) / V <= 1024u * 8u) {
+        const uint32_t vecs = vx_i8_pad(k) / V;  // (the codes behind k are written too)
 #define VX_QUANTIZE(TPR, NV)                                                                                                              \
     if (vecs <= TPR * NV) {                                                                                                               \
         constexpr uint32_t wg = TPR < 256 ? 256 : TPR;                                                                                    \
         hipLaunchKernelGGL((vx_i8_quantize_kernel<T, TPR, NV>), dim3((n_rows + wg / TPR - 1) / (wg / TPR)), dim3(wg), 0, st, x, n_rows, k, o, limit); \
         return hipGetLastError();                                                                                                         \
     }
-    VX_QUANTIZE(64, 1)
-    VX_QUANTIZE(64, 2)
-    VX_QUANTIZE(256, 1)
-    VX_QUANTIZE(256, 2)
-    VX_QUANTIZE(256, 4)
-    VX_QUANTIZE(256, 8)
-    VX_QUANTIZE(1024, 4)
-    VX_QUANTIZE(1024, 8)
-    VX_QUANTIZE(1024, 16)
+        VX_QUANTIZE(64, 1)
+        VX_QUANTIZE(64, 2)
+        VX_QUANTIZE(256, 1)
+        VX_QUANTIZE(256, 2)
+        VX_QUANTIZE(256, 4)
+        VX_QUANTIZE(256, 8)
+        VX_QUANTIZE(1024, 4)
+        VX_QUANTIZE(1024, 8)
 #undef VX_QUANTIZE
-    return hipErrorInvalidValue;
+    }
+    if (vx_i8_pad(k) <= 4u * 256u) hipLaunchKernelGGL((vx_i8_quantize_any_kernel<T, 4>), dim3(n_rows), dim3(256), 0, st, x, k, o, limit);
+    else hipLaunchKernelGGL((vx_i8_quantize_any_kernel<T, 16>), dim3(n_rows), dim3(256), 0, st, x, k, o, limit);
+    return hipGetLastError();
 }
 
-// ---- products ----
 // ---- products of few rows: the weights' bytes ----
 // A workgroup of NW waves takes NT weight tiles (paired: gate and up tiles by turns) by 16 MT rows. Its waves deal out the 64-column
 // tiles in turn, so that the weights stream in order, each lane's 16 bytes being its MFMA operand; U tiles are requested
@@ -292,23 +360,14 @@ __global__ __launch_bounds__(64 * NW) void vx_i8_stream_kernel(VxI8Args a, uint3
         if constexpr (EPI == VX_I8_HIDDEN) row = slot / a.top;
         const float s = a.a.scales[row];
         const float* ws = a.w.scales + ((uint64_t)e * a.w.n_tiles + t0 + (kSwiglu ? 2 * n : n)) * 16u + 4u * (lane >> 4);
-        const auto scaled = [&](const v4i& v, const float4 f) {
-            return make_float4((float)v[0] * f.x * s, (float)v[1] * f.y * s, (float)v[2] * f.z * s, (float)v[3] * f.w * s);
-        };
-        float4 y = scaled(total((kSwiglu ? 2 * n : n) * MT + m), *(const float4*)ws);
-        if constexpr (kSwiglu) {
-            const float4 u = scaled(total((2 * n + 1) * MT + m), *(const float4*)(ws + 16));
-            y = make_float4(vx_swiglu(y.x, u.x), vx_swiglu(y.y, u.y), vx_swiglu(y.z, u.z), vx_swiglu(y.w, u.w));
+        const v4i sum = total((kSwiglu ? 2 * n : n) * MT + m), up = kSwiglu ? total((2 * n + 1) * MT + m) : sum;
+        if constexpr (kGrouped) {
+            const float4 f = *(const float4*)ws;
+            *(float4*)(a.part + (size_t)(EPI == VX_I8_SLOT ? slot : p) * a.part_stride + c) =
+                kSwiglu ? vx_swiglu(sum, f, up, *(const float4*)(ws + 16), s) : vx_scaled<false>(sum, f, s, f);  // (rows of whole float4)
+        } else {
+            vx_outputs<kSwiglu>(a, p, c, cols, sum, up, ws, s);
         }
-        if constexpr (EPI == VX_I8_STORE) {
-            if (a.bias) {
-                const float4 b = vx_load4<false>(a.bias, c, VELOX_DT_F32, cols - c);
-                y = make_float4(y.x + b.x, y.y + b.y, y.z + b.z, y.w + b.w);
-            }
-        }
-        if constexpr (kGrouped) *(float4*)(a.part + (size_t)(EPI == VX_I8_SLOT ? slot : p) * a.part_stride + c) = y;  // (rows of whole float4)
-        else if (a.vec) vx_finish<true>(a, p, c, cols, y);
-        else vx_finish<false>(a, p, c, cols, y);
     }
 }
 
@@ -318,6 +377,166 @@ hipError_t vx_i8_stream_launch(const VxI8Args& a, hipStream_t st) {
     const uint32_t items = EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT ? a.max_items : (a.n_rows + 16u * MT - 1u) / (16u * MT);
     hipLaunchKernelGGL((vx_i8_stream_kernel<NT, MT, NW, EPI>), dim3(items * n_blocks), dim3(64 * NW), 0, st, a, n_blocks);
     return hipGetLastError();
+}
+
+// ---- products of one row, put into 8 bits on the way ----
+// NT tile rows of weights by one wave: tiles first, first + step, ... of each, U of them requested at a time, against codes in
+// LDS (`x`: this lane's row, 16 (lane / 16) bytes in).
+template <int NT>
+struct VxStream {
+    static constexpr int U = NT == 1 ? 8 : 4;
+    __amdgpu_buffer_rsrc_t rs[NT];
+    uint32_t k_tiles, lane;
+    v4i w[2][U][NT], acc[NT];
+    __device__ __forceinline__ VxStream(const VxI8Mat& m, uint32_t e, uint32_t t0) : k_tiles(m.k_tiles), lane(threadIdx.x & 63u) {
+        const uint32_t run = m.k_tiles * 1024u;
+        const uint8_t* at = (const uint8_t*)m.codes + ((uint64_t)e * m.n_tiles + t0) * run;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            rs[n] = __builtin_amdgcn_make_buffer_rsrc((void*)(at + (uint64_t)n * run), 0, t0 + n < m.n_tiles ? (int)run : 0, 0x00020000);
+            acc[n] = v4i{0, 0, 0, 0};
+        }
+    }
+    template <int SET>
+    __device__ __forceinline__ void load(uint32_t kt, uint32_t step) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) w[SET][u][n] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rs[n], (int)((kt + u * step) * 1024u + lane * 16u), 0, 2));
+    }
+    template <int SET>
+    __device__ __forceinline__ void multiply(uint32_t kt, uint32_t step, const uint8_t* x) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t k = kt + u * step;  // (behind the last the weights are zeros)
+            const v4i c = *(const v4i*)(x + 64u * (k < k_tiles ? k : k_tiles - 1u));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[SET][u][n], c, acc[n], 0, 0, 0);
+        }
+    }
+    // load<0>(first, step) has been called
+    __device__ __forceinline__ void run(uint32_t first, uint32_t step, const uint8_t* x) {
+        for (uint32_t kt = first; kt < k_tiles; kt += 2u * U * step) {
+            load<1>(kt + U * step, step);
+            multiply<0>(kt, step, x);
+            load<0>(kt + 2u * U * step, step);
+            multiply<1>(kt + U * step, step, x);
+        }
+    }
+};
+
+constexpr uint32_t kRowWaves = 4;
+
+// Up to four rows (STORE, SWIGLU), or one slot's row for its expert (HIDDEN): the first weights are requested, the workgroup
+// puts the rows into 8 bits in LDS, its waves take the columns' tiles in turn. Saves the launch that quantizes: one row of 4096 x
+// 4096 fp32.
+template <class T, int NV, int NT, int EPI>
+__global__ __launch_bounds__(64 * kRowWaves) void vx_i8_row_kernel(VxI8Args a, VxI8View x, uint32_t n_blocks) {
+    constexpr bool kSwiglu = EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ v4i sums[kRowWaves][NT][64];
+    __shared__ uint32_t red[kRowWaves];
+    __shared__ float scales[4];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+    const uint32_t slot = uniform(blockIdx.x / n_blocks), t0 = uniform(blockIdx.x % n_blocks) * NT, kp = vx_i8_pad(a.w.k);
+    uint32_t e = 0, row0 = 0, rows = a.n_rows;
+    if constexpr (EPI == VX_I8_HIDDEN) {
+        e = uniform(a.ids[slot] - a.first);
+        if (e >= a.w.count) return;
+        row0 = uniform(slot / a.top);
+        rows = 1;
+    }
+    VxStream<NT> s(a.w, e, t0);
+    s.template load<0>(wave, kRowWaves);
+    for (uint32_t r = 0; r < rows; ++r) {
+        const float f = vx_hold_row<T, 64 * kRowWaves, NV, EPI == VX_I8_HIDDEN && NV == 8>((const T*)x.data + (size_t)(row0 + r) * x.rs, a.w.k, lds + r * kp, threadIdx.x, red);
+        if (threadIdx.x == 0) scales[r] = f;
+    }
+    __syncthreads();
+    const uint32_t mine = lane & 15u;
+    s.run(wave, kRowWaves, lds + (mine < rows ? mine : 0u) * kp + 16u * (lane >> 4));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) sums[wave][n][lane] = s.acc[n];
+    __syncthreads();
+    constexpr uint32_t OUT = kSwiglu ? NT / 2 : NT;
+    const uint32_t cols = kSwiglu ? a.w.n / 2u : a.w.n;
+    for (uint32_t o = wave; o < OUT; o += kRowWaves) {
+        const uint32_t n = kSwiglu ? 2u * o : o, c = 16u * (t0 / (kSwiglu ? 2u : 1u) + o) + 4u * (lane >> 4);
+        if (mine >= rows || c >= cols) continue;
+        v4i sum = sums[0][n][lane], up = sums[0][kSwiglu ? n + 1u : n][lane];
+#pragma unroll
+        for (uint32_t w = 1; w < kRowWaves; ++w) {
+            sum += sums[w][n][lane];
+            if (kSwiglu) up += sums[w][n + 1u][lane];
+        }
+        const float* ws = a.w.scales + ((uint64_t)e * a.w.n_tiles + t0 + n) * 16u + 4u * (lane >> 4);
+        if constexpr (EPI == VX_I8_HIDDEN) *(float4*)(a.part + (size_t)slot * a.part_stride + c) = vx_swiglu(sum, *(const float4*)ws, up, *(const float4*)(ws + 16), scales[0]);
+        else vx_outputs<kSwiglu>(a, mine, c, cols, sum, up, ws, scales[mine]);
+    }
+}
+
+// 16 outputs of a row: each wave takes slots of the row in turn, puts the slot's hidden row into 8 bits in its own piece of LDS
+// while its expert's weights are on their way, and multiplies; the answers meet in LDS and are added in the slots' order.
+constexpr uint32_t kAnswerWaves = 8, kAnswerMost = 8u * 4u * 64u;  // values of a hidden row
+__global__ __launch_bounds__(64 * kAnswerWaves) void vx_i8_answer_kernel(VxI8Args a, VxCombineArgs c, uint32_t n_blocks) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ float answers[kVxMaxTop][16];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+    const uint32_t row = uniform(blockIdx.x / n_blocks), t = uniform(blockIdx.x % n_blocks), kp = vx_i8_pad(a.w.k);
+    uint8_t* codes = lds + wave * kp;
+    for (uint32_t j = wave; j < c.top; j += kAnswerWaves) {
+        const uint32_t slot = row * c.top + j, e = uniform(c.ids[slot] - c.first);
+        if (e >= c.count) continue;
+        VxStream<1> s(a.w, e, t);
+        s.load<0>(0, 1);
+        const float f = vx_hold_row<float, 64, 8, false>(a.part + (size_t)slot * a.part_stride, (a.w.k + 3u) & ~3u, codes, lane, nullptr);
+        vx_wave_sync();
+        s.run(0, 1, codes + 16u * (lane >> 4));
+        vx_wave_sync();
+        if ((lane & 15u) == 0) {
+            const float* ws = a.w.scales + ((uint64_t)e * a.w.n_tiles + t) * 16u + 4u * (lane >> 4);
+            *(float4*)&answers[j][4u * (lane >> 4)] = vx_scaled<false>(s.acc[0], *(const float4*)ws, f, *(const float4*)ws);
+        }
+    }
+    __syncthreads();
+    const uint32_t n = 16u * t + threadIdx.x;
+    if (threadIdx.x >= 16u || n >= c.n) return;
+    float sum = 0.0f;
+    for (uint32_t j = 0; j < c.top; ++j) {
+        const uint32_t slot = row * c.top + j;
+        if (c.ids[slot] - c.first < c.count) sum = __builtin_fmaf(c.weights[slot], answers[j][threadIdx.x], sum);
+    }
+    const float res = c.res.data ? vx_load(c.res.data, (size_t)row * c.res.rs + n, c.res.dtype) : 0.0f;
+    vx_store(c.out.data, (size_t)row * c.out.rs + n, c.out.dtype, res + sum);
+}
+
+template <class T, int NV, int NT, int EPI>
+hipError_t vx_i8_row_launch_v(const VxI8Args& a, const VxI8View& x, hipStream_t st) {
+    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_row_kernel<T, NV, NT, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, 1 << 17);
+    if (set != hipSuccess) return set;
+    const uint32_t n_blocks = (a.w.n_tiles + NT - 1u) / NT, rows = EPI == VX_I8_HIDDEN ? a.n_rows * a.top : 1u;
+    hipLaunchKernelGGL((vx_i8_row_kernel<T, NV, NT, EPI>), dim3(rows * n_blocks), dim3(64 * kRowWaves), vx_i8_pad(a.w.k) * (EPI == VX_I8_HIDDEN ? 1u : a.n_rows), st, a, x, n_blocks);
+    return hipGetLastError();
+}
+template <class T, int NT, int EPI>
+hipError_t vx_i8_row_launch(const VxI8Args& a, const VxI8View& x, hipStream_t st) {
+    const uint32_t vecs = vx_i8_pad(a.w.k) / (16u / sizeof(T));
+    if (vecs <= 64u * kRowWaves) return vx_i8_row_launch_v<T, 1, NT, EPI>(a, x, st);
+    if (vecs <= 4u * 64u * kRowWaves) return vx_i8_row_launch_v<T, 4, NT, EPI>(a, x, st);
+    return vx_i8_row_launch_v<T, 8, NT, EPI>(a, x, st);
+}
+template <int NT, int EPI>
+hipError_t vx_i8_row_launch_t(const VxI8Args& a, const VxI8View& x, hipStream_t st) {
+    if (x.dtype == VELOX_DT_F32) return vx_i8_row_launch<float, NT, EPI>(a, x, st);
+    if (x.dtype == VELOX_DT_F16) return vx_i8_row_launch<_Float16, NT, EPI>(a, x, st);
+    return vx_i8_row_launch<__bf16, NT, EPI>(a, x, st);
+}
+// Rows of whole 16-byte vectors.
+bool vx_whole_rows(const VxI8View& x, uint32_t k) {
+    const uint32_t v = x.dtype == VELOX_DT_F32 ? 4u : 8u;
+    return ((uintptr_t)x.data & 15u) == 0 && x.rs % v == 0 && k % v == 0;
 }
 
 // ---- products of many rows: tiles through LDS ----
@@ -559,14 +778,11 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
                     if constexpr (kSwiglu) {
                         const uint32_t c = 4u * (lane % LANES), b = c / 16u * 32u + c % 16u;
                         const v4i g = *(const v4i*)(at + b), u = *(const v4i*)(at + b + 16u);
-                        y[j] = make_float4(vx_swiglu((float)g[0] * w0.x * sr, (float)u[0] * w1.x * sr), vx_swiglu((float)g[1] * w0.y * sr, (float)u[1] * w1.y * sr),
-                                           vx_swiglu((float)g[2] * w0.z * sr, (float)u[2] * w1.z * sr), vx_swiglu((float)g[3] * w0.w * sr, (float)u[3] * w1.w * sr));
+                        y[j] = vx_swiglu(g, w0, u, w1, sr);
                     } else {
                         const v4i c = *(const v4i*)(at + 4u * (lane % LANES));
-                        y[j] = make_float4((float)c[0] * w0.x * sr, (float)c[1] * w0.y * sr, (float)c[2] * w0.z * sr, (float)c[3] * w0.w * sr);
-                        if constexpr (EPI == VX_I8_STORE) {
-                            if (a.bias) y[j] = make_float4(y[j].x + w1.x, y[j].y + w1.y, y[j].z + w1.z, y[j].w + w1.w);
-                        }
+                        if (EPI == VX_I8_STORE && a.bias) y[j] = vx_scaled<true>(c, w0, sr, w1);
+                        else y[j] = vx_scaled<false>(c, w0, sr, w1);
                     }
                 }
 #pragma unroll
@@ -629,15 +845,9 @@ hipError_t vx_launch_i8_pack(const VxI8Mat& m, uint32_t first, uint32_t number, 
 
 hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& out, const uint32_t* limit,
                                  hipStream_t st) {
-    const uint32_t elt = x.dtype == VELOX_DT_F32 ? 4u : 2u;
-    if (((uintptr_t)x.data & 15u) == 0 && x.rs * elt % 16u == 0 && vx_i8_pad(k) * elt <= 1024u * 16u * 16u) {
-        if (x.dtype == VELOX_DT_F32) return vx_quantize_launch<float>(x, n_rows, k, out, limit, st);
-        if (x.dtype == VELOX_DT_F16) return vx_quantize_launch<_Float16>(x, n_rows, k, out, limit, st);
-        return vx_quantize_launch<__bf16>(x, n_rows, k, out, limit, st);
-    }
-    if (limit) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(vx_i8_quantize_any_kernel, dim3(n_rows), dim3(256), 0, st, x, k, out);
-    return hipGetLastError();
+    if (x.dtype == VELOX_DT_F32) return vx_quantize_launch<float>(x, n_rows, k, out, limit, st);
+    if (x.dtype == VELOX_DT_F16) return vx_quantize_launch<_Float16>(x, n_rows, k, out, limit, st);
+    return vx_quantize_launch<__bf16>(x, n_rows, k, out, limit, st);
 }
 
 // Positions of a block of a grouped product: tiles of 128 once an expert has 32 on average (4096 rows of 8 in 256 experts, 64 of
@@ -672,4 +882,28 @@ hipError_t vx_launch_i8_product(const VxI8Args& a, int epi, hipStream_t st) {
         case VX_I8_SLOT: return vx_i8_choose<VX_I8_SLOT>(a, st);
         default: return hipErrorInvalidValue;
     }
+}
+
+// One or two rows that stay in the workgroup's registers (4096 x 4096 fp32: one row 7.6 -> 6.2 us, two 8.4 and 8.4 but a launch less
+// for the host, four 9.0 -> 12.0; 29568 values, which do not: 44.5 -> 54).
+bool vx_i8_by_row(const VxI8View& x, uint32_t n_rows, uint32_t k) {
+    return n_rows <= 2u && vx_whole_rows(x, k) && k * (x.dtype == VELOX_DT_F32 ? 4u : 2u) <= 8u * 16u * 64u * kRowWaves;
+}
+hipError_t vx_launch_i8_row(const VxI8Args& a, const VxI8View& x, int epi, hipStream_t st) {
+    if (epi == VX_I8_SWIGLU) return vx_i8_row_launch_t<2, VX_I8_SWIGLU>(a, x, st);
+    return vx_i8_row_launch_t<1, VX_I8_STORE>(a, x, st);
+}
+
+// Up to four rows whose hidden rows stay in a wave's registers (6 of 64 experts of 2048 x 1408: one row 26.6 -> 18.5 us, four
+// 40.7 -> 37.2, eight 47 -> 67; hidden rows of 14336, four rows: 121 -> 371).
+bool vx_i8_ffn_by_slot(const VxI8View& x, uint32_t n_rows, uint32_t hidden, uint32_t inner) {
+    return n_rows <= 4u && vx_whole_rows(x, hidden) && inner <= kAnswerMost;
+}
+hipError_t vx_launch_i8_slots(const VxI8Args& a, const VxI8View& x, hipStream_t st) { return vx_i8_row_launch_t<2, VX_I8_HIDDEN>(a, x, st); }
+hipError_t vx_launch_i8_answers(const VxI8Args& a, const VxCombineArgs& c, hipStream_t st) {
+    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_answer_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 1 << 17);
+    if (set != hipSuccess) return set;
+    const uint32_t n_blocks = a.w.n_tiles;
+    hipLaunchKernelGGL(vx_i8_answer_kernel, dim3(c.n_rows * n_blocks), dim3(64 * kAnswerWaves), vx_i8_pad(a.w.k) * kAnswerWaves, st, a, c, n_blocks);
+    return hipGetLastError();
 }

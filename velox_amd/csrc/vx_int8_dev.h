@@ -5,6 +5,8 @@
 
 namespace {
 
+typedef int v4i __attribute__((ext_vector_type(4)));
+
 __device__ __forceinline__ float vx_load(const void* p, size_t i, uint32_t dtype) {
     if (dtype == VELOX_DT_F32) return ((const float*)p)[i];
     if (dtype == VELOX_DT_F16) return (float)((const _Float16*)p)[i];

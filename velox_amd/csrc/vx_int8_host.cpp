@@ -155,22 +155,24 @@ int velox_hip_int8_product(const VeloxHipInt8Matrix* m, const VeloxHipRows* x, c
     std::memset(&a, 0, sizeof(a));
     a.w = view(m);
     a.n_rows = n_rows;
-    if (x) {
-        Space s(workspace);
-        a.a.rs = vx_i8_pad(m->k);
-        a.a.codes = s.take<int8_t>(n_rows * a.a.rs);
-        a.a.scales = s.take<float>(n_rows);
-        if (!workspace || !aligned(workspace, 16) || workspace_bytes < s.used) return VELOX_HIP_EINVAL;
-        const hipError_t e = vx_launch_i8_quantize(view(x), n_rows, m->k, a.a, nullptr, st);
-        if (e != hipSuccess) return (int)e;
-    } else {
-        a.a = VxI8Rows{q->codes, q->scales, q->row_stride};
-    }
     a.bias = d_bias;
     if (residual) a.res = view(residual);
     a.out = view(out);
     a.vec = whole(out) && (!residual || whole(residual));
-    return (int)vx_launch_i8_product(a, m->paired ? VX_I8_SWIGLU : VX_I8_STORE, st);
+    const int epi = m->paired ? VX_I8_SWIGLU : VX_I8_STORE;
+    if (!x) {
+        a.a = VxI8Rows{q->codes, q->scales, q->row_stride};
+        return (int)vx_launch_i8_product(a, epi, st);
+    }
+    Space s(workspace);
+    a.a.rs = vx_i8_pad(m->k);
+    a.a.codes = s.take<int8_t>(n_rows * a.a.rs);
+    a.a.scales = s.take<float>(n_rows);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < s.used) return VELOX_HIP_EINVAL;
+    if (x->data != out->data && vx_i8_by_row(view(x), n_rows, m->k)) return  // (every workgroup reads x)
+            (int)vx_launch_i8_row(a, view(x), epi, st);
+    const hipError_t e = vx_launch_i8_quantize(view(x), n_rows, m->k, a.a, nullptr, st);
+    return e != hipSuccess ? (int)e : (int)vx_launch_i8_product(a, epi, st);
 }
 
 int velox_hip_expert_route(const VeloxHipRouteConfig* cfg, const VeloxHipRows* logits, const float* d_bias, uint32_t n_rows,
@@ -242,37 +244,13 @@ int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Ma
     const FfnSpace f = ffn_space(gu, dn, n_rows, top_k, workspace);
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < f.bytes) return VELOX_HIP_EINVAL;
     const uint32_t slots = n_rows * top_k;
-    VxGroupArgs g;
-    g.ids = d_ids;
-    g.n_slots = slots;
-    g.first = first;
-    g.count = gu.count;
-    g.order = f.order;
-    g.offsets = f.offsets;
-    g.hist = f.hist;
-    g.items = f.items;
-    g.n_items = f.n_items;
-    g.item_rows = vx_i8_item_rows(slots, gu.count);
-    hipError_t e = vx_launch_group(g, st);
-    if (e == hipSuccess) e = vx_launch_i8_quantize(view(x), n_rows, gu.k, f.x, nullptr, st);
     VxI8Args a;
     std::memset(&a, 0, sizeof(a));
     a.w = gu;
-    a.a = f.x;
-    a.g = VxGrouped{f.order, f.offsets, f.items, f.n_items};
+    a.n_rows = n_rows;
     a.top = top_k;
-    a.max_items = max_items(slots, gu.count, g.item_rows);
-    a.item_rows = g.item_rows;
     a.part = f.hidden;
     a.part_stride = f.hidden_stride;
-    if (e == hipSuccess) e = vx_launch_i8_product(a, VX_I8_HIDDEN, st);
-    if (e == hipSuccess)
-        e = vx_launch_i8_quantize(VxI8View{f.hidden, f.hidden_stride, VELOX_DT_F32}, slots, dn.k, f.h, f.offsets + gu.count, st);
-    a.w = dn;
-    a.a = f.h;
-    a.part = f.part;
-    a.part_stride = f.part_stride;
-    if (e == hipSuccess) e = vx_launch_i8_product(a, VX_I8_SLOT, st);
     VxCombineArgs c;
     std::memset(&c, 0, sizeof(c));
     c.ids = d_ids;
@@ -287,6 +265,39 @@ int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Ma
     if (residual) c.res = view(residual);
     c.out = view(out);
     c.vec = whole(out) && (!residual || whole(residual));
+    if (vx_i8_ffn_by_slot(view(x), n_rows, gu.k, dn.k)) {
+        a.ids = d_ids;
+        a.first = first;
+        hipError_t e = vx_launch_i8_slots(a, view(x), st);
+        a.w = dn;
+        if (e == hipSuccess) e = vx_launch_i8_answers(a, c, st);
+        return (int)e;
+    }
+    VxGroupArgs g;
+    g.ids = d_ids;
+    g.n_slots = slots;
+    g.first = first;
+    g.count = gu.count;
+    g.order = f.order;
+    g.offsets = f.offsets;
+    g.hist = f.hist;
+    g.items = f.items;
+    g.n_items = f.n_items;
+    g.item_rows = vx_i8_item_rows(slots, gu.count);
+    hipError_t e = vx_launch_group(g, st);
+    if (e == hipSuccess) e = vx_launch_i8_quantize(view(x), n_rows, gu.k, f.x, nullptr, st);
+    a.a = f.x;
+    a.g = VxGrouped{f.order, f.offsets, f.items, f.n_items};
+    a.max_items = max_items(slots, gu.count, g.item_rows);
+    a.item_rows = g.item_rows;
+    if (e == hipSuccess) e = vx_launch_i8_product(a, VX_I8_HIDDEN, st);
+    if (e == hipSuccess)
+        e = vx_launch_i8_quantize(VxI8View{f.hidden, f.hidden_stride, VELOX_DT_F32}, slots, (dn.k + 3u) & ~3u, f.h, f.offsets + gu.count, st);
+    a.w = dn;
+    a.a = f.h;
+    a.part = f.part;
+    a.part_stride = f.part_stride;
+    if (e == hipSuccess) e = vx_launch_i8_product(a, VX_I8_SLOT, st);
     if (e == hipSuccess) e = vx_launch_combine(c, st);
     return (int)e;
 }
