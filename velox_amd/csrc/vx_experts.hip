@@ -300,40 +300,41 @@ __global__ __launch_bounds__(kGroupThreads) void vx_group_count_kernel(VxGroupAr
         a.hist[(size_t)blockIdx.x * a.count + e] = n;
     }
 }
-// Exclusive sums of u and v (the latter below 2^32) over the workgroup's threads, and the totals; room: 2 kGroupWaves words.
-__device__ __forceinline__ uint2 vx_scan(uint2 v, uint32_t* room, uint2& total) {
+// Exclusive sums of v over the workgroup's threads, the total in `total`; room: kGroupWaves words.
+__device__ __forceinline__ uint32_t vx_scan(uint32_t v, uint32_t* room, uint32_t& total) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint2 s = v;
+    uint32_t s = v;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t x = __shfl_up(s.x, off), y = __shfl_up(s.y, off);
-        if (lane >= (uint32_t)off) {
-            s.x += x;
-            s.y += y;
-        }
+        const uint32_t o = __shfl_up(s, off);
+        if (lane >= (uint32_t)off) s += o;
     }
-    if (lane == 63u) {
-        room[2u * wave] = s.x;
-        room[2u * wave + 1u] = s.y;
-    }
+    if (lane == 63u) room[wave] = s;
     __syncthreads();
-    uint2 before = make_uint2(0, 0);
-    total = before;
+    uint32_t before = 0;
+    total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kGroupWaves; ++w) {
-        if (w < wave) before = make_uint2(before.x + room[2u * w], before.y + room[2u * w + 1u]);
-        total = make_uint2(total.x + room[2u * w], total.y + room[2u * w + 1u]);
+        if (w < wave) before += room[w];
+        total += room[w];
     }
-    return make_uint2(before.x + s.x - v.x, before.y + s.y - v.y);
+    return before + s - v;
+}
+// Experts by size, in steps of 32 slots: their blocks of a grouped product are listed from the largest class down, so that the
+// last workgroups of a launch are short ones (the order within a class is any: blocks do not depend on each other).
+__device__ __forceinline__ uint32_t vx_size_class(uint32_t slots) {
+    const uint32_t c = (slots + 31u) / 32u;
+    return c < 63u ? c : 63u;
 }
 // PER: experts of a thread, neighbours.
 template <uint32_t PER>
 __global__ __launch_bounds__(kGroupThreads) void vx_group_place_kernel(VxGroupArgs a) {
     __shared__ uint32_t tally[kGroupWaves * (kVxI8MaxCount + 1u)];
-    __shared__ uint32_t room[2u * kGroupWaves];
+    __shared__ uint32_t room[kGroupWaves], sizes[64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n = a.count + 1u, block = blockIdx.x, blocks = gridDim.x;
     const uint32_t run = block * kGroupSlots + wave * kGroupRun;
     const VxKeys k = vx_keys(a, run);
+    if (threadIdx.x < 64u) sizes[threadIdx.x] = 0;
     uint32_t mine[PER], front[PER];
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(kGroupThreads) void vx_group_place_kernel(VxGroupAr
         }
     }
     vx_tally(a, k, tally);
-    uint2 sum = make_uint2(0, 0);  // slots and blocks of a grouped product
+    uint32_t sum = 0;
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
         const uint32_t e = threadIdx.x * PER + j;
@@ -357,20 +358,41 @@ __global__ __launch_bounds__(kGroupThreads) void vx_group_place_kernel(VxGroupAr
 #pragma unroll
             for (uint32_t w = 0; w < kGroupWaves; ++w) mine[j] += tally[w * n + e];
         }
-        sum.x += mine[j];
-        sum.y += (mine[j] + a.item_rows - 1u) / a.item_rows;
+        sum += mine[j];
     }
-    uint2 total, at = vx_scan(sum, room, total);
+    uint32_t total, at = vx_scan(sum, room, total);
+    const bool items = a.items && block == 0;
+    uint32_t rank[PER];
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) {
+        const uint32_t e = threadIdx.x * PER + j, c = (mine[j] + a.item_rows - 1u) / a.item_rows;
+        rank[j] = items && e < a.count && c ? atomicAdd(&sizes[vx_size_class(mine[j])], c) : 0u;
+    }
+    if (items) {  // (the workgroup)
+        __syncthreads();
+        if (wave == 0) {  // lane l: the items of larger classes than l's
+            const uint32_t c = sizes[63u - lane];
+            uint32_t s = c;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t o = __shfl_up(s, off);
+                if (lane >= (uint32_t)off) s += o;
+            }
+            sizes[63u - lane] = s - c;
+            if (lane == 63u) *a.n_items = s;
+        }
+        __syncthreads();
+    }
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
         const uint32_t e = threadIdx.x * PER + j;
         if (e < a.count) {
-            if (block == 0) {
-                a.offsets[e] = at.x;
-                if (a.items)
-                    for (uint32_t p = 0; p < mine[j]; p += a.item_rows) a.items[at.y++] = make_uint2(e, at.x + p);
+            if (block == 0) a.offsets[e] = at;
+            if (items && mine[j]) {
+                uint2* to = a.items + sizes[vx_size_class(mine[j])] + rank[j];
+                for (uint32_t p = 0; p < mine[j]; p += a.item_rows) *to++ = make_uint2(e, at + p);
             }
-            uint32_t place = at.x + front[j];  // each wave's first place of the expert
+            uint32_t place = at + front[j];  // each wave's first place of the expert
 #pragma unroll
             for (uint32_t w = 0; w < kGroupWaves; ++w) {
                 const uint32_t c = tally[w * n + e];
@@ -378,12 +400,9 @@ __global__ __launch_bounds__(kGroupThreads) void vx_group_place_kernel(VxGroupAr
                 place += c;
             }
         }
-        at.x += mine[j];
+        at += mine[j];
     }
-    if (block == 0 && threadIdx.x == 0) {
-        a.offsets[a.count] = total.x;
-        if (a.items) *a.n_items = total.y;
-    }
+    if (block == 0 && threadIdx.x == 0) a.offsets[a.count] = total;
     __syncthreads();
     uint32_t* places = tally + wave * n;
 #pragma unroll
@@ -399,7 +418,7 @@ __global__ __launch_bounds__(kGroupThreads) void vx_group_place_kernel(VxGroupAr
         }
         vx_wave_sync();
     }
-    for (uint32_t p = total.x + block * kGroupThreads + threadIdx.x; p < a.n_slots; p += blocks * kGroupThreads) a.order[p] = kVxNoExpert;
+    for (uint32_t p = total + block * kGroupThreads + threadIdx.x; p < a.n_slots; p += blocks * kGroupThreads) a.order[p] = kVxNoExpert;
 }
 
 // ---- the sum of a row's experts ----

@@ -544,15 +544,16 @@ bool vx_whole_rows(const VxI8View& x, uint32_t k) {
 // v_mfma_i32_32x32x32_i8 (D[n = 8 (i / 4) + 4 (lane / 32) + i % 4][row = lane % 32]). 128 columns of both go straight to LDS at
 // a time, two stages; a column quarter's operands are read while the one before is multiplied, and the barrier between
 // two stages stands in front of the last quarter's products, behind which everything of the stage is in registers.
-// Weights lie in LDS as in memory (1 KiB tiles, operand reads of 256 neighbouring bytes); of an activation row's eight
-// 16-byte units, unit u lies at u ^ (row % 8), so that eight rows' reads of one unit meet all banks.
+// Weights lie in LDS as in memory (1 KiB tiles, operand reads of 256 neighbouring bytes); an activation row's 16-byte units
+// are exchanged by row, so that sixteen rows' reads of one unit meet all 64 banks.
 typedef int v16i __attribute__((ext_vector_type(16)));
 
-// 16 bytes a lane from memory to lds + 16 lane.
-__device__ __forceinline__ void vx_to_lds(uint32_t lds, const void* from, uint32_t off) {
+// 16 bytes a lane from memory to lds + 16 lane; once: with the non-temporal hint.
+__device__ __forceinline__ void vx_to_lds(uint32_t lds, const void* from, uint32_t off, bool once) {
     const uint64_t v = (uint64_t)(uintptr_t)from;  // (a scalar operand, wherever the compiler formed it)
     const uint64_t base = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
+    if (once) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
 }
 __device__ __forceinline__ void vx_to_lds(uint32_t lds, const void* from) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "m0", "memory");
@@ -564,38 +565,22 @@ __device__ __forceinline__ uint32_t vx_xcd_run(uint32_t b, uint32_t total) {
     return x * q + (x < r ? x : r) + i;
 }
 
-template <int WN, int WM, int FN, int FM, int S, int EPI>
-__global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, uint32_t row0, uint32_t n_blocks, uint32_t m_blocks) {
-    constexpr int W = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, STAGE = (TN + TM) * 128;
+template <int WN, int WM, int FN, int FM, int S, int KQ, int EPI>
+__device__ __forceinline__ void vx_i8_tile(const VxI8Args& a, uint8_t* lds, uint32_t nb, uint32_t e, uint32_t first, uint32_t end, bool once) {
+    constexpr int W = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, RB = 32 * KQ, STAGE = (TN + TM) * RB;  // RB: bytes of a row
     constexpr bool kGrouped = EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };  // (quotients are formed in vector registers)
-    uint32_t nb, e = 0, first, end = a.n_rows;
-    if constexpr (kGrouped) {
-        const uint32_t total = uniform(*a.g.n_items) * n_blocks;
-        if (blockIdx.x >= total) return;
-        const uint32_t id = vx_xcd_run(blockIdx.x, total);
-        const uint2 it = a.g.items[id / n_blocks];
-        nb = uniform(id % n_blocks);
-        e = uniform(it.x);
-        first = uniform(it.y);
-        end = uniform(a.g.offsets[e + 1u]);
-    } else {
-        // patches of up to 4 row blocks by all weight blocks, the rows first
-        const uint32_t id = vx_xcd_run(blockIdx.x, n_blocks * m_blocks), patch = id / (4u * n_blocks);
-        const uint32_t high = m_blocks - 4u * patch < 4u ? m_blocks - 4u * patch : 4u, in = id - patch * 4u * n_blocks;
-        nb = uniform(in / high);
-        first = uniform(row0 + (4u * patch + in % high) * TM);
-    }
     const uint32_t wn = wave / WM, wm = wave % WM;
-    const uint32_t steps = a.w.k_tiles / 2u, tile0 = nb * (TN / 16);
+    const uint32_t steps = a.w.k_tiles * 2u / KQ, tile0 = nb * (TN / 16);
 
-    // where this wave's share of a stage comes from: weight tiles (two pieces of 1 KiB each), groups of 8 rows
-    constexpr int PW = TN / 16 / W, PA = TM / 8 / W;
+    // where this wave's share of a stage comes from: weight tiles (KQ / 2 pieces of 1 KiB each), pieces of 1024 / RB rows (where
+    // they do not come out even, the last piece comes more than once)
+    constexpr int PW = TN / 16 / W, APIECES = TM * RB / 1024, PA = (APIECES + W - 1) / W, UNITS = RB / 16, AROWS = 64 / UNITS;
+    const auto swizzle = [](uint32_t row) { return KQ == 4 ? row >> 1 & 7u : row >> 2 & 3u; };
     const uint8_t* pw[PW];
     const uint8_t* pa[PA];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    const auto piece = [&](int j) { return APIECES % W == 0 || wave * PA + j < APIECES ? wave * PA + j : (uint32_t)APIECES - 1u; };
 #pragma unroll
     for (int j = 0; j < PW; ++j) {
         const uint32_t t = tile0 + wave * PW + j;
@@ -603,30 +588,29 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
     }
 #pragma unroll
     for (int j = 0; j < PA; ++j) {
-        const uint32_t p = first + (wave * PA + j) * 8u + (lane >> 3);
+        const uint32_t p = first + piece(j) * AROWS + lane / UNITS;
         uint32_t row = p < end ? p : end - 1u;
         if constexpr (EPI == VX_I8_HIDDEN) row = a.g.order[row] / a.top;
-        pa[j] = (const uint8_t*)a.a.codes + (uint64_t)row * a.a.rs + (((lane & 7u) ^ (lane >> 3)) * 16u);
+        pa[j] = (const uint8_t*)a.a.codes + (uint64_t)row * a.a.rs + ((lane % UNITS ^ swizzle(piece(j) * AROWS + lane / UNITS)) * 16u);
     }
     // piece j of this wave's share of a stage into LDS, its pointer moved on
     auto fetch = [&](auto j_, uint32_t stage) {
         constexpr int j = decltype(j_)::value;
         const uint32_t base = lds0 + stage * STAGE;
         if constexpr (j < PW) {
-            vx_to_lds(base + (wave * PW + j) * 2048u, pw[j], lane * 16u);
-            vx_to_lds(base + (wave * PW + j) * 2048u + 1024u, pw[j] + 1024, lane * 16u);
-            pw[j] += 2048;
+            vx_to_lds(base + (wave * PW + j) * (16u * RB), pw[j], lane * 16u, once);
+            if constexpr (KQ == 4) vx_to_lds(base + (wave * PW + j) * (16u * RB) + 1024u, pw[j] + 1024, lane * 16u, once);
+            pw[j] += 16 * RB;
         } else {
-            vx_to_lds(base + TN * 128 + (wave * PA + j - PW) * 1024u, pa[j - PW]);
-            pa[j - PW] += 128;
+            vx_to_lds(base + TN * RB + piece(j - PW) * 1024u, pa[j - PW]);
+            pa[j - PW] += RB;
         }
     };
-    auto fetch_all = [&](uint32_t stage) { vx_each<PW + PA>([&](auto j) { fetch(j, stage); }); };
     // operands of column quarter s: the weights' by tile, the rows' by their unit's place
-    const uint32_t w_at = wn * FN * 4096u + ((lane >> 4) & 1u) * 2048u + (lane >> 5) * 256u + (lane & 15u) * 16u;
-    uint32_t a_at[4];
+    const uint32_t w_at = wn * FN * (32u * RB) + ((lane >> 4) & 1u) * (16u * RB) + (lane >> 5) * 256u + (lane & 15u) * 16u;
+    uint32_t a_at[KQ];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) a_at[s] = TN * 128u + (wm * FM * 32u + (lane & 31u)) * 128u + (((2u * s + (lane >> 5)) ^ (lane & 7u)) * 16u);
+    for (int s = 0; s < KQ; ++s) a_at[s] = TN * RB + (wm * FM * 32u + (lane & 31u)) * RB + (((2u * s + (lane >> 5)) ^ swizzle(lane & 31u)) * 16u);
     // what the epilogue needs: outputs 4 (lane % LANES) .. + 3 of the wave's, the rows lane % 32 of its blocks
     constexpr bool kSwiglu = EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN;
     constexpr int ROW = 32 * FN + 4, LANES = (kSwiglu ? 16 : 32) * FN / 4, AT_ONCE = 64 / LANES;
@@ -665,8 +649,8 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
     auto read = [&](auto s_, auto r_, uint32_t stage, auto to_) {
         constexpr int s = decltype(s_)::value, r = decltype(r_)::value, to = decltype(to_)::value;
         const uint8_t* base = lds + stage * STAGE;
-        if constexpr (r >= 1 && r <= FM) fa[to][r - 1] = *(const v4i*)(base + a_at[s] + (r - 1) * 4096);
-        else fw[to][r ? r - FM : 0] = *(const v4i*)(base + w_at + (r ? r - FM : 0) * 4096 + (s >> 1) * 1024 + (s & 1) * 512);
+        if constexpr (r >= 1 && r <= FM) fa[to][r - 1] = *(const v4i*)(base + a_at[s] + (r - 1) * (32 * RB));
+        else fw[to][r ? r - FM : 0] = *(const v4i*)(base + w_at + (r ? r - FM : 0) * (32 * RB) + (s >> 1) * 1024 + (s & 1) * 512);
     };
     // The products of the operands in set `from`; between them the next quarter's reads and (LO <= j < HI) the pieces of a
     // stage's fetch. The order is fixed: left to itself the compiler puts the reads together and waits for them.
@@ -688,7 +672,7 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    constexpr int PIECES = 2 * PW + PA, HALF = (PW + PA) / 2;  // loads of a wave's share of a stage
+    constexpr int PIECES = KQ / 2 * PW + PA, HALF = (PW + PA) / 2;  // loads of a wave's share of a stage
     auto ready = [&](auto left_) {  // this wave's loads but the last `left` are in LDS, its reads in registers; then everybody's are
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(left_)::value) : "memory");
     };
@@ -698,16 +682,19 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
     // this step's last quarter (NEXT), half in the next one's first (REST).
     auto step = [&](auto rest_, auto next_) {
         constexpr bool REST = decltype(rest_)::value != 0, NEXT = decltype(next_)::value != 0;
-        quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<HALF>{}, vx_int<(REST ? PW + PA : HALF)>{}, behind(S - 1));
-        quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
-        quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+        constexpr int ALL = REST ? PW + PA : HALF;
+        quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<HALF>{}, vx_int<ALL>{}, behind(S - 1));
+        if constexpr (KQ == 4) {
+            quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+            quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+        }
         ready(vx_int<(REST ? (S - 2) * PIECES : 0)>{});
         quarter(vx_int<1>{}, vx_int<0>{}, behind(1), vx_int<0>{}, vx_int<(NEXT ? HALF : 0)>{}, st);
         st = behind(1);
     };
 #pragma unroll
     for (int j = 0; j < S - 1; ++j)
-        if ((uint32_t)j < steps) vx_each<PW + PA>([&](auto piece) { fetch(piece, j); });
+        if ((uint32_t)j < steps) vx_each<PW + PA>([&](auto p) { fetch(p, j); });
     if (steps >= (uint32_t)S) ready(vx_int<(S - 2) * PIECES>{});
     else ready(vx_int<0>{});
     vx_each<FN + FM>([&](auto r) { read(vx_int<0>{}, r, 0, vx_int<0>{}); });
@@ -722,8 +709,10 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
     }
     for (; i + 1u < steps; ++i) step(vx_int<0>{}, vx_int<0>{});
     quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
-    quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
-    quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+    if constexpr (KQ == 4) {
+        quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+        quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+    }
     quarter(vx_int<1>{}, vx_int<-1>{}, 0, vx_int<0>{}, vx_int<0>{}, 0);
 
     // Epilogue, one block of 32 rows at a time: the sums go through LDS, where the lane of row lane % 32 writes those of n =
@@ -812,25 +801,68 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
     }
 }
 
+// Plain products: patches of up to 4 row blocks by all weight blocks on an XCD, the rows first.
+template <int WN, int WM, int FN, int FM, int S, int KQ, int EPI>
+__global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, uint32_t row0, uint32_t n_blocks, uint32_t m_blocks) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };  // (quotients are formed in vector registers)
+    const uint32_t id = vx_xcd_run(blockIdx.x, n_blocks * m_blocks), patch = id / (4u * n_blocks);
+    const uint32_t high = m_blocks - 4u * patch < 4u ? m_blocks - 4u * patch : 4u, in = id - patch * 4u * n_blocks;
+    vx_i8_tile<WN, WM, FN, FM, S, KQ, EPI>(a, lds, uniform(in / high), 0, uniform(row0 + (4u * patch + in % high) * 32u * WM * FM), a.n_rows, false);
+}
+
+// Grouped products: blocks of up to 256 of an expert's positions by 256 weight rows, eight waves of 64 weight rows by half of the
+// positions. As many blocks of 64 positions are fetched and multiplied as there are (by tiles of 128, padded, 4096 rows of 8 experts,
+// 64 of 256 here, took 978 us, so 840), and the fewer they are, the more stages LDS holds. An expert whose weights one block
+// reads passes the caches by (512 rows: 506 -> 470 us). What bounds it there: the weights' way to LDS (without the products 783 us,
+// without any loads 517).
+constexpr uint32_t kItemRows = 256u;
+template <int L>
+struct VxLive {
+    static constexpr int stages = L == 1 ? 4 : L == 2 ? 3 : 2;
+    static constexpr uint32_t lds = stages * (256 + 64 * L) * 128;
+};
+template <int EPI>
+__global__ __launch_bounds__(512) void vx_i8_items_kernel(VxI8Args a, uint32_t n_blocks) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+    if (blockIdx.x >= uniform(*a.g.n_items) * n_blocks) return;
+    const uint32_t nb = uniform(blockIdx.x % n_blocks);  // (an item's blocks over all XCDs: items are of unequal length)
+    const uint2 it = a.g.items[blockIdx.x / n_blocks];
+    const uint32_t e = uniform(it.x), first = uniform(it.y), end = uniform(a.g.offsets[e + 1u]);
+    const uint32_t live = end - first < kItemRows ? (end - first + 63u) / 64u : kItemRows / 64u;
+    const bool once = end - first <= kItemRows && first == uniform(a.g.offsets[e]);
+    vx_each<4>([&](auto l_) {
+        constexpr int L = decltype(l_)::value + 1;
+        if (live == L) vx_i8_tile<4, 2, 2, L, VxLive<L>::stages, 4, EPI>(a, lds, nb, e, first, end, once);
+    });
+}
+
 constexpr uint32_t kTileStep = 1u << 20;  // rows of a launch
 
-template <int WN, int WM, int FN, int FM, int S, int EPI>
+template <int WN, int WM, int FN, int FM, int S, int KQ, int EPI>
 hipError_t vx_i8_tile_launch(const VxI8Args& a, hipStream_t st) {
-    constexpr uint32_t TN = 32 * WN * FN, TM = 32 * WM * FM, lds = S * (TN + TM) * 128;
-    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_tile_kernel<WN, WM, FN, FM, S, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    constexpr uint32_t TN = 32 * WN * FN, TM = 32 * WM * FM, lds = S * (TN + TM) * 32 * KQ;
+    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_tile_kernel<WN, WM, FN, FM, S, KQ, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (set != hipSuccess) return set;
     const uint32_t n_blocks = (a.w.n_tiles * 16u + TN - 1u) / TN;
-    if (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) {
-        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, S, EPI>), dim3(a.max_items * n_blocks), dim3(64 * WN * WM), lds, st, a, 0u, n_blocks, 0u);
-        return hipGetLastError();
-    }
     for (uint32_t r = 0; r < a.n_rows; r += kTileStep) {
         const uint32_t rows = a.n_rows - r < kTileStep ? a.n_rows - r : kTileStep, m_blocks = (rows + TM - 1u) / TM;
-        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, S, EPI>), dim3(n_blocks * m_blocks), dim3(64 * WN * WM), lds, st, a, r, n_blocks, m_blocks);
+        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, S, KQ, EPI>), dim3(n_blocks * m_blocks), dim3(64 * WN * WM), lds, st, a, r, n_blocks, m_blocks);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
     return hipSuccess;
+}
+template <int EPI>
+hipError_t vx_i8_items_launch(const VxI8Args& a, hipStream_t st) {
+    constexpr uint32_t lds = VxLive<1>::lds;
+    static_assert(lds <= 160 * 1024 && VxLive<3>::lds <= VxLive<1>::lds && VxLive<2>::lds <= VxLive<1>::lds && VxLive<4>::lds <= VxLive<1>::lds, "a CU's LDS");
+    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_items_kernel<EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (set != hipSuccess) return set;
+    const uint32_t n_blocks = (a.w.n_tiles + 15u) / 16u;
+    hipLaunchKernelGGL((vx_i8_items_kernel<EPI>), dim3(a.max_items * n_blocks), dim3(512), lds, st, a, n_blocks);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -850,29 +882,32 @@ hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k,
     return vx_quantize_launch<__bf16>(x, n_rows, k, out, limit, st);
 }
 
-// Positions of a block of a grouped product: tiles of 128 once an expert has 32 on average (4096 rows of 8 in 256 experts, 64 of
-// them here: 2590 us by 16 -> 1171 by 128; 32 rows: 288 -> 302).
-uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count) { return slots >= 32u * count ? 128u : 16u; }
+// Positions of a block of a grouped product, by how many slots there are for an expert (64 of 256 experts of 7168 x 2048 here, 8 for
+// a row): 32 rows 185 us by 16 and by 32, 128 rows 295 and 279, 256 rows 374 by 32 and 361 by tiles, 512 rows 607 and 470.
+uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count) { return slots >= 32u * count ? kItemRows : slots >= 12u * count ? 32u : 16u; }
 
 // Up to 16 rows the streaming kernel with one weight tile a workgroup (4096 x 4096, one row: two tiles 6.1 us, one 5.0) or,
-// where more rows share a tile of a large matrix, two (8192 x 8192, 16 rows: 16.1, 14.2); up to 32 rows two or four tiles and eight
-// waves (8192 x 8192: 15.3; 37888 x 3584 paired: two 35.7, four 32.1). From 33 rows on tiles through LDS: 128 x 32 in four stages (64 rows of
-// 8192 x 8192: 18.1, streaming 21.3), from 65 on 128 x 128 (300 rows 109 by 16 -> 43), its 256 x 256 form where those tiles come to two rounds of the CUs (8192 rows of 8192 x 8192: 554 -> 471 us, of 8192 x 29568:
-// 1893 -> 1553; 2048 rows of 4096 x 4096, half a round: 40 -> 54).
+// where more rows share a tile of a large matrix, two (8192 x 8192, 16 rows: 16.1, 14.2); up to 32 rows two tiles and eight
+// waves, or where six fill the CUs still, six and four (8192 x 8192: 15.3; 37888 x 3584 paired: 35.7 and 29.6). From 33 rows on tiles through LDS: 128 x 32 in four stages
+// (64 rows of 8192 x 8192: 18.1, streaming 21.3), from 65 on 128 x 128 (300 rows 109 by 16 -> 43), 256 x 256 by eight waves where
+// those tiles come to more than a round of the CUs (8192 rows of 8192 x 8192: 554 -> 443 us, of 8192 x 29568: 1893 -> 1480; 1024 rows
+// of 14336 x 4096, 224 tiles: 71 -> 58; 2048 rows of 4096 x 4096, half a round: 40 -> 47).
 template <int EPI>
 hipError_t vx_i8_choose(const VxI8Args& a, hipStream_t st) {
     if constexpr (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) {
-        if (a.item_rows == 128u) return vx_i8_tile_launch<2, 2, 2, 2, 2, EPI>(a, st);
-    } else if (a.n_rows > 64u) {
-        if ((uint64_t)((a.w.n_tiles + 15u) / 16u) * ((a.n_rows + 255u) / 256u) >= 512u) return vx_i8_tile_launch<2, 2, 4, 4, 2, EPI>(a, st);
-        return vx_i8_tile_launch<2, 2, 2, 2, 2, EPI>(a, st);
+        if (a.item_rows == kItemRows) return vx_i8_items_launch<EPI>(a, st);
+        return a.item_rows == 32u ? vx_i8_stream_launch<2, 2, 4, EPI>(a, st) : vx_i8_stream_launch<2, 1, 4, EPI>(a, st);
+    } else {
+        constexpr bool one = EPI == VX_I8_STORE;  // (the others take tiles by pairs)
+        if (a.n_rows > 64u) {
+            if ((uint64_t)((a.w.n_tiles + 15u) / 16u) * ((a.n_rows + 255u) / 256u) >= 192u) return vx_i8_tile_launch<4, 2, 2, 4, 2, 4, EPI>(a, st);
+            return vx_i8_tile_launch<2, 2, 2, 2, 2, 4, EPI>(a, st);
+        }
+        if (a.n_rows > 32u) return vx_i8_tile_launch<4, 1, 1, 1, 4, 4, EPI>(a, st);
+        if (a.n_rows > 16u) return a.w.n_tiles >= 1536u ? vx_i8_stream_launch<6, 2, 4, EPI>(a, st) : vx_i8_stream_launch<2, 2, 8, EPI>(a, st);
+        if (one && (a.n_rows <= 4u || a.w.n_tiles < 512u)) return vx_i8_stream_launch<one ? 1 : 2, 1, 4, EPI>(a, st);
+        return vx_i8_stream_launch<2, 1, 4, EPI>(a, st);
     }
-    constexpr bool one = EPI == VX_I8_STORE || EPI == VX_I8_SLOT;  // (the others take tiles by pairs)
-    if constexpr (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) return vx_i8_stream_launch<2, 1, 4, EPI>(a, st);
-    if (a.n_rows > 32u) return vx_i8_tile_launch<4, 1, 1, 1, 4, EPI>(a, st);
-    if (a.n_rows > 16u) return a.w.n_tiles >= 2048u ? vx_i8_stream_launch<4, 2, 8, EPI>(a, st) : vx_i8_stream_launch<2, 2, 8, EPI>(a, st);
-    if (one && (a.n_rows <= 4u || a.w.n_tiles < 512u)) return vx_i8_stream_launch<one ? 1 : 2, 1, 4, EPI>(a, st);
-    return vx_i8_stream_launch<2, 1, 4, EPI>(a, st);
 }
 hipError_t vx_launch_i8_product(const VxI8Args& a, int epi, hipStream_t st) {
     switch (epi) {

@@ -16,13 +16,14 @@ from . import _lib as L
 from .int8 import Int8Matrix, _floats, _memory, _plain
 from .paged import _call, _gpu, _need, _numbers, _space, _words
 
+_lib = L.load  # (the library is looked up by the calls, not where this module is read)
 _SCORES = {"softmax": L.ROUTE_SOFTMAX, "sigmoid": L.ROUTE_SIGMOID}
 _MARKS = {"max": L.GROUP_LARGEST, "two": L.GROUP_TWO}
 
 
 def _whole(t: torch.Tensor, shape: tuple, device: torch.device, what: str) -> int:
     """The address of a contiguous int32 tensor of a shape."""
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous int32 tensor of shape {shape} on {device} is wanted")
     return t.data_ptr()
 
@@ -34,21 +35,29 @@ def route(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", bias: to
     the top_groups best groups where there are several; weights are the scores (renormalize: divided by their sum) times
     scale. -infinity masks an expert; a row without enough experts ends in -1 with weight 0."""
     device = _gpu(logits, "logits")
-    _need(scores in _SCORES and group_by in _MARKS, f"scores is one of {tuple(_SCORES)}, group_by one of {tuple(_MARKS)}")
+    how, mark = _SCORES.get(scores), _MARKS.get(group_by)
+    if how is None or mark is None:
+        raise ValueError(f"scores is one of {tuple(_SCORES)}, group_by one of {tuple(_MARKS)}")
     xr, n = _plain(logits, device, "logits")
     experts = logits.shape[1]
-    _need(groups >= 1 and experts % groups == 0 and 1 <= top_groups <= groups and 1 <= experts <= 1024 and groups <= 64,
-          "1 to 1024 experts in up to 64 groups of one size are wanted, and 1 to `groups` of the groups")
-    _need(1 <= top_k <= min(64, experts // groups * top_groups), "top_k: 1 to 64, no more than there are experts in top_groups groups")
+    if not (1 <= groups <= 64 and 1 <= experts <= 1024 and experts % groups == 0 and 1 <= top_groups <= groups):
+        raise ValueError("1 to 1024 experts in up to 64 groups of one size are wanted, and 1 to `groups` of the groups")
+    if not 1 <= top_k <= min(64, experts // groups * top_groups):
+        raise ValueError("top_k: 1 to 64, no more than there are experts in top_groups groups")
     if ids is None:
-        ids = torch.empty(n, top_k, dtype=torch.int32, device=device)
+        ids = torch.empty((n, top_k), dtype=torch.int32, device=device)
+        i = ids.data_ptr()
+    else:
+        i = _whole(ids, (n, top_k), device, "ids")
     if weights is None:
-        weights = torch.empty(n, top_k, dtype=torch.float32, device=device)
-    i, w = _whole(ids, (n, top_k), device, "ids"), _floats(weights, (n, top_k), device, "weights")
+        weights = torch.empty((n, top_k), dtype=torch.float32, device=device)
+        w = weights.data_ptr()
+    else:
+        w = _floats(weights, (n, top_k), device, "weights")
     b = _floats(bias, (experts,), device, "bias") if bias is not None else None
     if n:
-        cfg = L.RouteConfig(experts, top_k, _SCORES[scores], groups, top_groups, _MARKS[group_by], bool(renormalize), scale)
-        _call(L.load().velox_hip_expert_route, device.index, cfg, xr, b, n, i, w)
+        cfg = L.RouteConfig(experts, top_k, how, groups, top_groups, mark, 1 if renormalize else 0, scale)
+        _call(_lib().velox_hip_expert_route, device.index, cfg, xr, b, n, i, w)
     return ids, weights
 
 
@@ -61,8 +70,8 @@ def group_workspace(slots: int, count: int, device="cuda") -> torch.Tensor | Non
     """What group() needs for up to `slots` slots of `count` experts (None: nothing)."""
     n = C.c_uint64()
     _numbers("slots and count", slots, count)
-    L.check(L.load().velox_hip_expert_group_bytes(slots, count, C.byref(n)), "expert_group_bytes")
-    return _memory(n.value, _device_index(device))
+    L.check(_lib().velox_hip_expert_group_bytes(slots, count, C.byref(n)), "expert_group_bytes")
+    return _memory(n.value, device if isinstance(device, torch.device) else _device_index(device)) if n.value else None
 
 
 def group(ids: torch.Tensor, count: int, first: int = 0, *, order: torch.Tensor | None = None, offsets: torch.Tensor | None = None,
@@ -71,18 +80,25 @@ def group(ids: torch.Tensor, count: int, first: int = 0, *, order: torch.Tensor 
     count - 1, an expert's in their own order at order[offsets[e] : offsets[e + 1]]; -1 behind the last."""
     device = _gpu(ids, "ids")
     slots = ids.numel()
-    _whole(ids, tuple(ids.shape), device, "ids")
-    _numbers("first and count", first, count)
-    _need(1 <= count <= 1024 and slots <= 1 << 20, "1 to 1024 experts and up to 2^20 slots are wanted")
+    at = _whole(ids, ids.shape, device, "ids")
+    if (first | count) >> 32:
+        _numbers("first and count", first, count)
+    if not 1 <= count <= 1024 or slots > 1 << 20:
+        raise ValueError("1 to 1024 experts and up to 2^20 slots are wanted")
     if order is None:
         order = torch.empty(slots, dtype=torch.int32, device=device)
+        o = order.data_ptr()
+    else:
+        o = _words(order, slots, device, "order")
     if offsets is None:
         offsets = torch.empty(count + 1, dtype=torch.int32, device=device)
-    o, f = _words(order, slots, device, "order"), _words(offsets, count + 1, device, "offsets")
+        f = offsets.data_ptr()
+    else:
+        f = _words(offsets, count + 1, device, "offsets")
     if workspace is None:
         workspace = group_workspace(slots, count, device)
     space, size = _space(workspace, device)
-    _call(L.load().velox_hip_expert_group, device.index, ids.data_ptr(), slots, first, count, o, f, space, size)
+    _call(_lib().velox_hip_expert_group, device.index, at, slots, first, count, o, f, space, size)
     return order, offsets
 
 
@@ -101,22 +117,22 @@ def ffn(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_up: Int8
     ids add nothing. out: a new tensor of x's type, or the one given (may be x or the residual). workspace: ffn_workspace
     (None: made here)."""
     device = gate_up.device
-    _need(gate_up.paired and not down.paired and down.device == device and gate_up.count == down.count and gate_up.n == 2 * down.k and
-          gate_up.k == down.n, "gate_up (paired) [2 inner][hidden] and down [hidden][inner] of as many experts are wanted")
+    if not (gate_up.paired and not down.paired and down.device == device and gate_up.count == down.count and gate_up.outputs == down.k and
+            gate_up.k == down.n):
+        raise ValueError("gate_up (paired) [2 inner][hidden] and down [hidden][inner] of as many experts are wanted")
     xr, n = _plain(x, device, "x", gate_up.k)
-    _need(isinstance(ids, torch.Tensor) and ids.dim() == 2 and ids.shape[0] == n and 1 <= ids.shape[1] <= 64, f"ids: [{n}][1 to 64] is wanted")
-    top = ids.shape[1]
-    _need(n * top <= 1 << 20, "up to 2^20 slots (rows times top_k) are wanted")
-    _numbers("first", first)
+    top = ids.shape[1] if isinstance(ids, torch.Tensor) and ids.dim() == 2 else 0
+    if not 1 <= top <= 64 or n * top > 1 << 20:
+        raise ValueError("ids: [row][1 to 64] is wanted, up to 2^20 slots in all")
+    if first >> 32:
+        _numbers("first", first)
     i, w = _whole(ids, (n, top), device, "ids"), _floats(weights, (n, top), device, "weights")
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    o, on = _plain(out, device, "out", gate_up.k)
-    _need(on == n, f"out: {n} rows are wanted")
-    res = None
-    if residual is not None:
-        res, rn = _plain(residual, device, "residual", gate_up.k)
-        _need(rn == n, f"residual: {n} rows are wanted")
+        out = torch.empty((n, gate_up.k), dtype=x.dtype, device=device)
+        o = L.Rows(out.data_ptr(), xr.dtype, 1, gate_up.k, 0)
+    else:
+        o, _ = _plain(out, device, "out", gate_up.k, n)
+    res = _plain(residual, device, "residual", gate_up.k, n)[0] if residual is not None else None
     if n == 0:
         return out
     if workspace is None:

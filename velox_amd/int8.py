@@ -16,7 +16,7 @@ from . import _lib as L
 from .paged import _DTYPES, _call, _gpu, _need, _no_gradient, _numbers, _space
 
 
-def _plain(t: torch.Tensor, device: torch.device, what: str, width: int = 0) -> tuple[L.Rows, int]:
+def _plain(t: torch.Tensor, device: torch.device, what: str, width: int = 0, rows: int = -1) -> tuple[L.Rows, int]:
     """[row][element] as VeloxHipRows, and its rows; the elements of a row are next to each other."""
     code = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
     if code is None or t.device != device or t.dim() != 2:
@@ -24,8 +24,8 @@ def _plain(t: torch.Tensor, device: torch.device, what: str, width: int = 0) -> 
     if t.requires_grad:
         _no_gradient(t, what)
     n, d = t.shape
-    if width and d != width:
-        raise ValueError(f"{what}: rows of {width} elements are wanted, got {d}")
+    if (width and d != width) or (rows >= 0 and n != rows):
+        raise ValueError(f"{what}: {rows if rows >= 0 else n} rows of {width or d} elements are wanted, got {n} of {d}")
     rs, es = t.stride()
     if es != 1 and d > 1:
         raise ValueError(f"{what}: a row's elements have to be next to each other")
@@ -34,7 +34,7 @@ def _plain(t: torch.Tensor, device: torch.device, what: str, width: int = 0) -> 
 
 def _floats(t: torch.Tensor, shape: tuple, device: torch.device, what: str) -> int:
     """The address of a contiguous float32 tensor of a shape."""
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous float32 tensor of shape {shape} on {device} is wanted")
     if t.requires_grad:
         _no_gradient(t, what)
@@ -73,6 +73,7 @@ class Int8Matrix:
             codes, scales = codes.unsqueeze(0), scales.unsqueeze(0)
         self.count, self.n, self.k = codes.shape
         self.paired, self.device = bool(paired), device
+        self.outputs = self.n // 2 if self.paired else self.n  # values of a product's row
         at = _floats(scales, (self.count, self.n), device, "scales")
         _numbers("codes", self.count, self.n, self.k)
         self.lib = L.load()
@@ -93,10 +94,6 @@ class Int8Matrix:
         rows = quantize(w.reshape(-1, w.shape[-1]))
         return cls(rows.codes.view(*w.shape[:-1], -1)[..., :w.shape[-1]], rows.scales.view(w.shape[:-1]), paired=paired)
 
-    @property
-    def outputs(self) -> int:
-        """Values of a product's row."""
-        return self.n // 2 if self.paired else self.n
 
 
 def quantize(x: torch.Tensor, out: Int8Rows | None = None) -> Int8Rows:
@@ -127,9 +124,10 @@ def product(x: torch.Tensor | Int8Rows, w: Int8Matrix, *, bias: torch.Tensor | N
     into 8 bits on the way (workspace: product_workspace, None: made here), or Int8Rows. out: a new tensor of `dtype`
     (default: x's type, float32 for Int8Rows), or the one given."""
     device = w.device
-    _need(w.count == 1, "w: one matrix is wanted (experts.ffn takes several)")
+    if w.count != 1:
+        raise ValueError("w: one matrix is wanted (experts.ffn takes several)")
     if isinstance(x, Int8Rows):
-        _need(x.k == w.k and x.codes.device == device, f"x: rows of {w.k} values on {device} are wanted")
+        _need(x.k == w.k and x.codes.device == device, "x: rows of the matrix's k values on its device are wanted")
         n, xr, xq, space, size, kind = len(x), None, x.desc, None, 0, torch.float32
     else:
         xr, n = _plain(x, device, "x", w.k)
@@ -137,19 +135,22 @@ def product(x: torch.Tensor | Int8Rows, w: Int8Matrix, *, bias: torch.Tensor | N
         if workspace is None and n:
             workspace = product_workspace(w, n)
         space, size = _space(workspace, device)
-    cols = w.n // 2 if w.paired else w.n
     if out is None:
-        out = torch.empty(n, cols, dtype=dtype or kind, device=device)
+        kind = dtype or kind
+        if kind not in _DTYPES:
+            raise ValueError("dtype: float32, float16 or bfloat16 is wanted")
+        cols = w.outputs
+        out = torch.empty((n, cols), dtype=kind, device=device)
+        o = L.Rows(out.data_ptr(), _DTYPES[kind], 1, cols, 0)
     else:
         _need(dtype is None or out.dtype == dtype, "out: another type than dtype")
-    o, on = _plain(out, device, "out", cols)
-    _need(on == n, f"out: {n} rows are wanted")
-    _need(not w.paired or (bias is None and residual is None), "a paired product takes no bias and no residual")
+        o, _ = _plain(out, device, "out", w.outputs, n)
+    if w.paired and (bias is not None or residual is not None):
+        raise ValueError("a paired product takes no bias and no residual")
     at = _floats(bias, (w.n,), device, "bias") if bias is not None else None
     res, mode = None, L.GEMV_SWIGLU if w.paired else L.GEMV_STORE
     if residual is not None:
-        res, rn = _plain(residual, device, "residual", cols)
-        _need(rn == n, f"residual: {n} rows are wanted")
+        res, _ = _plain(residual, device, "residual", w.n, n)
         mode = L.GEMV_RESIDUAL
     if n:
         _call(w.lib.velox_hip_int8_product, w._index, w._ref, xr, xq, n, at, res, o, mode, space, size)
