@@ -95,7 +95,7 @@ hipError_t vx_launch_i8_pack(const VxI8Mat& m, uint32_t first, uint32_t number, 
 hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& out, const uint32_t* limit,
                                  hipStream_t st);
 hipError_t vx_launch_i8_product(const VxI8Args& a, int epi, hipStream_t st);
-uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count);  // positions of a block of a grouped product
+uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count, uint32_t n_tiles);  // positions of a block of a grouped product
 // Few rows, quantized by the workgroups that multiply them: whether x's rows are; plain products, the hidden values of
 // every slot (a.part: [slot]), the experts' answers and their sum.
 bool vx_i8_by_row(const VxI8View& x, uint32_t n_rows, uint32_t k);

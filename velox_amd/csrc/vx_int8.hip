@@ -838,6 +838,18 @@ __global__ __launch_bounds__(512) void vx_i8_items_kernel(VxI8Args a, uint32_t n
     });
 }
 
+// The same by blocks of 64 positions and 64 weight rows, for experts so small that the larger blocks would leave most CUs idle.
+constexpr uint32_t kSmallItemRows = 64u;
+template <int EPI>
+__global__ __launch_bounds__(256) void vx_i8_small_items_kernel(VxI8Args a, uint32_t n_blocks) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+    if (blockIdx.x >= uniform(*a.g.n_items) * n_blocks) return;
+    const uint2 it = a.g.items[blockIdx.x / n_blocks];
+    const uint32_t e = uniform(it.x);
+    vx_i8_tile<2, 2, 1, 1, 4, 4, EPI>(a, lds, uniform(blockIdx.x % n_blocks), e, uniform(it.y), uniform(a.g.offsets[e + 1u]), false);
+}
+
 constexpr uint32_t kTileStep = 1u << 20;  // rows of a launch
 
 template <int WN, int WM, int FN, int FM, int S, int KQ, int EPI>
@@ -856,8 +868,13 @@ hipError_t vx_i8_tile_launch(const VxI8Args& a, hipStream_t st) {
 }
 template <int EPI>
 hipError_t vx_i8_items_launch(const VxI8Args& a, hipStream_t st) {
-    constexpr uint32_t lds = VxLive<1>::lds;
+    constexpr uint32_t lds = VxLive<1>::lds, small = 4 * (64 + 64) * 128;
     static_assert(lds <= 160 * 1024 && VxLive<3>::lds <= VxLive<1>::lds && VxLive<2>::lds <= VxLive<1>::lds && VxLive<4>::lds <= VxLive<1>::lds, "a CU's LDS");
+    if (a.item_rows == kSmallItemRows) {
+        const uint32_t n_blocks = (a.w.n_tiles + 3u) / 4u;
+        hipLaunchKernelGGL((vx_i8_small_items_kernel<EPI>), dim3(a.max_items * n_blocks), dim3(256), small, st, a, n_blocks);
+        return hipGetLastError();
+    }
     static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_items_kernel<EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (set != hipSuccess) return set;
     const uint32_t n_blocks = (a.w.n_tiles + 15u) / 16u;
@@ -883,25 +900,39 @@ hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k,
 }
 
 // Positions of a block of a grouped product, by how many slots there are for an expert (64 of 256 experts of 7168 x 2048 here, 8 for
-// a row): 32 rows 185 us by 16 and by 32, 128 rows 295 and 279, 256 rows 374 by 32 and 361 by tiles, 512 rows 607 and 470.
-uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count) { return slots >= 32u * count ? kItemRows : slots >= 12u * count ? 32u : 16u; }
+// a row): 32 rows 185 us by 16 and by 32, 128 rows 295 and 279, 256 rows 374 by 32 and 361 by tiles, 512 rows 607 and 470. Where
+// blocks of 256 would not even be one for each CU, 64 (257 rows through 5 experts of 576 x 1100).
+uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count, uint32_t n_tiles) {
+    if (slots < 32u * count) return slots >= 12u * count ? 32u : 16u;
+    return (uint64_t)(slots / kItemRows + count) * ((n_tiles + 15u) / 16u) < 256u ? kSmallItemRows : kItemRows;
+}
 
 // Up to 16 rows the streaming kernel with one weight tile a workgroup (4096 x 4096, one row: two tiles 6.1 us, one 5.0) or,
 // where more rows share a tile of a large matrix, two (8192 x 8192, 16 rows: 16.1, 14.2); up to 32 rows two tiles and eight
-// waves, or where six fill the CUs still, six and four (8192 x 8192: 15.3; 37888 x 3584 paired: 35.7 and 29.6). From 33 rows on tiles through LDS: 128 x 32 in four stages
-// (64 rows of 8192 x 8192: 18.1, streaming 21.3), from 65 on 128 x 128 (300 rows 109 by 16 -> 43), 256 x 256 by eight waves where
-// those tiles come to more than a round of the CUs (8192 rows of 8192 x 8192: 554 -> 443 us, of 8192 x 29568: 1893 -> 1480; 1024 rows
-// of 14336 x 4096, 224 tiles: 71 -> 58; 2048 rows of 4096 x 4096, half a round: 40 -> 47).
+// waves, or where six fill the CUs still, six and four (8192 x 8192: 15.3; 37888 x 3584 paired: 35.7 and 29.6). From 33 rows on tiles
+// through LDS, as large as leave the CUs work: 128 x 32 up to 64 rows (8192 x 8192: 18.1, streaming 21.3), then
+//   64 x 64 (four stages) up to 100 tiles of 128 x 128 (1037 rows of 960 x 576: 8.3 -> 4.9 us, 200 of 4096 x 14336: 67 -> 29),
+//   128 x 64 (three stages) up to 160 (1000 rows of 2048 x 2048: 10.9 by 64 x 64, 10.1, 16.0 by 128 x 128),
+//   128 x 128 (three stages: one workgroup a CU) up to 256 (300 rows of 8192 x 8192: 43 by two stages, 31.6),
+//   128 x 128 (two stages: two workgroups a CU) up to 191 tiles of 256 x 256 (2048 rows of 4096 x 4096: 39, by 256 x 256 47),
+//   256 x 256: eight waves (8192 rows of 8192 x 8192: 554 by 128 x 128, 466 by four waves, 443), four where the columns are many
+//   (of 8192 x 29568: 1555 by eight, 1535; the clock is down to 1.6 GHz then, by power).
 template <int EPI>
 hipError_t vx_i8_choose(const VxI8Args& a, hipStream_t st) {
     if constexpr (EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT) {
-        if (a.item_rows == kItemRows) return vx_i8_items_launch<EPI>(a, st);
+        if (a.item_rows >= kSmallItemRows) return vx_i8_items_launch<EPI>(a, st);
         return a.item_rows == 32u ? vx_i8_stream_launch<2, 2, 4, EPI>(a, st) : vx_i8_stream_launch<2, 1, 4, EPI>(a, st);
     } else {
         constexpr bool one = EPI == VX_I8_STORE;  // (the others take tiles by pairs)
+        const auto tiles = [&](uint32_t by) { return (uint64_t)((a.w.n_tiles * 16u + by - 1u) / by) * ((a.n_rows + by - 1u) / by); };
         if (a.n_rows > 64u) {
-            if ((uint64_t)((a.w.n_tiles + 15u) / 16u) * ((a.n_rows + 255u) / 256u) >= 192u) return vx_i8_tile_launch<4, 2, 2, 4, 2, 4, EPI>(a, st);
-            return vx_i8_tile_launch<2, 2, 2, 2, 2, 4, EPI>(a, st);
+            if (tiles(256u) >= 192u)
+                return a.w.k > 16384u ? vx_i8_tile_launch<2, 2, 4, 4, 2, 4, EPI>(a, st) : vx_i8_tile_launch<4, 2, 2, 4, 2, 4, EPI>(a, st);
+            const uint64_t t = tiles(128u);
+            if (t > 256u) return vx_i8_tile_launch<2, 2, 2, 2, 2, 4, EPI>(a, st);
+            if (t > 160u) return vx_i8_tile_launch<2, 2, 2, 2, 3, 4, EPI>(a, st);
+            if (t > 100u) return vx_i8_tile_launch<2, 2, 2, 1, 3, 4, EPI>(a, st);
+            return vx_i8_tile_launch<2, 2, 1, 1, 4, 4, EPI>(a, st);
         }
         if (a.n_rows > 32u) return vx_i8_tile_launch<4, 1, 1, 1, 4, 4, EPI>(a, st);
         if (a.n_rows > 16u) return a.w.n_tiles >= 1536u ? vx_i8_stream_launch<6, 2, 4, EPI>(a, st) : vx_i8_stream_launch<2, 2, 8, EPI>(a, st);

@@ -283,7 +283,7 @@ int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Ma
     g.hist = f.hist;
     g.items = f.items;
     g.n_items = f.n_items;
-    g.item_rows = vx_i8_item_rows(slots, gu.count);
+    g.item_rows = vx_i8_item_rows(slots, gu.count, gu.n_tiles > dn.n_tiles ? gu.n_tiles : dn.n_tiles);
     hipError_t e = vx_launch_group(g, st);
     if (e == hipSuccess) e = vx_launch_i8_quantize(view(x), n_rows, gu.k, f.x, nullptr, st);
     a.a = f.x;
