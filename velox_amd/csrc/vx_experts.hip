@@ -326,12 +326,12 @@ __device__ __forceinline__ uint32_t vx_size_class(uint32_t slots) {
     const uint32_t c = (slots + 31u) / 32u;
     return c < 63u ? c : 63u;
 }
-// PER: experts of a thread, neighbours.
+// PER: experts of a thread, neighbours. Workgroup `block` of `blocks`.
 template <uint32_t PER>
-__global__ __launch_bounds__(kGroupThreads) void vx_group_place_kernel(VxGroupArgs a) {
+__device__ __forceinline__ void vx_group_place(const VxGroupArgs& a, uint32_t block, uint32_t blocks) {
     __shared__ uint32_t tally[kGroupWaves * (kVxI8MaxCount + 1u)];
     __shared__ uint32_t room[kGroupWaves], sizes[64];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n = a.count + 1u, block = blockIdx.x, blocks = gridDim.x;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, n = a.count + 1u;
     const uint32_t run = block * kGroupSlots + wave * kGroupRun;
     const VxKeys k = vx_keys(a, run);
     if (threadIdx.x < 64u) sizes[threadIdx.x] = 0;
@@ -421,6 +421,23 @@ __global__ __launch_bounds__(kGroupThreads) void vx_group_place_kernel(VxGroupAr
     for (uint32_t p = total + block * kGroupThreads + threadIdx.x; p < a.n_slots; p += blocks * kGroupThreads) a.order[p] = kVxNoExpert;
 }
 
+template <uint32_t PER>
+__global__ __launch_bounds__(kGroupThreads) void vx_group_place_kernel(VxGroupArgs a) {
+    vx_group_place<PER>(a, blockIdx.x, gridDim.x);
+}
+// Few slots and their rows, which do not need each other, in one launch: workgroup 0 groups, r + 1 puts row r into 8 bits.
+template <class T, int NV, uint32_t PER>
+__global__ __launch_bounds__(kGroupThreads) void vx_prepare_kernel(VxGroupArgs a, VxI8View x, uint32_t k, VxI8Rows o) {
+    __shared__ uint32_t red[kGroupWaves];
+    if (blockIdx.x == 0) {
+        vx_group_place<PER>(a, 0, 1);
+        return;
+    }
+    const uint32_t r = blockIdx.x - 1u;
+    const float s = vx_hold_row<T, kGroupThreads, NV, false>((const T*)x.data + (size_t)r * x.rs, k, (uint8_t*)o.codes + (size_t)r * o.rs, threadIdx.x, red);
+    if (threadIdx.x == 0) o.scales[r] = s;
+}
+
 // ---- the sum of a row's experts ----
 // A workgroup takes 1024 outputs of a row, a thread four. Lane j of a wave looks at the row's slot j; the slots of our
 // experts are then added in order, four of their answers on the way at a time.
@@ -473,9 +490,36 @@ hipError_t vx_launch_route(const VxRouteArgs& args, hipStream_t st) {
 
 uint32_t vx_group_blocks(uint32_t n_slots) { return n_slots ? (n_slots + kGroupSlots - 1u) / kGroupSlots : 1u; }
 
-hipError_t vx_launch_group(const VxGroupArgs& args, hipStream_t st) {
-    VxGroupArgs a = args;
+namespace {
+VxGroupArgs vx_keyed(VxGroupArgs a) {
     a.key_bits = 32u - (uint32_t)__builtin_clz(a.count);  // keys 0 .. count
+    return a;
+}
+template <class T, int NV>
+hipError_t vx_prepare(const VxGroupArgs& a, const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& o, hipStream_t st) {
+    if (a.count <= kGroupThreads) hipLaunchKernelGGL((vx_prepare_kernel<T, NV, 1>), dim3(n_rows + 1u), dim3(kGroupThreads), 0, st, a, x, k, o);
+    else hipLaunchKernelGGL((vx_prepare_kernel<T, NV, kVxI8MaxCount / kGroupThreads>), dim3(n_rows + 1u), dim3(kGroupThreads), 0, st, a, x, k, o);
+    return hipGetLastError();
+}
+template <class T>
+hipError_t vx_prepare_t(const VxGroupArgs& a, const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& o, hipStream_t st) {
+    return vx_i8_pad(k) * sizeof(T) <= 2u * 16u * kGroupThreads ? vx_prepare<T, 2>(a, x, n_rows, k, o, st) : vx_prepare<T, 8>(a, x, n_rows, k, o, st);
+}
+}  // namespace
+
+hipError_t vx_launch_group_and_quantize(const VxGroupArgs& args, const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& o, hipStream_t st) {
+    if (vx_group_blocks(args.n_slots) > 1u || !vx_whole_rows(x, k) || vx_i8_pad(k) * (x.dtype == VELOX_DT_F32 ? 4u : 2u) > 8u * 16u * kGroupThreads) {
+        const hipError_t e = vx_launch_group(args, st);
+        return e != hipSuccess ? e : vx_launch_i8_quantize(x, n_rows, k, o, nullptr, st);
+    }
+    const VxGroupArgs a = vx_keyed(args);
+    if (x.dtype == VELOX_DT_F32) return vx_prepare_t<float>(a, x, n_rows, k, o, st);
+    if (x.dtype == VELOX_DT_F16) return vx_prepare_t<_Float16>(a, x, n_rows, k, o, st);
+    return vx_prepare_t<__bf16>(a, x, n_rows, k, o, st);
+}
+
+hipError_t vx_launch_group(const VxGroupArgs& args, hipStream_t st) {
+    const VxGroupArgs a = vx_keyed(args);
     const uint32_t blocks = vx_group_blocks(a.n_slots);
     if (blocks > 1u) {
         hipLaunchKernelGGL(vx_group_count_kernel, dim3(blocks), dim3(kGroupThreads), 0, st, a);

@@ -91,6 +91,7 @@ struct VxCombineArgs {
 
 hipError_t vx_launch_i8_pack(const VxI8Mat& m, uint32_t first, uint32_t number, const int8_t* codes, uint64_t ms, uint64_t rs,
                              const float* scales, uint64_t ss, hipStream_t st);
+bool vx_whole_rows(const VxI8View& x, uint32_t k);
 // rows < *limit where limit is set
 hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& out, const uint32_t* limit,
                                  hipStream_t st);
@@ -106,4 +107,6 @@ hipError_t vx_launch_i8_answers(const VxI8Args& a, const VxCombineArgs& c, hipSt
 hipError_t vx_launch_route(const VxRouteArgs& a, hipStream_t st);
 uint32_t vx_group_blocks(uint32_t n_slots);
 hipError_t vx_launch_group(const VxGroupArgs& a, hipStream_t st);
+// Both, in one launch where the slots are few (they do not need each other).
+hipError_t vx_launch_group_and_quantize(const VxGroupArgs& a, const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& out, hipStream_t st);
 hipError_t vx_launch_combine(const VxCombineArgs& a, hipStream_t st);

@@ -284,8 +284,7 @@ int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Ma
     g.items = f.items;
     g.n_items = f.n_items;
     g.item_rows = vx_i8_item_rows(slots, gu.count, gu.n_tiles > dn.n_tiles ? gu.n_tiles : dn.n_tiles);
-    hipError_t e = vx_launch_group(g, st);
-    if (e == hipSuccess) e = vx_launch_i8_quantize(view(x), n_rows, gu.k, f.x, nullptr, st);
+    hipError_t e = vx_launch_group_and_quantize(g, view(x), n_rows, gu.k, f.x, st);
     a.a = f.x;
     a.g = VxGrouped{f.order, f.offsets, f.items, f.n_items};
     a.max_items = max_items(slots, gu.count, g.item_rows);
