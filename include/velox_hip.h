@@ -563,8 +563,8 @@ int velox_hip_pages_compact(const VeloxHipPagedCache* c, hipStream_t stream);
 int velox_hip_pages_status(const VeloxHipPagedCache* c, uint32_t* refused, uint32_t* free_pages, hipStream_t stream);
 
 /* ---- 8-bit integer products (no counterpart in the reference, whose weights are fp32, fp16, 4 bits or fp8) ----
- * Weights and activations in whole numbers of [-128, 127] with one fp32 scale for each weight row (output channel) and
- * each activation row (token). As the paged cache's, every entry point checks its arguments (EINVAL), launches on `stream`
+ * Weights in whole numbers of [-128, 127], activations of [-127, 127], with one fp32 scale for each weight row (output
+ * channel) and each activation row (token). As the paged cache's, every entry point checks its arguments (EINVAL), launches on `stream`
  * with the stream's device current, allocates nothing, does not synchronize and can be captured into a hipGraph; a call's
  * workspace is the call's own until the stream has passed it. Rows are VeloxHipRows with heads 1 (head_stride is not
  * looked at).
@@ -601,7 +601,8 @@ int velox_hip_int8_quantize(const VeloxHipRows* x, uint32_t n_rows, uint32_t k, 
 /* y[r][n] = (sum_k c[r][k] w[n][k]) scale[n] scale[r], the sum exact, the scales' products in fp32; then
  * VELOX_GEMV_STORE: out = y (+ bias[n]); VELOX_GEMV_RESIDUAL: out = residual + y (+ bias[n]) (residual may be out itself:
  * the same data and stride; other overlaps are not allowed); VELOX_GEMV_SWIGLU (a paired matrix, and only that):
- * out[r][j] = silu(gate_j) up_j. fp32 throughout, rounded once to out's type. The rows come as x, quantized on the way
+ * out[r][j] = silu(gate_j) up_j. fp32 throughout, rounded once to out's type. out may begin where x does; other overlaps with the rows are not
+ * allowed. The rows come as x, quantized on the way
  * (workspace: velox_hip_int8_product_bytes, 16-byte aligned), or as q, already in 8 bits (no workspace); the other is
  * NULL. m->count is 1. Fewer than 2^24 rows. */
 int velox_hip_int8_product_bytes(const VeloxHipInt8Matrix* m, uint32_t n_rows, uint64_t* bytes);

@@ -443,8 +443,8 @@ __global__ __launch_bounds__(kGroupThreads) void vx_prepare_kernel(VxGroupArgs a
 // experts are then added in order, four of their answers on the way at a time.
 constexpr uint32_t kCombineCols = 1024u;
 template <bool VEC>
-__global__ __launch_bounds__(256) void vx_combine_kernel(VxCombineArgs a, uint32_t blocks) {
-    const uint32_t r = blockIdx.x / blocks, c = blockIdx.x % blocks * kCombineCols + 4u * threadIdx.x, lane = threadIdx.x & 63u;
+__global__ __launch_bounds__(256) void vx_combine_kernel(VxCombineArgs a) {
+    const uint32_t r = blockIdx.x, c = blockIdx.y * kCombineCols + 4u * threadIdx.x, lane = threadIdx.x & 63u;
     const size_t slot0 = (size_t)r * a.top;
     const bool mine = lane < a.top && a.ids[slot0 + lane] - a.first < a.count;
     const float w = mine ? a.weights[slot0 + lane] : 0.0f;
@@ -533,7 +533,7 @@ hipError_t vx_launch_group(const VxGroupArgs& args, hipStream_t st) {
 
 hipError_t vx_launch_combine(const VxCombineArgs& a, hipStream_t st) {
     const uint32_t blocks = (a.n + kCombineCols - 1u) / kCombineCols;
-    if (a.vec) hipLaunchKernelGGL((vx_combine_kernel<true>), dim3(a.n_rows * blocks), dim3(256), 0, st, a, blocks);
-    else hipLaunchKernelGGL((vx_combine_kernel<false>), dim3(a.n_rows * blocks), dim3(256), 0, st, a, blocks);
+    if (a.vec) hipLaunchKernelGGL((vx_combine_kernel<true>), dim3(a.n_rows, blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((vx_combine_kernel<false>), dim3(a.n_rows, blocks), dim3(256), 0, st, a);
     return hipGetLastError();
 }

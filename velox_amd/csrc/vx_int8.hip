@@ -1,4 +1,6 @@
 // vx_int8.hip -- products of 8-bit integers with a scale for each token and channel.
+#include <atomic>
+
 #include "vx_int8_dev.h"
 
 namespace {
@@ -313,6 +315,16 @@ struct VxStream {
     }
 };
 
+// Lets a kernel take `bytes` of dynamic LDS, once on each device (`allowed`: a bit for each).
+hipError_t vx_allow_lds(const void* kernel, uint32_t bytes, std::atomic<uint64_t>& allowed) {
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess || (allowed.load(std::memory_order_relaxed) >> (device & 63) & 1u)) return e;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == hipSuccess) allowed.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
+    return e;
+}
+
 constexpr uint32_t kRowWaves = 4;
 
 // Up to four rows (STORE, SWIGLU), or one slot's row for its expert (HIDDEN): the first weights are requested, the workgroup
@@ -402,7 +414,8 @@ __global__ __launch_bounds__(64 * kAnswerWaves) void vx_i8_answer_kernel(VxI8Arg
 
 template <class T, int NV, int NT, int EPI>
 hipError_t vx_i8_row_launch_v(const VxI8Args& a, const VxI8View& x, hipStream_t st) {
-    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_row_kernel<T, NV, NT, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, 1 << 17);
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t set = vx_allow_lds((const void*)vx_i8_row_kernel<T, NV, NT, EPI>, 1 << 17, allowed);
     if (set != hipSuccess) return set;
     const uint32_t n_blocks = (a.w.n_tiles + NT - 1u) / NT, rows = EPI == VX_I8_HIDDEN ? a.n_rows * a.top : 1u;
     hipLaunchKernelGGL((vx_i8_row_kernel<T, NV, NT, EPI>), dim3(rows * n_blocks), dim3(64 * kRowWaves), vx_i8_pad(a.w.k) * (EPI == VX_I8_HIDDEN ? 1u : a.n_rows), st, a, x, n_blocks);
@@ -738,7 +751,8 @@ constexpr uint32_t kTileStep = 1u << 20;  // rows of a launch
 template <int WN, int WM, int FN, int FM, int S, int KQ, int EPI>
 hipError_t vx_i8_tile_launch(const VxI8Args& a, hipStream_t st) {
     constexpr uint32_t TN = 32 * WN * FN, TM = 32 * WM * FM, lds = S * (TN + TM) * 32 * KQ;
-    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_tile_kernel<WN, WM, FN, FM, S, KQ, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t set = vx_allow_lds((const void*)vx_i8_tile_kernel<WN, WM, FN, FM, S, KQ, EPI>, lds, allowed);
     if (set != hipSuccess) return set;
     const uint32_t n_blocks = (a.w.n_tiles * 16u + TN - 1u) / TN;
     for (uint32_t r = 0; r < a.n_rows; r += kTileStep) {
@@ -758,7 +772,8 @@ hipError_t vx_i8_items_launch(const VxI8Args& a, hipStream_t st) {
         hipLaunchKernelGGL((vx_i8_small_items_kernel<EPI>), dim3(a.max_items * n_blocks), dim3(256), small, st, a, n_blocks);
         return hipGetLastError();
     }
-    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_items_kernel<EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t set = vx_allow_lds((const void*)vx_i8_items_kernel<EPI>, lds, allowed);
     if (set != hipSuccess) return set;
     const uint32_t n_blocks = (a.w.n_tiles + 15u) / 16u;
     hipLaunchKernelGGL((vx_i8_items_kernel<EPI>), dim3(a.max_items * n_blocks), dim3(512), lds, st, a, n_blocks);
@@ -777,9 +792,18 @@ hipError_t vx_launch_i8_pack(const VxI8Mat& m, uint32_t first, uint32_t number, 
 
 hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k, const VxI8Rows& out, const uint32_t* limit,
                                  hipStream_t st) {
-    if (x.dtype == VELOX_DT_F32) return vx_quantize_launch<float>(x, n_rows, k, out, limit, st);
-    if (x.dtype == VELOX_DT_F16) return vx_quantize_launch<_Float16>(x, n_rows, k, out, limit, st);
-    return vx_quantize_launch<__bf16>(x, n_rows, k, out, limit, st);
+    constexpr uint32_t kStep = 1u << 21;  // (a launch has fewer than 2^32 threads, up to 1024 of them a row; limit: fewer rows)
+    const uint32_t elt = x.dtype == VELOX_DT_F32 ? 4u : 2u;
+    for (uint32_t r = 0; r < n_rows; r += kStep) {
+        const VxI8View part{(uint8_t*)x.data + (uint64_t)r * x.rs * elt, x.rs, x.dtype};
+        const VxI8Rows to{out.codes + (uint64_t)r * out.rs, out.scales + r, out.rs};
+        const uint32_t rows = n_rows - r < kStep ? n_rows - r : kStep;
+        const hipError_t e = x.dtype == VELOX_DT_F32   ? vx_quantize_launch<float>(part, rows, k, to, limit, st)
+                             : x.dtype == VELOX_DT_F16 ? vx_quantize_launch<_Float16>(part, rows, k, to, limit, st)
+                                                       : vx_quantize_launch<__bf16>(part, rows, k, to, limit, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // Positions of a block of a grouped product, by how many slots there are for an expert (64 of 256 experts of 7168 x 2048 here, 8 for
@@ -856,7 +880,8 @@ bool vx_i8_ffn_by_slot(const VxI8View& x, uint32_t n_rows, uint32_t hidden, uint
 }
 hipError_t vx_launch_i8_slots(const VxI8Args& a, const VxI8View& x, hipStream_t st) { return vx_i8_row_launch_t<2, VX_I8_HIDDEN>(a, x, st); }
 hipError_t vx_launch_i8_answers(const VxI8Args& a, const VxCombineArgs& c, hipStream_t st) {
-    static const hipError_t set = hipFuncSetAttribute((const void*)vx_i8_answer_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 1 << 17);
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t set = vx_allow_lds((const void*)vx_i8_answer_kernel, 1 << 17, allowed);
     if (set != hipSuccess) return set;
     const uint32_t n_blocks = a.w.n_tiles;
     hipLaunchKernelGGL(vx_i8_answer_kernel, dim3(c.n_rows * n_blocks), dim3(64 * kAnswerWaves), vx_i8_pad(a.w.k) * kAnswerWaves, st, a, c, n_blocks);
