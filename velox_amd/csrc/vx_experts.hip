@@ -77,19 +77,26 @@ __device__ __forceinline__ uint64_t vx_open_groups(const VxRouteArgs& a, const F
 // experts), the row is done again in 64 bits. The largest is found top_k times:
 // by DPP in the wave, its place by ballots. The chosen scores are formed in 64 bits. What bounds it: instructions (256 experts, 8 of
 // them in 4 of 8 groups: about 600 a row).
-template <uint32_t ITEMS>
+template <class T, uint32_t ITEMS>
 __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
     __shared__ double room[4][ITEMS * 64u + kVxMaxGroups];
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), r = blockIdx.x * 4u + wave;
     if (r >= a.n_rows) return;  // (waves share nothing)
-    const size_t base = (size_t)r * a.x.rs;
+    // (all of a row's loads are requested at once: what is not there they give as 0)
+    const T* row = (const T*)a.x.data + (size_t)r * a.x.rs;
+    const auto xs = __builtin_amdgcn_make_buffer_rsrc((void*)row, 0, (int)(a.n_experts * sizeof(T)), 0x00020000);
+    const auto bs = __builtin_amdgcn_make_buffer_rsrc((void*)a.bias, 0, a.bias ? (int)(a.n_experts * 4u) : 0, 0x00020000);
+    const auto logit = [&](uint32_t e) -> float {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(xs, (int)(e * 4u), 0, 0));
+        else return (float)__builtin_bit_cast(T, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(xs, (int)(e * 2u), 0, 0));
+    };
     float x[ITEMS], bias[ITEMS];
 #pragma unroll
-    for (uint32_t i = 0; i < ITEMS; ++i) {
-        const uint32_t e = lane + 64u * i;
-        x[i] = e < a.n_experts ? vx_load(a.x.data, base + e, a.x.dtype) : -INFINITY;
-        bias[i] = a.bias && e < a.n_experts ? a.bias[e] : 0.0f;
-    }
+    for (uint32_t i = 0; i < ITEMS; ++i) x[i] = logit(lane + 64u * i);
+#pragma unroll
+    for (uint32_t i = 0; i < ITEMS; ++i) bias[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(bs, (int)((lane + 64u * i) * 4u), 0, 0));
+#pragma unroll
+    for (uint32_t i = 0; i < ITEMS; ++i) x[i] = lane + 64u * i < a.n_experts ? x[i] : -INFINITY;
     float top = -INFINITY;
 #pragma unroll
     for (uint32_t i = 0; i < ITEMS; ++i) {
@@ -204,7 +211,7 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
             uint32_t at = 0xFFFFFFFFu;
             for (uint32_t e = lane; e < a.n_experts; e += 64u) {
                 // (without a bias equal scores of different logits keep the logits' order: the largest logit comes first)
-                const double v = marked && !(open >> (e / size) & 1u) ? -INFINITY : by_logits && all[e] > -INFINITY ? (double)vx_load(a.x.data, base + e, a.x.dtype) : all[e];
+                const double v = marked && !(open >> (e / size) & 1u) ? -INFINITY : by_logits && all[e] > -INFINITY ? (double)logit(e) : all[e];
                 if (v > best) {
                     best = v;
                     at = e;
@@ -226,8 +233,7 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
     }
     double s = 0.0;
     if (id != kVxNoExpert) {
-        const float v = vx_load(a.x.data, base + id, a.x.dtype);
-        s = exact(fminf(v, 3.40282347e38f));
+        s = exact(fminf(logit(id), 3.40282347e38f));
         if (whole) s = all_sum > 0.0 ? s / all_sum : 0.0;
     }
     if (a.renorm) {
@@ -475,17 +481,23 @@ __global__ __launch_bounds__(256) void vx_combine_kernel(VxCombineArgs a) {
 
 }  // namespace
 
+template <class T>
+static hipError_t vx_route_launch(const VxRouteArgs& a, hipStream_t st) {
+    const dim3 grid((a.n_rows + 3u) / 4u);
+    if (a.n_experts <= 64u) hipLaunchKernelGGL((vx_route_kernel<T, 1>), grid, dim3(256), 0, st, a);
+    else if (a.n_experts <= 128u) hipLaunchKernelGGL((vx_route_kernel<T, 2>), grid, dim3(256), 0, st, a);
+    else if (a.n_experts <= 256u) hipLaunchKernelGGL((vx_route_kernel<T, 4>), grid, dim3(256), 0, st, a);
+    else if (a.n_experts <= 512u) hipLaunchKernelGGL((vx_route_kernel<T, 8>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((vx_route_kernel<T, 16>), grid, dim3(256), 0, st, a);
+    return hipGetLastError();
+}
 hipError_t vx_launch_route(const VxRouteArgs& args, hipStream_t st) {
     VxRouteArgs a = args;
     a.group_lanes = 0;
     while ((2u << a.group_lanes) * a.groups <= 64u) ++a.group_lanes;
-    const dim3 grid((a.n_rows + 3u) / 4u);
-    if (a.n_experts <= 64u) hipLaunchKernelGGL((vx_route_kernel<1>), grid, dim3(256), 0, st, a);
-    else if (a.n_experts <= 128u) hipLaunchKernelGGL((vx_route_kernel<2>), grid, dim3(256), 0, st, a);
-    else if (a.n_experts <= 256u) hipLaunchKernelGGL((vx_route_kernel<4>), grid, dim3(256), 0, st, a);
-    else if (a.n_experts <= 512u) hipLaunchKernelGGL((vx_route_kernel<8>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((vx_route_kernel<16>), grid, dim3(256), 0, st, a);
-    return hipGetLastError();
+    if (a.x.dtype == VELOX_DT_F32) return vx_route_launch<float>(a, st);
+    if (a.x.dtype == VELOX_DT_F16) return vx_route_launch<_Float16>(a, st);
+    return vx_route_launch<__bf16>(a, st);
 }
 
 uint32_t vx_group_blocks(uint32_t n_slots) { return n_slots ? (n_slots + kGroupSlots - 1u) / kGroupSlots : 1u; }

@@ -816,8 +816,8 @@ uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count, uint32_t n_tiles) {
 
 // Up to 16 rows the streaming kernel with one weight tile a workgroup (4096 x 4096, one row: two tiles 6.1 us, one 5.0) or,
 // where more rows share a tile of a large matrix, two (8192 x 8192, 16 rows: 16.1, 14.2); up to 32 rows two tiles and eight
-// waves, or where six fill the CUs still, six and four (8192 x 8192: 15.3; 37888 x 3584 paired: 35.7 and 29.6). From 33 rows on tiles
-// through LDS, as large as leave the CUs work: 128 x 32 up to 64 rows (8192 x 8192: 18.1, streaming 21.3), then
+// waves (8192 x 8192: 17.3, four and four 27.7), four and four from 1024 tiles on (28672 x 4096 paired: 30.0, 23.9), six and four where
+// those were over two workgroups a CU (37888 x 3584 paired: 35.6, 31.9, 29.6). From 33 rows on tiles through LDS, as large as leave the CUs work: 128 x 32 up to 64 rows (8192 x 8192: 18.1, streaming 21.3), then
 //   64 x 64 (four stages) up to 100 tiles of 128 x 128 (1037 rows of 960 x 576: 8.3 -> 4.9 us, 200 of 4096 x 14336: 67 -> 29),
 //   128 x 64 (three stages) up to 160 (1000 rows of 2048 x 2048: 10.9 by 64 x 64, 10.1, 16.0 by 128 x 128),
 //   128 x 128 (three stages: one workgroup a CU) up to 256 (300 rows of 8192 x 8192: 43 by two stages, 31.6),
@@ -842,7 +842,10 @@ hipError_t vx_i8_choose(const VxI8Args& a, hipStream_t st) {
             return vx_i8_tile_launch<2, 2, 1, 1, 4, 4, EPI>(a, st);
         }
         if (a.n_rows > 32u) return vx_i8_tile_launch<4, 1, 1, 1, 4, 4, EPI>(a, st);
-        if (a.n_rows > 16u) return a.w.n_tiles >= 1536u ? vx_i8_stream_launch<6, 2, 4, EPI>(a, st) : vx_i8_stream_launch<2, 2, 8, EPI>(a, st);
+        if (a.n_rows > 16u) {
+            if (a.w.n_tiles > 2048u) return vx_i8_stream_launch<6, 2, 4, EPI>(a, st);
+            return a.w.n_tiles >= 1024u ? vx_i8_stream_launch<4, 2, 4, EPI>(a, st) : vx_i8_stream_launch<2, 2, 8, EPI>(a, st);
+        }
         if (one && (a.n_rows <= 4u || a.w.n_tiles < 512u)) return vx_i8_stream_launch<one ? 1 : 2, 1, 4, EPI>(a, st);
         return vx_i8_stream_launch<2, 1, 4, EPI>(a, st);
     }
