@@ -180,6 +180,35 @@ def test_product_of_rows_already_in_8_bits_any_output_type_and_place(m):
         check(x, w, sw, res, residual=before)
 
 
+@pytest.mark.parametrize("m", [1, 2, 3, 20, 40, 100, 700])
+def test_product_in_the_rows_place(m):
+    """out begins where x does: every row is in 8 bits before the first output is written."""
+    for i, dtype in enumerate(T):
+        w, sw = weights(256, 256, 5 + i)
+        mat = int8.Int8Matrix(w, sw)
+        x = rows(m, 256, dtype, 4)
+        before = x.clone()
+        apart = int8.product(x, mat, residual=x)
+        assert int8.product(x, mat, residual=x, out=x) is x
+        assert torch.equal(x, apart)
+        check(before, w, sw, x, residual=before)
+
+
+@pytest.mark.parametrize("m,step", [(2, 2 ** 31 + 8), (20, 2 ** 28 + 8), (100, 2 ** 26 + 8), (300, 2 ** 24 + 3)])
+def test_rows_that_lie_past_32_bits(m, step):
+    n, k = 80, 144
+    x, res, room = (torch.empty((m - 1) * step + 160, device="cuda", dtype=torch.float16) for _ in range(3))
+    xr, rr, out = x.as_strided((m, k), (step, 1)), res.as_strided((m, n), (step, 1)), room.as_strided((m, n), (step, 1))
+    xr.copy_(rows(m, k, "f16", 1))
+    rr.copy_(rows(m, n, "f16", 2))
+    w, sw = weights(n, k, 3)
+    mat = int8.Int8Matrix(w, sw)
+    int8.product(xr, mat, residual=rr, out=out)
+    check(xr.clone(), w, sw, out, residual=rr.clone())
+    q = int8.quantize(xr)
+    assert torch.equal(int8.product(q, mat, residual=rr, dtype=torch.float16), out)
+
+
 def test_rows_behind_the_last_are_left_as_they_were():
     for m in (1, 7, 16, 33, 130, 257):
         x = rows(m, 256, "f32", 2)
