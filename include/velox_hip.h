@@ -564,8 +564,8 @@ int velox_hip_pages_status(const VeloxHipPagedCache* c, uint32_t* refused, uint3
 
 /* ---- 8-bit integer products (no counterpart in the reference, whose weights are fp32, fp16, 4 bits or fp8) ----
  * Weights in whole numbers of [-128, 127], activations of [-127, 127], with one fp32 scale for each weight row (output
- * channel) and each activation row (token). As the paged cache's, every entry point checks its arguments (EINVAL), launches on `stream`
- * with the stream's device current, allocates nothing, does not synchronize and can be captured into a hipGraph; a call's
+ * channel) and each activation row (token). As the paged cache's, every entry point checks its arguments (EINVAL), launches on
+ * `stream` with the stream's device current, allocates nothing, does not synchronize and can be captured into a hipGraph; a call's
  * workspace is the call's own until the stream has passed it. Rows are VeloxHipRows with heads 1 (head_stride is not
  * looked at).
  *
@@ -601,10 +601,9 @@ int velox_hip_int8_quantize(const VeloxHipRows* x, uint32_t n_rows, uint32_t k, 
 /* y[r][n] = (sum_k c[r][k] w[n][k]) scale[n] scale[r], the sum exact, the scales' products in fp32; then
  * VELOX_GEMV_STORE: out = y (+ bias[n]); VELOX_GEMV_RESIDUAL: out = residual + y (+ bias[n]) (residual may be out itself:
  * the same data and stride; other overlaps are not allowed); VELOX_GEMV_SWIGLU (a paired matrix, and only that):
- * out[r][j] = silu(gate_j) up_j. fp32 throughout, rounded once to out's type. out may begin where x does; other overlaps with the rows are not
- * allowed. The rows come as x, quantized on the way
- * (workspace: velox_hip_int8_product_bytes, 16-byte aligned), or as q, already in 8 bits (no workspace); the other is
- * NULL. m->count is 1. Fewer than 2^24 rows. */
+ * out[r][j] = silu(gate_j) up_j. fp32 throughout, rounded once to out's type. out may begin where x does; other overlaps with
+ * the rows are not allowed. The rows come as x, quantized on the way (workspace: velox_hip_int8_product_bytes, 16-byte
+ * aligned), or as q, already in 8 bits (no workspace); the other is NULL. m->count is 1. Fewer than 2^24 rows. */
 int velox_hip_int8_product_bytes(const VeloxHipInt8Matrix* m, uint32_t n_rows, uint64_t* bytes);
 int velox_hip_int8_product(const VeloxHipInt8Matrix* m, const VeloxHipRows* x, const VeloxHipInt8Rows* q, uint32_t n_rows,
                            const float* d_bias, const VeloxHipRows* residual, const VeloxHipRows* out, int mode,
@@ -619,8 +618,8 @@ int velox_hip_int8_product(const VeloxHipInt8Matrix* m, const VeloxHipRows* x, c
  *   sum is 0). Without a bias the order is that of the logits themselves; choice values with one, and sums of two, compare
  *   as in 64 bits, so that nearly equal ones keep their order. A logit of -infinity or NaN takes its expert out of the row
  *   and of the softmax's sum, a bias that is not finite takes it out of every row; a logit of +infinity counts as the
- *   largest finite number. Where fewer than
- *   top_k experts are left, the rest of ids is VELOX_HIP_NO_EXPERT and of weights 0: a row of -infinity is padding. */
+ *   largest finite number. Where fewer than top_k experts are left, the rest of ids is VELOX_HIP_NO_EXPERT and of weights 0:
+ *   a row of -infinity is padding. */
 #define VELOX_HIP_NO_EXPERT 0xFFFFFFFFu
 #define VELOX_ROUTE_SOFTMAX 0u
 #define VELOX_ROUTE_SIGMOID 1u
@@ -647,8 +646,9 @@ int velox_hip_expert_group(const uint32_t* d_ids, uint32_t n_slots, uint32_t fir
 /* out[r] = residual[r] (NULL: 0) + sum over j of weights[r][j] down_e(h), h = silu(gate_e(x[r])) up_e(x[r]), e = ids[r][j]
  * - first. gate_up (paired, n = 2 inner, k = hidden) and down (n = hidden, k = inner) hold the experts first .. first +
  * count - 1; other ids (VELOX_HIP_NO_EXPERT, experts that live elsewhere) add nothing, a row may name an expert twice. x and
- * h enter the products in 8 bits (h from fp32), sums are fp32 in the order of j, rounded once to out's type. out may be x or the residual (the same data and stride). n_rows * top_k <= 2^20; workspace:
- * velox_hip_expert_ffn_bytes of the same matrices, enough for up to n_rows rows of any types, 16-byte aligned. */
+ * h enter the products in 8 bits (h from fp32), sums are fp32 in the order of j, rounded once to out's type. out may be x or
+ * the residual (the same data and stride). n_rows * top_k <= 2^20; workspace: velox_hip_expert_ffn_bytes of the same
+ * matrices, enough for up to n_rows rows of any types, 16-byte aligned. */
 int velox_hip_expert_ffn_bytes(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Matrix* down, uint32_t n_rows,
                                uint32_t top_k, uint64_t* bytes);
 int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Matrix* down, uint32_t first,
@@ -865,8 +865,8 @@ void velox_hip_mla_layer_step(VeloxHipMla* m, uint32_t layer, uint32_t batch, ui
 /* The attention stack of a decode step: the layer step of layers 0 .. num_layers - 1 in order, as the
  * reference's graph step launches its MLA kernel per layer (src/codegen.rs:2980-3003), with each
  * layer's W_o partials folded into the next layer's RMSNorm instead of a residual launch (hidden
- * ends equal to num_layers successive layer steps, bit for bit). The MoE FFN the reference model
- * places between the attention layers is outside this backend (not in the benchmark configurations).
+ * ends equal to num_layers successive layer steps, bit for bit). The feed-forward half that
+ * the reference model places between the attention layers is the caller's (velox_hip_expert_*, between layer steps).
  * Capturable; errors through velox_hip_last_error(). */
 void velox_hip_mla_decode_step(VeloxHipMla* m, uint32_t batch, uint64_t active_mask, hipStream_t stream);
 /* Algorithmic HBM bytes of one layer step (weights + scales + latent rows 0..pos + activations). */

@@ -86,7 +86,9 @@ __global__ __launch_bounds__(256) void vx_i8_pack_kernel(VxI8Mat m, uint32_t fir
 }
 
 // ---- rows in 8 bits ----
-// Bound by the bytes (8192 rows of 29568 bf16, 726 MB: 138 us).
+// Scale and codes of a row, which is read once: as many threads a row as hold it in registers (a wave for short rows, which
+// then share nothing). Bound by the bytes (8192 rows of 29568 bf16, 727 MB: 127 to 172 us, 5.7 to 4.2 TB/s), for few rows by latency
+// (32 rows of 3584 fp32: 4.9 us).
 template <class T, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void vx_i8_quantize_kernel(VxI8View x, uint32_t n_rows, uint32_t k, VxI8Rows o, const uint32_t* limit) {
     constexpr int WG = TPR < 256 ? 256 : TPR;
@@ -162,6 +164,8 @@ hipError_t vx_quantize_launch(const VxI8View& x, uint32_t n_rows, uint32_t k, co
 // tiles in turn, so that the weights stream in order, each lane's 16 bytes being its MFMA operand; U tiles are requested
 // while U are multiplied, those behind the last by bounds-checked loads that give zeros. The waves' sums meet in LDS. The
 // weights are the A operand, so that a lane ends with four neighbouring outputs: D[n = 4 (lane / 16) + i][row = lane % 16].
+// Bound by the weights' bytes: 32 rows of 37888 x 3584 28.4 to 29 us (4.7 TB/s), 32 rows by 8 of 256 experts of 7168 x 2048,
+// 64 here, 107 and 56 us for the two products (6.7 TB/s).
 template <int NT, int MT, int NW, int EPI>
 __global__ __launch_bounds__(64 * NW) void vx_i8_stream_kernel(VxI8Args a, uint32_t n_blocks) {
     constexpr bool kGrouped = EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT, kSwiglu = EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN;
@@ -327,9 +331,10 @@ hipError_t vx_allow_lds(const void* kernel, uint32_t bytes, std::atomic<uint64_t
 
 constexpr uint32_t kRowWaves = 4;
 
-// Up to four rows (STORE, SWIGLU), or one slot's row for its expert (HIDDEN): the first weights are requested, the workgroup
-// puts the rows into 8 bits in LDS, its waves take the columns' tiles in turn. Saves the launch that quantizes: one row of 4096 x
-// 4096 fp32.
+// One or two rows (STORE, SWIGLU), or one slot's row for its expert (HIDDEN): the first weights are requested, the workgroup
+// puts the rows into 8 bits in LDS, its waves take the columns' tiles in turn. Saves the launch that quantizes (one row of 4096 x
+// 4096 fp32: 7.6 -> 6.2 us). Bound by latency: the row, its largest value, then 16 KB of weights a wave; one slot's gate and up
+// (6 of 64 experts of 2048 x 1408, 35 MB): 9.3 us.
 template <class T, int NV, int NT, int EPI>
 __global__ __launch_bounds__(64 * kRowWaves) void vx_i8_row_kernel(VxI8Args a, VxI8View x, uint32_t n_blocks) {
     constexpr bool kSwiglu = EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN;
@@ -377,7 +382,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void vx_i8_row_kernel(VxI8Args a, V
 }
 
 // 16 outputs of a row: each wave takes slots of the row in turn, puts the slot's hidden row into 8 bits in its own piece of LDS
-// while its expert's weights are on their way, and multiplies; the answers meet in LDS and are added in the slots' order.
+// while its expert's weights are on their way, and multiplies; the answers meet in LDS and are added in the slots' order. Bound by
+// latency as above (6 of 64 experts of 2048 x 1408, 17 MB: 9.5 us).
 constexpr uint32_t kAnswerWaves = 8, kAnswerMost = 8u * 4u * 64u;  // values of a hidden row
 __global__ __launch_bounds__(64 * kAnswerWaves) void vx_i8_answer_kernel(VxI8Args a, VxCombineArgs c, uint32_t n_blocks) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -441,7 +447,9 @@ hipError_t vx_i8_row_launch_t(const VxI8Args& a, const VxI8View& x, hipStream_t 
 // a time, two stages; a column quarter's operands are read while the one before is multiplied, and the barrier between
 // two stages stands in front of the last quarter's products, behind which everything of the stage is in registers.
 // Weights lie in LDS as in memory (1 KiB tiles, operand reads of 256 neighbouring bytes); an activation row's 16-byte units
-// are exchanged by row, so that sixteen rows' reads of one unit meet all 64 banks.
+// are exchanged by row, so that sixteen rows' reads of one unit meet all 64 banks. What bounds it: at 256 x 256 power (8192 rows of
+// 8192 x 29568 in 1480 to 1580 us, 2.5 to 2.7 Pop/s, the matrix cores busy in 74 % of the clocks at 1.4 to 1.7 GHz; 8192 cubed with
+// the products removed 371 of 461 us, with the loads removed 388), with few columns the way there and back (64 x 64: 5.2 us).
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 // 16 bytes a lane from memory to lds + 16 lane; once: with the non-temporal hint.
@@ -709,8 +717,8 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
 
 // Grouped products: blocks of up to 256 of an expert's positions by 256 weight rows, eight waves of 64 weight rows by half of the
 // positions. As many blocks of 64 positions are fetched and multiplied as there are (by tiles of 128, padded, 4096 rows of 8 experts,
-// 64 of 256 here, took 978 us, so 840), and the fewer they are, the more stages LDS holds. An expert whose weights one block
-// reads passes the caches by (512 rows: 506 -> 470 us). What bounds it there: the weights' way to LDS (without the products 783 us,
+// 64 of 256 here, took 978 us, so 830), and the fewer they are, the more stages LDS holds. An expert whose weights one block
+// reads passes the caches by (512 rows: 506 -> 465 us). What bounds it there: the weights' way to LDS (without the products 783 us,
 // without any loads 517).
 constexpr uint32_t kItemRows = 256u;
 template <int L>
@@ -808,7 +816,7 @@ hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k,
 
 // Positions of a block of a grouped product, by how many slots there are for an expert (64 of 256 experts of 7168 x 2048 here, 8 for
 // a row): 32 rows 185 us by 16 and by 32, 128 rows 295 and 279, 256 rows 374 by 32 and 361 by tiles, 512 rows 607 and 470. Where
-// blocks of 256 would not even be one for each CU, 64 (257 rows through 5 experts of 576 x 1100).
+// blocks of 256 would not even be one for each CU, 64 (257 rows through 5 experts of 576 x 1100: 36 -> 28 us).
 uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count, uint32_t n_tiles) {
     if (slots < 32u * count) return slots >= 12u * count ? 32u : 16u;
     return (uint64_t)(slots / kItemRows + count) * ((n_tiles + 15u) / 16u) < 256u ? kSmallItemRows : kItemRows;
@@ -817,7 +825,8 @@ uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count, uint32_t n_tiles) {
 // Up to 16 rows the streaming kernel with one weight tile a workgroup (4096 x 4096, one row: two tiles 6.1 us, one 5.0) or,
 // where more rows share a tile of a large matrix, two (8192 x 8192, 16 rows: 16.1, 14.2); up to 32 rows two tiles and eight
 // waves (8192 x 8192: 17.3, four and four 27.7), four and four from 1024 tiles on (28672 x 4096 paired: 30.0, 23.9), six and four where
-// those were over two workgroups a CU (37888 x 3584 paired: 35.6, 31.9, 29.6). From 33 rows on tiles through LDS, as large as leave the CUs work: 128 x 32 up to 64 rows (8192 x 8192: 18.1, streaming 21.3), then
+// those were over two workgroups a CU (37888 x 3584 paired: 35.6, 31.9, 29.6). From 33 rows on tiles through LDS, as large as
+// leave the CUs work: 128 x 32 up to 64 rows (8192 x 8192: 18.1, streaming 21.3), then
 //   64 x 64 (four stages) up to 100 tiles of 128 x 128 (1037 rows of 960 x 576: 8.3 -> 4.9 us, 200 of 4096 x 14336: 67 -> 29),
 //   128 x 64 (three stages) up to 160 (1000 rows of 2048 x 2048: 10.9 by 64 x 64, 10.1, 16.0 by 128 x 128),
 //   128 x 128 (three stages: one workgroup a CU) up to 256 (300 rows of 8192 x 8192: 43 by two stages, 31.6),
