@@ -32,7 +32,7 @@ __device__ __forceinline__ bool vx_above(float a, float as, float b, float bs) {
 // A row's groups that take part, as a mask, by marks of the choice values in `all` (LDS, one wave's). L lanes a group.
 template <class F>
 __device__ __forceinline__ uint64_t vx_open_groups(const VxRouteArgs& a, const F* all, F* marks, bool& unsure) {
-    const uint32_t lane = threadIdx.x & 63u, size = a.n_experts / a.groups, L = 1u << a.group_lanes, g = lane >> a.group_lanes, sub = lane & (L - 1u);
+    const uint32_t lane = threadIdx.x & 63u, size = a.group_size, L = 1u << a.group_lanes, g = lane >> a.group_lanes, sub = lane & (L - 1u);
     F best = -INFINITY, next = -INFINITY;
     if (g < a.groups)
         for (uint32_t j = sub; j < size; j += L) {
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
         for (uint32_t i = 0; i < ITEMS; ++i) pick[i] = x[i];
     }
     uint64_t open = ~0ull;
-    const uint32_t size = a.n_experts / a.groups;
+    const auto shut = [&](uint32_t e) { return marked && !(open >> (e * a.by_size >> 20 & 63u) & 1u); };
     if (marked) {
         float* all = (float*)room[wave];
 #pragma unroll
@@ -149,34 +149,80 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
         for (uint32_t i = 0; i < ITEMS; ++i) {
             const uint32_t e = lane + 64u * i;
             float v = by_logits ? x[i] : pick[i] + 0.0f;
-            if (e >= a.n_experts || (marked && !(open >> (e / size) & 1u))) v = -INFINITY;
+            if (e >= a.n_experts || shut(e)) v = -INFINITY;
             key[i] = vx_word_of(v);
         }
-        float before = 0.0f;
-        for (uint32_t j = 0; j < a.top + (by_logits ? 0u : 1u); ++j) {
-            uint32_t best = key[0];
+        constexpr bool kSorted = ITEMS <= 4;  // each lane's experts from the largest down, equal ones by index: its first is looked at
+        uint32_t place[ITEMS];
 #pragma unroll
-            for (uint32_t i = 1; i < ITEMS; ++i) best = best > key[i] ? best : key[i];
+        for (uint32_t i = 0; i < ITEMS; ++i) place[i] = lane + 64u * i;
+        if constexpr (kSorted) {
+#pragma unroll
+            for (uint32_t end = ITEMS - 1u; end > 0u; --end)
+#pragma unroll
+                for (uint32_t i = 0; i < end; ++i) {
+                    const bool turn = key[i + 1] > key[i];
+                    const uint32_t k0 = key[i], p0 = place[i];
+                    key[i] = turn ? key[i + 1] : k0;
+                    key[i + 1] = turn ? k0 : key[i + 1];
+                    place[i] = turn ? place[i + 1] : p0;
+                    place[i + 1] = turn ? p0 : place[i + 1];
+                }
+        }
+        uint32_t found = 0, mine = 0, next = 0;  // lane j: the key of the j-th choice; the one behind the last
+        for (;; ++found) {
+            uint32_t best = key[0];
+            if constexpr (!kSorted) {
+#pragma unroll
+                for (uint32_t i = 1; i < ITEMS; ++i) best = best > key[i] ? best : key[i];
+            }
             best = vx_wave_max(best);
             if (best <= none) break;
-            if (!by_logits) {
-                const float v = vx_float_of(best);
-                unsure = unsure || (j && !vx_above(before, fabsf(before), v, fabsf(v)));
-                before = v;
-                if (j == a.top) break;
+            if (found == a.top) {
+                next = best;
+                break;
             }
-            uint32_t at = 0;  // the lowest index that has it
-            uint64_t lanes = 0;
+            uint32_t e;
+            if constexpr (kSorted) {
+                uint64_t lanes = __ballot(key[0] == best);
+                if (ITEMS > 1 && (lanes & (lanes - 1u))) {  // the lowest index that has it
+                    for (uint32_t end = 64u;; end += 64u) {
+                        const uint64_t m = __ballot(key[0] == best && place[0] < end);
+                        if (!m) continue;
+                        lanes = m;
+                        break;
+                    }
+                }
+                const uint32_t l = (uint32_t)__builtin_ctzll(lanes);
+                e = (uint32_t)__builtin_amdgcn_readlane((int)place[0], (int)l);
+                const bool taken = lane == l;
 #pragma unroll
-            for (uint32_t i = 0; i < ITEMS; ++i) {
-                const uint64_t m = __ballot(key[i] == best);
-                at = lanes ? at : i;
-                lanes = lanes ? lanes : m;
+                for (uint32_t i = 0; i < ITEMS; ++i) {
+                    key[i] = taken ? (i + 1 < ITEMS ? key[i + 1 < ITEMS ? i + 1 : i] : 0u) : key[i];
+                    if (i + 1 < ITEMS) place[i] = taken ? place[i + 1 < ITEMS ? i + 1 : i] : place[i];
+                }
+            } else {
+                uint32_t at = 0;  // the lowest index that has it
+                uint64_t lanes = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < ITEMS; ++i) {
+                    const uint64_t m = __ballot(key[i] == best);
+                    at = lanes ? at : i;
+                    lanes = lanes ? lanes : m;
+                }
+                const uint32_t l = (uint32_t)__builtin_ctzll(lanes);
+#pragma unroll
+                for (uint32_t i = 0; i < ITEMS; ++i) key[i] = i == at && lane == l ? 0u : key[i];
+                e = l + 64u * at;
             }
-            const uint32_t l = (uint32_t)__builtin_ctzll(lanes);
-#pragma unroll
-            for (uint32_t i = 0; i < ITEMS; ++i) key[i] = i == at && lane == l ? 0u : key[i];
-            id = lane == j ? l + 64u * at : id;
+            id = lane == found ? e : id;
+            mine = lane == found ? best : mine;
+            if (by_logits && found + 1u == a.top) break;
+        }
+        if (!by_logits) {  // neighbours in the order, and the last that is in and the first that is out, have to be apart
+            const float v = vx_float_of(mine), up = __shfl_up(v, 1), last = __shfl(v, (int)(a.top - 1u)), first_out = vx_float_of(next);
+            unsure = __ballot(lane && lane < found && !vx_above(up, fabsf(up), v, fabsf(v))) != 0;
+            unsure = unsure || (next && !vx_above(last, fabsf(last), first_out, fabsf(first_out)));
         }
     }
     // 64-bit scores: of what was chosen; of all where the softmax's sum is wanted, or the choice is made again
@@ -211,7 +257,7 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
             uint32_t at = 0xFFFFFFFFu;
             for (uint32_t e = lane; e < a.n_experts; e += 64u) {
                 // (without a bias equal scores of different logits keep the logits' order: the largest logit comes first)
-                const double v = marked && !(open >> (e / size) & 1u) ? -INFINITY : by_logits && all[e] > -INFINITY ? (double)logit(e) : all[e];
+                const double v = shut(e) ? -INFINITY : by_logits && all[e] > -INFINITY ? (double)logit(e) : all[e];
                 if (v > best) {
                     best = v;
                     at = e;
@@ -238,8 +284,7 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
     }
     if (a.renorm) {
         double sum = s;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
+        for (uint32_t off = 1; off < a.top; off <<= 1) sum += __shfl_xor(sum, (int)off);  // (behind lane top - 1 all are 0)
         s = sum > 0.0 ? s / sum : 0.0;
     }
     if (lane >= a.top) return;
@@ -495,6 +540,8 @@ static hipError_t vx_route_launch(const VxRouteArgs& a, hipStream_t st) {
 }
 hipError_t vx_launch_route(const VxRouteArgs& args, hipStream_t st) {
     VxRouteArgs a = args;
+    a.group_size = a.n_experts / a.groups;
+    a.by_size = (1u << 20) / a.group_size + 1u;  // (too large by less than 1023 / 2^20 of a group, below 1 / group_size)
     a.group_lanes = 0;
     while ((2u << a.group_lanes) * a.groups <= 64u) ++a.group_lanes;
     if (a.x.dtype == VELOX_DT_F32) return vx_route_launch<float>(a, st);

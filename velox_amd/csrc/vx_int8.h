@@ -64,7 +64,8 @@ struct VxRouteArgs {
     float scale;
     uint32_t* ids;
     float* weights;
-    uint32_t group_lanes;      // set by the launcher: 2^group_lanes lanes for each group
+    // set by the launcher: 2^group_lanes lanes for each group; experts of one; e < 1024 is of group e * by_size >> 20
+    uint32_t group_lanes, group_size, by_size;
 };
 
 struct VxGroupArgs {
