@@ -145,6 +145,25 @@ def test_route_scores_next_to_each_other():
     check_route(x, 16, bias=torch.full((128,), 0.125, device="cuda"))
 
 
+@pytest.mark.parametrize("n", [64, 200, 256, 1024])
+def test_route_a_few_or_many_too_near_to_tell(n):
+    """Logits with clusters of 2 to 100 neighbours that differ by less than fp32 scores show, some of them equal; groups
+    whose marks do as well."""
+    g = gen(n)
+    x = torch.randn(40, n, generator=g, device="cuda")
+    for r in range(40):
+        size = (2, 3, 10, 63, 64, 65, 100, n)[r % 8]
+        at = torch.randperm(n, generator=g, device="cuda")[:size]
+        x[r, at] = 3.0 + (r % 5) * 0.5 + torch.randint(0, 8, (len(at),), generator=g, device="cuda") * 2.0 ** -21
+    bias = torch.zeros(n, device="cuda")
+    some = torch.randint(0, 2, (n,), generator=g, device="cuda") * 0.25
+    for kw in (dict(bias=bias, scores="sigmoid"), dict(bias=some, scores="sigmoid", renormalize=True), dict(bias=bias), dict(bias=some, renormalize=True),
+               dict(bias=bias, scores="sigmoid", groups=4, top_groups=2, group_by="two"), dict(groups=4, top_groups=2, group_by="two"),
+               dict(bias=some, groups=8, top_groups=3)):
+        for top in (1, 8) if "groups" in kw else (1, 8, 64):
+            check_route(x, top, **kw)
+
+
 def test_route_strided_rows_and_given_outputs():
     wide = torch.randn(20, 100, generator=gen(2), device="cuda").bfloat16()
     x = wide[:, 13:77]

@@ -73,10 +73,12 @@ __device__ __forceinline__ uint64_t vx_open_groups(const VxRouteArgs& a, const F
 }
 
 // One wave per row; lane l holds experts l, l + 64, ... Without a bias the order is the logits'. With one, and for sums of two
-// marks, choice values are first formed in fp32; where two that decide are too near to each other for that (about one row in 300 of 256
-// experts), the row is done again in 64 bits. The largest is found top_k times: by DPP in the wave, its place by ballots. The
-// chosen scores are formed in 64 bits. What bounds it: instructions, about 1000 a row (16384 rows of 256 experts, 8 of them in 4
-// of 8 groups: 40 us, of which reading takes 4); one row 5.9 us.
+// marks, choice values are first formed in fp32. Where two marks that decide are too near to each other for that, the groups are chosen
+// again in 64 bits; where two choices are (about one row in 300 of 256 experts), the experts that may be among the chosen are
+// ordered again in 64 bits, each by how many are above it (all experts again, one choice after the other, took 10 us, which a launch
+// with one such row waited for: 4096 rows 18.7 -> 9.9 us). The largest is found top_k times: by DPP in the wave, its place
+// by ballots. The chosen scores are formed in 64 bits. What bounds it: instructions, about 800 of the vector unit and 350 of the
+// scalar one a row (16384 rows of 256 experts, 8 of them in 4 of 8 groups: 25 us, of which reading takes 4); one row 5.5 us.
 template <class T, uint32_t ITEMS>
 __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
     __shared__ double room[4][ITEMS * 64u + kVxMaxGroups];
@@ -139,19 +141,51 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
         for (uint32_t i = 0; i < ITEMS; ++i) all[lane + 64u * i] = pick[i];
         vx_wave_sync();
         open = vx_open_groups<float>(a, all, all + ITEMS * 64u, unsure);
-        unsure = unsure && (!by_logits || a.two);
+    }
+    // 64-bit scores. The softmax's sum is formed where it is wanted, once.
+    const auto exact = [&](float v) { return a.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : v > -INFINITY ? exp((double)v - (double)top) : 0.0; };
+    double all_sum = 0.0;
+    bool summed = a.sigmoid != 0;
+    // (a rolled loop's numbers come from LDS: with an index that is not a constant the registers' arrays would go to memory)
+    const auto spread = [&](double* all) {
+#pragma unroll
+        for (uint32_t i = 0; i < ITEMS; ++i) all[lane + 64u * i] = __builtin_bit_cast(double, make_float2(x[i], bias[i]));
+    };
+    const auto sum_all = [&](double* all) {
+        summed = true;
+        spread(all);
+#pragma unroll 1
+        for (uint32_t i = 0; i < ITEMS; ++i) all_sum += exact(__builtin_bit_cast(float2, all[lane + 64u * i]).x);
+#pragma unroll 1
+        for (int off = 1; off < 64; off <<= 1) all_sum += __shfl_xor(all_sum, off);
+    };
+    const auto score = [&](float v) { return a.sigmoid ? exact(v) : all_sum > 0.0 ? exact(v) / all_sum : 0.0; };
+    const auto choices = [&](double* all) {
+        if (!summed) sum_all(all);
+        spread(all);
+#pragma unroll 1
+        for (uint32_t i = 0; i < ITEMS; ++i) {
+            const float2 v = __builtin_bit_cast(float2, all[lane + 64u * i]);
+            all[lane + 64u * i] = v.x > -INFINITY && fabsf(v.y) < INFINITY ? score(v.x) + (double)v.y : -INFINITY;
+        }
+        vx_wave_sync();
+    };
+    if (unsure && (!by_logits || a.two)) {
+        double* all = room[wave];
+        bool never = false;
+        choices(all);
+        open = vx_open_groups<double>(a, all, all + ITEMS * 64u, never);
     }
     uint32_t id = kVxNoExpert;  // lane j: the j-th choice
-    if (!unsure) {
+    {
         uint32_t key[ITEMS];
         const uint32_t none = vx_word_of(-INFINITY);
-#pragma unroll
-        for (uint32_t i = 0; i < ITEMS; ++i) {
+        const auto value = [&](uint32_t i) {
             const uint32_t e = lane + 64u * i;
-            float v = by_logits ? x[i] : pick[i] + 0.0f;
-            if (e >= a.n_experts || shut(e)) v = -INFINITY;
-            key[i] = vx_word_of(v);
-        }
+            return e >= a.n_experts || shut(e) ? -INFINITY : by_logits ? x[i] : pick[i] + 0.0f;
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < ITEMS; ++i) key[i] = vx_word_of(value(i));
         constexpr bool kSorted = ITEMS <= 4;  // each lane's experts from the largest down, equal ones by index: its first is looked at
         uint32_t place[ITEMS];
 #pragma unroll
@@ -221,61 +255,82 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
         }
         if (!by_logits) {  // neighbours in the order, and the last that is in and the first that is out, have to be apart
             const float v = vx_float_of(mine), up = __shfl_up(v, 1), last = __shfl(v, (int)(a.top - 1u)), first_out = vx_float_of(next);
-            unsure = __ballot(lane && lane < found && !vx_above(up, fabsf(up), v, fabsf(v))) != 0;
-            unsure = unsure || (next && !vx_above(last, fabsf(last), first_out, fabsf(first_out)));
+            const bool near = (lane && lane < found && !vx_above(up, fabsf(up), v, fabsf(v))) || (next && !vx_above(last, fabsf(last), first_out, fabsf(first_out)));
+            if (__ballot(near)) {
+                // Again, in 64 bits: of the experts that are not certainly below the last choice, as a list by index, each lane's
+                // goes behind as many as are above it.
+                const auto candidate = [&](uint32_t i) {
+                    const float c = value(i);
+                    return c > -INFINITY && (found < a.top || !vx_above(last, fabsf(last), c, fabsf(c)));
+                };
+                uint32_t n = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < ITEMS; ++i) n += (uint32_t)__popcll(__ballot(candidate(i)));
+                if (!summed) sum_all(room[wave]);
+                id = kVxNoExpert;
+                if (n <= 64u) {
+                    uint4* list = (uint4*)room[wave];  // {index, logit, bias}
+                    uint32_t front = 0;
+#pragma unroll
+                    for (uint32_t i = 0; i < ITEMS; ++i) {
+                        const bool in = candidate(i);
+                        const uint64_t m = __ballot(in);
+                        if (in) list[front + (uint32_t)__popcll(m & ((1ull << lane) - 1ull))] =
+                            make_uint4(lane + 64u * i, __builtin_bit_cast(uint32_t, x[i]), __builtin_bit_cast(uint32_t, bias[i]), 0u);
+                        front += (uint32_t)__popcll(m);
+                    }
+                    vx_wave_sync();
+                    const uint4 c = list[lane < n ? lane : 0u];
+                    const double d = score(__builtin_bit_cast(float, c.y)) + (double)__builtin_bit_cast(float, c.z);
+                    vx_wave_sync();
+                    double* values = room[wave];
+                    uint32_t* order = (uint32_t*)(values + 64);
+                    values[lane] = d;
+                    vx_wave_sync();
+                    uint32_t above = 0;
+                    for (uint32_t j = 0; j < n; ++j) {
+                        const double o = values[j];
+                        above += o > d || (o == d && j < lane);
+                    }
+                    if (lane < n) order[above] = c.x;
+                    vx_wave_sync();
+                    if (lane < a.top && lane < n) id = order[lane];
+                } else {
+                    double* all = room[wave];
+                    choices(all);
+                    for (uint32_t j = 0; j < a.top; ++j) {
+                        double most = -INFINITY;
+                        uint32_t at = 0xFFFFFFFFu;
+                        for (uint32_t e = lane; e < a.n_experts; e += 64u) {
+                            const double o = shut(e) ? -INFINITY : all[e];
+                            if (o > most) {
+                                most = o;
+                                at = e;
+                            }
+                        }
+#pragma unroll
+                        for (int off = 1; off < 64; off <<= 1) {
+                            const double ob = __shfl_xor(most, off);
+                            const uint32_t oa = __shfl_xor(at, off);
+                            if (ob > most || (ob == most && oa < at)) {
+                                most = ob;
+                                at = oa;
+                            }
+                        }
+                        if (at == 0xFFFFFFFFu) break;
+                        if ((at & 63u) == lane) all[at] = -INFINITY;
+                        if (lane == j) id = at;
+                    }
+                }
+            }
         }
     }
-    // 64-bit scores: of what was chosen; of all where the softmax's sum is wanted, or the choice is made again
-    double all_sum = 0.0;
-    const bool whole = !a.sigmoid && (unsure || !a.renorm);
-    const auto exact = [&](float v) { return a.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : v > -INFINITY ? exp((double)v - (double)top) : 0.0; };
-    if (whole) {
+    const bool whole = !a.sigmoid && !a.renorm;
+    if (whole && !summed) {
 #pragma unroll
         for (uint32_t i = 0; i < ITEMS; ++i) all_sum += exact(x[i]);
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) all_sum += __shfl_xor(all_sum, off);
-    }
-    if (unsure) {
-        double* all = room[wave];
-#pragma unroll 1
-        for (uint32_t i = 0; i < ITEMS; ++i) {
-            float v = x[0], b = bias[0];
-#pragma unroll
-            for (uint32_t q = 1; q < ITEMS; ++q) {
-                v = i == q ? x[q] : v;
-                b = i == q ? bias[q] : b;
-            }
-            const double s = a.sigmoid ? exact(v) : all_sum > 0.0 ? exact(v) / all_sum : 0.0;
-            all[lane + 64u * i] = v > -INFINITY && fabsf(b) < INFINITY ? s + (double)b : -INFINITY;
-        }
-        vx_wave_sync();
-        bool never = false;
-        if (marked) open = vx_open_groups<double>(a, all, all + ITEMS * 64u, never);
-        id = kVxNoExpert;
-        for (uint32_t j = 0; j < a.top; ++j) {
-            double best = -INFINITY;
-            uint32_t at = 0xFFFFFFFFu;
-            for (uint32_t e = lane; e < a.n_experts; e += 64u) {
-                // (without a bias equal scores of different logits keep the logits' order: the largest logit comes first)
-                const double v = shut(e) ? -INFINITY : by_logits && all[e] > -INFINITY ? (double)logit(e) : all[e];
-                if (v > best) {
-                    best = v;
-                    at = e;
-                }
-            }
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const double ob = __shfl_xor(best, off);
-                const uint32_t oa = __shfl_xor(at, off);
-                if (ob > best || (ob == best && oa < at)) {
-                    best = ob;
-                    at = oa;
-                }
-            }
-            if (at == 0xFFFFFFFFu) break;
-            if ((at & 63u) == lane) all[at] = -INFINITY;
-            if (lane == j) id = at;
-        }
     }
     double s = 0.0;
     if (id != kVxNoExpert) {
