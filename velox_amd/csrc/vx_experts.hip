@@ -443,16 +443,22 @@ __device__ __forceinline__ void vx_group_place(const VxGroupArgs& a, uint32_t bl
     const VxKeys k = vx_keys(a, run);
     if (threadIdx.x < 64u) sizes[threadIdx.x] = 0;
     uint32_t mine[PER], front[PER];
+    // 32 workgroups' counts on the way at a time (behind the last they are 0)
+    const auto hist = __builtin_amdgcn_make_buffer_rsrc((void*)a.hist, 0, blocks > 1u ? (int)(blocks * a.count * 4u) : 0, 0x00020000);
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
         const uint32_t e = threadIdx.x * PER + j;
         mine[j] = front[j] = 0;
         if (blocks > 1u && e < a.count) {
-#pragma unroll 16
-            for (uint32_t b = 0; b < blocks; ++b) {
-                const uint32_t c = a.hist[(size_t)b * a.count + e];
-                front[j] += b < block ? c : 0u;
-                mine[j] += c;
+            for (uint32_t b0 = 0; b0 < blocks; b0 += 32u) {
+                uint32_t c[32];
+#pragma unroll
+                for (uint32_t b = 0; b < 32u; ++b) c[b] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(hist, (int)(((b0 + b) * a.count + e) * 4u), 0, 0);
+#pragma unroll
+                for (uint32_t b = 0; b < 32u; ++b) {
+                    front[j] += b0 + b < block ? c[b] : 0u;
+                    mine[j] += c[b];
+                }
             }
         }
     }
