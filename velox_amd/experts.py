@@ -9,6 +9,7 @@ given. There is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -66,12 +67,18 @@ def _device_index(device) -> torch.device:
     return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
 
 
+@functools.lru_cache(maxsize=1024)
+def _group_bytes(slots: int, count: int) -> int:
+    n = C.c_uint64()
+    L.check(_lib().velox_hip_expert_group_bytes(slots, count, C.byref(n)), "expert_group_bytes")
+    return n.value
+
+
 def group_workspace(slots: int, count: int, device="cuda") -> torch.Tensor | None:
     """What group() needs for up to `slots` slots of `count` experts (None: nothing)."""
-    n = C.c_uint64()
     _numbers("slots and count", slots, count)
-    L.check(_lib().velox_hip_expert_group_bytes(slots, count, C.byref(n)), "expert_group_bytes")
-    return _memory(n.value, device if isinstance(device, torch.device) else _device_index(device)) if n.value else None
+    n = _group_bytes(slots, count)
+    return _memory(n, device if isinstance(device, torch.device) else _device_index(device)) if n else None
 
 
 def group(ids: torch.Tensor, count: int, first: int = 0, *, order: torch.Tensor | None = None, offsets: torch.Tensor | None = None,
