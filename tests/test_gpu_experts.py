@@ -295,6 +295,17 @@ def test_ffn_where_slots_stop_being_done_one_by_one(n, inner, hidden):
         m.check(x, ids, w, m(x, ids, w))
 
 
+@pytest.mark.parametrize("n,hidden,inner", [(100, 256, 14336), (65, 100, 16001), (600, 48, 14336), (1500, 300, 8200)])
+def test_ffn_of_very_unequal_products(n, hidden, inner):
+    """A wide first product by large blocks, a narrow second one by parts of them, the last part partly filled or empty."""
+    m = Mixture(4, hidden, inner, seed=n)
+    x = rows(n, hidden, "bf16", 3)
+    ids, w = choice(n, 2, 4, 5, low=-1)
+    m.check(x, ids, w, m(x, ids, w))
+    ids[:, 0] = 2  # all rows to one expert
+    m.check(x, ids, w, m(x, ids, w))
+
+
 def test_ffn_weights_past_32_bits():
     """18 experts of 8192 x 16384: the last one's gate and up lie 4.5 GB in."""
     m = Mixture(18, 8192, 16384)

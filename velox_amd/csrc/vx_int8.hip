@@ -742,16 +742,21 @@ __global__ __launch_bounds__(512) void vx_i8_items_kernel(VxI8Args a, uint32_t n
     });
 }
 
-// The same by blocks of 64 positions and 64 weight rows, for experts so small that the larger blocks would leave most CUs idle.
+// The same by blocks of 64 positions and 64 weight rows, an item being `parts` of them: for experts so small that the larger
+// blocks would leave most CUs idle, and for one product of two whose larger blocks would (below 192 of them: 100 rows, 2 of 4 experts of
+// 256 x 14336, 123 -> 58 us by 64 x 64 in the second product; 300 rows, 2 of 8 of 4096 x 8192, 160 blocks, 237 -> 215; 1000 rows,
+// 2 of 8 of 4096 x 14336, 240 blocks, 568 -> 641).
 constexpr uint32_t kSmallItemRows = 64u;
 template <int EPI>
-__global__ __launch_bounds__(256) void vx_i8_small_items_kernel(VxI8Args a, uint32_t n_blocks) {
+__global__ __launch_bounds__(256) void vx_i8_small_items_kernel(VxI8Args a, uint32_t n_blocks, uint32_t parts) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
-    if (blockIdx.x >= uniform(*a.g.n_items) * n_blocks) return;
-    const uint2 it = a.g.items[blockIdx.x / n_blocks];
-    const uint32_t e = uniform(it.x);
-    vx_i8_tile<2, 2, 1, 1, 4, 4, EPI>(a, lds, uniform(blockIdx.x % n_blocks), e, uniform(it.y), uniform(a.g.offsets[e + 1u]), false);
+    const uint32_t block = uniform(blockIdx.x / n_blocks), item = uniform(block / parts);
+    if (item >= uniform(*a.g.n_items)) return;
+    const uint2 it = a.g.items[item];
+    const uint32_t e = uniform(it.x), first = uniform(it.y) + block % parts * kSmallItemRows, end = uniform(a.g.offsets[e + 1u]);
+    if (first >= end) return;
+    vx_i8_tile<2, 2, 1, 1, 4, 4, EPI>(a, lds, uniform(blockIdx.x % n_blocks), e, uniform(first), end, false);
 }
 
 constexpr uint32_t kTileStep = 1u << 20;  // rows of a launch
@@ -775,9 +780,9 @@ template <int EPI>
 hipError_t vx_i8_items_launch(const VxI8Args& a, hipStream_t st) {
     constexpr uint32_t lds = VxLive<1>::lds, small = 4 * (64 + 64) * 128;
     static_assert(lds <= 160 * 1024 && VxLive<3>::lds <= VxLive<1>::lds && VxLive<2>::lds <= VxLive<1>::lds && VxLive<4>::lds <= VxLive<1>::lds, "a CU's LDS");
-    if (a.item_rows == kSmallItemRows) {
-        const uint32_t n_blocks = (a.w.n_tiles + 3u) / 4u;
-        hipLaunchKernelGGL((vx_i8_small_items_kernel<EPI>), dim3(a.max_items * n_blocks), dim3(256), small, st, a, n_blocks);
+    if (a.item_rows == kSmallItemRows || (uint64_t)a.max_items * ((a.w.n_tiles + 15u) / 16u) < 192u) {
+        const uint32_t n_blocks = (a.w.n_tiles + 3u) / 4u, parts = a.item_rows / kSmallItemRows;
+        hipLaunchKernelGGL((vx_i8_small_items_kernel<EPI>), dim3(a.max_items * parts * n_blocks), dim3(256), small, st, a, n_blocks, parts);
         return hipGetLastError();
     }
     static std::atomic<uint64_t> allowed{0};
