@@ -164,6 +164,53 @@ def test_route_a_few_or_many_too_near_to_tell(n):
             check_route(x, top, **kw)
 
 
+def test_route_groups_whose_marks_cancel():
+    """Marks of two values far larger than their sum are off by more than the marks beside them are apart: a group in the
+    middle of the order, or one that is out, may be the one that is wrong."""
+    score = torch.tensor([0.6, 0.2, 0.5, 0.4, 0.45, 0.4, 0.1, 0.1], dtype=torch.float64)  # marks 0.8, 0.9, 0.85, 0.2
+    x = torch.log(score / (1 - score)).float().cuda().unsqueeze(0)
+    bias = torch.zeros(8, device="cuda")
+    bias[0], bias[1] = 1e7, -1e7
+    kw = dict(scores="sigmoid", bias=bias, groups=4, group_by="two")
+    check_route(x, 4, top_groups=2, **kw)
+    assert sorted(experts.route(x, 4, top_groups=2, **kw)[0][0].tolist()) == [2, 3, 4, 5]
+    for n, groups in ((8, 4), (64, 8), (256, 8), (60, 20), (512, 64), (1024, 16)):
+        size = n // groups
+        x = torch.randn(24, n, generator=gen(n), device="cuda")
+        x[5, :size], x[6, 2 * size:] = -math.inf, -math.inf  # groups without an expert
+        for large in (3e4, 1e5, 1e7, 1e12):
+            bias = torch.randn(n, generator=gen(n + 1), device="cuda") * 0.05
+            for g in range(0, groups, 3):
+                bias[g * size], bias[g * size + 1] = large, -large
+                bias[g * size + 2:(g + 1) * size] = -2 * large  # (the two are the group's mark)
+            for scores in ("sigmoid", "softmax"):
+                for top_groups in {1, 2, groups // 2, groups - 1}:
+                    check_route(x, min(4, size * top_groups), scores=scores, bias=bias, groups=groups, top_groups=top_groups, group_by="two")
+
+
+def test_route_marks_past_fp32():
+    """Two biases next to the largest number: their sum is a number in 64 bits, and above that of a group without an expert."""
+    most = torch.finfo(torch.float32).max
+    x = torch.randn(20, 24, generator=gen(7), device="cuda")
+    x[4, :4] = -math.inf
+    x[5, 4:8] = -math.inf
+    x[6, 4:] = -math.inf
+    x[7, :20] = -math.inf
+    x[8] = -math.inf
+    for signs in ((-1, -1), (1, 1), (1, -1)):
+        for at in (0, 1, 5):  # the group
+            bias = torch.zeros(24, device="cuda")
+            bias[4 * at:4 * at + 4] = -most
+            bias[4 * at], bias[4 * at + 1] = signs[0] * most, signs[1] * most
+            both = bias.clone()
+            both[8:12] = -most
+            for b in (bias, both, torch.full_like(bias, -most), torch.full_like(bias, most)):
+                for scores in ("sigmoid", "softmax"):
+                    for top_groups in (1, 2, 5, 6):
+                        check_route(x, 4, scores=scores, bias=b, groups=6, top_groups=top_groups, group_by="two")
+                        check_route(x, 4, scores=scores, bias=b, groups=6, top_groups=top_groups)
+
+
 def test_route_strided_rows_and_given_outputs():
     wide = torch.randn(20, 100, generator=gen(2), device="cuda").bfloat16()
     x = wide[:, 13:77]

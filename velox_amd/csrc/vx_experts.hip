@@ -25,9 +25,10 @@ __device__ __forceinline__ uint32_t vx_word_of(float f) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float vx_float_of(uint32_t w) { return __builtin_bit_cast(float, w & 0x80000000u ? w & 0x7FFFFFFFu : ~w); }
-// Whether a is above b for certain, where they are sums of numbers of sizes as and bs, each off by less than 2^-19 (1 + its
+// Whether a is above b for certain, where they are sums of numbers of sizes as and bs, each off by less than kVxOff (1 + its
 // size): a score in fp32 is off by 22 of its half steps at most (a sum of 1024), its sum with a bias by one more.
-__device__ __forceinline__ bool vx_above(float a, float as, float b, float bs) { return a - b > 1.9073486e-6f * (4.0f + as + bs); }
+constexpr float kVxOff = 1.9073486e-6f;  // 2^-19
+__device__ __forceinline__ bool vx_above(float a, float as, float b, float bs) { return a - b > kVxOff * (4.0f + as + bs); }
 
 // A row's groups that take part, as a mask, by marks of the choice values in `all` (LDS, one wave's). L lanes a group.
 template <class F>
@@ -50,7 +51,7 @@ __device__ __forceinline__ uint64_t vx_open_groups(const VxRouteArgs& a, const F
     const F mark = a.two && next > -INFINITY ? best + next : best;
     if (sub == 0 && g < a.groups) {
         marks[g] = mark;
-        if constexpr (sizeof(F) == 4) marks[kVxMaxGroups + g] = fabsf(best) + (a.two && next > -INFINITY ? fabsf(next) : 0.0f);
+        if constexpr (sizeof(F) == 4) marks[kVxMaxGroups + g] = best > -INFINITY ? fabsf(best) + (a.two && next > -INFINITY ? fabsf(next) : 0.0f) : 0.0f;
     }
     vx_wave_sync();
     uint32_t before = 0;  // lane g: the marks in front of group g's
@@ -59,14 +60,17 @@ __device__ __forceinline__ uint64_t vx_open_groups(const VxRouteArgs& a, const F
         const F m = marks[j];
         before += m > my || (m == my && j < lane);
     }
-    const uint64_t open = __ballot(lane < a.groups && before < a.top_groups);
+    const bool in = lane < a.groups && before < a.top_groups;
+    const uint64_t open = __ballot(in);
     if constexpr (sizeof(F) == 4) {
-        // the last mark that is in and the first that is out have to be apart
-        const uint64_t last = __ballot(lane < a.groups && before == a.top_groups - 1u), out = __ballot(lane < a.groups && before == a.top_groups);
-        if (out) {
-            const int in_at = (int)__builtin_ctzll(last), out_at = (int)__builtin_ctzll(out);
-            unsure = marks[out_at] > -INFINITY && !vx_above(marks[in_at], marks[kVxMaxGroups + in_at], marks[out_at], marks[kVxMaxGroups + out_at]);
-        }
+        // The least that a group that is in may be has to be above the most that one that is out may be: not the neighbours' in the
+        // order alone, since a mark of two may be off by far more than it is (1e7 + -1e7). One whose parts, or whose sum, overflow may
+        // be anything; a group without an expert is -infinity.
+        const float size = marks[kVxMaxGroups + (lane < a.groups ? lane : 0u)], off = kVxOff * (2.0f + size);
+        const bool known = size < INFINITY;
+        const float low = in ? (known ? my - off : -INFINITY) : INFINITY, high = in || lane >= a.groups ? -INFINITY : known ? my + off : INFINITY;
+        const uint32_t out = vx_wave_max(vx_word_of(high)), least = ~vx_wave_max(~vx_word_of(low));
+        unsure = out > vx_word_of(-INFINITY) && least <= out;
     }
     vx_wave_sync();
     return open;
