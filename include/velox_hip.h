@@ -633,13 +633,15 @@ typedef struct VeloxHipRouteConfig {
     uint32_t renormalize;        /* 0 or 1 */
     float scale;                 /* finite */
 } VeloxHipRouteConfig;
-/* logits [n_rows][n_experts] (heads 1), ids and weights [n_rows][top_k]. Fewer than 2^24 rows. */
+/* logits [n_rows][n_experts] (heads 1), ids and weights [n_rows][top_k], memory of their own (EINVAL where they overlap each
+ * other, the logits' rows or the bias). Fewer than 2^24 rows. */
 int velox_hip_expert_route(const VeloxHipRouteConfig* cfg, const VeloxHipRows* logits, const float* d_bias, uint32_t n_rows,
                            uint32_t* d_ids, float* d_weights, hipStream_t stream);
 /* The n_slots slots of d_ids (row r, place j: slot r * top_k + j) in the order of their experts first .. first + count - 1,
  * an expert's slots in their own order: d_order[offsets[e] .. offsets[e + 1]) are expert first + e's, d_offsets has count + 1
  * entries. Slots of other ids are left out; d_order behind the last offset is VELOX_HIP_NO_EXPERT. n_slots <= 2^20,
- * count <= 1024; workspace: velox_hip_expert_group_bytes (may be 0 bytes: NULL), 16-byte aligned. */
+ * count <= 1024; workspace: velox_hip_expert_group_bytes (may be 0 bytes: NULL), 16-byte aligned. The four are memory of
+ * their own (EINVAL where two overlap). */
 int velox_hip_expert_group_bytes(uint32_t n_slots, uint32_t count, uint64_t* bytes);
 int velox_hip_expert_group(const uint32_t* d_ids, uint32_t n_slots, uint32_t first, uint32_t count, uint32_t* d_order,
                            uint32_t* d_offsets, void* workspace, uint64_t workspace_bytes, hipStream_t stream);

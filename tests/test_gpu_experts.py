@@ -247,6 +247,35 @@ def test_group(rows, top, total, first, count):
         check_group(torch.full_like(ids, -2 ** 31), count, first)
 
 
+@pytest.mark.parametrize("n", [7, 1024, 1025, 9000])
+def test_group_memory_side_by_side_and_overlapping(n):
+    """Neighbours in one piece of memory are apart; a call in the ids' own place is refused at every size."""
+    room = torch.full((2 * n + 5,), -7, dtype=torch.int32, device="cuda")
+    ids, order, offsets = room[:n], room[n:2 * n], room[2 * n:]
+    ids.copy_(torch.randint(-1, 4, (n,), generator=gen(n), device="cuda", dtype=torch.int32))
+    want = experts.group(ids.clone(), 4)
+    got = experts.group(ids, 4, order=order, offsets=offsets)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    before = room.clone()
+    for call in (lambda: experts.group(ids, 4, order=ids), lambda: experts.group(ids, 4, order=room[1:n + 1]), lambda: experts.group(ids, 4, offsets=room[n - 1:n + 4])):
+        with pytest.raises(RuntimeError):
+            call()
+    assert torch.equal(room, before)
+
+
+def test_route_memory_side_by_side_and_overlapping():
+    """ids and weights between strided rows of logits, which they do not touch; where they do, the call is refused."""
+    room = torch.randn(9, 200, generator=gen(3), device="cuda")
+    x = room[:, :64]
+    want = experts.route(x.contiguous(), 4)
+    ids, w = room[2, 64:100].view(torch.int32).view(9, 4), room[5, 164:200].view(9, 4)
+    got = experts.route(x, 4, ids=ids, weights=w)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for kw in (dict(ids=room[2, 63:99].view(torch.int32).view(9, 4)), dict(weights=room.flatten()[1165:1201].view(9, 4)), dict(ids=ids, weights=ids.view(torch.float32))):
+        with pytest.raises(RuntimeError):
+            experts.route(x, 4, **kw)
+
+
 # ---- the experts' products ----
 
 class Mixture:

@@ -136,6 +136,46 @@ def test_refuses_group_arguments(hiplib):
         last = size
 
 
+def test_refuses_group_memory_that_overlaps(hiplib):
+    """Several workgroups read ids while others write order: every pair of the four has to be apart, by a byte at least."""
+    n, count = 5000, 8
+    rc, need = u64(hiplib.velox_hip_expert_group_bytes, n, count)
+    assert rc == 0 and need > 0
+    own = dict(ids=P, order=2 * P, offsets=3 * P, space=4 * P)
+    size = dict(ids=4 * n, order=4 * n, offsets=4 * (count + 1), space=need)
+    for a in own:
+        for b in own:
+            if a == b:
+                continue
+            ends = [0, 16, size[b] - 4, 4 - size[a]]  # where a begins, from b on: its start, inside, its last word, a's last word
+            for at in ends if "space" not in (a, b) else [0, 16, (size[b] - 1) // 16 * 16, -((size[a] - 1) // 16 * 16)]:
+                kw = dict(own, **{a: own[b] + at})
+                assert hiplib.velox_hip_expert_group(kw["ids"], n, 0, count, kw["order"], kw["offsets"], kw["space"], need, None) == L.EINVAL, (a, b, at)
+    for m in (1, 1024):  # one workgroup too
+        assert hiplib.velox_hip_expert_group(P, m, 0, count, P, 2 * P, None, 0, None) == L.EINVAL
+        assert hiplib.velox_hip_expert_group(P, m, 0, count, 2 * P, P + 4 * m - 4, None, 0, None) == L.EINVAL
+
+
+def test_refuses_route_memory_that_overlaps(hiplib):
+    n, c = 40, route_config()  # 64 experts, 4 of them
+    bytes_ = 4 * n * 4
+
+    def call(x=rows(), bias=None, ids=3 * P, w=4 * P):
+        return hiplib.velox_hip_expert_route(ref(c), ref(x), bias, n, ids, w, None)
+
+    for at in (0, 4, bytes_ - 4, 4 - bytes_):
+        assert call(w=3 * P + at) == L.EINVAL, at
+    last = P + 4 * 1024 * (n - 1)  # the last row's logits
+    for at in (P, P + 4 * 63, P + 4 * 1024 - 4 * 100, last, last + 4 * 63, P - bytes_ + 4):
+        for kw in (dict(ids=at), dict(w=at)):
+            assert call(**kw) == L.EINVAL, (at, kw)
+    half = rows(dtype=L.DT_BF16)
+    for at in (P, P + 124, P + 2 * 1024 * 7 + 124, P + 2 * 1024 * (n - 1) + 124):
+        assert call(x=half, ids=at) == L.EINVAL, at
+    for at in (5 * P, 5 * P + 252, 5 * P - bytes_ + 4):
+        assert call(bias=5 * P, ids=at) == L.EINVAL and call(bias=5 * P, w=at) == L.EINVAL, at
+
+
 def test_refuses_ffn_arguments(hiplib):
     gu, dn = matrix(n=128, k=256, count=4, paired=1), matrix(n=256, k=64, count=4)
 

@@ -44,6 +44,17 @@ bool same_or_apart(const VeloxHipRows* a, const VeloxHipRows* b, uint32_t n_rows
     return a->data != b->data || (elt(a->dtype) == elt(b->dtype) && (n_rows <= 1u || a->row_stride == b->row_stride));
 }
 
+// Whether [at, at + bytes) and n_rows rows of `len` bytes, `stride` bytes apart, have a byte in common.
+bool meet(const void* at, uint64_t bytes, const void* rows, uint64_t n_rows, uint64_t len, uint64_t stride) {
+    const uint64_t lo = (uint64_t)(uintptr_t)at, base = (uint64_t)(uintptr_t)rows;
+    if (!bytes || !n_rows || !len || base >= lo + bytes) return false;
+    if (base + len > lo) return true;
+    if (!stride) return false;
+    const uint64_t r = (lo - base - len) / stride + 1u;  // the first row that ends behind lo
+    return r < n_rows && base + r * stride < lo + bytes;
+}
+bool meet(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) { return meet(a, a_bytes, b, 1, b_bytes, 0); }
+
 // Every row begins at a whole multiple of four elements.
 bool whole(const VeloxHipRows* r) { return aligned(r->data, 4u * elt(r->dtype)) && r->row_stride % 4u == 0; }
 
@@ -180,6 +191,12 @@ int velox_hip_expert_route(const VeloxHipRouteConfig* cfg, const VeloxHipRows* l
     if (!route_ok(cfg) || !rows_ok(logits) || n_rows > kVxI8MaxRows || !aligned(d_bias, 4)) return VELOX_HIP_EINVAL;
     if (!n_rows) return VELOX_HIP_OK;
     if (!d_ids || !d_weights || !aligned(d_ids, 4) || !aligned(d_weights, 4)) return VELOX_HIP_EINVAL;
+    const uint64_t words = 4ull * n_rows * cfg->top_k, e = elt(logits->dtype);  // (waves read while others write)
+    if (meet(d_ids, words, d_weights, words)) return VELOX_HIP_EINVAL;
+    for (const void* to : {(const void*)d_ids, (const void*)d_weights})
+        if (meet(to, words, logits->data, n_rows, e * cfg->n_experts, e * logits->row_stride) ||
+            (d_bias && meet(to, words, d_bias, 4ull * cfg->n_experts)))
+            return VELOX_HIP_EINVAL;
     VxRouteArgs a;
     std::memset(&a, 0, sizeof(a));
     a.x = view(logits);
@@ -211,6 +228,11 @@ int velox_hip_expert_group(const uint32_t* d_ids, uint32_t n_slots, uint32_t fir
         return VELOX_HIP_EINVAL;
     const uint64_t need = 4ull * group_words(n_slots, count);
     if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need)) return VELOX_HIP_EINVAL;
+    const void* const at[4] = {d_ids, d_order, d_offsets, workspace};  // (workgroups read while others write)
+    const uint64_t bytes[4] = {4ull * n_slots, 4ull * n_slots, 4ull * (count + 1u), need};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (meet(at[i], bytes[i], at[j], bytes[j])) return VELOX_HIP_EINVAL;
     VxGroupArgs a;
     std::memset(&a, 0, sizeof(a));
     a.ids = d_ids;

@@ -34,7 +34,8 @@ def route(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", bias: to
           ids: torch.Tensor | None = None, weights: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(ids int32, weights float32), both [row][top_k]: the experts with the largest score (+ bias) of logits [row][expert], of
     the top_groups best groups where there are several; weights are the scores (renormalize: divided by their sum) times
-    scale. -infinity masks an expert; a row without enough experts ends in -1 with weight 0."""
+    scale. -infinity masks an expert; a row without enough experts ends in -1 with weight 0. ids and weights are memory of
+    their own."""
     device = _gpu(logits, "logits")
     how, mark = _SCORES.get(scores), _MARKS.get(group_by)
     if how is None or mark is None:
@@ -84,7 +85,8 @@ def group_workspace(slots: int, count: int, device="cuda") -> torch.Tensor | Non
 def group(ids: torch.Tensor, count: int, first: int = 0, *, order: torch.Tensor | None = None, offsets: torch.Tensor | None = None,
           workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(order int32 [slot], offsets int32 [count + 1]): the slots of ids (row * top_k + place) by expert first .. first +
-    count - 1, an expert's in their own order at order[offsets[e] : offsets[e + 1]]; -1 behind the last."""
+    count - 1, an expert's in their own order at order[offsets[e] : offsets[e + 1]]; -1 behind the last. ids, order, offsets
+    and workspace are memory of their own."""
     device = _gpu(ids, "ids")
     slots = ids.numel()
     at = _whole(ids, ids.shape, device, "ids")
