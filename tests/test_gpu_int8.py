@@ -233,6 +233,18 @@ def test_layout_of_strided_codes_and_quantized_weights():
     check(x, c, sw, int8.product(x, m))
 
 
+def test_outputs_whose_rows_overlap_are_refused():
+    w, sw = weights(48, 200, 1)
+    mat = int8.Int8Matrix(w, sw)
+    x, room = rows(3, 200, "f32", 2), torch.full((200,), 4.0, device="cuda")
+    for stride in (0, 47):
+        with pytest.raises(ValueError):
+            int8.product(x, mat, out=room.as_strided((3, 48), (stride, 1)))
+    assert (room == 4).all()
+    int8.product(x[:1], mat, out=room.as_strided((1, 48), (0, 1)))  # one row has no other
+    check(x[:1], w, sw, room[:48].view(1, 48))
+
+
 def test_captured_and_replayed_beside_eager_calls_on_another_stream():
     k, n = 1000, 300
     w, sw = weights(n, k, 1)

@@ -216,3 +216,25 @@ def test_python_refuses_tensors_of_the_host():
         experts.route(torch.zeros(2, 4), 1)
     with pytest.raises(ValueError):
         experts.group(torch.zeros(2, 4, dtype=torch.int32), 3)
+
+
+@pytest.mark.parametrize("stride", [0, 1, 47])
+def test_refuses_outputs_whose_rows_overlap(hiplib, stride):
+    assert product(hiplib, matrix(), out=rows(data=1 << 24, rs=stride)) == L.EINVAL
+    assert product(hiplib, matrix(), q=held(), out=rows(data=1 << 24, rs=stride)) == L.EINVAL
+    assert product(hiplib, matrix(n=96, paired=1), out=rows(data=1 << 24, rs=stride), mode=L.GEMV_SWIGLU) == L.EINVAL
+    out = rows(data=1 << 24, rs=stride)  # (the residual's own place does not help)
+    assert product(hiplib, matrix(), out=out, res=out, mode=L.GEMV_RESIDUAL) == L.EINVAL
+    gu, dn = matrix(n=128, k=48, count=4, paired=1), matrix(n=48, k=64, count=4)
+    assert hiplib.velox_hip_expert_ffn(ref(gu), ref(dn), 0, ref(rows()), P, P, 2, 2, None, ref(out), P, 1 << 50, None) == L.EINVAL
+
+
+def test_python_refuses_outputs_whose_rows_overlap():
+    torch = pytest.importorskip("torch")
+    from velox_amd import int8
+    cpu, room = torch.device("cpu"), torch.zeros(100)
+    for stride in (0, 1, 7):
+        with pytest.raises(ValueError):
+            int8._result(room.as_strided((3, 8), (stride, 1)), cpu, 8, 3)
+        assert int8._result(room.as_strided((1, 8), (stride, 1)), cpu, 8, 1).row_stride == stride
+    assert int8._result(room.as_strided((3, 8), (8, 1)), cpu, 8, 3).row_stride == 8

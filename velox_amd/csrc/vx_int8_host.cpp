@@ -34,6 +34,8 @@ uint32_t elt(uint32_t dtype) { return dtype == VELOX_DT_F32 ? 4u : 2u; }
 bool rows_ok(const VeloxHipRows* r) {
     return r && r->data && r->dtype <= VELOX_DT_BF16 && r->heads == 1 && aligned(r->data, elt(r->dtype));
 }
+// Rows that are written: each has a place of its own.
+bool out_ok(const VeloxHipRows* r, uint32_t n_rows, uint32_t cols) { return rows_ok(r) && (n_rows <= 1u || r->row_stride >= cols); }
 VxI8View view(const VeloxHipRows* r) { return VxI8View{r->data, r->row_stride, r->dtype}; }
 bool q_ok(const VeloxHipInt8Rows* q, uint32_t k) {
     return q && q->codes && q->scales && aligned(q->codes, 16) && aligned(q->scales, 4) && q->row_stride % 128u == 0 &&
@@ -155,7 +157,8 @@ int velox_hip_int8_product_bytes(const VeloxHipInt8Matrix* m, uint32_t n_rows, u
 int velox_hip_int8_product(const VeloxHipInt8Matrix* m, const VeloxHipRows* x, const VeloxHipInt8Rows* q, uint32_t n_rows,
                            const float* d_bias, const VeloxHipRows* residual, const VeloxHipRows* out, int mode, void* workspace,
                            uint64_t workspace_bytes, hipStream_t st) {
-    if (!matrix_ok(m) || m->count != 1 || n_rows > kVxI8MaxRows || !x == !q || !rows_ok(out)) return VELOX_HIP_EINVAL;
+    if (!matrix_ok(m) || m->count != 1 || n_rows > kVxI8MaxRows || !x == !q || !out_ok(out, n_rows, m->paired ? m->n / 2u : m->n))
+        return VELOX_HIP_EINVAL;
     if (mode < VELOX_GEMV_STORE || mode > VELOX_GEMV_SWIGLU || (mode == VELOX_GEMV_SWIGLU) != (m->paired != 0)) return VELOX_HIP_EINVAL;
     if ((mode == VELOX_GEMV_RESIDUAL) != (residual != nullptr) || (d_bias && mode == VELOX_GEMV_SWIGLU) || !aligned(d_bias, 4))
         return VELOX_HIP_EINVAL;
@@ -256,7 +259,8 @@ int velox_hip_expert_ffn_bytes(const VeloxHipInt8Matrix* gate_up, const VeloxHip
 int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Matrix* down, uint32_t first, const VeloxHipRows* x,
                          const uint32_t* d_ids, const float* d_weights, uint32_t n_rows, uint32_t top_k, const VeloxHipRows* residual,
                          const VeloxHipRows* out, void* workspace, uint64_t workspace_bytes, hipStream_t st) {
-    if (!ffn_ok(gate_up, down, n_rows, top_k) || !matrix_ok(gate_up) || !matrix_ok(down) || !rows_ok(x) || !rows_ok(out))
+    if (!ffn_ok(gate_up, down, n_rows, top_k) || !matrix_ok(gate_up) || !matrix_ok(down) || !rows_ok(x) ||
+        !out_ok(out, n_rows, down->n))
         return VELOX_HIP_EINVAL;
     if ((uint64_t)first + gate_up->count > kVxNoExpert || !same_or_apart(x, out, n_rows)) return VELOX_HIP_EINVAL;
     if (residual && (!rows_ok(residual) || !same_or_apart(residual, out, n_rows))) return VELOX_HIP_EINVAL;

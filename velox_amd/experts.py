@@ -14,7 +14,7 @@ import functools
 import torch
 
 from . import _lib as L
-from .int8 import Int8Matrix, _floats, _memory, _plain
+from .int8 import Int8Matrix, _floats, _memory, _plain, _result
 from .paged import _call, _gpu, _need, _numbers, _space, _words
 
 _lib = L.load  # (the library is looked up by the calls, not where this module is read)
@@ -140,7 +140,7 @@ def ffn(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_up: Int8
         out = torch.empty((n, gate_up.k), dtype=x.dtype, device=device)
         o = L.Rows(out.data_ptr(), xr.dtype, 1, gate_up.k, 0)
     else:
-        o, _ = _plain(out, device, "out", gate_up.k, n)
+        o = _result(out, device, gate_up.k, n)
     res = _plain(residual, device, "residual", gate_up.k, n)[0] if residual is not None else None
     if n == 0:
         return out

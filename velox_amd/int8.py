@@ -32,6 +32,14 @@ def _plain(t: torch.Tensor, device: torch.device, what: str, width: int = 0, row
     return L.Rows(t.data_ptr(), code, 1, rs, 0), n
 
 
+def _result(t: torch.Tensor, device: torch.device, width: int, rows: int) -> L.Rows:
+    """The given output: as _plain, its rows apart from each other."""
+    o, n = _plain(t, device, "out", width, rows)
+    if n > 1 and o.row_stride < width:
+        raise ValueError(f"out: rows that do not overlap are wanted, got {width} elements every {o.row_stride}")
+    return o
+
+
 def _floats(t: torch.Tensor, shape: tuple, device: torch.device, what: str) -> int:
     """The address of a contiguous float32 tensor of a shape."""
     if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
@@ -144,7 +152,7 @@ def product(x: torch.Tensor | Int8Rows, w: Int8Matrix, *, bias: torch.Tensor | N
         o = L.Rows(out.data_ptr(), _DTYPES[kind], 1, cols, 0)
     else:
         _need(dtype is None or out.dtype == dtype, "out: another type than dtype")
-        o, _ = _plain(out, device, "out", w.outputs, n)
+        o = _result(out, device, w.outputs, n)
     if w.paired and (bias is not None or residual is not None):
         raise ValueError("a paired product takes no bias and no residual")
     at = _floats(bias, (w.n,), device, "bias") if bias is not None else None
