@@ -238,3 +238,17 @@ def test_python_refuses_outputs_whose_rows_overlap():
             int8._result(room.as_strided((3, 8), (stride, 1)), cpu, 8, 3)
         assert int8._result(room.as_strided((1, 8), (stride, 1)), cpu, 8, 1).row_stride == stride
     assert int8._result(room.as_strided((3, 8), (8, 1)), cpu, 8, 3).row_stride == 8
+
+
+def test_python_refuses_rows_and_lengths_past_32_bits():
+    """ctypes would hand them on modulo 2^32, and all but the first rows, or the first values, would be left out."""
+    torch = pytest.importorskip("torch")
+    from velox_amd import int8
+    cpu = torch.device("cpu")
+    for t in (torch.zeros(1, 8).expand((1 << 32) + 5, 8), torch.zeros(1, 8, dtype=torch.bfloat16).expand(1 << 32, 8),
+              torch.empty(0).as_strided((0, (1 << 32) + 8), (1, 1))):
+        with pytest.raises(ValueError):
+            int8._plain(t, cpu, "x")
+        with pytest.raises(ValueError):
+            int8._plain(t, cpu, "x", t.shape[1])
+    assert int8._plain(torch.zeros(1, 8).expand((1 << 32) - 1, 8), cpu, "x")[1] == (1 << 32) - 1  # (the C ABI refuses these)

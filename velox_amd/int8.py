@@ -24,6 +24,8 @@ def _plain(t: torch.Tensor, device: torch.device, what: str, width: int = 0, row
     if t.requires_grad:
         _no_gradient(t, what)
     n, d = t.shape
+    if (n | d) >> 32:
+        _numbers(what, n, d)
     if (width and d != width) or (rows >= 0 and n != rows):
         raise ValueError(f"{what}: {rows if rows >= 0 else n} rows of {width or d} elements are wanted, got {n} of {d}")
     rs, es = t.stride()
