@@ -245,6 +245,15 @@ def test_outputs_whose_rows_overlap_are_refused():
     check(x[:1], w, sw, room[:48].view(1, 48))
 
 
+def test_weights_of_more_rows_than_a_call_takes():
+    """1024 matrices of 16385 rows, 2^24 + 1024 in all: as the last matrices alone."""
+    w = torch.randn(1024, 16385, 3, generator=gen(1), device="cuda", dtype=torch.float16)
+    many = int8.Int8Matrix.quantized(w)
+    for at in (0, 511, 1023):
+        one = int8.Int8Matrix.quantized(w[at])
+        assert torch.equal(many._codes.view(1024, -1)[at], one._codes) and torch.equal(many._scales.view(1024, -1)[at], one._scales)
+
+
 def test_captured_and_replayed_beside_eager_calls_on_another_stream():
     k, n = 1000, 300
     w, sw = weights(n, k, 1)

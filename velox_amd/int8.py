@@ -16,6 +16,9 @@ from . import _lib as L
 from .paged import _DTYPES, _call, _gpu, _need, _no_gradient, _numbers, _space
 
 
+_ROWS = 1 << 23  # of many more rows, those of a call (the C ABI takes fewer than 2^24)
+
+
 def _plain(t: torch.Tensor, device: torch.device, what: str, width: int = 0, rows: int = -1) -> tuple[L.Rows, int]:
     """[row][element] as VeloxHipRows, and its rows; the elements of a row are next to each other."""
     code = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
@@ -66,6 +69,13 @@ class Int8Rows:
         self.scales = torch.empty(rows, dtype=torch.float32, device=device)
         self.desc = L.Int8RowsDesc(self.codes.data_ptr(), self.scales.data_ptr(), self.codes.shape[1])
 
+    def _part(self, first: int, last: int) -> "Int8Rows":
+        """Rows first .. last - 1, in their place."""
+        p = Int8Rows.__new__(Int8Rows)
+        p.k, p.codes, p.scales = self.k, self.codes[first:last], self.scales[first:last]
+        p.desc = L.Int8RowsDesc(p.codes.data_ptr(), p.scales.data_ptr(), self.codes.shape[1])
+        return p
+
     def __len__(self) -> int:
         return self.codes.shape[0]
 
@@ -100,10 +110,12 @@ class Int8Matrix:
     @classmethod
     def quantized(cls, w: torch.Tensor, *, paired: bool = False) -> "Int8Matrix":
         """Of weights [n][k] or [matrix][n][k] of float32, float16 or bfloat16: each row by its largest value (quantize)."""
-        _need(isinstance(w, torch.Tensor) and w.dim() in (2, 3), "w: [n][k] or [matrix][n][k] is wanted")
-        rows = quantize(w.reshape(-1, w.shape[-1]))
+        _need(isinstance(w, torch.Tensor) and w.dim() in (2, 3) and min(w.shape) > 0, "w: [n][k] or [matrix][n][k] is wanted")
+        x = w.reshape(-1, w.shape[-1])
+        rows = Int8Rows(*x.shape, _gpu(x, "w"))
+        for r in range(0, len(rows), _ROWS):
+            quantize(x[r:r + _ROWS], rows._part(r, r + _ROWS))
         return cls(rows.codes.view(*w.shape[:-1], -1)[..., :w.shape[-1]], rows.scales.view(w.shape[:-1]), paired=paired)
-
 
 
 def quantize(x: torch.Tensor, out: Int8Rows | None = None) -> Int8Rows:
