@@ -209,6 +209,23 @@ def test_rows_that_lie_past_32_bits(m, step):
     assert torch.equal(int8.product(q, mat, residual=rr, dtype=torch.float16), out)
 
 
+@pytest.mark.parametrize("dtype", T)
+@pytest.mark.parametrize("n,k", [(96, 320), (1030, 200), (66, 2056)])
+def test_a_row_gives_the_same_bits_in_any_batch(n, k, dtype):
+    """Rows alone, among few and among many go through different kernels: the same sums, scales and roundings in each."""
+    x, w, sw = rows(1200, k, dtype, 3), *weights(2 * n, k, 4)
+    bias, res = torch.randn(2 * n, generator=gen(5), device="cuda"), rows(1200, 2 * n, dtype, 6)
+    plain, paired = int8.Int8Matrix(w, sw), int8.Int8Matrix(w, sw, paired=True)
+    calls = (lambda r: int8.product(x[r], plain), lambda r: int8.product(x[r], plain, bias=bias), lambda r: int8.product(x[r], plain, residual=res[r]),
+             lambda r: int8.product(x[r], plain, bias=bias, residual=res[r]), lambda r: int8.product(x[r], paired),
+             lambda r: int8.product(x[r], plain, residual=res[r], dtype=torch.float32), lambda r: int8.product(x[r], plain, bias=bias, residual=res[r].double().float()))
+    for call in calls:
+        whole = call(slice(0, 1200))
+        for m in (1, 2, 3, 16, 17, 20, 33, 40, 64, 65, 100, 300):
+            for at in (0, 1200 - m):
+                assert torch.equal(call(slice(at, at + m)), whole[at:at + m]), (m, at)
+
+
 def test_rows_behind_the_last_are_left_as_they_were():
     for m in (1, 7, 16, 33, 130, 257):
         x = rows(m, 256, "f32", 2)

@@ -17,22 +17,16 @@ __device__ __forceinline__ void vx_each(F f) {  // f(vx_int<0>) .. f(vx_int<N - 
     }
 }
 
-// Outputs n .. n + 3 of row r (of `cols` in a row), y their products with the bias: the residual added, stored.
-template <bool VEC>
-__device__ __forceinline__ void vx_finish(const VxI8Args& a, size_t r, uint32_t n, uint32_t cols, float4 y) {
-    const uint32_t left = cols - n;
-    if (a.res.data) {
-        const float4 v = vx_load4<VEC>(a.res.data, r * a.res.rs + n, a.res.dtype, left);
-        y.x += v.x;
-        y.y += v.y;
-        y.z += v.z;
-        y.w += v.w;
-    }
-    vx_store4<VEC>(a.out.data, r * a.out.rs + n, a.out.dtype, left, y);
+// A row's bits do not depend on the kernel that it goes through: sums of whole numbers are exact, and what follows is done by the
+// functions here with the roundings as they are written (nothing is contracted into an fma but what says fma).
+__device__ __forceinline__ float4 vx_add(const float4& a, const float4& b) {
+#pragma clang fp contract(off)
+    return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
-// Four sums with the weight rows' scales, the row's scale and (BIAS) the bias: the same roundings in every kernel.
+// Four sums with the weight rows' scales, the row's scale and (BIAS) the bias.
 template <bool BIAS>
 __device__ __forceinline__ float4 vx_scaled(const v4i& c, const float4& w, float s, const float4& b) {
+#pragma clang fp contract(off)
     float y[4];
     const float f[4] = {w.x, w.y, w.z, w.w}, d[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -42,10 +36,20 @@ __device__ __forceinline__ float4 vx_scaled(const v4i& c, const float4& w, float
     }
     return make_float4(y[0], y[1], y[2], y[3]);
 }
-__device__ __forceinline__ float vx_swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+__device__ __forceinline__ float vx_swiglu(float g, float u) {
+#pragma clang fp contract(off)
+    return g / (1.0f + expf(-g)) * u;
+}
 __device__ __forceinline__ float4 vx_swiglu(const v4i& g, const float4& wg, const v4i& u, const float4& wu, float s) {
     const float4 none = make_float4(0, 0, 0, 0), a = vx_scaled<false>(g, wg, s, none), b = vx_scaled<false>(u, wu, s, none);
     return make_float4(vx_swiglu(a.x, b.x), vx_swiglu(a.y, b.y), vx_swiglu(a.z, b.z), vx_swiglu(a.w, b.w));
+}
+// Outputs n .. n + 3 of row r (of `cols` in a row), y their products with the bias: the residual added, stored.
+template <bool VEC>
+__device__ __forceinline__ void vx_finish(const VxI8Args& a, size_t r, uint32_t n, uint32_t cols, float4 y) {
+    const uint32_t left = cols - n;
+    if (a.res.data) y = vx_add(y, vx_load4<VEC>(a.res.data, r * a.res.rs + n, a.res.dtype, left));
+    vx_store4<VEC>(a.out.data, r * a.out.rs + n, a.out.dtype, left, y);
 }
 // Outputs c .. c + 3 of a plain product's row r (of `cols` in a row), from their sums.
 template <bool SWIGLU>
@@ -684,7 +688,7 @@ __device__ __forceinline__ void vx_i8_tile(const VxI8Args& a, uint8_t* lds, uint
                     if constexpr (kGrouped) {
                         *(float4*)(a.part + (size_t)to[j] * a.part_stride + n) = y[j];  // (rows of whole float4)
                     } else if constexpr (DT < 3u) {
-                        if constexpr (RES) y[j] = make_float4(y[j].x + res[j].x, y[j].y + res[j].y, y[j].z + res[j].z, y[j].w + res[j].w);
+                        if constexpr (RES) y[j] = vx_add(y[j], res[j]);
                         vx_store4<true>(a.out.data, (size_t)to[j] * a.out.rs + n, DT, cols - n, y[j]);
                     } else {
                         vx_finish<false>(a, to[j], n, cols, y[j]);
