@@ -473,22 +473,22 @@ __device__ __forceinline__ uint32_t vx_xcd_run(uint32_t b, uint32_t total) {
     return x * q + (x < r ? x : r) + i;
 }
 
-template <int WN, int WM, int FN, int FM, int S, int KQ, int EPI>
+template <int WN, int WM, int FN, int FM, int S, int EPI>
 __device__ __forceinline__ void vx_i8_tile(const VxI8Args& a, uint8_t* lds, uint32_t nb, uint32_t e, uint32_t first, uint32_t end, bool once) {
-    constexpr int W = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, RB = 32 * KQ, STAGE = (TN + TM) * RB;  // RB: bytes of a row
+    constexpr int W = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, RB = 128, STAGE = (TN + TM) * RB;  // RB: bytes of a row
     constexpr bool kGrouped = EPI == VX_I8_HIDDEN || EPI == VX_I8_SLOT;
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t wn = wave / WM, wm = wave % WM;
-    const uint32_t steps = a.w.k_tiles * 2u / KQ, tile0 = nb * (TN / 16);
+    const uint32_t steps = a.w.k_tiles / 2u, tile0 = nb * (TN / 16);
 
-    // where this wave's share of a stage comes from: weight tiles (KQ / 2 pieces of 1 KiB each), pieces of 1024 / RB rows (where
-    // they do not come out even, the last piece comes more than once)
-    constexpr int PW = TN / 16 / W, APIECES = TM * RB / 1024, PA = (APIECES + W - 1) / W, UNITS = RB / 16, AROWS = 64 / UNITS;
-    const auto swizzle = [](uint32_t row) { return KQ == 4 ? row >> 1 & 7u : row >> 2 & 3u; };
+    // where this wave's share of a stage comes from: weight tiles (two pieces of 1 KiB each), pieces of eight rows
+    constexpr int PW = TN / 16 / W, PA = TM / 8 / W, UNITS = RB / 16, AROWS = 64 / UNITS;
+    static_assert(PW * 16 * W == TN && PA * 8 * W == TM, "the waves' shares are equal");
+    const auto swizzle = [](uint32_t row) { return row >> 1 & 7u; };
     const uint8_t* pw[PW];
     const uint8_t* pa[PA];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    const auto piece = [&](int j) { return APIECES % W == 0 || wave * PA + j < APIECES ? wave * PA + j : (uint32_t)APIECES - 1u; };
+    const auto piece = [&](int j) { return wave * PA + j; };
 #pragma unroll
     for (int j = 0; j < PW; ++j) {
         const uint32_t t = tile0 + wave * PW + j;
@@ -507,7 +507,7 @@ __device__ __forceinline__ void vx_i8_tile(const VxI8Args& a, uint8_t* lds, uint
         const uint32_t base = lds0 + stage * STAGE;
         if constexpr (j < PW) {
             vx_to_lds(base + (wave * PW + j) * (16u * RB), pw[j], lane * 16u, once);
-            if constexpr (KQ == 4) vx_to_lds(base + (wave * PW + j) * (16u * RB) + 1024u, pw[j] + 1024, lane * 16u, once);
+            vx_to_lds(base + (wave * PW + j) * (16u * RB) + 1024u, pw[j] + 1024, lane * 16u, once);
             pw[j] += 16 * RB;
         } else {
             vx_to_lds(base + TN * RB + piece(j - PW) * 1024u, pa[j - PW]);
@@ -516,9 +516,9 @@ __device__ __forceinline__ void vx_i8_tile(const VxI8Args& a, uint8_t* lds, uint
     };
     // operands of column quarter s: the weights' by tile, the rows' by their unit's place
     const uint32_t w_at = wn * FN * (32u * RB) + ((lane >> 4) & 1u) * (16u * RB) + (lane >> 5) * 256u + (lane & 15u) * 16u;
-    uint32_t a_at[KQ];
+    uint32_t a_at[4];
 #pragma unroll
-    for (int s = 0; s < KQ; ++s) a_at[s] = TN * RB + (wm * FM * 32u + (lane & 31u)) * RB + (((2u * s + (lane >> 5)) ^ swizzle(lane & 31u)) * 16u);
+    for (int s = 0; s < 4; ++s) a_at[s] = TN * RB + (wm * FM * 32u + (lane & 31u)) * RB + (((2u * s + (lane >> 5)) ^ swizzle(lane & 31u)) * 16u);
     // what the epilogue needs: outputs 4 (lane % LANES) .. + 3 of the wave's, the rows lane % 32 of its blocks
     constexpr bool kSwiglu = EPI == VX_I8_SWIGLU || EPI == VX_I8_HIDDEN;
     constexpr int ROW = 32 * FN + 4, LANES = (kSwiglu ? 16 : 32) * FN / 4, AT_ONCE = 64 / LANES;
@@ -575,12 +575,12 @@ __device__ __forceinline__ void vx_i8_tile(const VxI8Args& a, uint8_t* lds, uint
             constexpr int d0 = LO + i * (HI - LO) / P, d1 = LO + (i + 1) * (HI - LO) / P;
             if constexpr (d1 > d0) fetch(vx_int<d0>{}, into);
             if constexpr (d1 > d0 + 1) fetch(vx_int<d0 + 1>{}, into);
-            if constexpr (d1 > d0 + 2) fetch(vx_int<d0 + 2>{}, into);
+            static_assert(d1 <= d0 + 2);
             acc[n][m] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[from][n], fa[from][m], acc[n][m], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    constexpr int PIECES = KQ / 2 * PW + PA, HALF = (PW + PA) / 2;  // loads of a wave's share of a stage
+    constexpr int PIECES = 2 * PW + PA, HALF = (PW + PA) / 2;  // loads of a wave's share of a stage
     auto ready = [&](auto left_) {  // this wave's loads but the last `left` are in LDS, its reads in registers; then everybody's are
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(left_)::value) : "memory");
     };
@@ -592,10 +592,8 @@ __device__ __forceinline__ void vx_i8_tile(const VxI8Args& a, uint8_t* lds, uint
         constexpr bool REST = decltype(rest_)::value != 0, NEXT = decltype(next_)::value != 0;
         constexpr int ALL = REST ? PW + PA : HALF;
         quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<HALF>{}, vx_int<ALL>{}, behind(S - 1));
-        if constexpr (KQ == 4) {
-            quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
-            quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
-        }
+        quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+        quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
         ready(vx_int<(REST ? (S - 2) * PIECES : 0)>{});
         quarter(vx_int<1>{}, vx_int<0>{}, behind(1), vx_int<0>{}, vx_int<(NEXT ? HALF : 0)>{}, st);
         st = behind(1);
@@ -617,10 +615,8 @@ __device__ __forceinline__ void vx_i8_tile(const VxI8Args& a, uint8_t* lds, uint
     }
     for (; i + 1u < steps; ++i) step(vx_int<0>{}, vx_int<0>{});
     quarter(vx_int<0>{}, vx_int<1>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
-    if constexpr (KQ == 4) {
-        quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
-        quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
-    }
+    quarter(vx_int<1>{}, vx_int<2>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
+    quarter(vx_int<0>{}, vx_int<3>{}, st, vx_int<0>{}, vx_int<0>{}, 0);
     quarter(vx_int<1>{}, vx_int<-1>{}, 0, vx_int<0>{}, vx_int<0>{}, 0);
 
     // Epilogue, one block of 32 rows at a time: the sums go through LDS, where the lane of row lane % 32 writes those of n =
@@ -710,13 +706,13 @@ __device__ __forceinline__ void vx_i8_tile(const VxI8Args& a, uint8_t* lds, uint
 }
 
 // Plain products: patches of up to 4 row blocks by all weight blocks on an XCD, the rows first.
-template <int WN, int WM, int FN, int FM, int S, int KQ, int EPI>
+template <int WN, int WM, int FN, int FM, int S, int EPI>
 __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, uint32_t row0, uint32_t n_blocks, uint32_t m_blocks) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };  // (quotients are formed in vector registers)
     const uint32_t id = vx_xcd_run(blockIdx.x, n_blocks * m_blocks), patch = id / (4u * n_blocks);
     const uint32_t high = m_blocks - 4u * patch < 4u ? m_blocks - 4u * patch : 4u, in = id - patch * 4u * n_blocks;
-    vx_i8_tile<WN, WM, FN, FM, S, KQ, EPI>(a, lds, uniform(in / high), 0, uniform(row0 + (4u * patch + in % high) * 32u * WM * FM), a.n_rows, false);
+    vx_i8_tile<WN, WM, FN, FM, S, EPI>(a, lds, uniform(in / high), 0, uniform(row0 + (4u * patch + in % high) * 32u * WM * FM), a.n_rows, false);
 }
 
 // Grouped products: blocks of up to 256 of an expert's positions by 256 weight rows, eight waves of 64 weight rows by half of the
@@ -742,7 +738,7 @@ __global__ __launch_bounds__(512) void vx_i8_items_kernel(VxI8Args a, uint32_t n
     const bool once = end - first <= kItemRows && first == uniform(a.g.offsets[e]);
     vx_each<4>([&](auto l_) {
         constexpr int L = decltype(l_)::value + 1;
-        if (live == L) vx_i8_tile<4, 2, 2, L, VxLive<L>::stages, 4, EPI>(a, lds, nb, e, first, end, once);
+        if (live == L) vx_i8_tile<4, 2, 2, L, VxLive<L>::stages, EPI>(a, lds, nb, e, first, end, once);
     });
 }
 
@@ -760,21 +756,21 @@ __global__ __launch_bounds__(256) void vx_i8_small_items_kernel(VxI8Args a, uint
     const uint2 it = a.g.items[item];
     const uint32_t e = uniform(it.x), first = uniform(it.y) + block % parts * kSmallItemRows, end = uniform(a.g.offsets[e + 1u]);
     if (first >= end) return;
-    vx_i8_tile<2, 2, 1, 1, 4, 4, EPI>(a, lds, uniform(blockIdx.x % n_blocks), e, uniform(first), end, false);
+    vx_i8_tile<2, 2, 1, 1, 4, EPI>(a, lds, uniform(blockIdx.x % n_blocks), e, uniform(first), end, false);
 }
 
 constexpr uint32_t kTileStep = 1u << 20;  // rows of a launch
 
-template <int WN, int WM, int FN, int FM, int S, int KQ, int EPI>
+template <int WN, int WM, int FN, int FM, int S, int EPI>
 hipError_t vx_i8_tile_launch(const VxI8Args& a, hipStream_t st) {
-    constexpr uint32_t TN = 32 * WN * FN, TM = 32 * WM * FM, lds = S * (TN + TM) * 32 * KQ;
+    constexpr uint32_t TN = 32 * WN * FN, TM = 32 * WM * FM, lds = S * (TN + TM) * 128;
     static std::atomic<uint64_t> allowed{0};
-    const hipError_t set = vx_allow_lds((const void*)vx_i8_tile_kernel<WN, WM, FN, FM, S, KQ, EPI>, lds, allowed);
+    const hipError_t set = vx_allow_lds((const void*)vx_i8_tile_kernel<WN, WM, FN, FM, S, EPI>, lds, allowed);
     if (set != hipSuccess) return set;
     const uint32_t n_blocks = (a.w.n_tiles * 16u + TN - 1u) / TN;
     for (uint32_t r = 0; r < a.n_rows; r += kTileStep) {
         const uint32_t rows = a.n_rows - r < kTileStep ? a.n_rows - r : kTileStep, m_blocks = (rows + TM - 1u) / TM;
-        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, S, KQ, EPI>), dim3(n_blocks * m_blocks), dim3(64 * WN * WM), lds, st, a, r, n_blocks, m_blocks);
+        hipLaunchKernelGGL((vx_i8_tile_kernel<WN, WM, FN, FM, S, EPI>), dim3(n_blocks * m_blocks), dim3(64 * WN * WM), lds, st, a, r, n_blocks, m_blocks);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
@@ -852,14 +848,14 @@ hipError_t vx_i8_choose(const VxI8Args& a, hipStream_t st) {
         const auto tiles = [&](uint32_t by) { return (uint64_t)((a.w.n_tiles * 16u + by - 1u) / by) * ((a.n_rows + by - 1u) / by); };
         if (a.n_rows > 64u) {
             if (tiles(256u) >= 192u)
-                return a.w.k > 16384u ? vx_i8_tile_launch<2, 2, 4, 4, 2, 4, EPI>(a, st) : vx_i8_tile_launch<4, 2, 2, 4, 2, 4, EPI>(a, st);
+                return a.w.k > 16384u ? vx_i8_tile_launch<2, 2, 4, 4, 2, EPI>(a, st) : vx_i8_tile_launch<4, 2, 2, 4, 2, EPI>(a, st);
             const uint64_t t = tiles(128u);
-            if (t > 256u) return vx_i8_tile_launch<2, 2, 2, 2, 2, 4, EPI>(a, st);
-            if (t > 160u) return vx_i8_tile_launch<2, 2, 2, 2, 3, 4, EPI>(a, st);
-            if (t > 100u) return vx_i8_tile_launch<2, 2, 2, 1, 3, 4, EPI>(a, st);
-            return vx_i8_tile_launch<2, 2, 1, 1, 4, 4, EPI>(a, st);
+            if (t > 256u) return vx_i8_tile_launch<2, 2, 2, 2, 2, EPI>(a, st);
+            if (t > 160u) return vx_i8_tile_launch<2, 2, 2, 2, 3, EPI>(a, st);
+            if (t > 100u) return vx_i8_tile_launch<2, 2, 2, 1, 3, EPI>(a, st);
+            return vx_i8_tile_launch<2, 2, 1, 1, 4, EPI>(a, st);
         }
-        if (a.n_rows > 32u) return vx_i8_tile_launch<4, 1, 1, 1, 4, 4, EPI>(a, st);
+        if (a.n_rows > 32u) return vx_i8_tile_launch<4, 1, 1, 1, 4, EPI>(a, st);
         if (a.n_rows > 16u) {
             if (a.w.n_tiles > 2048u) return vx_i8_stream_launch<6, 2, 4, EPI>(a, st);
             return a.w.n_tiles >= 1024u ? vx_i8_stream_launch<4, 2, 4, EPI>(a, st) : vx_i8_stream_launch<2, 2, 8, EPI>(a, st);
