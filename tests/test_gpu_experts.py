@@ -371,6 +371,24 @@ def test_ffn_where_slots_stop_being_done_one_by_one(n, inner, hidden):
         m.check(x, ids, w, m(x, ids, w))
 
 
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("count,top,hidden,inner", [(40, 16, 96, 2047), (40, 16, 100, 2048), (40, 16, 104, 2049), (40, 17, 96, 2048), (300, 16, 64, 48), (4, 4, 4096, 1024),
+                                                    (2, 2, 2048, 2048), (1, 1, 4096, 2048), (1, 2, 4096, 2048), (3, 8, 1024, 1500), (5, 16, 96, 2048)])
+def test_ffn_slot_by_slot_and_by_groups(count, top, hidden, inner, n):
+    """A few rows, on both sides of where slots are no longer done one by one: by the places, by how often an expert's weights
+    would be read. The same bits as in a larger batch, which goes by groups."""
+    m = Mixture(count, hidden, inner, seed=count + top)
+    ids, w = choice(40, top, count, 5, low=-1)
+    for dtype in T:
+        x = rows(40, hidden, dtype, 3)
+        got = m(x[:n], ids[:n], w[:n])
+        m.check(x[:n], ids[:n], w[:n], got)
+        assert torch.equal(got, m(x, ids, w)[:n])
+        kept = x[:n].clone()
+        m(kept, ids[:n], w[:n], residual=kept, out=kept)
+        assert torch.equal(kept, m(x, ids, w, residual=x)[:n])
+
+
 @pytest.mark.parametrize("n,hidden,inner", [(100, 256, 14336), (65, 100, 16001), (600, 48, 14336), (1500, 300, 8200)])
 def test_ffn_of_very_unequal_products(n, hidden, inner):
     """A wide first product by large blocks, a narrow second one by parts of them, the last part partly filled or empty."""

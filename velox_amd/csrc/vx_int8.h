@@ -102,7 +102,7 @@ uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count, uint32_t n_tiles);  // 
 // every slot (a.part: [slot]), the experts' answers and their sum.
 bool vx_i8_by_row(const VxI8View& x, uint32_t n_rows, uint32_t k);
 hipError_t vx_launch_i8_row(const VxI8Args& a, const VxI8View& x, int epi, hipStream_t st);
-bool vx_i8_ffn_by_slot(const VxI8View& x, uint32_t n_rows, uint32_t hidden, uint32_t inner);
+bool vx_i8_ffn_by_slot(const VxI8View& x, uint32_t n_rows, uint32_t top, uint32_t count, uint32_t hidden, uint32_t inner);
 hipError_t vx_launch_i8_slots(const VxI8Args& a, const VxI8View& x, hipStream_t st);
 hipError_t vx_launch_i8_answers(const VxI8Args& a, const VxCombineArgs& c, hipStream_t st);
 hipError_t vx_launch_route(const VxRouteArgs& a, hipStream_t st);

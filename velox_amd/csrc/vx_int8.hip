@@ -890,10 +890,24 @@ hipError_t vx_launch_i8_row(const VxI8Args& a, const VxI8View& x, int epi, hipSt
     return vx_i8_row_launch_t<1, VX_I8_STORE>(a, x, st);
 }
 
-// Up to four rows whose hidden rows stay in a wave's registers (6 of 64 experts of 2048 x 1408: one row 26.6 -> 18.5 us, four
-// 40.7 -> 37.2, eight 47 -> 67; hidden rows of 14336, four rows: 121 -> 371).
-bool vx_i8_ffn_by_slot(const VxI8View& x, uint32_t n_rows, uint32_t hidden, uint32_t inner) {
-    return n_rows <= 4u && vx_whole_rows(x, hidden) && inner <= kAnswerMost;
+// Up to four rows whose hidden rows stay in a wave's registers (more: 14336, four rows 121 -> 371 us) and whose slots are dealt to the
+// answers' eight waves at most twice (one row, 32 of 64 experts of 1024 x 512: 30.1 and 30.3, all 64 44.7 -> 52.8). It saves three
+// launches, up to 8 us, but reads an expert's weights for each slot that names it: worth it while the slots that a choice of the
+// held experts at random would give to experts that other rows have too cost less than that again, 4 MB and the weights' bytes
+// each, 110 MB in all. Grouped and slot by slot, us (a launch behind the other, weights out of the caches):
+//   6 of 64 experts of 2048 x 1408, 1 to 4 rows: 25.8 19.1, 30.8 25.8, 40.5 33.5, 45.7 38.8 (six 52.9 55.9);
+//   8 of 8 of 7168 x 2048: 71.4 62.6, by groups from two rows on (74.7 115, 75.0 165, 74.7 214);
+//   8 of 32 of 4096 x 1024: 34.5 26.6, 48.6 37.7, 57.0 54.0, four by groups (61.6 70.1);
+//   2 of 2 of 4096 x 2048: 24.3 18.2, 25.4 22.6, from three rows on by groups (25.6 30.6, 25.8 35.5);
+//   64 places of 5 of 96 x 2048: by groups (25.3 76.5 to 28.9 152).
+// Where only a part of the experts is held, fewer slots are here than the rule counts with: 8 of 64 of 2048 x 1408, 8 here, three rows
+// go by groups, 17.1 for 12.9.
+bool vx_i8_ffn_by_slot(const VxI8View& x, uint32_t n_rows, uint32_t top, uint32_t count, uint32_t hidden, uint32_t inner) {
+    if (n_rows > 4u || top > 2u * kAnswerWaves || inner > kAnswerMost || !vx_whole_rows(x, hidden)) return false;
+    double unnamed = 1.0;  // the share of the experts that no row names
+    for (uint32_t r = 0; r < n_rows; ++r) unnamed *= top < count ? 1.0 - (double)top / count : 0.0;
+    const double again = n_rows * top - count * (1.0 - unnamed);
+    return again * (3.0 * hidden * inner + 4e6) <= 110e6;
 }
 hipError_t vx_launch_i8_slots(const VxI8Args& a, const VxI8View& x, hipStream_t st) { return vx_i8_row_launch_t<2, VX_I8_HIDDEN>(a, x, st); }
 hipError_t vx_launch_i8_answers(const VxI8Args& a, const VxCombineArgs& c, hipStream_t st) {

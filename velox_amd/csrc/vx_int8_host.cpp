@@ -291,7 +291,7 @@ int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Ma
     if (residual) c.res = view(residual);
     c.out = view(out);
     c.vec = whole(out) && (!residual || whole(residual));
-    if (vx_i8_ffn_by_slot(view(x), n_rows, gu.k, dn.k)) {
+    if (vx_i8_ffn_by_slot(view(x), n_rows, top_k, gu.count, gu.k, dn.k)) {
         a.ids = d_ids;
         a.first = first;
         hipError_t e = vx_launch_i8_slots(a, view(x), st);
