@@ -68,9 +68,9 @@ __device__ __forceinline__ uint64_t vx_open_groups(const VxRouteArgs& a, const F
         // be anything; a group without an expert is -infinity.
         const float size = marks[kVxMaxGroups + (lane < a.groups ? lane : 0u)], off = kVxOff * (2.0f + size);
         const bool known = size < INFINITY;
-        const float low = in ? (known ? my - off : -INFINITY) : INFINITY, high = in || lane >= a.groups ? -INFINITY : known ? my + off : INFINITY;
-        const uint32_t out = vx_wave_max(vx_word_of(high)), least = ~vx_wave_max(~vx_word_of(low));
-        unsure = out > vx_word_of(-INFINITY) && least <= out;
+        const float low = known ? my - off : -INFINITY, high = in || lane >= a.groups ? -INFINITY : known ? my + off : INFINITY;
+        const uint32_t out = vx_wave_max(vx_word_of(high));
+        unsure = out > vx_word_of(-INFINITY) && __ballot(in && vx_word_of(low) <= out);
     }
     vx_wave_sync();
     return open;
@@ -82,7 +82,7 @@ __device__ __forceinline__ uint64_t vx_open_groups(const VxRouteArgs& a, const F
 // ordered again in 64 bits, each by how many are above it (all experts again, one choice after the other, took 10 us, which a launch
 // with one such row waited for: 4096 rows 18.7 -> 9.9 us). The largest is found top_k times: by DPP in the wave, its place
 // by ballots. The chosen scores are formed in 64 bits. What bounds it: instructions, about 800 of the vector unit and 350 of the
-// scalar one a row (16384 rows of 256 experts, 8 of them in 4 of 8 groups: 25 us, of which reading takes 4); one row 5.5 us.
+// scalar one a row (16384 rows of 256 experts, 8 of them in 4 of 8 groups: 28 us, of which reading takes 4); one row 5.1 us.
 template <class T, uint32_t ITEMS>
 __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
     __shared__ double room[4][ITEMS * 64u + kVxMaxGroups];
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(256) void vx_route_kernel(VxRouteArgs a) {
 // A workgroup takes kGroupSlots slots, a wave kGroupRun neighbours of them. Slots of one expert within a wave find each other by
 // ballots of their keys' bits, so that ranks follow the slots' order; waves' and workgroups' counts are summed in order.
 // Several workgroups count first (their counts through memory), then place; one does both at once. Bound by latency: one workgroup
-// 3.0 us, 131072 slots of 256 experts 4.8 and 9.3 us (each workgroup sums the counts of those in front of it).
+// 3.1 us, 131072 slots of 256 experts 4.6 and 9.5 us (each workgroup sums the counts of those in front of it).
 constexpr uint32_t kGroupWaves = 4, kGroupRun = 256, kGroupSlots = kGroupWaves * kGroupRun, kGroupSteps = kGroupRun / 64u;
 constexpr uint32_t kGroupThreads = 64u * kGroupWaves;
 
