@@ -613,10 +613,10 @@ int velox_hip_int8_product(const VeloxHipInt8Matrix* m, const VeloxHipRows* x, c
  * route: of n_experts experts the top_k with the largest choice values, in descending order, equal ones by index.
  *   score: SOFTMAX exp(x_e) / sum over the row, SIGMOID 1 / (1 + exp(-x_e)); choice value: score + bias[e] (d_bias NULL: 0).
  *   With groups > 1 (groups of n_experts / groups neighbours) only the experts of the top_groups groups with the largest
- *   marks take part, a group's mark being the LARGEST of its choice values or the sum of its TWO largest (equal marks by
- *   index). weights[r][j] = scale * score, divided by the row's sum of chosen scores first with renormalize (0 where that
- *   sum is 0). Without a bias the order is that of the logits themselves; choice values with one, and sums of two, compare
- *   as in 64 bits, so that nearly equal ones keep their order. A logit of -infinity or NaN takes its expert out of the row
+ *   marks take part, a group's mark being the LARGEST of its choice values or the sum of its TWO largest (one alone where
+ *   no other is left; equal marks by index). weights[r][j] = scale * score, divided by the row's sum of chosen scores first
+ *   with renormalize (0 where that sum is 0). Without a bias the order is that of the logits themselves; choice values with
+ *   one, and sums of two, compare as in 64 bits, so that nearly equal ones keep their order. A logit of -infinity or NaN takes its expert out of the row
  *   and of the softmax's sum, a bias that is not finite takes it out of every row; a logit of +infinity counts as the
  *   largest finite number. Where fewer than top_k experts are left, the rest of ids is VELOX_HIP_NO_EXPERT and of weights 0:
  *   a row of -infinity is padding. */

@@ -91,8 +91,12 @@ __global__ __launch_bounds__(256) void vx_i8_pack_kernel(VxI8Mat m, uint32_t fir
 
 // ---- rows in 8 bits ----
 // Scale and codes of a row, which is read once: as many threads a row as hold it in registers (a wave for short rows, which
-// then share nothing). Bound by the bytes (8192 rows of 29568 bf16, 727 MB: 127 to 172 us, 5.7 to 4.2 TB/s), for few rows by latency
-// (32 rows of 3584 fp32: 4.9 us).
+// then share nothing). Bound by the bytes in fp32 (8192 rows of 14336, 587 MB: 108 us, 5.4 TB/s), in 16 bits by the values that lie next to
+// a half, for which a wave goes over its values again: 8192 rows of 29568 bf16, 727 MB, take 157 to 175 us (4.6 to 4.2 TB/s) with a few
+// channels far above the others, as hidden states have (one value in 3000), 281 with normally distributed ones (one in 380: bf16 numbers
+// are few, and so are their quotients). For few rows by latency (32 rows of 3584 fp32: 4.8 us). 64 values of 16 bits a thread of 1024
+// (rows of 32769 to 65536 values) do not all stay in registers (44 to 48 bytes a thread go to memory); they still beat the kernel below
+// with the former values (4096 rows of 40960: 166 and 216 us), not with the latter (267 and 215).
 template <class T, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void vx_i8_quantize_kernel(VxI8View x, uint32_t n_rows, uint32_t k, VxI8Rows o, const uint32_t* limit) {
     constexpr int WG = TPR < 256 ? 256 : TPR;
@@ -104,7 +108,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void vx_i8_quantize_kernel(V
     if (t == 0) o.scales[r] = s;
 }
 
-// Rows at any place and of any length, value by value: NE of them a thread in registers, those behind read twice.
+// Rows at any place and of any length, value by value: NE of them a thread in registers, those behind read twice. Each value's
+// remainder is formed, so the values do not matter: 8192 rows of 4096 bf16 25 us, of 29568 289 (2.5 TB/s), fp32 32 and 414.
 template <class T, int NE>
 __global__ __launch_bounds__(256) void vx_i8_quantize_any_kernel(VxI8View x, uint32_t k, VxI8Rows o, const uint32_t* limit) {
     __shared__ uint32_t red[4];
@@ -387,7 +392,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void vx_i8_row_kernel(VxI8Args a, V
 
 // 16 outputs of a row: each wave takes slots of the row in turn, puts the slot's hidden row into 8 bits in its own piece of LDS
 // while its expert's weights are on their way, and multiplies; the answers meet in LDS and are added in the slots' order. Bound by
-// latency as above (6 of 64 experts of 2048 x 1408, 17 MB: 9.5 us).
+// latency as above (6 of 64 experts of 2048 x 1408, 17 MB: 9.5 to 10 us by 128 workgroups, half of the CUs).
 constexpr uint32_t kAnswerWaves = 8, kAnswerMost = 8u * 4u * 64u;  // values of a hidden row
 __global__ __launch_bounds__(64 * kAnswerWaves) void vx_i8_answer_kernel(VxI8Args a, VxCombineArgs c, uint32_t n_blocks) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -718,8 +723,8 @@ __global__ __launch_bounds__(64 * WN * WM) void vx_i8_tile_kernel(VxI8Args a, ui
 // Grouped products: blocks of up to 256 of an expert's positions by 256 weight rows, eight waves of 64 weight rows by half of the
 // positions. As many blocks of 64 positions are fetched and multiplied as there are (by tiles of 128, padded, 4096 rows of 8 experts,
 // 64 of 256 here, took 978 us, so 830), and the fewer they are, the more stages LDS holds. An expert whose weights one block
-// reads passes the caches by (512 rows: 506 -> 465 us). What bounds it there: the weights' way to LDS (without the products 783 us,
-// without any loads 517).
+// reads passes the caches by (512 rows: 506 -> 465 us). What bounds it there: the weights' way to LDS (the call 839 us; in a build without
+// the products, the operands still read, 775, without the rows' loads 801, without the weights' 534, without either 493).
 constexpr uint32_t kItemRows = 256u;
 template <int L>
 struct VxLive {
@@ -819,9 +824,18 @@ hipError_t vx_launch_i8_quantize(const VxI8View& x, uint32_t n_rows, uint32_t k,
     return hipSuccess;
 }
 
-// Positions of a block of a grouped product, by how many slots there are for an expert (64 of 256 experts of 7168 x 2048 here, 8 for
-// a row): 32 rows 185 us by 16 and by 32, 128 rows 295 and 279, 256 rows 374 by 32 and 361 by tiles, 512 rows 607 and 470. Where
-// blocks of 256 would not even be one for each CU, 64 (257 rows through 5 experts of 576 x 1100: 36 -> 28 us).
+// Positions of a block of a grouped product, by the call's slots for each expert held. How many of them go to experts elsewhere is not
+// known on the host, so the borders, 12 and 32, lie between what measures best where all are held and where a quarter is. Calls by blocks
+// of 16, 32, 64 and 256, us, 8 places a row of experts of 7168 x 2048:
+//   slots for each held      64 of 64 here              64 of 256 here
+//     8 (64 rows)       453   459   489   508      374   376   418   438
+//    16 (128)           650   547   510   530      435   436   481   501
+//    32 (256)          1136   867   555   549      471   474   508   526
+//    64 (512)          2102  1517   711   606      693   568   528   545
+//   128 (1024)         4012  2785  1019   730     1198   906   574   564
+// and 6 of 64 of 2048 x 1408, 128 rows (12 slots): 119, 116, 120, 135. What that costs at the borders: all held, 16 to 31 slots, 7 to 12 %
+// over blocks of 64; a quarter held, 32 slots, 11 % over blocks of 16. Where blocks of 256 would not even be one for each CU, 64
+// (257 rows through 5 experts of 576 x 1100: 36 -> 28 us).
 uint32_t vx_i8_item_rows(uint32_t slots, uint32_t count, uint32_t n_tiles) {
     if (slots < 32u * count) return slots >= 12u * count ? 32u : 16u;
     return (uint64_t)(slots / kItemRows + count) * ((n_tiles + 15u) / 16u) < 256u ? kSmallItemRows : kItemRows;

@@ -122,7 +122,8 @@ __device__ __forceinline__ uint32_t vx_threads_max(uint32_t v, uint32_t* red) {
 // A row of k values (a whole number of 16-byte vectors, so placed) by THREADS threads, t this one's number, as codes at `to`
 // (memory or LDS), k filled up to a multiple of 128; its scale. Up to NV vectors a thread stay in registers between the search
 // for the largest value and the rounding, those behind are read again (MORE). Loads behind the row give 0. Values next to
-// a half, one in 5000, are done again by a rolled loop: little code, which comes through the instruction cache once.
+// a half, one in 5000 (bf16: one in 380 of normally distributed ones), are done again by a rolled loop: little code, which comes
+// through the instruction cache once.
 template <class T, int THREADS, int NV, bool MORE>
 __device__ __forceinline__ float vx_hold_row(const T* from, uint32_t k, uint8_t* to, uint32_t t, uint32_t* red) {
     constexpr uint32_t V = 16 / sizeof(T), STEP = THREADS * V;
