@@ -602,8 +602,9 @@ int velox_hip_int8_quantize(const VeloxHipRows* x, uint32_t n_rows, uint32_t k, 
  * VELOX_GEMV_STORE: out = y (+ bias[n]); VELOX_GEMV_RESIDUAL: out = residual + y (+ bias[n]) (residual may be out itself:
  * the same data and stride; other overlaps are not allowed); VELOX_GEMV_SWIGLU (a paired matrix, and only that):
  * out[r][j] = silu(gate_j) up_j. fp32 throughout, rounded once to out's type. out's rows do not overlap each other (EINVAL
- * where its stride is less than a row); out may begin where x does; other overlaps with the rows are not allowed. The rows come as x, quantized on the way (workspace: velox_hip_int8_product_bytes, 16-byte
- * aligned), or as q, already in 8 bits (no workspace); the other is NULL. m->count is 1. Fewer than 2^24 rows. */
+ * where its stride is less than a row); out may begin where x does; other overlaps with the rows are not allowed. The rows
+ * come as x, quantized on the way (workspace: velox_hip_int8_product_bytes, 16-byte aligned), or as q, already in 8 bits (no
+ * workspace); the other is NULL. m->count is 1. Fewer than 2^24 rows. */
 int velox_hip_int8_product_bytes(const VeloxHipInt8Matrix* m, uint32_t n_rows, uint64_t* bytes);
 int velox_hip_int8_product(const VeloxHipInt8Matrix* m, const VeloxHipRows* x, const VeloxHipInt8Rows* q, uint32_t n_rows,
                            const float* d_bias, const VeloxHipRows* residual, const VeloxHipRows* out, int mode,
@@ -616,10 +617,10 @@ int velox_hip_int8_product(const VeloxHipInt8Matrix* m, const VeloxHipRows* x, c
  *   marks take part, a group's mark being the LARGEST of its choice values or the sum of its TWO largest (one alone where
  *   no other is left; equal marks by index). weights[r][j] = scale * score, divided by the row's sum of chosen scores first
  *   with renormalize (0 where that sum is 0). Without a bias the order is that of the logits themselves; choice values with
- *   one, and sums of two, compare as in 64 bits, so that nearly equal ones keep their order. A logit of -infinity or NaN takes its expert out of the row
- *   and of the softmax's sum, a bias that is not finite takes it out of every row; a logit of +infinity counts as the
- *   largest finite number. Where fewer than top_k experts are left, the rest of ids is VELOX_HIP_NO_EXPERT and of weights 0:
- *   a row of -infinity is padding. */
+ *   one, and sums of two, compare as in 64 bits, so that nearly equal ones keep their order. A logit of -infinity or NaN
+ *   takes its expert out of the row and of the softmax's sum, a bias that is not finite takes it out of every row; a logit of
+ *   +infinity counts as the largest finite number. Where fewer than top_k experts are left, the rest of ids is
+ *   VELOX_HIP_NO_EXPERT and of weights 0: a row of -infinity is padding. */
 #define VELOX_HIP_NO_EXPERT 0xFFFFFFFFu
 #define VELOX_ROUTE_SOFTMAX 0u
 #define VELOX_ROUTE_SIGMOID 1u
@@ -649,8 +650,9 @@ int velox_hip_expert_group(const uint32_t* d_ids, uint32_t n_slots, uint32_t fir
  * - first. gate_up (paired, n = 2 inner, k = hidden) and down (n = hidden, k = inner) hold the experts first .. first +
  * count - 1; other ids (VELOX_HIP_NO_EXPERT, experts that live elsewhere) add nothing, a row may name an expert twice. x and
  * h enter the products in 8 bits (h from fp32), sums are fp32 in the order of j, rounded once to out's type. out may be x or
- * the residual (the same data and stride); its rows do not overlap each other (EINVAL) nor anything else that is given. n_rows * top_k <= 2^20; workspace: velox_hip_expert_ffn_bytes of the same
- * matrices, enough for up to n_rows rows of any types, 16-byte aligned. */
+ * the residual (the same data and stride); its rows do not overlap each other (EINVAL) nor anything else that is given.
+ * n_rows * top_k <= 2^20; workspace: velox_hip_expert_ffn_bytes of the same matrices, enough for up to n_rows rows of any
+ * types, 16-byte aligned. */
 int velox_hip_expert_ffn_bytes(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Matrix* down, uint32_t n_rows,
                                uint32_t top_k, uint64_t* bytes);
 int velox_hip_expert_ffn(const VeloxHipInt8Matrix* gate_up, const VeloxHipInt8Matrix* down, uint32_t first,

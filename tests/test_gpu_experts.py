@@ -400,6 +400,24 @@ def test_ffn_of_very_unequal_products(n, hidden, inner):
     m.check(x, ids, w, m(x, ids, w))
 
 
+@pytest.mark.parametrize("hidden,inner", [(131072, 48), (48, 131072), (131072, 2048)])
+def test_ffn_of_the_longest_rows(hidden, inner):
+    m = Mixture(2, hidden, inner)
+    for n in (1, 3, 6, 40, 200):
+        for dtype in ("f32", "bf16"):
+            x = rows(n, hidden, dtype, n)
+            ids, w = choice(n, 2, 2, 5, low=-1)
+            m.check(x, ids, w, m(x, ids, w))
+
+
+def test_ffn_of_the_most_experts():
+    m = Mixture(1024, 64, 32)
+    for n, top in ((1, 8), (4, 64), (100, 8), (700, 64)):
+        x = rows(n, 64, "f16", n)
+        ids, w = choice(n, top, 1024, 5, low=-1)
+        m.check(x, ids, w, m(x, ids, w))
+
+
 def test_ffn_weights_past_32_bits():
     """18 experts of 8192 x 16384: the last one's gate and up lie 4.5 GB in."""
     m = Mixture(18, 8192, 16384)

@@ -160,6 +160,16 @@ def test_product_at_the_largest_sums():
     check(x, w, sw, int8.product(x, int8.Int8Matrix(w, sw)))
 
 
+@pytest.mark.parametrize("m", [1, 3, 17, 40, 100, 300])
+def test_product_of_the_most_outputs(m):
+    """2^20 weight rows; paired, 2^19 gate and up rows."""
+    n, k = 1 << 20, 72
+    x = rows(m, k, "bf16", m)
+    w, sw = weights(n, k, 3)
+    check(x, w, sw, int8.product(x, int8.Int8Matrix(w, sw)))
+    check(x, w, sw, int8.product(x, int8.Int8Matrix(w, sw, paired=True)), paired=True)
+
+
 @pytest.mark.parametrize("m", [1, 5, 40, 200])
 def test_product_of_rows_already_in_8_bits_any_output_type_and_place(m):
     k, n = 500, 70
